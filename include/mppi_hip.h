@@ -37,8 +37,9 @@ extern "C" {
 #define MPPI_ABI_VERSION 8
 #define MPPI_LOG_CAP 4096
 #define MPPI_NOALLOC_MAX_K 262144   /* most samples mppi_update_from_returns_noalloc accepts */
+#define MPPI_DRAW_MAX_K 16777216    /* most samples per row mppi_draw_from_returns accepts */
 
-enum { MPPI_F32 = 0, MPPI_F64 = 1 };
+enum { MPPI_F32 = 0, MPPI_F64 = 1, MPPI_F16 = 2, MPPI_BF16 = 3 };   /* planners: the first two */
 enum { MPPI_REWARD_DENSE = 0, MPPI_REWARD_SPARSE = 1, MPPI_REWARD_TRACKING = 2, MPPI_REWARD_COOLING = 3 };
 enum { MPPI_TAIL_REPEAT = 0, MPPI_TAIL_MEAN = 1 };
 enum {
@@ -299,6 +300,57 @@ int mppi_update_from_returns(int32_t device, const double* act_KxHM, const doubl
  * mppi_planner_create or at the first call on that device (which should therefore be made before a capture). */
 int mppi_update_from_returns_noalloc(int32_t device, const double* d_act_KxHM, const double* d_R, int32_t K, int32_t HM,
                                      double kappa, double* d_act_seq_out, void* stream);
+
+/* Which samples a draw may pick, and how it weighs them: w_k = exp(kappa (R_k - max R)), the weights of `MPPI.update`
+ * (trajopt/algos/mppi.py:60-62), among the samples that pass three filters, applied in this order.  Samples are ordered
+ * by return, best first, equal ones by index; a sample whose return is not finite takes no part.
+ *   top_k: the first top_k of the order (0: all);
+ *   top_p: of these, the ones with less than top_p times their whole mass before them (1: all that have mass);
+ *   min_p: of these, the ones with w_k >= min_p, i.e. at least that fraction of the best sample's weight (0: all).
+ * kappa is finite and >= 0, top_p in (0, 1], min_p in [0, 1].  An array of one value per row (device memory) stands in
+ * for a number where its pointer is not NULL; its values cannot be checked here, and one outside its range leaves its row
+ * without samples (a negative top_k: all samples). */
+typedef struct mppi_draw_filter {
+    double kappa;
+    int64_t top_k;
+    double top_p;
+    double min_p;
+    const double* kappa_of;
+    const int64_t* top_k_of;
+    const double* top_p_of;
+    const double* min_p_of;
+} mppi_draw_filter;
+
+/* D draws from each of `rows` rows of K returns: index[row][d] = the smallest k with  sum_{j <= k} w_j > u[row][d] W  over
+ * the samples that the filter keeps, W their mass, and weight[row][d] = w_k / W (weight may be NULL).  u in [0, 1); values
+ * outside are taken as the nearest end.  A row without samples gives index -1 and weight 0.  No counterpart in the reference,
+ * whose update is the mean over the same weights (trajopt/algos/mppi.py:56-65).
+ * All arrays are device memory: returns of type `dtype` (MPPI_F32, F64, F16, BF16), element k of row r at
+ * r * row_stride + k * col_stride elements; u (rows, D), index (rows, D) and weight (rows, D) contiguous.  The work is
+ * enqueued on `stream` (NULL: the default stream); nothing is allocated or synchronised, and it may be captured.  K up to
+ * MPPI_DRAW_MAX_K (-6 beyond).  The current device of the calling thread is left as it was. */
+int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32_t rows, int32_t K, int64_t row_stride,
+                           int64_t col_stride, const double* d_u, int32_t D, const mppi_draw_filter* filter, int64_t* d_index,
+                           float* d_weight, void* stream);
+
+/* Norm of the gradients of a critic (or of any tensors) and clipping to a largest norm, for the training steps between
+ * planning epochs (sandbox/examples/ac_reacher_7dof_mppi.py:146-229; the reference leaves them unclipped).
+ *   MPPI_NORM_L2: sqrt(sum g^2), MPPI_NORM_MAX: max |g|, over all entries of all n tensors;
+ *   clip: out_i = g_i s with s = max_norm / norm if norm > max_norm, else 1.  A norm that is not finite changes nothing.
+ * Tensor i has sizes[i] contiguous entries of type dtypes[i] (MPPI_F32, MPPI_F16 or MPPI_BF16) at the device address
+ * d_grads[i], a multiple of the entry's size; the four arrays themselves are host memory and are read before the call returns.
+ * d_out[i] = d_grads[i] clips in place; otherwise nothing that is written may overlap another tensor (-1).  Sums of squares
+ * are fp64.  *d_norm (device memory) receives the norm before clipping, rounded to float.  d_workspace: device memory of at
+ * least mppi_gradient_workspace bytes, 8-byte aligned, that nothing else uses until the work on `stream` is done.  The work
+ * is enqueued on `stream` (NULL: the default stream); nothing is allocated on the device or synchronised, and it may be
+ * captured (with the addresses it was given).  The current device of the calling thread is left as it was. */
+enum { MPPI_NORM_L2 = 0, MPPI_NORM_MAX = 1 };
+int mppi_gradient_workspace(int32_t n, size_t* bytes);
+int mppi_gradient_norm(int32_t device, int32_t n, const void* const* d_grads, const int64_t* sizes, const int32_t* dtypes,
+                       int32_t norm_type, float* d_norm, void* d_workspace, size_t workspace_bytes, void* stream);
+int mppi_clip_gradients(int32_t device, int32_t n, const void* const* d_grads, void* const* d_out, const int64_t* sizes,
+                        const int32_t* dtypes, int32_t norm_type, double max_norm, float* d_norm, void* d_workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* Host utility: the first n values of numpy's legacy normal stream after `np.random.seed(seed)` -- what the
  * reference's rollout workers draw (trajopt/utils.py:118-139) -- bit for bit, generated in bulk on nthreads host

@@ -1,0 +1,296 @@
+"""Draws from exponentiated returns against the definition in 64 bits (oracle/ref_learn.py).
+
+An index has to be the oracle's: the numbers u are random, and the chance that one lies within the kernels' rounding
+(below 2^-40 of the mass) of a border between two samples is below 1e-7 over all of these tests.  A weight is rounded to
+float32 once (2^-24 relative); the fp64 exponentials behind it are good to 1e-13 at the largest distance that can be drawn
+(kappa (Rmax - R) < 44, times 2^-53, a few of them)."""
+import numpy as np
+import pytest
+
+from oracle import ref_learn
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["float64", "float32", "float16", "bfloat16"]
+WEIGHT_RTOL = 2.0 ** -24 * (1 + 1e-5) + 1e-13
+
+FILTERS = [
+    dict(),
+    dict(top_k=1),
+    dict(top_k=7),
+    dict(top_p=0.5),
+    dict(min_p=0.3),
+    dict(top_k=40, top_p=0.9, min_p=0.02),
+    dict(top_k=1 << 20, top_p=0.999, min_p=1e-6),
+]
+
+
+def _draw(R, u, **kw):
+    from trajopt_amd.device import draw_from_returns
+    return draw_from_returns(R, u, **kw)
+
+
+def _check(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0, got=None):
+    """R, u: CUDA tensors (rows, K), (rows, D); parameters numbers or CUDA tensors."""
+    index, weight = got if got is not None else _draw(R, u, kappa=kappa, top_k=top_k, top_p=top_p, min_p=min_p)
+    assert index.shape == weight.shape == u.shape and str(index.dtype) == "torch.int64" and str(weight.dtype) == "torch.float32"
+    Rn, un = R.double().cpu().numpy(), u.double().cpu().numpy()
+    index, weight = index.cpu().numpy(), weight.cpu().numpy()
+    one = lambda v, b: v.cpu().numpy()[b] if hasattr(v, "cpu") else v  # noqa: E731
+    for b in range(Rn.shape[0]):
+        i, w = ref_learn.draw(Rn[b], un[b], one(kappa, b), one(top_k, b), one(top_p, b), one(min_p, b))
+        assert np.array_equal(index[b], i), (b, np.flatnonzero(index[b] != i)[:5], index[b][index[b] != i][:5], i[index[b] != i][:5])
+        assert np.all(np.abs(weight[b] - w) <= WEIGHT_RTOL * w + 1e-45), (b, np.abs(weight[b] - w).max())
+
+
+def _returns(rows, K, dtype, seed, spread=2.0, masked=0.0):
+    import torch
+    rng = np.random.RandomState(seed)
+    R = torch.tensor(-20.0 + spread * rng.normal(size=(rows, K)), device="cuda").to(getattr(torch, dtype))
+    if masked:
+        bad = torch.tensor([np.nan, -np.inf, np.inf, 0.0], dtype=R.dtype, device="cuda")
+        bad[3] = torch.finfo(R.dtype).min
+        at = torch.tensor(rng.uniform(size=(rows, K)) < masked, device="cuda")
+        R = torch.where(at, bad[torch.tensor(rng.randint(0, 4, size=(rows, K)), device="cuda")], R)
+    return R
+
+
+def _numbers(rows, D, seed):
+    import torch
+    return torch.tensor(np.random.RandomState(1000 + seed).uniform(size=(rows, D)), device="cuda")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("f", range(len(FILTERS)))
+@pytest.mark.parametrize("rows,K,D", [(1, 1, 1), (3, 2, 3), (5, 63, 2), (1, 64, 9), (4, 65, 1), (2, 511, 70), (2, 513, 3), (1, 4099, 20)])
+def test_draws(dtype, f, rows, K, D):
+    R, u = _returns(rows, K, dtype, K + f), _numbers(rows, D, K)
+    _check(R, u, kappa=1.5, **FILTERS[f])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,K", [(2, 255), (2, 257), (2, 1023), (2, 1025), (2, 2047), (2, 2049), (3, 4097), (2, 8191), (2, 8193), (2, 16383),
+                                    (2, 16385), (1, 32769), (2, 65535), (1, 65537), (1, 131071), (1, 524291)])
+def test_long_rows(dtype, rows, K):
+    R = _returns(rows, K, dtype, K, masked=0.05)
+    _check(R, _numbers(rows, 5, K), kappa=0.7, top_k=K // 3, top_p=0.8)
+    _check(R, _numbers(rows, 33, K), kappa=1.1, top_p=0.97, min_p=1e-4)
+    _check(R, _numbers(rows, 2, K), kappa=3.0, top_k=50)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kappa", [0.0, 1e-3, 25.0, 300.0, 1e6])
+def test_temperatures(dtype, kappa):
+    """From uniform (kappa 0) to the best sample alone."""
+    for K in (50, 3000, 40000):
+        R, u = _returns(2, K, dtype, K), _numbers(2, 11, K)
+        _check(R, u, kappa=kappa)
+        _check(R, u, kappa=kappa, top_k=K // 2, top_p=0.6)
+        _check(R, u, kappa=kappa, min_p=0.2, top_p=0.9)
+
+
+@pytest.mark.parametrize("K", [10, 700, 5000, 70000])
+@pytest.mark.parametrize("levels", [1, 2, 5])
+def test_ties_go_to_the_lowest_index(K, levels):
+    """Few different returns: every border lies among equal samples."""
+    import torch
+    rng = np.random.RandomState(K + levels)
+    R = torch.tensor(rng.randint(0, levels, size=(2, K)).astype(np.float32) * 0.25, device="cuda")
+    if levels > 1:
+        R = torch.where(R == 0, torch.tensor([0.0, -0.0], device="cuda").repeat(K)[:K], R)      # both zeros are one value
+    u = _numbers(2, 17, K)
+    for f in (dict(top_k=K // 2), dict(top_k=3), dict(top_p=0.37), dict(top_p=0.9, top_k=(2 * K) // 3), dict(min_p=0.9), dict(min_p=1.0)):
+        _check(R, u, kappa=2.0, **f)
+    half = R.to(torch.bfloat16)
+    _check(half, u, kappa=0.0, top_k=K // 3, top_p=0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_a_mask_empties(dtype):
+    import torch
+    for K in (5, 600, 9000, 66000):
+        R = _returns(6, K, dtype, K, masked=0.3)
+        R[0] = float("nan")
+        R[1] = -float("inf")
+        R[2] = torch.finfo(R.dtype).min                     # finite: every sample weighs the same
+        R[3] = float("-inf")
+        R[3, K - 1] = -3.0                                   # one sample left
+        R[4] = torch.finfo(R.dtype).min
+        R[4, K // 2] = 1.0
+        u = _numbers(6, 4, K)
+        for f in (dict(), dict(top_k=3), dict(top_p=0.5), dict(top_k=5, top_p=0.9, min_p=0.1)):
+            _check(R, u, kappa=1.0, **f)
+        index, weight = _draw(R, u)
+        assert (index[:2] == -1).all() and (weight[:2] == 0).all() and (index[3] == K - 1).all() and (index[4] == K // 2).all()
+
+
+def test_range_of_the_type():
+    """Returns as far apart as the type allows, and neighbours one rounding apart."""
+    import torch
+    for dtype in (torch.float64, torch.float32):
+        big = torch.finfo(dtype).max
+        R = torch.tensor([[-big, big, 0.0, big, -big, 1.0, torch.finfo(dtype).tiny / 4]], dtype=dtype, device="cuda")
+        u = torch.linspace(0, 0.99, 23, dtype=torch.float64, device="cuda").reshape(1, -1)
+        for f in (dict(), dict(top_k=1), dict(top_k=3), dict(top_p=0.5)):
+            _check(R, u, kappa=1.0, **f)
+            _check(R / 4, u, kappa=0.0, **f)
+        one = torch.ones(1, 1000, dtype=dtype, device="cuda")
+        eps = torch.finfo(dtype).eps
+        close = one + eps * torch.arange(1000, device="cuda", dtype=dtype)[torch.randperm(1000, generator=torch.Generator().manual_seed(1)).cuda()]
+        for K in (1000, 64000):
+            _check(close.repeat(1, K // 1000), u, kappa=1.0, top_k=K // 3 + 1, top_p=0.7)
+
+
+def test_numbers_at_the_ends():
+    import torch
+    for K in (40, 5000, 80000):
+        R = _returns(1, K, "float32", K)
+        R[0, 0] = -1000.0                                    # weighs nothing: u = 0 must not pick it
+        R[0, K - 1] = float("-inf")
+        u = torch.tensor([[0.0, 1 - 2.0 ** -53, 1.0, 2.0, -1.0, float("nan"), float("inf"), -float("inf")]], dtype=torch.float64, device="cuda")
+        index, weight = _draw(R, u, kappa=2.0, top_p=0.99)
+        w = ref_learn.kept_weights(R[0].double().cpu().numpy(), 2.0, 0, 0.99)
+        first, last = np.flatnonzero(w * 2.0 ** 40 > 1)[[0, -1]]
+        assert index.cpu().tolist()[0] == [first, last, last, last, first, first, last, first]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides(dtype):
+    import torch
+    for rows, K in ((3, 50), (4, 3001), (2, 20000), (2, 70001)):
+        u = _numbers(rows, 6, K)
+        wide = _returns(rows, K + 7, dtype, K)
+        _check(wide[:, 3:K + 3], u, kappa=1.0, top_k=20, top_p=0.9)           # rows at every alignment
+        tall = _returns(K, rows, dtype, K)
+        _check(tall.t(), u, kappa=1.0, top_p=0.8)                              # samples a row apart
+        _check(wide[:, ::2][:, :K // 2], u, kappa=1.0, min_p=0.05)
+        _check(wide[:1, :K].expand(rows, K), u, kappa=1.0, top_p=0.8)          # one row for all
+    R, u = _returns(1, 999, dtype, 5), _numbers(1, 3, 5)
+    index, weight = _draw(R[0], u[0], kappa=0.5)
+    assert index.shape == (3,)
+    _check(R, u, kappa=0.5, got=(index[None], weight[None]))
+    index, weight = _draw(R, u.float(), kappa=0.5)
+    _check(R, u.float().double(), kappa=0.5, got=(index, weight))
+
+
+@pytest.mark.parametrize("K", [30, 500, 6000, 70000])
+def test_parameters_per_row(K):
+    import torch
+    rows = 12
+    rng = np.random.RandomState(K)
+    R, u = _returns(rows, K, "float32", K, masked=0.02), _numbers(rows, 5, K)
+    kappa = torch.tensor(np.exp(rng.uniform(-2, 3, rows)), device="cuda")
+    top_k = torch.tensor(rng.randint(0, K, rows), device="cuda")
+    top_p = torch.tensor(rng.uniform(0.05, 1.0, rows), device="cuda")
+    min_p = torch.tensor(rng.uniform(0.0, 0.2, rows), device="cuda")
+    top_p[3] = 1.0
+    top_k[4] = 0
+    top_k[5] = K + 100
+    _check(R, u, kappa=kappa, top_k=top_k, top_p=top_p, min_p=min_p)
+    _check(R, u, kappa=kappa, top_k=5, top_p=top_p, min_p=0.0)
+    # values no call could pass as numbers leave their row without samples (a negative top_k: with all)
+    kappa[0], kappa[1], kappa[2] = -1.0, float("nan"), float("inf")
+    top_p[6], top_p[7], min_p[8], min_p[9], top_k[10] = 0.0, float("nan"), 1.5, float("nan"), -3
+    index, _ = _draw(R, u, kappa=kappa, top_k=top_k, top_p=top_p, min_p=min_p)
+    assert (index[[0, 1, 2, 6, 7, 8, 9]] == -1).all() and (index[[3, 4, 5, 10, 11]] >= 0).all()
+    index32, _ = _draw(R, u, kappa=kappa.float().double(), top_k=top_k.int(), top_p=top_p, min_p=min_p)
+    assert index32.shape == index.shape
+
+
+def test_many_rows_and_many_draws():
+    R, u = _returns(700, 130, "float32", 1), _numbers(700, 1, 1)
+    _check(R, u, kappa=2.0, top_k=64, top_p=0.95, min_p=0.01)
+    R, u = _returns(3, 200, "float64", 2), _numbers(3, 5000, 2)
+    _check(R, u, kappa=0.3)
+    R, u = _returns(2, 9000, "float32", 3), _numbers(2, 2000, 3)
+    _check(R, u, kappa=0.5, top_p=0.9)
+    R, u = _returns(1, 100000, "bfloat16", 4), _numbers(1, 600, 4)
+    _check(R, u, kappa=0.5, top_p=0.9, top_k=60000)
+
+
+def test_nothing_to_do():
+    import torch
+    R, u = _returns(2, 10, "float32", 0), _numbers(2, 0, 0)
+    assert _draw(R, u)[0].shape == (2, 0)
+    assert _draw(R[:0], _numbers(0, 4, 0))[0].shape == (0, 4)
+    with pytest.raises(RuntimeError):
+        _draw(R[:, :0], _numbers(2, 1, 0))
+    assert torch.cuda.current_device() == 0
+
+
+def test_rows_behind_the_last_are_left_alone():
+    """The library writes rows x D values and nothing else."""
+    import ctypes
+    import torch
+    from trajopt_amd import _lib as L
+    for K in (40, 5000, 70000):
+        R, u = _returns(3, K, "float32", 1), _numbers(3, 2, 1)
+        index = torch.full((12,), 77, dtype=torch.int64, device="cuda")
+        weight = torch.full((12,), 7.0, device="cuda")
+        f = L.DrawFilterC(kappa=1.0, top_k=5, top_p=0.9, min_p=0.0)
+        torch.cuda.synchronize()
+        index2, weight2 = _draw(R, u, kappa=1.0, top_k=5, top_p=0.9)
+        from trajopt_amd.device import _draw_call
+        _draw_call(torch, R, L.F32, 3, K, K, 1, u, 2, f, index[3:], weight[3:])
+        torch.cuda.synchronize()
+        assert (index[:3] == 77).all() and (index[9:] == 77).all() and (weight[:3] == 7).all() and (weight[9:] == 7).all()
+        assert torch.equal(index[3:9].reshape(3, 2), index2) and torch.equal(weight[3:9].reshape(3, 2), weight2)
+        assert ctypes.sizeof(f) == 64
+
+
+@pytest.mark.parametrize("K", [40, 3000, 100000])
+def test_captured_and_replayed(K):
+    """Two graphs and eager calls in turn; every replay against the eager result of its own inputs."""
+    import torch
+    R, u = _returns(2, K, "float32", K), _numbers(2, 9, K)
+    _draw(R, u, kappa=1.0, top_k=30, top_p=0.9)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    ins = [(R.clone(), u.clone()), (R.flip(1).contiguous(), u.clone())]
+    with torch.cuda.stream(side):
+        for r, v in ins:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(_draw(r, v, kappa=1.0, top_k=30, top_p=0.9))
+            graphs.append(g)
+    torch.cuda.synchronize()
+    for turn in range(4):
+        for (r, v), g, out in zip(ins, graphs, outs):
+            v.copy_(_numbers(2, 9, 50 + turn))
+            r.copy_(_returns(2, K, "float32", 90 + turn))
+            g.replay()
+            want = _draw(r, v, kappa=1.0, top_k=30, top_p=0.9)
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        _check(ins[0][0], ins[0][1], kappa=1.0, top_k=30, top_p=0.9, got=outs[0])
+
+
+def test_two_streams_at_once_and_repeated_calls():
+    """Same bits every time, whatever runs beside it."""
+    import torch
+    sets = [(_returns(1, K, "float32", K), _numbers(1, 8, K)) for K in (100000, 90001, 70000, 300)]
+    want = [_draw(R, u, kappa=0.5, top_k=5000, top_p=0.9) for R, u in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(5):
+        for k, (R, u) in enumerate(sets):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(_draw(R, u, kappa=0.5, top_k=5000, top_p=0.9))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        for g in gs:
+            assert torch.equal(w[0], g[0]) and torch.equal(w[1], g[1])
+
+
+def test_shares_of_many_draws():
+    """The frequencies of 200 000 draws are the weights (five standard deviations of a binomial count)."""
+    import torch
+    R = _returns(1, 6, "float32", 8, spread=0.7)
+    n = 200000
+    index, weight = _draw(R, torch.rand(1, n, dtype=torch.float64, device="cuda", generator=torch.Generator("cuda").manual_seed(3)), kappa=1.0)
+    share = torch.bincount(index[0], minlength=6).double().cpu().numpy() / n
+    w = ref_learn.kept_weights(R[0].double().cpu().numpy(), 1.0)
+    w /= w.sum()
+    assert np.all(np.abs(share - w) < 5 * np.sqrt(w * (1 - w) / n))

@@ -12,7 +12,8 @@ MAXV = 32
 NOALLOC_MAX_K = 262144
 _d, _i32, _u64, _vp = C.c_double, C.c_int32, C.c_uint64, C.c_void_p
 
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3
+NORMS = {"l2": 0, "max": 1}
 REWARD_TYPES = {"dense": 0, "sparse": 1, "tracking": 2, "cooling": 3}
 TAIL = {"repeat": 0, "mean": 1}
 (READ_RETURNS, READ_ACT_SEQ, READ_ARGMAX, READ_ACTIONS, READ_NEXT_OBS, READ_REWARDS, READ_STATUS, READ_RMAX,
@@ -42,6 +43,11 @@ class PlannerCfgC(C.Structure):
         ("kappa", _d), ("gamma", _d),
         ("sigma", _d * MAXV), ("beta", _d * 3), ("mean", _d * MAXV),
     ]
+
+
+class DrawFilterC(C.Structure):
+    _fields_ = [("kappa", _d), ("top_k", C.c_int64), ("top_p", _d), ("min_p", _d),
+                ("kappa_of", _vp), ("top_k_of", _vp), ("top_p_of", _vp), ("min_p_of", _vp)]
 
 
 class MppiError(RuntimeError):
@@ -92,6 +98,11 @@ _PROTOS = {
     "mppi_env_forward": (C.c_int, [_vp, _i32, _vp, _vp]),
     "mppi_update_from_returns": (C.c_int, [_i32, _vp, _vp, _i32, _i32, _d, _vp]),
     "mppi_update_from_returns_noalloc": (C.c_int, [_i32, _vp, _vp, _i32, _i32, _d, _vp, _vp]),
+    "mppi_draw_from_returns": (C.c_int, [_i32, _vp, _i32, _i32, _i32, C.c_int64, C.c_int64, _vp, _i32,
+                                         C.POINTER(DrawFilterC), _vp, _vp, _vp]),
+    "mppi_gradient_workspace": (C.c_int, [_i32, C.POINTER(C.c_size_t)]),
+    "mppi_gradient_norm": (C.c_int, [_i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, C.c_size_t, _vp]),
+    "mppi_clip_gradients": (C.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _i32, _d, _vp, _vp, C.c_size_t, _vp]),
     "mppi_numpy_normals": (C.c_int, [C.c_uint32, C.c_size_t, _vp, _i32, _vp]),
     "mppi_numpy_normals_many": (C.c_int, [_vp, _i32, C.c_size_t, _vp, _i32]),
     "mppi_numpy_normals_test_margin": (None, [_d]),

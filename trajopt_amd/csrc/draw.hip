@@ -1,0 +1,453 @@
+// Draws from exponentiated returns: for every row of K returns the samples that pass top-k, top-p and min-p are weighed by
+// w_i = exp(kappa (R_i - max R)), and given uniform numbers u pick the smallest i with  sum_{j <= i} w_j > u W.
+//
+// Numbers.  A return that is NaN or infinite weighs nothing, as in the planner's updates.  Weights are evaluated in fp64 and
+// summed as 64-bit fixed point, q_i = round(w_i 2^S): integer sums do not depend on their order, so the histograms may use
+// atomics, a row gives the same answer however it is split, and ties are exact.  S is chosen from the row's own mass (its
+// fp64 sum, rounded up to a power of two), so the sum stays below 2^63 and K roundings of half a unit are at most
+// K 2^-62 of the mass.  Samples with kappa (max - R) > (S + 1) ln 2 round to zero; they cannot be drawn, so they are left
+// out from the start.
+//
+// Borders.  The samples kept by top-k and top-p are a prefix of the order (return descending, index ascending), so either
+// filter is one pair (key of the last kept return, how many of the samples equal to it are kept).  It is found without
+// sorting: a histogram of counts (top-k) or masses (top-p) over bins that are linear in kappa (max - R), then, while the bin
+// with the border holds more than LIST samples of different returns, histograms over the bits of its keys, and last the
+// ranks of the LIST candidates by comparing each with each.
+#include "abi_common.hpp"
+#include "../../include/mppi_hip.h"
+
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <new>
+
+using mppi::fail;
+
+namespace {
+
+// ------------------------------------------------------------------------------------------
+// returns of every type as float or double, and keys that order like them
+// ------------------------------------------------------------------------------------------
+struct Half { uint16_t bits; };
+struct Bfloat { uint16_t bits; };
+__device__ __forceinline__ double value_of(double x) { return x; }
+__device__ __forceinline__ float value_of(float x) { return x; }
+__device__ __forceinline__ float value_of(Half x) { return (float)__builtin_bit_cast(_Float16, x.bits); }
+__device__ __forceinline__ float value_of(Bfloat x) { return __uint_as_float((unsigned)x.bits << 16); }
+
+template <class T> struct Traits { using V = float; using U = uint32_t; };
+template <> struct Traits<double> { using V = double; using U = uint64_t; };
+
+// monotone in x; adding zero gives both zeros one key
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+    return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ double of_key(uint64_t k) {
+    return __longlong_as_double((long long)((k & 0x8000000000000000ull) ? k ^ 0x8000000000000000ull : ~k));
+}
+
+struct DrawArgs {
+    const void* R;
+    long long row_stride, col_stride;
+    int rows, K, D;
+    const double* u;
+    mppi_draw_filter f;
+    long long* index;
+    float* weight;
+};
+
+// ------------------------------------------------------------------------------------------
+// sums and scans over a workgroup of NT threads
+// ------------------------------------------------------------------------------------------
+template <class X> __device__ __forceinline__ X wave_scan(X v, int lane) {          // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const X o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+template <int NT, class X> __device__ X group_scan(X v, X* s_tot, X& total) {        // exclusive; s_tot: NT / 64 + 1 values
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const X inc = wave_scan(v, lane);
+    if (lane == 63) s_tot[wave] = inc;
+    __syncthreads();
+    X before = 0, all = 0;
+    for (int w = 0; w < NT / 64; w++) {
+        const X t = s_tot[w];
+        if (w < wave) before += t;
+        all += t;
+    }
+    __syncthreads();
+    total = all;
+    return before + inc - v;
+}
+template <int NT, class X, class Op> __device__ X group_reduce(X v, X* s_tot, Op op) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v = op(v, (X)__shfl_xor(v, d, 64));
+    if (lane == 0) s_tot[wave] = v;
+    __syncthreads();
+    v = s_tot[0];
+    for (int w = 1; w < NT / 64; w++) v = op(v, s_tot[w]);
+    __syncthreads();
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------
+// one row per workgroup, read from memory in every pass
+// ------------------------------------------------------------------------------------------
+template <class T, int NT> struct Row {
+    using V = typename Traits<T>::V;
+    using U = typename Traits<T>::U;
+    static constexpr int VEC = 16 / sizeof(T);          // samples a thread takes at a time: 16 bytes
+    static constexpr int BINS = NT, LIST = 256;
+    struct Shared {
+        unsigned cnt[BINS];
+        unsigned long long mass[BINS];
+        unsigned long long tot[NT / 64 + 1];
+        U list_key[LIST];
+        unsigned list_idx[LIST];
+        unsigned long long list_q[LIST], list_before[LIST];
+        unsigned list_rank[LIST], list_ties[LIST];
+        unsigned n_list;
+        unsigned long long pick_before;
+        unsigned pick_bin, pick_n;
+        U border_key;
+        unsigned border_keep, border_all;
+    };
+    const T* R;
+    long long cs;
+    int K, S;
+    double kappa, best, cut;          // cut: kappa (best - R) beyond which a sample is left out
+    Shared& s;
+
+    __device__ Row(Shared& s_) : s(s_) {}
+
+    __device__ double distance(V x) const { return kappa > 0.0 ? kappa * (best - (double)x) : 0.0; }
+    __device__ unsigned long long mass_of(V x) const { return (unsigned long long)__double2ull_rn(ldexp(exp(-distance(x)), S)); }
+
+    // f(x, i): every sample in reach; those left out come as -inf
+    template <class F> __device__ void each(F f) const {
+        for (long long i0 = (long long)threadIdx.x * VEC; i0 < K; i0 += (long long)NT * VEC) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (i0 + j < K) f(load(i0 + j), (int)(i0 + j));
+        }
+    }
+    __device__ V load(long long i) const {
+        const V x = value_of(R[i * cs]);
+        if (!isfinite(x)) return (V)-INFINITY;
+        return distance(x) > cut ? (V)-INFINITY : x;
+    }
+
+    // Border of a prefix of the order: `target` counts samples (MASS false: the border is the target-th sample) or mass (the
+    // last sample with less than the target before it).  Only samples with keys >= from take part.  A target beyond what
+    // there is leaves no border (false).
+    template <bool MASS> __device__ bool border(unsigned long long target, U from) {
+        // range of kappa (best - R) over the samples in reach
+        double far = 0.0;
+        each([&](V x, int) {
+            if (x > (V)-INFINITY && key_of(x) >= from) far = fmax(far, distance(x));
+        });
+        far = group_reduce<NT>(far, (double*)s.tot, [](double a, double b) { return fmax(a, b); });
+        const double per = far > 0.0 ? BINS / far : 0.0;
+        U lo = from, hi = ~(U)0;
+        int shift = -1;                                  // -1: bins linear in the distance; else bits of hi - key
+        unsigned long long before = 0;
+        unsigned n = 0;
+        auto bin_of = [&](V x, U key) -> int {
+            if (shift >= 0) return (int)((hi - key) >> shift);
+            const int b = (int)(distance(x) * per);
+            return b < BINS ? b : BINS - 1;
+        };
+        while (true) {
+            s.cnt[threadIdx.x] = 0;
+            s.mass[threadIdx.x] = 0;
+            __syncthreads();
+            each([&](V x, int) {
+                const U key = key_of(x);
+                if (x > (V)-INFINITY && key >= lo && key <= hi) {
+                    const int b = bin_of(x, key);
+                    atomicAdd(&s.cnt[b], 1u);
+                    if (MASS) atomicAdd(&s.mass[b], mass_of(x));
+                }
+            });
+            __syncthreads();
+            const unsigned long long v = MASS ? s.mass[threadIdx.x] : (unsigned long long)s.cnt[threadIdx.x];
+            unsigned long long total;
+            const unsigned long long at = before + group_scan<NT>(v, s.tot, total);
+            if (before + total < target) return false;   // (first pass only: later ones hold the border)
+            if (at < target && target <= at + v) {
+                s.pick_bin = threadIdx.x;
+                s.pick_n = s.cnt[threadIdx.x];
+                s.pick_before = at;
+            }
+            __syncthreads();
+            const int b = (int)s.pick_bin;
+            n = s.pick_n;
+            before = s.pick_before;
+            // keys of that bin
+            if (shift < 0) {
+                U klo = ~(U)0, khi = 0;
+                each([&](V x, int) {
+                    const U key = key_of(x);
+                    if (x > (V)-INFINITY && key >= lo && bin_of(x, key) == b) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
+                });
+                klo = group_reduce<NT>(klo, (U*)s.tot, [](U a, U c) { return a < c ? a : c; });
+                khi = group_reduce<NT>(khi, (U*)s.tot, [](U a, U c) { return a > c ? a : c; });
+                lo = klo;
+                hi = khi;
+            } else {
+                const U top = hi - ((U)b << shift), width = ((U)1 << shift) - 1;
+                lo = top - lo > width ? top - width : lo;
+                hi = top;
+            }
+            if (n <= LIST || lo == hi) break;
+            shift = 0;
+            while (((hi - lo) >> shift) >= (U)BINS) shift++;
+        }
+        if (lo == hi) {                                  // all n of one return
+            if (threadIdx.x == 0) {
+                s.border_key = lo;
+                s.border_all = n;
+                if (MASS) {
+                    const unsigned long long q = mass_of(of_key(lo));
+                    s.border_keep = (unsigned)((target - before + q - 1) / q);
+                } else {
+                    s.border_keep = (unsigned)(target - before);
+                }
+            }
+            __syncthreads();
+            return true;
+        }
+        if (threadIdx.x == 0) s.n_list = 0;
+        if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
+        __syncthreads();
+        each([&](V x, int i) {
+            const U key = key_of(x);
+            if (x > (V)-INFINITY && key >= lo && key <= hi) {
+                const unsigned at = atomicAdd(&s.n_list, 1u);
+                s.list_key[at] = key;
+                s.list_idx[at] = (unsigned)i;
+                s.list_q[at] = MASS ? mass_of(x) : 0;
+            }
+        });
+        __syncthreads();
+        // rank of every candidate: the threads share the comparisons
+        const unsigned parts = NT / n;                   // n <= LIST <= NT
+        const unsigned e = threadIdx.x / parts, part = threadIdx.x % parts;
+        if (e < n) {
+            const U key = s.list_key[e];
+            const unsigned idx = s.list_idx[e];
+            unsigned rank = 0, ties = 0;
+            unsigned long long ahead = 0;
+            for (unsigned o = part; o < n; o += parts) {
+                const U ok = s.list_key[o];
+                const bool first = ok > key || (ok == key && s.list_idx[o] < idx);
+                rank += first ? 1u : 0u;
+                ties += ok == key ? (first ? 0x10001u : 0x1u) : 0u;        // low half: all equal ones, high half: those ahead
+                if (MASS) ahead += first ? s.list_q[o] : 0ull;
+            }
+            atomicAdd(&s.list_rank[e], rank);
+            atomicAdd(&s.list_ties[e], ties);
+            if (MASS) atomicAdd(&s.list_before[e], ahead);
+        }
+        __syncthreads();
+        if (threadIdx.x < n) {
+            const unsigned long long at = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
+            const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
+            if (at < target && target <= at + own) {
+                s.border_key = s.list_key[threadIdx.x];
+                s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
+                s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+};
+
+template <class T, int NT> __global__ void __launch_bounds__(NT) draw_rows_kernel(DrawArgs a) {
+    using W = Row<T, NT>;
+    using V = typename W::V;
+    using U = typename W::U;
+    __shared__ typename W::Shared s;
+    W r(s);
+    const long long row = blockIdx.x;
+    r.R = (const T*)a.R + row * a.row_stride;
+    r.cs = a.col_stride;
+    r.K = a.K;
+    r.kappa = a.f.kappa_of ? a.f.kappa_of[row] : a.f.kappa;
+    const double top_p = a.f.top_p_of ? a.f.top_p_of[row] : a.f.top_p;
+    const double min_p = a.f.min_p_of ? a.f.min_p_of[row] : a.f.min_p;
+    const long long top_k = a.f.top_k_of ? a.f.top_k_of[row] : a.f.top_k;
+    long long* index = a.index + row * a.D;
+    float* weight = a.weight ? a.weight + row * a.D : nullptr;
+    const double* u = a.u + row * a.D;
+
+    auto nothing = [&]() {
+        for (int d = threadIdx.x; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
+    };
+    if (!(r.kappa >= 0.0 && r.kappa < INFINITY)) return nothing();
+
+    // best return, then the scale from the mass
+    r.best = 0.0;
+    r.cut = INFINITY;
+    V best = (V)-INFINITY;
+    r.each([&](V x, int) { best = x > best ? x : best; });
+    best = group_reduce<NT>(best, (V*)s.tot, [](V x, V y) { return x > y ? x : y; });
+    if (!(best > (V)-INFINITY)) return nothing();
+    r.best = (double)best;
+    double mass = 0.0;
+    r.each([&](V x, int) { if (x > (V)-INFINITY) mass += exp(-r.distance(x)); });
+    mass = group_reduce<NT>(mass, (double*)s.tot, [](double x, double y) { return x + y; });
+    int e;
+    (void)frexp(mass, &e);                                // mass < 2^e
+    r.S = 62 - e;
+    r.cut = (r.S + 1) * 0.6931471805599453;
+
+    U from = 0;                                           // border: keys above it, and the first `keep` samples that equal it
+    unsigned keep = UINT_MAX, ties = 0;
+    if (top_k > 0 && top_k < a.K && r.template border<false>((unsigned long long)top_k, 0)) {
+        from = s.border_key; keep = s.border_keep; ties = s.border_all;
+    }
+    __syncthreads();
+    auto kept_mass = [&](double least) {                  // of the samples with w >= least inside the border
+        unsigned long long sum = 0;
+        r.each([&](V x, int) {
+            if (x > (V)-INFINITY) {
+                const U key = key_of(x);
+                if (key > from || (key == from && keep >= ties)) {
+                    const double w = exp(-r.distance(x));
+                    if (w >= least) sum += __double2ull_rn(ldexp(w, r.S));
+                }
+            }
+        });
+        sum = group_reduce<NT>(sum, s.tot, [](unsigned long long x, unsigned long long y) { return x + y; });
+        if (keep < ties && exp(-r.distance(of_key(from))) >= least) sum += keep * r.mass_of(of_key(from));
+        return sum;
+    };
+    if (!(top_p >= 1.0)) {
+        const unsigned long long all = kept_mass(0.0);
+        const double part = ceil(top_p * (double)all);    // a whole number: "mass before < top_p W" is "mass before < part"
+        if (!(part >= 1.0)) return nothing();
+        const unsigned long long target = part < (double)all ? (unsigned long long)part : all;
+        if (r.template border<true>(target, from)) {
+            // inside the samples that top-k kept: its own border never lies behind theirs
+            if (s.border_key != from || s.border_keep < keep) { from = s.border_key; keep = s.border_keep; ties = s.border_all; }
+        }
+        __syncthreads();
+    }
+    const unsigned long long all = kept_mass(min_p);
+    if (all == 0) return nothing();
+
+    // running mass in the order of the samples, a tile of NT VEC samples at a time
+    unsigned long long running = 0;
+    unsigned equal = 0;
+    for (long long t0 = 0; t0 < a.K; t0 += (long long)NT * W::VEC) {
+        V x[W::VEC];
+        unsigned mine = 0;
+#pragma unroll
+        for (int j = 0; j < W::VEC; j++) {
+            const long long i = t0 + (long long)threadIdx.x * W::VEC + j;
+            x[j] = i < a.K ? r.load(i) : (V)-INFINITY;
+            mine += x[j] > (V)-INFINITY && key_of(x[j]) == from ? 1u : 0u;
+        }
+        unsigned tile_equal;
+        unsigned rank = equal + group_scan<NT>(mine, (unsigned*)s.tot, tile_equal);
+        unsigned long long q[W::VEC], sum = 0;
+#pragma unroll
+        for (int j = 0; j < W::VEC; j++) {
+            q[j] = 0;
+            if (x[j] > (V)-INFINITY) {
+                const U key = key_of(x[j]);
+                const bool in = key > from || (key == from && rank < keep);
+                rank += key == from ? 1u : 0u;
+                if (in) {
+                    const double w = exp(-r.distance(x[j]));
+                    q[j] = w >= min_p ? __double2ull_rn(ldexp(w, r.S)) : 0ull;
+                }
+            }
+            sum += q[j];
+        }
+        unsigned long long tile;
+        const unsigned long long at = running + group_scan<NT>(sum, s.tot, tile);
+        for (int d = 0; d < a.D; d++) {
+            const double want = u[d] * (double)all;
+            unsigned long long target = want > 0.0 ? (want < (double)all ? (unsigned long long)want : all) : 0ull;
+            target = target < all ? target : all - 1;
+            if (target >= at && target < at + sum) {
+                unsigned long long c = at;
+#pragma unroll
+                for (int j = 0; j < W::VEC; j++) {
+                    if (target >= c && target < c + q[j]) {
+                        index[d] = t0 + (long long)threadIdx.x * W::VEC + j;
+                        if (weight) weight[d] = (float)(ldexp(exp(-r.distance(x[j])), r.S) / (double)all);
+                    }
+                    c += q[j];
+                }
+            }
+        }
+        running += tile;
+        equal += tile_equal;
+    }
+}
+
+template <class T> hipError_t launch(const DrawArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((draw_rows_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a);
+    return hipGetLastError();
+}
+
+int check_filter(const mppi_draw_filter* f) {
+    if (!f->kappa_of && !(f->kappa >= 0.0 && std::isfinite(f->kappa))) return fail(-1, "kappa must be finite and not negative");
+    if (!f->top_k_of && f->top_k < 0) return fail(-1, "top_k must not be negative (0: every sample)");
+    if (!f->top_p_of && !(f->top_p > 0.0 && f->top_p <= 1.0)) return fail(-1, "top_p must lie in (0, 1]");
+    if (!f->min_p_of && !(f->min_p >= 0.0 && f->min_p <= 1.0)) return fail(-1, "min_p must lie in [0, 1]");
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32_t rows, int32_t K, int64_t row_stride,
+                           int64_t col_stride, const double* d_u, int32_t D, const mppi_draw_filter* filter, int64_t* d_index,
+                           float* d_weight, void* stream) try {
+    if (!filter) return fail(-1, "null argument");
+    if (rows < 0 || K < 1 || D < 0) return fail(-1, "rows and D must not be negative, K must be positive");
+    if (K > MPPI_DRAW_MAX_K)
+        return fail(-6, "mppi_draw_from_returns: K = " + std::to_string(K) + " exceeds " + std::to_string(MPPI_DRAW_MAX_K) + " samples");
+    if (row_stride < 0 || col_stride < 0) return fail(-1, "strides must not be negative");
+    if (dtype < MPPI_F32 || dtype > MPPI_BF16) return fail(-1, "dtype must be MPPI_F32, MPPI_F64, MPPI_F16 or MPPI_BF16");
+    const int rc = check_filter(filter);
+    if (rc) return rc;
+    if (rows == 0 || D == 0) return 0;
+    if (!d_R || !d_u || !d_index) return fail(-1, "null argument");
+    mppi::DeviceGuard guard;
+    HIP_OK(guard.enter(device));
+    DrawArgs a;
+    a.R = d_R; a.row_stride = row_stride; a.col_stride = col_stride;
+    a.rows = rows; a.K = K; a.D = D;
+    a.u = d_u; a.f = *filter;
+    a.index = (long long*)d_index; a.weight = d_weight;
+    hipStream_t s = (hipStream_t)stream;
+    switch (dtype) {
+    case MPPI_F32: HIP_OK(launch<float>(a, s)); break;
+    case MPPI_F64: HIP_OK(launch<double>(a, s)); break;
+    case MPPI_F16: HIP_OK(launch<Half>(a, s)); break;
+    default: HIP_OK(launch<Bfloat>(a, s)); break;
+    }
+    return 0;
+} catch (const std::exception& e) {
+    return fail(-8, std::string("host exception: ") + e.what());
+}
+
+}  // extern "C"

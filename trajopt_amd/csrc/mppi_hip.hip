@@ -34,6 +34,7 @@
 #include <vector>
 
 #include "../../include/mppi_hip.h"
+#include "abi_common.hpp"
 #include "numpy_stream.h"
 #include "env_core.hpp"
 #include "models_gen.hpp"
@@ -44,16 +45,10 @@ using namespace mppi;
 // errors
 // ------------------------------------------------------------------------------------------
 static thread_local std::string g_err;
-static int fail(int code, const std::string& msg) {
+int mppi::fail(int code, const std::string& msg) {
     g_err = msg;
     return code;
 }
-#define HIP_OK(expr)                                                                                   \
-    do {                                                                                               \
-        hipError_t e_ = (expr);                                                                        \
-        if (e_ != hipSuccess)                                                                          \
-            return fail(-2, std::string(#expr) + ": " + hipGetErrorString(e_));                        \
-    } while (0)
 
 #include "kernels.hpp"
 
