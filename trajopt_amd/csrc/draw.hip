@@ -64,41 +64,70 @@ struct DrawArgs {
 };
 
 // ------------------------------------------------------------------------------------------
-// sums and scans over a workgroup of NT threads
+// sums, extremes and scans: lanes through DPP (no trip to LDS), waves through LDS
 // ------------------------------------------------------------------------------------------
-template <class X> __device__ __forceinline__ X wave_scan(X v, int lane) {          // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const X o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
+template <int CTRL, int ROWS, class X> __device__ __forceinline__ X dpp(X v, X other) {      // other where no lane is read from
+    if constexpr (sizeof(X) == 4) {
+        return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, other), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const unsigned long long a = __builtin_bit_cast(unsigned long long, v), o = __builtin_bit_cast(unsigned long long, other);
+        const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp((int)(unsigned)o, (int)(unsigned)a, CTRL, ROWS, 0xf, false);
+        const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp((int)(o >> 32), (int)(a >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(X, (unsigned long long)hi << 32 | lo);
     }
+}
+template <class X> __device__ __forceinline__ X lane_value(X v, int lane) {                  // lane: the same in every lane
+    if constexpr (sizeof(X) == 4) {
+        return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        const unsigned long long a = __builtin_bit_cast(unsigned long long, v);
+        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)a, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(a >> 32), lane);
+        return __builtin_bit_cast(X, (unsigned long long)hi << 32 | lo);
+    }
+}
+// inclusive, in the order of the lanes: within rows of 16, then the last lane of rows 0 and 2 into rows 1 and 3, then lane 31
+// into rows 2 and 3
+template <class X, class Op> __device__ __forceinline__ X wave_scan(X v, X none, Op op) {
+    v = op(v, dpp<0x111, 0xf>(v, none));
+    v = op(v, dpp<0x112, 0xf>(v, none));
+    v = op(v, dpp<0x114, 0xf>(v, none));
+    v = op(v, dpp<0x118, 0xf>(v, none));
+    v = op(v, dpp<0x142, 0xa>(v, none));
+    v = op(v, dpp<0x143, 0xc>(v, none));
     return v;
 }
-template <int NT, class X> __device__ X group_scan(X v, X* s_tot, X& total) {        // exclusive; s_tot: NT / 64 + 1 values
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const X inc = wave_scan(v, lane);
-    if (lane == 63) s_tot[wave] = inc;
+struct Add { template <class X> __device__ __forceinline__ X operator()(X a, X b) const { return a + b; } };
+struct Max { template <class X> __device__ __forceinline__ X operator()(X a, X b) const { return a > b ? a : b; } };
+struct Min { template <class X> __device__ __forceinline__ X operator()(X a, X b) const { return a < b ? a : b; } };
+
+// over the NT threads of a workgroup; s_tot: NT / 64 values nobody else uses before the next barrier
+template <int NT, class X, class Op> __device__ __forceinline__ X group_reduce(X v, X none, X* s_tot, Op op) {
+    v = wave_scan(v, none, op);
+    if (NT == 64) return lane_value(v, 63);
+    if ((threadIdx.x & 63) == 63) s_tot[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s_tot[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) v = op(v, s_tot[w]);
+    __syncthreads();
+    return v;
+}
+template <int NT, class X> __device__ __forceinline__ X group_scan(X v, X* s_tot, X& total) {        // exclusive sums
+    const int wave = threadIdx.x >> 6;
+    const X inc = wave_scan(v, (X)0, Add());
+    if (NT == 64) { total = lane_value(inc, 63); return inc - v; }
+    if ((threadIdx.x & 63) == 63) s_tot[wave] = inc;
     __syncthreads();
     X before = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < NT / 64; w++) {
         const X t = s_tot[w];
-        if (w < wave) before += t;
+        before += w < wave ? t : (X)0;
         all += t;
     }
     __syncthreads();
     total = all;
     return before + inc - v;
-}
-template <int NT, class X, class Op> __device__ X group_reduce(X v, X* s_tot, Op op) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v = op(v, (X)__shfl_xor(v, d, 64));
-    if (lane == 0) s_tot[wave] = v;
-    __syncthreads();
-    v = s_tot[0];
-    for (int w = 1; w < NT / 64; w++) v = op(v, s_tot[w]);
-    __syncthreads();
-    return v;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -157,7 +186,7 @@ template <class T, int NT> struct Row {
         each([&](V x, int) {
             if (x > (V)-INFINITY && key_of(x) >= from) far = fmax(far, distance(x));
         });
-        far = group_reduce<NT>(far, (double*)s.tot, [](double a, double b) { return fmax(a, b); });
+        far = group_reduce<NT>(far, 0.0, (double*)s.tot, Max());
         const double per = far > 0.0 ? BINS / far : 0.0;
         U lo = from, hi = ~(U)0;
         int shift = -1;                                  // -1: bins linear in the distance; else bits of hi - key
@@ -201,8 +230,8 @@ template <class T, int NT> struct Row {
                     const U key = key_of(x);
                     if (x > (V)-INFINITY && key >= lo && bin_of(x, key) == b) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
                 });
-                klo = group_reduce<NT>(klo, (U*)s.tot, [](U a, U c) { return a < c ? a : c; });
-                khi = group_reduce<NT>(khi, (U*)s.tot, [](U a, U c) { return a > c ? a : c; });
+                klo = group_reduce<NT>(klo, ~(U)0, (U*)s.tot, Min());
+                khi = group_reduce<NT>(khi, (U)0, (U*)s.tot, Max());
                 lo = klo;
                 hi = khi;
             } else {
@@ -303,12 +332,12 @@ template <class T, int NT> __global__ void __launch_bounds__(NT) draw_rows_kerne
     r.cut = INFINITY;
     V best = (V)-INFINITY;
     r.each([&](V x, int) { best = x > best ? x : best; });
-    best = group_reduce<NT>(best, (V*)s.tot, [](V x, V y) { return x > y ? x : y; });
+    best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.tot, Max());
     if (!(best > (V)-INFINITY)) return nothing();
     r.best = (double)best;
     double mass = 0.0;
     r.each([&](V x, int) { if (x > (V)-INFINITY) mass += exp(-r.distance(x)); });
-    mass = group_reduce<NT>(mass, (double*)s.tot, [](double x, double y) { return x + y; });
+    mass = group_reduce<NT>(mass, 0.0, (double*)s.tot, Add());
     int e;
     (void)frexp(mass, &e);                                // mass < 2^e
     r.S = 62 - e;
@@ -331,7 +360,7 @@ template <class T, int NT> __global__ void __launch_bounds__(NT) draw_rows_kerne
                 }
             }
         });
-        sum = group_reduce<NT>(sum, s.tot, [](unsigned long long x, unsigned long long y) { return x + y; });
+        sum = group_reduce<NT>(sum, 0ull, s.tot, Add());
         if (keep < ties && exp(-r.distance(of_key(from))) >= least) sum += keep * r.mass_of(of_key(from));
         return sum;
     };
@@ -401,8 +430,435 @@ template <class T, int NT> __global__ void __launch_bounds__(NT) draw_rows_kerne
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// one row per workgroup, held in registers
+// ------------------------------------------------------------------------------------------
+struct Param {
+    double kappa, top_p, min_p;
+    long long top_k;
+    __device__ Param(const mppi_draw_filter& f, long long row)
+        : kappa(f.kappa_of ? f.kappa_of[row] : f.kappa), top_p(f.top_p_of ? f.top_p_of[row] : f.top_p),
+          min_p(f.min_p_of ? f.min_p_of[row] : f.min_p), top_k(f.top_k_of ? f.top_k_of[row] : f.top_k) {}
+    __device__ bool valid() const { return kappa >= 0.0 && kappa < INFINITY; }
+};
+// u in [0, 1) -> a whole number below the mass
+__device__ __forceinline__ unsigned long long target_of(double u, unsigned long long mass) {
+    const double want = u * (double)mass;
+    const unsigned long long t = want > 0.0 ? (want < (double)mass ? (unsigned long long)want : mass) : 0ull;
+    return t < mass ? t : mass - 1;
+}
+
+// A thread holds G groups of VEC neighbouring samples (16 bytes of the row each); group g of thread t starts at sample
+// (g NT + t) VEC, so that a load covers neighbouring 16-byte pieces over the lanes and the order of the samples is g-major.
+template <class T, int NT, int G> struct Held {
+    using V = typename Traits<T>::V;
+    using U = typename Traits<T>::U;
+    static constexpr int VEC = 16 / sizeof(T), ITEMS = G * VEC, NW = NT / 64;
+    static constexpr int BINS = NT, LIST = NT >= 1024 ? 256 : NT / 2 < 64 ? 64 : NT / 2;
+    static constexpr bool KEEP = ITEMS <= 16 && NT < 1024;        // masses stay in registers; else they are evaluated again where needed
+    static constexpr int DIRECT = 8;                 // up to this many draws are looked up by every thread in its own samples
+    static constexpr int ENTRIES = (G * NW + 63) / 64;
+    struct Shared {
+        unsigned cnt[BINS];
+        unsigned long long mass[BINS];
+        unsigned long long tot[G * NW > 32 ? G * NW : 32];
+        U list_key[LIST];
+        unsigned list_idx[LIST];
+        unsigned long long list_q[LIST], list_before[LIST];
+        unsigned list_rank[LIST], list_ties[LIST];
+        unsigned n_list;
+        unsigned long long pick_before;
+        unsigned pick_bin, pick_n;
+        U border_key;
+        unsigned border_keep, border_all;
+        unsigned long long ends[G * NT];             // mass up to the end of every group
+        unsigned char kept[G * NT];                  // its samples that may be drawn
+    };
+    Shared& s;
+    V x[G][VEC];
+    unsigned long long q[KEEP ? G : 1][KEEP ? VEC : 1];
+    double kappa, best, scale;
+
+    __device__ Held(Shared& s_) : s(s_) {}
+    __device__ __forceinline__ static int first(int g) { return (g * NT + (int)threadIdx.x) * VEC; }
+    __device__ __forceinline__ static bool on(V v) { return v > (V)-INFINITY; }
+    __device__ __forceinline__ double distance(V v) const { return kappa > 0.0 ? kappa * (best - (double)v) : 0.0; }
+    __device__ __forceinline__ double weight(V v) const { return exp(-distance(v)); }
+    __device__ __forceinline__ unsigned long long mass_of(V v) const { return __double2ull_rn(weight(v) * scale); }
+    __device__ __forceinline__ unsigned long long mass_at(int g, int j) const {
+        if constexpr (KEEP) return q[g][j];
+        return on(x[g][j]) ? mass_of(x[g][j]) : 0ull;
+    }
+    template <class F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) f(g, j, x[g][j]);
+    }
+
+    __device__ __forceinline__ static void load(const T* R, long long cs, int i, int K, V (&out)[VEC]) {
+        if (cs == 1 && i + VEC <= K) {
+            T raw[VEC];
+            __builtin_memcpy(raw, R + i, 16);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) out[j] = value_of(raw[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) out[j] = i + j < K ? value_of(R[(long long)(i + j) * cs]) : (V)-INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; j++) out[j] = isfinite(out[j]) ? out[j] : (V)-INFINITY;
+    }
+
+    // exclusive sums of v[g] in the order of the samples
+    template <class X> __device__ __forceinline__ void scan(const X (&v)[G], X (&base)[G], X& total) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        X* tot = (X*)s.tot;
+        if (NW == 1) {
+            X run = 0;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const X inc = wave_scan(v[g], (X)0, Add());
+                base[g] = run + inc - v[g];
+                run += lane_value(inc, 63);
+            }
+            total = run;
+            return;
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const X inc = wave_scan(v[g], (X)0, Add());
+            base[g] = inc - v[g];
+            if (lane == 63) tot[g * NW + wave] = inc;
+        }
+        __syncthreads();
+        X mine[ENTRIES], sum = 0;                    // lane l: entries l ENTRIES ...
+#pragma unroll
+        for (int e = 0; e < ENTRIES; e++) {
+            const int at = lane * ENTRIES + e;
+            mine[e] = at < G * NW ? tot[at] : (X)0;
+            sum += mine[e];
+        }
+        const X inc = wave_scan(sum, (X)0, Add());
+        total = lane_value(inc, 63);
+        X run = inc - sum;
+#pragma unroll
+        for (int e = 0; e < ENTRIES; e++) { const X t = mine[e]; mine[e] = run; run += t; }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int at = __builtin_amdgcn_readfirstlane(g * NW + wave);
+            X b = 0;
+#pragma unroll
+            for (int e = 0; e < ENTRIES; e++)
+                if (at % ENTRIES == e) b = lane_value(mine[e], at / ENTRIES);
+            base[g] += b;
+        }
+        __syncthreads();
+    }
+
+    // Border of a prefix of the order among the samples that are on (`far`: bound of their distances): `target` counts
+    // samples (MASS false: the border is the target-th sample) or mass (the last sample with less than the target before
+    // it).  A target beyond what there is leaves no border (false).
+    template <bool MASS> __device__ bool border(unsigned long long target, double far) {
+        const double per = far > 0.0 ? BINS / far : 0.0;
+        U lo = 0, hi = ~(U)0;
+        int shift = -1, bin = 0;                     // -1: bins linear in the distance; else bits of hi - key
+        unsigned long long before = 0;
+        unsigned n = 0;
+        auto bin_of = [&](V v, U key) -> int {
+            if (shift >= 0) return (int)((hi - key) >> shift);
+            const int b = (int)(distance(v) * per);
+            return b < BINS ? b : BINS - 1;
+        };
+        while (true) {
+            s.cnt[threadIdx.x] = 0;
+            if (MASS) s.mass[threadIdx.x] = 0;
+            if (threadIdx.x == 0) s.n_list = 0;
+            if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
+            __syncthreads();
+            each([&](int g, int j, V v) {
+                const U key = key_of(v);
+                if (on(v) && key >= lo && key <= hi) {
+                    const int b = bin_of(v, key);
+                    atomicAdd(&s.cnt[b], 1u);
+                    if (MASS) atomicAdd(&s.mass[b], mass_at(g, j));
+                }
+            });
+            __syncthreads();
+            const unsigned c = s.cnt[threadIdx.x];
+            const unsigned long long own = MASS ? s.mass[threadIdx.x] : (unsigned long long)c;
+            unsigned long long total;
+            const unsigned long long at = before + group_scan<NT>(own, s.tot, total);
+            if (before + total < target) return false;           // (first pass only: later ones hold the border)
+            if (at < target && target <= at + own) { s.pick_bin = threadIdx.x; s.pick_n = c; s.pick_before = at; }
+            __syncthreads();
+            bin = (int)s.pick_bin;
+            n = s.pick_n;
+            before = s.pick_before;
+            if (n <= LIST) break;
+            // the keys of that bin
+            if (shift < 0) {
+                U klo = ~(U)0, khi = 0;
+                each([&](int, int, V v) {
+                    const U key = key_of(v);
+                    if (on(v) && bin_of(v, key) == bin) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
+                });
+                lo = group_reduce<NT>(klo, ~(U)0, (U*)s.tot, Min());
+                hi = group_reduce<NT>(khi, (U)0, (U*)s.tot, Max());
+            } else {
+                const U top = hi - ((U)bin << shift), width = ((U)1 << shift) - 1;
+                lo = top - lo > width ? top - width : lo;
+                hi = top;
+            }
+            if (lo == hi) break;
+            shift = 0;
+            while (((hi - lo) >> shift) >= (U)BINS) shift++;
+        }
+        if (n > LIST) {                              // all n of one return
+            if (threadIdx.x == 0) {
+                s.border_key = lo;
+                s.border_all = n;
+                if (MASS) {
+                    const unsigned long long one = mass_of(of_key(lo));
+                    s.border_keep = (unsigned)((target - before + one - 1) / one);
+                } else {
+                    s.border_keep = (unsigned)(target - before);
+                }
+            }
+            __syncthreads();
+            return true;
+        }
+        each([&](int g, int j, V v) {
+            const U key = key_of(v);
+            if (on(v) && key >= lo && key <= hi && bin_of(v, key) == bin) {
+                const unsigned e = atomicAdd(&s.n_list, 1u);
+                s.list_key[e] = key;
+                s.list_idx[e] = (unsigned)(first(g) + j);
+                if (MASS) s.list_q[e] = mass_at(g, j);
+            }
+        });
+        __syncthreads();
+        // rank of every candidate: the threads share the comparisons
+        const unsigned parts = NT / n;               // 1 <= n <= LIST <= NT
+        const unsigned e = threadIdx.x / parts, part = threadIdx.x - e * parts;
+        if (e < n) {
+            const U key = s.list_key[e];
+            const unsigned idx = s.list_idx[e];
+            unsigned rank = 0, ties = 0;
+            unsigned long long ahead = 0;
+            for (unsigned o = part; o < n; o += parts) {
+                const U ok = s.list_key[o];
+                const bool lead = ok > key || (ok == key && s.list_idx[o] < idx);
+                rank += lead ? 1u : 0u;
+                ties += ok == key ? (lead ? 0x10001u : 0x1u) : 0u;         // low half: all equal ones, high half: those ahead
+                if (MASS) ahead += lead ? s.list_q[o] : 0ull;
+            }
+            atomicAdd(&s.list_rank[e], rank);
+            atomicAdd(&s.list_ties[e], ties);
+            if (MASS) atomicAdd(&s.list_before[e], ahead);
+        }
+        __syncthreads();
+        if (threadIdx.x < n) {
+            const unsigned long long at = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
+            const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
+            if (at < target && target <= at + own) {
+                s.border_key = s.list_key[threadIdx.x];
+                s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
+                s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+
+    // switches off what lies behind the border that was found; returns the distance of the border
+    __device__ double cut_behind() {
+        const U from = s.border_key;
+        const unsigned keep = s.border_keep;
+        if (keep < s.border_all) {                   // some of the equal ones: the first in the order of the samples
+            unsigned mine[G], rank[G], total;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                mine[g] = 0;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) mine[g] += on(x[g][j]) && key_of(x[g][j]) == from ? 1u : 0u;
+            }
+            scan(mine, rank, total);
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if (on(x[g][j]) && key_of(x[g][j]) == from) {
+                        if (rank[g] >= keep) drop(g, j);
+                        rank[g]++;
+                    }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (key_of(x[g][j]) < from) drop(g, j);
+        __syncthreads();                             // s.border_* may be written again
+        return distance(of_key(from));
+    }
+    __device__ __forceinline__ void drop(int g, int j) {
+        x[g][j] = (V)-INFINITY;
+        if constexpr (KEEP) q[g][j] = 0;
+    }
+};
+
+template <class T, int NT, int G> __global__ void __launch_bounds__(NT) draw_held_kernel(DrawArgs a, int S) {
+    using H = Held<T, NT, G>;
+    using V = typename H::V;
+    constexpr int VEC = H::VEC;
+    __shared__ typename H::Shared s;
+    H h(s);
+    const long long row = blockIdx.x;
+    const T* R = (const T*)a.R + row * a.row_stride;
+#pragma unroll
+    for (int g = 0; g < G; g++) H::load(R, a.col_stride, H::first(g), a.K, h.x[g]);
+    const Param par(a.f, row);
+    long long* index = a.index + row * a.D;
+    float* weight = a.weight ? a.weight + row * a.D : nullptr;
+    const double* u = a.u + row * a.D;
+    auto nothing = [&]() {
+        for (int d = threadIdx.x; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
+    };
+
+    V best = (V)-INFINITY, worst = (V)INFINITY;
+    h.each([&](int, int, V v) {
+        best = v > best ? v : best;
+        worst = H::on(v) && v < worst ? v : worst;
+    });
+    best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.tot, Max());
+    worst = group_reduce<NT>(worst, (V)INFINITY, (V*)s.tot, Min());
+    if (!par.valid() || !H::on(best)) return nothing();
+    h.kappa = par.kappa;
+    h.best = (double)best;
+    h.scale = __longlong_as_double((long long)(1023 + S) << 52);          // 2^S
+    const double cut = (S + 1) * 0.6931471805599453;
+    double far = fmin(h.distance(worst), cut);
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+            if (h.distance(h.x[g][j]) > cut) h.x[g][j] = (V)-INFINITY;
+    if constexpr (H::KEEP) {
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) h.q[g][j] = 0;
+    }
+    if (par.top_k > 0 && par.top_k < a.K && h.template border<false>((unsigned long long)par.top_k, far)) far = h.cut_behind();
+    if constexpr (H::KEEP) {
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (H::on(h.x[g][j])) h.q[g][j] = h.mass_of(h.x[g][j]);
+    }
+    if (!(par.top_p >= 1.0)) {
+        unsigned long long mass = 0;
+        h.each([&](int g, int j, V) { mass += h.mass_at(g, j); });
+        mass = group_reduce<NT>(mass, 0ull, s.tot, Add());
+        const double part = ceil(par.top_p * (double)mass);   // a whole number: "mass before < top_p W" is "mass before < part"
+        if (!(part >= 1.0)) return nothing();
+        const unsigned long long target = part < (double)mass ? (unsigned long long)part : mass;
+        if (h.template border<true>(target, far)) (void)h.cut_behind();
+    }
+    if (!(par.min_p <= 0.0)) {
+        // exp(-distance) >= min_p; only next to the border does the exponential itself have to decide
+        const double edge = -log(par.min_p), near = 1e-9 * (1.0 + fabs(edge));
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const double d = h.distance(h.x[g][j]);
+                bool in = d < edge;
+                if (!(fabs(d - edge) > near)) in = h.weight(h.x[g][j]) >= par.min_p;
+                if (!in) h.drop(g, j);
+            }
+    }
+
+    unsigned long long sum[G], base[G], mass;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        sum[g] = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) sum[g] += h.mass_at(g, j);
+    }
+    h.scan(sum, base, mass);
+    if (mass == 0) return nothing();
+    auto answer = [&](int d, long long i, V v) {
+        index[d] = i;
+        if (weight) weight[d] = (float)(h.weight(v) * h.scale / (double)mass);
+    };
+    if (a.D <= H::DIRECT) {
+        for (int d = 0; d < a.D; d++) {
+            const unsigned long long target = target_of(u[d], mass);
+#pragma unroll
+            for (int g = 0; g < G; g++)
+                if (target - base[g] < sum[g]) {              // (below base: a huge number)
+                    unsigned long long c = base[g];
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        const unsigned long long m = h.mass_at(g, j);
+                        if (target - c < m) answer(d, H::first(g) + j, h.x[g][j]);
+                        c += m;
+                    }
+                }
+        }
+        return;
+    }
+    // many draws: a thread each, which finds the group by bisection and reads its samples again
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        unsigned char bits = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) bits |= (unsigned char)(H::on(h.x[g][j]) ? 1u << j : 0u);
+        s.ends[g * NT + threadIdx.x] = base[g] + sum[g];
+        s.kept[g * NT + threadIdx.x] = bits;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += NT) {
+        const unsigned long long target = target_of(u[d], mass);
+        int lo = 0, hi = G * NT - 1;                           // the first group whose end is above the target
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s.ends[mid] > target) hi = mid; else lo = mid + 1;
+        }
+        unsigned long long c = lo > 0 ? s.ends[lo - 1] : 0ull;
+        const unsigned bits = s.kept[lo];
+        V v[VEC];
+        H::load(R, a.col_stride, lo * VEC, a.K, v);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            const unsigned long long m = bits >> j & 1u ? h.mass_of(v[j]) : 0ull;
+            if (target - c < m) answer(d, (long long)lo * VEC + j, v[j]);
+            c += m;
+        }
+    }
+}
+
+int ceil_log2(int n) {
+    int e = 0;
+    while ((1ll << e) < n) e++;
+    return e;
+}
+
 template <class T> hipError_t launch(const DrawArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((draw_rows_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a);
+    constexpr int VEC = 16 / sizeof(T);
+    const int S = 62 - ceil_log2(a.K);
+    if (a.K <= 512)
+        hipLaunchKernelGGL((draw_held_kernel<T, 64, 8 / VEC>), dim3(a.rows), dim3(64), 0, s, a, S);
+    else if (a.K <= 4096)
+        hipLaunchKernelGGL((draw_held_kernel<T, 256, 16 / VEC>), dim3(a.rows), dim3(256), 0, s, a, S);
+    else if (a.K <= 16384)
+        hipLaunchKernelGGL((draw_held_kernel<T, 512, 32 / VEC>), dim3(a.rows), dim3(512), 0, s, a, S);
+    else if (sizeof(T) < 8 && a.K <= (sizeof(T) == 4 ? 32768 : 65536))
+        hipLaunchKernelGGL((draw_held_kernel<T, 1024, sizeof(T) == 2 ? 8 : 8>), dim3(a.rows), dim3(1024), 0, s, a, S);
+    else
+        hipLaunchKernelGGL((draw_rows_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
 
