@@ -36,6 +36,11 @@ __device__ __forceinline__ float value_of(float x) { return x; }
 __device__ __forceinline__ float value_of(Half x) { return (float)__builtin_bit_cast(_Float16, x.bits); }
 __device__ __forceinline__ float value_of(Bfloat x) { return __uint_as_float((unsigned)x.bits << 16); }
 
+__device__ __forceinline__ float minus_infinity(float*) { return -INFINITY; }
+__device__ __forceinline__ double minus_infinity(double*) { return -INFINITY; }
+__device__ __forceinline__ Half minus_infinity(Half*) { return {0xfc00}; }
+__device__ __forceinline__ Bfloat minus_infinity(Bfloat*) { return {0xff80}; }
+
 template <class T> struct Traits { using V = float; using U = uint32_t; };
 template <> struct Traits<double> { using V = double; using U = uint64_t; };
 
@@ -448,149 +453,113 @@ __device__ __forceinline__ unsigned long long target_of(double u, unsigned long 
     return t < mass ? t : mass - 1;
 }
 
-// A thread holds G groups of VEC neighbouring samples (16 bytes of the row each); group g of thread t starts at sample
-// (g NT + t) VEC, so that a load covers neighbouring 16-byte pieces over the lanes and the order of the samples is g-major.
-template <class T, int NT, int G> struct Held {
+// The row lies in LDS as it came (what takes no part as -inf of its type).  Thread t owns the C samples from t C on, in GP
+// pieces of 16 bytes; it visits them from piece t mod GP on, so that the lanes of a wave read from all banks.  All loops over
+// samples stay rolled: unrolled, a kernel of this many passes is larger than the instruction cache.
+template <class T, int NT, int BYTES> struct Shelf {
     using V = typename Traits<T>::V;
     using U = typename Traits<T>::U;
-    static constexpr int VEC = 16 / sizeof(T), ITEMS = G * VEC, NW = NT / 64;
-    static constexpr int BINS = NT, LIST = NT >= 1024 ? 256 : NT / 2 < 64 ? 64 : NT / 2;
-    static constexpr bool KEEP = ITEMS <= 16 && NT < 1024;        // masses stay in registers; else they are evaluated again where needed
-    static constexpr int DIRECT = 8;                 // up to this many draws are looked up by every thread in its own samples
-    static constexpr int ENTRIES = (G * NW + 63) / 64;
+    static constexpr int VEC = 16 / sizeof(T);
+    static constexpr int BINS = NT == 64 ? 256 : 1024, PER = BINS / NT, LIST = NT == 64 ? 64 : 128;
+    struct alignas(16) Piece { T v[VEC]; };
     struct Shared {
-        unsigned cnt[BINS];
-        unsigned long long mass[BINS];
-        unsigned long long tot[G * NW > 32 ? G * NW : 32];
-        U list_key[LIST];
-        unsigned list_idx[LIST];
-        unsigned long long list_q[LIST], list_before[LIST];
-        unsigned list_rank[LIST], list_ties[LIST];
-        unsigned n_list;
-        unsigned long long pick_before;
-        unsigned pick_bin, pick_n;
-        U border_key;
-        unsigned border_keep, border_all;
-        unsigned long long ends[G * NT];             // mass up to the end of every group
-        unsigned char kept[G * NT];                  // its samples that may be drawn
+        Piece row[BYTES / 16];
+        unsigned long long mass[BINS], ends[NT], tot[32], list_q[LIST], list_before[LIST], pick_before;
+        U list_key[LIST], border_key;
+        unsigned cnt[BINS], list_idx[LIST], list_rank[LIST], list_ties[LIST], n_list, pick_bin, pick_n, border_keep, border_all;
     };
     Shared& s;
-    V x[G][VEC];
-    unsigned long long q[KEEP ? G : 1][KEEP ? VEC : 1];
-    double kappa, best, scale;
+    int GP, start;                    // pieces per thread, the one this thread begins with
+    double kappa, best, cut, scale;   // cut: distance beyond which a mass rounds to zero
+    U from;                           // lowest key that takes part
 
-    __device__ Held(Shared& s_) : s(s_) {}
-    __device__ __forceinline__ static int first(int g) { return (g * NT + (int)threadIdx.x) * VEC; }
+    __device__ Shelf(Shared& s_) : s(s_) {}
     __device__ __forceinline__ static bool on(V v) { return v > (V)-INFINITY; }
-    __device__ __forceinline__ double distance(V v) const { return kappa > 0.0 ? kappa * (best - (double)v) : 0.0; }
-    __device__ __forceinline__ double weight(V v) const { return exp(-distance(v)); }
-    __device__ __forceinline__ unsigned long long mass_of(V v) const { return __double2ull_rn(weight(v) * scale); }
-    __device__ __forceinline__ unsigned long long mass_at(int g, int j) const {
-        if constexpr (KEEP) return q[g][j];
-        return on(x[g][j]) ? mass_of(x[g][j]) : 0ull;
+    __device__ __forceinline__ static V at(const Piece& p, int j) { return value_of(p.v[j]); }
+    // kappa (best - v); both ends of fp64 may be apart by more than its range, and 0 times that is 0
+    __device__ __forceinline__ double distance(V v) const {
+        const double d = best - (double)v;
+        return kappa * (sizeof(V) == 8 ? fmin(d, 1.7976931348623157e308) : d);
     }
-    template <class F> __device__ __forceinline__ void each(F f) const {
-#pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) f(g, j, x[g][j]);
-    }
+    __device__ __forceinline__ double weight(double d) const { return exp(-d); }
+    __device__ __forceinline__ unsigned long long mass_of(double d) const { return __double2ull_rn(weight(d) * scale); }
 
-    __device__ __forceinline__ static void load(const T* R, long long cs, int i, int K, V (&out)[VEC]) {
-        if (cs == 1 && i + VEC <= K) {
-            T raw[VEC];
-            __builtin_memcpy(raw, R + i, 16);
+    // f(v, d, key, i): every sample that takes part, its distance, key and index
+    template <class F> __device__ __forceinline__ void each(F f) {
+        const int own = (int)threadIdx.x * GP;
+        int g = start;
+#pragma unroll 1
+        for (int n = 0; n < GP; n++) {
+            const Piece p = s.row[own + g];
 #pragma unroll
-            for (int j = 0; j < VEC; j++) out[j] = value_of(raw[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) out[j] = i + j < K ? value_of(R[(long long)(i + j) * cs]) : (V)-INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; j++) out[j] = isfinite(out[j]) ? out[j] : (V)-INFINITY;
-    }
-
-    // exclusive sums of v[g] in the order of the samples
-    template <class X> __device__ __forceinline__ void scan(const X (&v)[G], X (&base)[G], X& total) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        X* tot = (X*)s.tot;
-        if (NW == 1) {
-            X run = 0;
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                const X inc = wave_scan(v[g], (X)0, Add());
-                base[g] = run + inc - v[g];
-                run += lane_value(inc, 63);
+            for (int j = 0; j < VEC; j++) {
+                const V v = at(p, j);
+                const double d = distance(v);
+                const U key = key_of(v);
+                if (on(v) && d <= cut && key >= from) f(v, d, key, (own + g) * VEC + j);
             }
-            total = run;
-            return;
+            g = g + 1 == GP ? 0 : g + 1;
         }
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            const X inc = wave_scan(v[g], (X)0, Add());
-            base[g] = inc - v[g];
-            if (lane == 63) tot[g * NW + wave] = inc;
-        }
-        __syncthreads();
-        X mine[ENTRIES], sum = 0;                    // lane l: entries l ENTRIES ...
-#pragma unroll
-        for (int e = 0; e < ENTRIES; e++) {
-            const int at = lane * ENTRIES + e;
-            mine[e] = at < G * NW ? tot[at] : (X)0;
-            sum += mine[e];
-        }
-        const X inc = wave_scan(sum, (X)0, Add());
-        total = lane_value(inc, 63);
-        X run = inc - sum;
-#pragma unroll
-        for (int e = 0; e < ENTRIES; e++) { const X t = mine[e]; mine[e] = run; run += t; }
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            const int at = __builtin_amdgcn_readfirstlane(g * NW + wave);
-            X b = 0;
-#pragma unroll
-            for (int e = 0; e < ENTRIES; e++)
-                if (at % ENTRIES == e) b = lane_value(mine[e], at / ENTRIES);
-            base[g] += b;
-        }
-        __syncthreads();
     }
 
-    // Border of a prefix of the order among the samples that are on (`far`: bound of their distances): `target` counts
-    // samples (MASS false: the border is the target-th sample) or mass (the last sample with less than the target before
-    // it).  A target beyond what there is leaves no border (false).
-    template <bool MASS> __device__ bool border(unsigned long long target, double far) {
+    // Border of a prefix of the order among the samples that take part (`far`: bound of their distances).  MASS false: the
+    // border is sample number `count` of the order; there is none (false) if there are fewer.  MASS true: it is the last
+    // sample with less than `part` of the mass before it (part < 1).
+    template <bool MASS> __device__ bool border(unsigned long long count, double part, double far) {
         const double per = far > 0.0 ? BINS / far : 0.0;
-        U lo = 0, hi = ~(U)0;
+        U lo = from, hi = ~(U)0;
         int shift = -1, bin = 0;                     // -1: bins linear in the distance; else bits of hi - key
-        unsigned long long before = 0;
+        unsigned long long before = 0, target = count;
         unsigned n = 0;
-        auto bin_of = [&](V v, U key) -> int {
+        auto bin_of = [&](double d, U key) -> int {
             if (shift >= 0) return (int)((hi - key) >> shift);
-            const int b = (int)(distance(v) * per);
+            const int b = (int)(d * per);
             return b < BINS ? b : BINS - 1;
         };
+#pragma unroll 1
         while (true) {
-            s.cnt[threadIdx.x] = 0;
-            if (MASS) s.mass[threadIdx.x] = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                s.cnt[threadIdx.x + i * NT] = 0;
+                if (MASS) s.mass[threadIdx.x + i * NT] = 0;
+            }
             if (threadIdx.x == 0) s.n_list = 0;
             if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
             __syncthreads();
-            each([&](int g, int j, V v) {
-                const U key = key_of(v);
-                if (on(v) && key >= lo && key <= hi) {
-                    const int b = bin_of(v, key);
+            each([&](V, double d, U key, int) {
+                if (key >= lo && key <= hi) {
+                    const int b = bin_of(d, key);
                     atomicAdd(&s.cnt[b], 1u);
-                    if (MASS) atomicAdd(&s.mass[b], mass_at(g, j));
+                    if (MASS) atomicAdd(&s.mass[b], mass_of(d));
                 }
             });
             __syncthreads();
-            const unsigned c = s.cnt[threadIdx.x];
-            const unsigned long long own = MASS ? s.mass[threadIdx.x] : (unsigned long long)c;
-            unsigned long long total;
-            const unsigned long long at = before + group_scan<NT>(own, s.tot, total);
-            if (before + total < target) return false;           // (first pass only: later ones hold the border)
-            if (at < target && target <= at + own) { s.pick_bin = threadIdx.x; s.pick_n = c; s.pick_before = at; }
+            unsigned long long own[PER], sum = 0, total;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int b = threadIdx.x * PER + i;
+                own[i] = MASS ? s.mass[b] : (unsigned long long)s.cnt[b];
+                sum += own[i];
+            }
+            unsigned long long run = before + group_scan<NT>(sum, s.tot, total);
+            if (shift < 0) {
+                if (MASS) {
+                    // a whole number: "mass before < part W" is "mass before < ceil(part W)"
+                    const double want = ceil(part * (double)total);
+                    if (!(want >= 1.0)) { from = ~(U)0; return false; }           // nothing is kept
+                    target = want < (double)total ? (unsigned long long)want : total;
+                }
+                if (total < target) return false;
+            }
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (run < target && target <= run + own[i]) {
+                    s.pick_bin = threadIdx.x * PER + i;
+                    s.pick_n = s.cnt[threadIdx.x * PER + i];
+                    s.pick_before = run;
+                }
+                run += own[i];
+            }
             __syncthreads();
             bin = (int)s.pick_bin;
             n = s.pick_n;
@@ -599,9 +568,8 @@ template <class T, int NT, int G> struct Held {
             // the keys of that bin
             if (shift < 0) {
                 U klo = ~(U)0, khi = 0;
-                each([&](int, int, V v) {
-                    const U key = key_of(v);
-                    if (on(v) && bin_of(v, key) == bin) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
+                each([&](V, double d, U key, int) {
+                    if (bin_of(d, key) == bin) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
                 });
                 lo = group_reduce<NT>(klo, ~(U)0, (U*)s.tot, Min());
                 hi = group_reduce<NT>(khi, (U)0, (U*)s.tot, Max());
@@ -618,224 +586,200 @@ template <class T, int NT, int G> struct Held {
             if (threadIdx.x == 0) {
                 s.border_key = lo;
                 s.border_all = n;
-                if (MASS) {
-                    const unsigned long long one = mass_of(of_key(lo));
-                    s.border_keep = (unsigned)((target - before + one - 1) / one);
-                } else {
-                    s.border_keep = (unsigned)(target - before);
+                const unsigned long long one = MASS ? mass_of(distance(of_key(lo))) : 1ull;
+                s.border_keep = (unsigned)((target - before + one - 1) / one);
+            }
+        } else {
+            each([&](V, double d, U key, int i) {
+                if (key >= lo && key <= hi && bin_of(d, key) == bin) {
+                    const unsigned e = atomicAdd(&s.n_list, 1u);
+                    s.list_key[e] = key;
+                    s.list_idx[e] = (unsigned)i;
+                    if (MASS) s.list_q[e] = mass_of(d);
                 }
+            });
+            __syncthreads();
+            // rank of every candidate: the threads share the comparisons
+            const unsigned parts = NT / n;           // 1 <= n <= LIST <= NT
+            const unsigned e = threadIdx.x / parts, first = threadIdx.x - e * parts;
+            if (e < n) {
+                const U key = s.list_key[e];
+                const unsigned idx = s.list_idx[e];
+                unsigned rank = 0, ties = 0;
+                unsigned long long ahead = 0;
+                for (unsigned o = first; o < n; o += parts) {
+                    const U ok = s.list_key[o];
+                    const bool lead = ok > key || (ok == key && s.list_idx[o] < idx);
+                    rank += lead ? 1u : 0u;
+                    ties += ok == key ? (lead ? 0x10001u : 0x1u) : 0u;     // low half: all equal ones, high half: those ahead
+                    if (MASS) ahead += lead ? s.list_q[o] : 0ull;
+                }
+                atomicAdd(&s.list_rank[e], rank);
+                atomicAdd(&s.list_ties[e], ties);
+                if (MASS) atomicAdd(&s.list_before[e], ahead);
             }
             __syncthreads();
-            return true;
-        }
-        each([&](int g, int j, V v) {
-            const U key = key_of(v);
-            if (on(v) && key >= lo && key <= hi && bin_of(v, key) == bin) {
-                const unsigned e = atomicAdd(&s.n_list, 1u);
-                s.list_key[e] = key;
-                s.list_idx[e] = (unsigned)(first(g) + j);
-                if (MASS) s.list_q[e] = mass_at(g, j);
-            }
-        });
-        __syncthreads();
-        // rank of every candidate: the threads share the comparisons
-        const unsigned parts = NT / n;               // 1 <= n <= LIST <= NT
-        const unsigned e = threadIdx.x / parts, part = threadIdx.x - e * parts;
-        if (e < n) {
-            const U key = s.list_key[e];
-            const unsigned idx = s.list_idx[e];
-            unsigned rank = 0, ties = 0;
-            unsigned long long ahead = 0;
-            for (unsigned o = part; o < n; o += parts) {
-                const U ok = s.list_key[o];
-                const bool lead = ok > key || (ok == key && s.list_idx[o] < idx);
-                rank += lead ? 1u : 0u;
-                ties += ok == key ? (lead ? 0x10001u : 0x1u) : 0u;         // low half: all equal ones, high half: those ahead
-                if (MASS) ahead += lead ? s.list_q[o] : 0ull;
-            }
-            atomicAdd(&s.list_rank[e], rank);
-            atomicAdd(&s.list_ties[e], ties);
-            if (MASS) atomicAdd(&s.list_before[e], ahead);
-        }
-        __syncthreads();
-        if (threadIdx.x < n) {
-            const unsigned long long at = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
-            const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
-            if (at < target && target <= at + own) {
-                s.border_key = s.list_key[threadIdx.x];
-                s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
-                s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
+            if (threadIdx.x < n) {
+                const unsigned long long run = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
+                const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
+                if (run < target && target <= run + own) {
+                    s.border_key = s.list_key[threadIdx.x];
+                    s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
+                    s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
+                }
             }
         }
         __syncthreads();
         return true;
     }
 
-    // switches off what lies behind the border that was found; returns the distance of the border
+    // leaves out what lies behind the border that was found; returns the distance of the border
     __device__ double cut_behind() {
-        const U from = s.border_key;
+        from = s.border_key;
         const unsigned keep = s.border_keep;
-        if (keep < s.border_all) {                   // some of the equal ones: the first in the order of the samples
-            unsigned mine[G], rank[G], total;
+        if (keep < s.border_all) {                   // of the equal ones, the first in the order of the samples stay
+            unsigned mine = 0, total;
+            each([&](V, double, U key, int) { mine += key == from ? 1u : 0u; });
+            unsigned rank = group_scan<NT>(mine, (unsigned*)s.tot, total);
+#pragma unroll 1
+            for (int g = 0; g < GP && mine > 0; g++) {
+                Piece& p = s.row[(int)threadIdx.x * GP + g];
 #pragma unroll
-            for (int g = 0; g < G; g++) {
-                mine[g] = 0;
-#pragma unroll
-                for (int j = 0; j < VEC; j++) mine[g] += on(x[g][j]) && key_of(x[g][j]) == from ? 1u : 0u;
+                for (int j = 0; j < VEC; j++) {
+                    const V v = at(p, j);
+                    if (on(v) && key_of(v) == from && rank++ >= keep) p.v[j] = minus_infinity((T*)nullptr);
+                }
             }
-            scan(mine, rank, total);
-#pragma unroll
-            for (int g = 0; g < G; g++)
-#pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    if (on(x[g][j]) && key_of(x[g][j]) == from) {
-                        if (rank[g] >= keep) drop(g, j);
-                        rank[g]++;
-                    }
         }
-#pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if (key_of(x[g][j]) < from) drop(g, j);
         __syncthreads();                             // s.border_* may be written again
-        return distance(of_key(from));
-    }
-    __device__ __forceinline__ void drop(int g, int j) {
-        x[g][j] = (V)-INFINITY;
-        if constexpr (KEEP) q[g][j] = 0;
+        return fmin(distance(of_key(from)), cut);
     }
 };
 
-template <class T, int NT, int G> __global__ void __launch_bounds__(NT) draw_held_kernel(DrawArgs a, int S) {
-    using H = Held<T, NT, G>;
+template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw_row_kernel(DrawArgs a, int S) {
+    using H = Shelf<T, NT, BYTES>;
     using V = typename H::V;
+    using U = typename H::U;
+    using Piece = typename H::Piece;
     constexpr int VEC = H::VEC;
     __shared__ typename H::Shared s;
     H h(s);
     const long long row = blockIdx.x;
     const T* R = (const T*)a.R + row * a.row_stride;
-#pragma unroll
-    for (int g = 0; g < G; g++) H::load(R, a.col_stride, H::first(g), a.K, h.x[g]);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    h.GP = (a.K + NT * VEC - 1) / (NT * VEC);
+    h.start = tid % h.GP;
     const Param par(a.f, row);
     long long* index = a.index + row * a.D;
     float* weight = a.weight ? a.weight + row * a.D : nullptr;
     const double* u = a.u + row * a.D;
     auto nothing = [&]() {
-        for (int d = threadIdx.x; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
+        for (int d = tid; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
     };
 
+    // the row into LDS, AHEAD pieces requested at a time
+    constexpr int AHEAD = 4;
     V best = (V)-INFINITY, worst = (V)INFINITY;
-    h.each([&](int, int, V v) {
-        best = v > best ? v : best;
-        worst = H::on(v) && v < worst ? v : worst;
-    });
+#pragma unroll 1
+    for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {
+        Piece in[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const int i = ((p0 + k) * NT + tid) * VEC;
+            if (a.col_stride == 1 && i + VEC <= a.K) {
+                __builtin_memcpy(&in[k], R + i, 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) in[k].v[j] = i + j < a.K ? R[(long long)(i + j) * a.col_stride] : minus_infinity((T*)nullptr);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            if (p0 + k >= h.GP) break;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const V v = H::at(in[k], j);
+                if (!isfinite(v)) {
+                    in[k].v[j] = minus_infinity((T*)nullptr);
+                } else {
+                    best = v > best ? v : best;
+                    worst = v < worst ? v : worst;
+                }
+            }
+            s.row[(p0 + k) * NT + tid] = in[k];
+        }
+    }
     best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.tot, Max());
     worst = group_reduce<NT>(worst, (V)INFINITY, (V*)s.tot, Min());
+    __syncthreads();
     if (!par.valid() || !H::on(best)) return nothing();
     h.kappa = par.kappa;
     h.best = (double)best;
     h.scale = __longlong_as_double((long long)(1023 + S) << 52);          // 2^S
-    const double cut = (S + 1) * 0.6931471805599453;
-    double far = fmin(h.distance(worst), cut);
-#pragma unroll
-    for (int g = 0; g < G; g++)
-#pragma unroll
-        for (int j = 0; j < VEC; j++)
-            if (h.distance(h.x[g][j]) > cut) h.x[g][j] = (V)-INFINITY;
-    if constexpr (H::KEEP) {
-#pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) h.q[g][j] = 0;
-    }
-    if (par.top_k > 0 && par.top_k < a.K && h.template border<false>((unsigned long long)par.top_k, far)) far = h.cut_behind();
-    if constexpr (H::KEEP) {
-#pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if (H::on(h.x[g][j])) h.q[g][j] = h.mass_of(h.x[g][j]);
-    }
-    if (!(par.top_p >= 1.0)) {
-        unsigned long long mass = 0;
-        h.each([&](int g, int j, V) { mass += h.mass_at(g, j); });
-        mass = group_reduce<NT>(mass, 0ull, s.tot, Add());
-        const double part = ceil(par.top_p * (double)mass);   // a whole number: "mass before < top_p W" is "mass before < part"
-        if (!(part >= 1.0)) return nothing();
-        const unsigned long long target = part < (double)mass ? (unsigned long long)part : mass;
-        if (h.template border<true>(target, far)) (void)h.cut_behind();
-    }
-    if (!(par.min_p <= 0.0)) {
-        // exp(-distance) >= min_p; only next to the border does the exponential itself have to decide
-        const double edge = -log(par.min_p), near = 1e-9 * (1.0 + fabs(edge));
-#pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                const double d = h.distance(h.x[g][j]);
-                bool in = d < edge;
-                if (!(fabs(d - edge) > near)) in = h.weight(h.x[g][j]) >= par.min_p;
-                if (!in) h.drop(g, j);
-            }
-    }
+    h.cut = (S + 1) * 0.6931471805599453;
+    h.from = 0;
+    double far = fmin(h.distance(worst), h.cut);
+    if (par.top_k > 0 && par.top_k < a.K && h.template border<false>((unsigned long long)par.top_k, 0.0, far)) far = h.cut_behind();
+    if (!(par.top_p >= 1.0) && h.template border<true>(0, par.top_p, far)) (void)h.cut_behind();
 
-    unsigned long long sum[G], base[G], mass;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        sum[g] = 0;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) sum[g] += h.mass_at(g, j);
-    }
-    h.scan(sum, base, mass);
+    unsigned long long sum = 0, mass;
+    h.each([&](V, double d, U, int) {
+        const double w = h.weight(d);
+        if (w >= par.min_p) sum += __double2ull_rn(w * h.scale);
+    });
+    const unsigned long long base = group_scan<NT>(sum, s.tot, mass);
     if (mass == 0) return nothing();
-    auto answer = [&](int d, long long i, V v) {
-        index[d] = i;
-        if (weight) weight[d] = (float)(h.weight(v) * h.scale / (double)mass);
-    };
-    if (a.D <= H::DIRECT) {
-        for (int d = 0; d < a.D; d++) {
-            const unsigned long long target = target_of(u[d], mass);
-#pragma unroll
-            for (int g = 0; g < G; g++)
-                if (target - base[g] < sum[g]) {              // (below base: a huge number)
-                    unsigned long long c = base[g];
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const unsigned long long m = h.mass_at(g, j);
-                        if (target - c < m) answer(d, H::first(g) + j, h.x[g][j]);
-                        c += m;
-                    }
-                }
-        }
-        return;
-    }
-    // many draws: a thread each, which finds the group by bisection and reads its samples again
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        unsigned char bits = 0;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) bits |= (unsigned char)(H::on(h.x[g][j]) ? 1u << j : 0u);
-        s.ends[g * NT + threadIdx.x] = base[g] + sum[g];
-        s.kept[g * NT + threadIdx.x] = bits;
-    }
+    s.ends[tid] = base + sum;
     __syncthreads();
-    for (int d = threadIdx.x; d < a.D; d += NT) {
-        const unsigned long long target = target_of(u[d], mass);
-        int lo = 0, hi = G * NT - 1;                           // the first group whose end is above the target
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s.ends[mid] > target) hi = mid; else lo = mid + 1;
-        }
-        unsigned long long c = lo > 0 ? s.ends[lo - 1] : 0ull;
-        const unsigned bits = s.kept[lo];
-        V v[VEC];
-        H::load(R, a.col_stride, lo * VEC, a.K, v);
+    // mass of sample i of the row, zero if it may not be drawn
+    auto mass_of_sample = [&](int i, double& w) -> unsigned long long {
+        const V v = H::at(s.row[i / VEC], i % VEC);
+        const double d = h.distance(v);
+        w = h.weight(d);
+        return H::on(v) && d <= h.cut && key_of(v) >= h.from && w >= par.min_p ? __double2ull_rn(w * h.scale) : 0ull;
+    };
+    auto answer = [&](int d, int i, double w) {
+        index[d] = i;
+        if (weight) weight[d] = (float)(w * h.scale / (double)mass);
+    };
+    const int C = h.GP * VEC;
+    // A wave for every draw (about 500 cycles each) or a thread for every draw (about 150 cycles for every sample it walks over)
+    if ((long long)(a.D + NT / 64 - 1) / (NT / 64) * 500 <= (long long)((a.D + NT - 1) / NT) * C * 150) {
+#pragma unroll 1
+        for (int d = wave; d < a.D; d += NT / 64) {
+            const unsigned long long target = target_of(u[d], mass);
+            int owner = 0;                                     // number of threads that end at or below the target
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            const unsigned long long m = bits >> j & 1u ? h.mass_of(v[j]) : 0ull;
-            if (target - c < m) answer(d, (long long)lo * VEC + j, v[j]);
-            c += m;
+            for (int k = 0; k < NT / 64; k++) owner += __popcll(__ballot(s.ends[k * 64 + lane] <= target));
+            const unsigned long long ahead = owner > 0 ? s.ends[owner - 1] : 0ull;
+            unsigned long long m[(BYTES / (int)sizeof(T) / NT + 63) / 64], run = ahead;
+            double w;
+#pragma unroll
+            for (int k = 0; k < (int)(sizeof(m) / sizeof(m[0])); k++) {
+                const int j = k * 64 + lane;
+                m[k] = j < C ? mass_of_sample(owner * C + j, w) : 0ull;
+                const unsigned long long inc = wave_scan(m[k], 0ull, Add());
+                if (target - (run + inc - m[k]) < m[k]) answer(d, owner * C + j, w);
+                run += lane_value(inc, 63);
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int d = tid; d < a.D; d += NT) {
+            const unsigned long long target = target_of(u[d], mass);
+            int lo = 0, hi = NT - 1;                           // the first thread that ends above the target
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (s.ends[mid] > target) hi = mid; else lo = mid + 1;
+            }
+            unsigned long long c = lo > 0 ? s.ends[lo - 1] : 0ull;
+#pragma unroll 1
+            for (int i = lo * C; i < (lo + 1) * C; i++) {
+                double w;
+                const unsigned long long m = mass_of_sample(i, w);
+                if (target - c < m) { answer(d, i, w); break; }
+                c += m;
+            }
         }
     }
 }
@@ -847,16 +791,14 @@ int ceil_log2(int n) {
 }
 
 template <class T> hipError_t launch(const DrawArgs& a, hipStream_t s) {
-    constexpr int VEC = 16 / sizeof(T);
     const int S = 62 - ceil_log2(a.K);
+    const size_t bytes = (size_t)a.K * sizeof(T);
     if (a.K <= 512)
-        hipLaunchKernelGGL((draw_held_kernel<T, 64, 8 / VEC>), dim3(a.rows), dim3(64), 0, s, a, S);
+        hipLaunchKernelGGL((draw_row_kernel<T, 64, 512 * sizeof(T)>), dim3(a.rows), dim3(64), 0, s, a, S);
     else if (a.K <= 4096)
-        hipLaunchKernelGGL((draw_held_kernel<T, 256, 16 / VEC>), dim3(a.rows), dim3(256), 0, s, a, S);
-    else if (a.K <= 16384)
-        hipLaunchKernelGGL((draw_held_kernel<T, 512, 32 / VEC>), dim3(a.rows), dim3(512), 0, s, a, S);
-    else if (sizeof(T) < 8 && a.K <= (sizeof(T) == 4 ? 32768 : 65536))
-        hipLaunchKernelGGL((draw_held_kernel<T, 1024, sizeof(T) == 2 ? 8 : 8>), dim3(a.rows), dim3(1024), 0, s, a, S);
+        hipLaunchKernelGGL((draw_row_kernel<T, 256, 4096 * sizeof(T)>), dim3(a.rows), dim3(256), 0, s, a, S);
+    else if (bytes <= 131072)
+        hipLaunchKernelGGL((draw_row_kernel<T, 1024, 131072>), dim3(a.rows), dim3(1024), 0, s, a, S);
     else
         hipLaunchKernelGGL((draw_rows_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a);
     return hipGetLastError();
