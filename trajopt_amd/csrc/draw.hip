@@ -109,30 +109,25 @@ struct Min { template <class X> __device__ __forceinline__ X operator()(X a, X b
 template <int NT, class X, class Op> __device__ __forceinline__ X group_reduce(X v, X none, X* s_tot, Op op) {
     v = wave_scan(v, none, op);
     if (NT == 64) return lane_value(v, 63);
-    if ((threadIdx.x & 63) == 63) s_tot[threadIdx.x >> 6] = v;
+    const int lane = threadIdx.x & 63;
+    if (lane == 63) s_tot[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = s_tot[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; w++) v = op(v, s_tot[w]);
+    v = wave_scan(lane < NT / 64 ? s_tot[lane] : none, none, op);       // (the lanes behind the totals add nothing)
     __syncthreads();
-    return v;
+    return lane_value(v, 63);
 }
 template <int NT, class X> __device__ __forceinline__ X group_scan(X v, X* s_tot, X& total) {        // exclusive sums
     const int wave = threadIdx.x >> 6;
     const X inc = wave_scan(v, (X)0, Add());
     if (NT == 64) { total = lane_value(inc, 63); return inc - v; }
-    if ((threadIdx.x & 63) == 63) s_tot[wave] = inc;
+    const int lane = threadIdx.x & 63;
+    if (lane == 63) s_tot[wave] = inc;
     __syncthreads();
-    X before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; w++) {
-        const X t = s_tot[w];
-        before += w < wave ? t : (X)0;
-        all += t;
-    }
+    const X own = lane < NT / 64 ? s_tot[lane] : (X)0;
+    const X tot = wave_scan(own, (X)0, Add());
     __syncthreads();
-    total = all;
-    return before + inc - v;
+    total = lane_value(tot, 63);
+    return lane_value(tot - own, __builtin_amdgcn_readfirstlane(wave)) + inc - v;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -455,65 +450,86 @@ __device__ __forceinline__ unsigned long long target_of(double u, unsigned long 
 
 // The row lies in LDS as it came (what takes no part as -inf of its type).  Thread t owns the C samples from t C on, in GP
 // pieces of 16 bytes; it visits them from piece t mod GP on, so that the lanes of a wave read from all banks.  All loops over
-// samples stay rolled: unrolled, a kernel of this many passes is larger than the instruction cache.
+// samples stay rolled: unrolled, a kernel of this many passes is larger than the instruction cache.  A pass tests values
+// against the lowest one that takes part, in the type of the row (fp32 or fp64); exponentials, in fp64, are evaluated only for
+// samples that pass.
 template <class T, int NT, int BYTES> struct Shelf {
     using V = typename Traits<T>::V;
     using U = typename Traits<T>::U;
     static constexpr int VEC = 16 / sizeof(T);
     static constexpr int BINS = NT == 64 ? 256 : 1024, PER = BINS / NT, LIST = NT == 64 ? 64 : 128;
+    static constexpr int FEW = BYTES >= 131072 ? 1024 : 0;     // up to this many samples that take part move together
     struct alignas(16) Piece { T v[VEC]; };
     struct Shared {
-        Piece row[BYTES / 16];
-        unsigned long long mass[BINS], ends[NT], tot[32], list_q[LIST], list_before[LIST], pick_before;
-        U list_key[LIST], border_key;
+        Piece row[(BYTES / (int)sizeof(T) + FEW) / VEC];
+        unsigned few_idx[FEW ? FEW : 1];
+        union {
+            unsigned long long mass[BINS];
+            unsigned long long ends[NT];             // (once the borders are found)
+        };
+        unsigned long long tot[32], list_q[LIST], list_before[LIST], pick_before;
+        V list_v[LIST], border;
         unsigned cnt[BINS], list_idx[LIST], list_rank[LIST], list_ties[LIST], n_list, pick_bin, pick_n, border_keep, border_all;
     };
     Shared& s;
-    int GP, start;                    // pieces per thread, the one this thread begins with
-    double kappa, best, cut, scale;   // cut: distance beyond which a mass rounds to zero
-    U from;                           // lowest key that takes part
+    int GP, start, base;              // pieces of this thread, the one it begins with, the row's first piece
+    int C;                            // samples per thread
+    double kappa, scale;
+    V best, from;                     // from: the lowest value that takes part
 
     __device__ Shelf(Shared& s_) : s(s_) {}
-    __device__ __forceinline__ static bool on(V v) { return v > (V)-INFINITY; }
     __device__ __forceinline__ static V at(const Piece& p, int j) { return value_of(p.v[j]); }
     // kappa (best - v); both ends of fp64 may be apart by more than its range, and 0 times that is 0
     __device__ __forceinline__ double distance(V v) const {
-        const double d = best - (double)v;
+        const double d = (double)best - (double)v;
         return kappa * (sizeof(V) == 8 ? fmin(d, 1.7976931348623157e308) : d);
     }
-    __device__ __forceinline__ double weight(double d) const { return exp(-d); }
-    __device__ __forceinline__ unsigned long long mass_of(double d) const { return __double2ull_rn(weight(d) * scale); }
+    __device__ __forceinline__ double weight(V v) const { return exp(-distance(v)); }
+    __device__ __forceinline__ unsigned long long mass_of(V v) const { return __double2ull_rn(weight(v) * scale); }
 
-    // f(v, d, key, i): every sample that takes part, its distance, key and index
-    template <class F> __device__ __forceinline__ void each(F f) {
+    // f(v, live, i): the pieces with samples that take part; live: bit j for sample v[j], whose index is i + j
+    template <class F> __device__ __forceinline__ void each(V low, V high, F f) {
         const int own = (int)threadIdx.x * GP;
         int g = start;
 #pragma unroll 1
         for (int n = 0; n < GP; n++) {
-            const Piece p = s.row[own + g];
+            const Piece p = s.row[base + own + g];
+            V v[VEC];
+            unsigned live = 0;
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                const V v = at(p, j);
-                const double d = distance(v);
-                const U key = key_of(v);
-                if (on(v) && d <= cut && key >= from) f(v, d, key, (own + g) * VEC + j);
+                v[j] = at(p, j);
+                live |= v[j] >= low && v[j] <= high ? 1u << j : 0u;
             }
+            if (live) f(v, live, (own + g) * VEC);
             g = g + 1 == GP ? 0 : g + 1;
         }
     }
+    // masses of a piece side by side: their exponentials are long chains of dependent operations
+    __device__ __forceinline__ void masses(const V (&v)[VEC], unsigned live, double least, unsigned long long (&q)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            const double w = weight(v[j]);
+            q[j] = (live >> j & 1u) && w >= least ? __double2ull_rn(w * scale) : 0ull;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; j++) asm volatile("" : "+v"(q[j]));       // (or each would be moved behind the test of its bit)
+    }
 
-    // Border of a prefix of the order among the samples that take part (`far`: bound of their distances).  MASS false: the
-    // border is sample number `count` of the order; there is none (false) if there are fewer.  MASS true: it is the last
-    // sample with less than `part` of the mass before it (part < 1).
-    template <bool MASS> __device__ bool border(unsigned long long count, double part, double far) {
-        const double per = far > 0.0 ? BINS / far : 0.0;
-        U lo = from, hi = ~(U)0;
-        int shift = -1, bin = 0;                     // -1: bins linear in the distance; else bits of hi - key
+    // Border of a prefix of the order among the samples that take part (none below `low`).  MASS false: the border is sample
+    // number `count` of the order; there is none (false) if there are fewer.  MASS true: it is the last sample with less
+    // than `part` of the mass before it (part < 1).
+    template <bool MASS> __device__ bool border(unsigned long long count, double part, V low) {
+        // bins linear in best - v first (monotone: every step rounds monotonically); per = 0 where that range overflows
+        const V per = best > low ? (V)BINS / (best - low) : (V)0;
+        V lo = from, hi = best;
+        int shift = -1, bin = 0;                     // -1: linear bins; else bits of key(hi) - key(v)
+        U top = key_of(hi);
         unsigned long long before = 0, target = count;
         unsigned n = 0;
-        auto bin_of = [&](double d, U key) -> int {
-            if (shift >= 0) return (int)((hi - key) >> shift);
-            const int b = (int)(d * per);
+        auto bin_of = [&](V v) -> int {
+            if (shift >= 0) return (int)((top - key_of(v)) >> shift);
+            const int b = (int)((best - v) * per);
             return b < BINS ? b : BINS - 1;
         };
 #pragma unroll 1
@@ -526,12 +542,16 @@ template <class T, int NT, int BYTES> struct Shelf {
             if (threadIdx.x == 0) s.n_list = 0;
             if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
             __syncthreads();
-            each([&](V, double d, U key, int) {
-                if (key >= lo && key <= hi) {
-                    const int b = bin_of(d, key);
-                    atomicAdd(&s.cnt[b], 1u);
-                    if (MASS) atomicAdd(&s.mass[b], mass_of(d));
-                }
+            each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
+                unsigned long long q[VEC];
+                if (MASS) masses(v, live, 0.0, q);
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if (live >> j & 1u) {
+                        const int b = bin_of(v[j]);
+                        atomicAdd(&s.cnt[b], 1u);
+                        if (MASS) atomicAdd(&s.mass[b], q[j]);
+                    }
             });
             __syncthreads();
             unsigned long long own[PER], sum = 0, total;
@@ -546,7 +566,7 @@ template <class T, int NT, int BYTES> struct Shelf {
                 if (MASS) {
                     // a whole number: "mass before < part W" is "mass before < ceil(part W)"
                     const double want = ceil(part * (double)total);
-                    if (!(want >= 1.0)) { from = ~(U)0; return false; }           // nothing is kept
+                    if (!(want >= 1.0)) { from = (V)INFINITY; return false; }     // nothing is kept
                     target = want < (double)total ? (unsigned long long)want : total;
                 }
                 if (total < target) return false;
@@ -565,53 +585,60 @@ template <class T, int NT, int BYTES> struct Shelf {
             n = s.pick_n;
             before = s.pick_before;
             if (n <= LIST) break;
-            // the keys of that bin
-            if (shift < 0) {
-                U klo = ~(U)0, khi = 0;
-                each([&](V, double d, U key, int) {
-                    if (bin_of(d, key) == bin) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
-                });
-                lo = group_reduce<NT>(klo, ~(U)0, (U*)s.tot, Min());
-                hi = group_reduce<NT>(khi, (U)0, (U*)s.tot, Max());
-            } else {
-                const U top = hi - ((U)bin << shift), width = ((U)1 << shift) - 1;
-                lo = top - lo > width ? top - width : lo;
-                hi = top;
-            }
+            // the values of that bin, from its lowest to its highest
+            V least = (V)INFINITY, most = (V)-INFINITY;
+            each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if ((live >> j & 1u) && bin_of(v[j]) == bin) { least = v[j] < least ? v[j] : least; most = v[j] > most ? v[j] : most; }
+            });
+            lo = group_reduce<NT>(least, (V)INFINITY, (V*)s.tot, Min());
+            hi = group_reduce<NT>(most, (V)-INFINITY, (V*)s.tot, Max());
             if (lo == hi) break;
+            top = key_of(hi);
             shift = 0;
-            while (((hi - lo) >> shift) >= (U)BINS) shift++;
+            while (((top - key_of(lo)) >> shift) >= (U)BINS) shift++;
         }
         if (n > LIST) {                              // all n of one return
             if (threadIdx.x == 0) {
-                s.border_key = lo;
+                s.border = lo;
                 s.border_all = n;
-                const unsigned long long one = MASS ? mass_of(distance(of_key(lo))) : 1ull;
+                const unsigned long long one = MASS ? mass_of(lo) : 1ull;
                 s.border_keep = (unsigned)((target - before + one - 1) / one);
             }
         } else {
-            each([&](V, double d, U key, int i) {
-                if (key >= lo && key <= hi && bin_of(d, key) == bin) {
-                    const unsigned e = atomicAdd(&s.n_list, 1u);
-                    s.list_key[e] = key;
-                    s.list_idx[e] = (unsigned)i;
-                    if (MASS) s.list_q[e] = mass_of(d);
+            each(lo, hi, [&](const V (&v)[VEC], unsigned live, int i) {
+                unsigned hit = 0;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
+                if (hit) {
+#pragma unroll 1
+                    for (int j = 0; j < VEC; j++)
+                        if (hit >> j & 1u) {
+                            const unsigned e = atomicAdd(&s.n_list, 1u);
+                            s.list_v[e] = at(s.row[base + i / VEC], j);
+                            s.list_idx[e] = (unsigned)(i + j);
+                        }
                 }
             });
             __syncthreads();
+            if (MASS) {
+                if (threadIdx.x < n) s.list_q[threadIdx.x] = mass_of(s.list_v[threadIdx.x]);
+                __syncthreads();
+            }
             // rank of every candidate: the threads share the comparisons
             const unsigned parts = NT / n;           // 1 <= n <= LIST <= NT
             const unsigned e = threadIdx.x / parts, first = threadIdx.x - e * parts;
             if (e < n) {
-                const U key = s.list_key[e];
+                const V v = s.list_v[e];
                 const unsigned idx = s.list_idx[e];
                 unsigned rank = 0, ties = 0;
                 unsigned long long ahead = 0;
                 for (unsigned o = first; o < n; o += parts) {
-                    const U ok = s.list_key[o];
-                    const bool lead = ok > key || (ok == key && s.list_idx[o] < idx);
+                    const V ov = s.list_v[o];
+                    const bool lead = ov > v || (ov == v && s.list_idx[o] < idx);
                     rank += lead ? 1u : 0u;
-                    ties += ok == key ? (lead ? 0x10001u : 0x1u) : 0u;     // low half: all equal ones, high half: those ahead
+                    ties += ov == v ? (lead ? 0x10001u : 0x1u) : 0u;       // low half: all equal ones, high half: those ahead
                     if (MASS) ahead += lead ? s.list_q[o] : 0ull;
                 }
                 atomicAdd(&s.list_rank[e], rank);
@@ -623,7 +650,7 @@ template <class T, int NT, int BYTES> struct Shelf {
                 const unsigned long long run = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
                 const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
                 if (run < target && target <= run + own) {
-                    s.border_key = s.list_key[threadIdx.x];
+                    s.border = s.list_v[threadIdx.x];
                     s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
                     s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
                 }
@@ -633,33 +660,90 @@ template <class T, int NT, int BYTES> struct Shelf {
         return true;
     }
 
-    // leaves out what lies behind the border that was found; returns the distance of the border
-    __device__ double cut_behind() {
-        from = s.border_key;
+    // raises `from` to a value that at least k threads' own values `mine` reach (one per thread), near the highest such
+    __device__ void raise(V mine, unsigned k) {
+        const V per = best > from ? (V)BINS / (best - from) : (V)0;
+        const bool in = mine >= from;
+        int b = in ? (int)((best - mine) * per) : 0;
+        b = b < BINS ? b : BINS - 1;
+#pragma unroll
+        for (int i = 0; i < PER; i++) s.cnt[threadIdx.x + i * NT] = 0;
+        __syncthreads();
+        if (in) atomicAdd(&s.cnt[b], 1u);
+        __syncthreads();
+        unsigned own[PER], sum = 0, total;
+#pragma unroll
+        for (int i = 0; i < PER; i++) { own[i] = s.cnt[threadIdx.x * PER + i]; sum += own[i]; }
+        unsigned run = group_scan<NT>(sum, (unsigned*)s.tot, total);
+        if (total < k) return;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if (run < k && k <= run + own[i]) s.pick_bin = threadIdx.x * PER + i;
+            run += own[i];
+        }
+        __syncthreads();
+        const V low = in && b <= (int)s.pick_bin ? mine : (V)INFINITY;
+        from = group_reduce<NT>(low, (V)INFINITY, (V*)s.tot, Min());
+    }
+
+    // If few samples take part, they move together (in their order, with their indices), and the passes that follow go over
+    // them alone.
+    __device__ void gather_few() {
+        unsigned mine = 0, pieces = 0, total;
+        const int own = (int)threadIdx.x * GP;
+        each(from, best, [&](const V (&)[VEC], unsigned live, int i) {
+            mine += (unsigned)__popc(live);
+            pieces |= 1u << (i / VEC - own);
+        });
+        unsigned to = group_scan<NT>(mine, (unsigned*)s.tot, total);
+        if (total > FEW) return;
+        constexpr int first = BYTES / 16;
+        if (threadIdx.x < FEW / VEC) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) s.row[first + threadIdx.x].v[j] = minus_infinity((T*)nullptr);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (; pieces; pieces &= pieces - 1) {
+            const int p = own + __ffs(pieces) - 1;
+#pragma unroll 1
+            for (int j = 0; j < VEC; j++)
+                if (at(s.row[p], j) >= from) {
+                    s.row[first + to / VEC].v[to % VEC] = s.row[p].v[j];
+                    s.few_idx[to] = (unsigned)(p * VEC + j);
+                    to++;
+                }
+        }
+        __syncthreads();
+        base = first;
+        GP = threadIdx.x < FEW / VEC ? 1 : 0;
+        start = 0;
+        C = VEC;
+    }
+
+    // leaves out what lies behind the border that was found
+    __device__ void cut_behind() {
+        from = s.border;
         const unsigned keep = s.border_keep;
         if (keep < s.border_all) {                   // of the equal ones, the first in the order of the samples stay
             unsigned mine = 0, total;
-            each([&](V, double, U key, int) { mine += key == from ? 1u : 0u; });
+            each(from, from, [&](const V (&)[VEC], unsigned live, int) { mine += (unsigned)__popc(live); });
             unsigned rank = group_scan<NT>(mine, (unsigned*)s.tot, total);
 #pragma unroll 1
             for (int g = 0; g < GP && mine > 0; g++) {
-                Piece& p = s.row[(int)threadIdx.x * GP + g];
+                Piece& p = s.row[base + (int)threadIdx.x * GP + g];
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const V v = at(p, j);
-                    if (on(v) && key_of(v) == from && rank++ >= keep) p.v[j] = minus_infinity((T*)nullptr);
-                }
+                for (int j = 0; j < VEC; j++)
+                    if (at(p, j) == from && rank++ >= keep) p.v[j] = minus_infinity((T*)nullptr);
             }
         }
-        __syncthreads();                             // s.border_* may be written again
-        return fmin(distance(of_key(from)), cut);
+        __syncthreads();                             // s.border may be written again
     }
 };
 
 template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw_row_kernel(DrawArgs a, int S) {
     using H = Shelf<T, NT, BYTES>;
     using V = typename H::V;
-    using U = typename H::U;
     using Piece = typename H::Piece;
     constexpr int VEC = H::VEC;
     __shared__ typename H::Shared s;
@@ -668,7 +752,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     const T* R = (const T*)a.R + row * a.row_stride;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     h.GP = (a.K + NT * VEC - 1) / (NT * VEC);
+    h.C = h.GP * VEC;
     h.start = tid % h.GP;
+    h.base = 0;
     const Param par(a.f, row);
     long long* index = a.index + row * a.D;
     float* weight = a.weight ? a.weight + row * a.D : nullptr;
@@ -677,8 +763,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         for (int d = tid; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
     };
 
+    const double u_wave = wave < a.D ? u[wave] : 0.0, u_thread = tid < a.D ? u[tid] : 0.0;      // asked for before anything waits
     // the row into LDS, AHEAD pieces requested at a time
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = BYTES >= 131072 ? 8 : 4;
     V best = (V)-INFINITY, worst = (V)INFINITY;
 #pragma unroll 1
     for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {
@@ -709,23 +796,29 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             s.row[(p0 + k) * NT + tid] = in[k];
         }
     }
+    const V mine = best;                                                  // best of what this thread loaded
     best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.tot, Max());
     worst = group_reduce<NT>(worst, (V)INFINITY, (V*)s.tot, Min());
     __syncthreads();
-    if (!par.valid() || !H::on(best)) return nothing();
+    if (!par.valid() || !(best > (V)-INFINITY)) return nothing();
     h.kappa = par.kappa;
-    h.best = (double)best;
+    h.best = best;
     h.scale = __longlong_as_double((long long)(1023 + S) << 52);          // 2^S
-    h.cut = (S + 1) * 0.6931471805599453;
-    h.from = 0;
-    double far = fmin(h.distance(worst), h.cut);
-    if (par.top_k > 0 && par.top_k < a.K && h.template border<false>((unsigned long long)par.top_k, 0.0, far)) far = h.cut_behind();
-    if (!(par.top_p >= 1.0) && h.template border<true>(0, par.top_p, far)) (void)h.cut_behind();
+    // samples this far behind have masses below half a unit, with a margin for the rounding of the bound itself
+    h.from = fmax(worst, (V)((double)best - (S + 1.01) * 0.6931471805599453 / h.kappa * (1.0 + 1e-6)));
+    // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
+    // thread next to nothing else passes that bound.
+    if (BYTES >= 131072 && par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
+    if (H::FEW && h.GP > 1) h.gather_few();
+    if (par.top_k > 0 && par.top_k < a.K && h.template border<false>((unsigned long long)par.top_k, 0.0, h.from)) h.cut_behind();
+    if (!(par.top_p >= 1.0) && h.template border<true>(0, par.top_p, h.from)) h.cut_behind();
 
     unsigned long long sum = 0, mass;
-    h.each([&](V, double d, U, int) {
-        const double w = h.weight(d);
-        if (w >= par.min_p) sum += __double2ull_rn(w * h.scale);
+    h.each(h.from, h.best, [&](const V (&v)[VEC], unsigned live, int) {
+        unsigned long long q[VEC];
+        h.masses(v, live, par.min_p, q);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) sum += q[j];
     });
     const unsigned long long base = group_scan<NT>(sum, s.tot, mass);
     if (mass == 0) return nothing();
@@ -733,21 +826,20 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     __syncthreads();
     // mass of sample i of the row, zero if it may not be drawn
     auto mass_of_sample = [&](int i, double& w) -> unsigned long long {
-        const V v = H::at(s.row[i / VEC], i % VEC);
-        const double d = h.distance(v);
-        w = h.weight(d);
-        return H::on(v) && d <= h.cut && key_of(v) >= h.from && w >= par.min_p ? __double2ull_rn(w * h.scale) : 0ull;
+        const V v = H::at(s.row[h.base + i / VEC], i % VEC);
+        w = h.weight(v);
+        return v >= h.from && w >= par.min_p ? __double2ull_rn(w * h.scale) : 0ull;
     };
     auto answer = [&](int d, int i, double w) {
-        index[d] = i;
+        index[d] = h.base ? (long long)s.few_idx[i] : i;
         if (weight) weight[d] = (float)(w * h.scale / (double)mass);
     };
-    const int C = h.GP * VEC;
+    const int C = h.C;
     // A wave for every draw (about 500 cycles each) or a thread for every draw (about 150 cycles for every sample it walks over)
     if ((long long)(a.D + NT / 64 - 1) / (NT / 64) * 500 <= (long long)((a.D + NT - 1) / NT) * C * 150) {
 #pragma unroll 1
         for (int d = wave; d < a.D; d += NT / 64) {
-            const unsigned long long target = target_of(u[d], mass);
+            const unsigned long long target = target_of(d == wave ? u_wave : u[d], mass);
             int owner = 0;                                     // number of threads that end at or below the target
 #pragma unroll
             for (int k = 0; k < NT / 64; k++) owner += __popcll(__ballot(s.ends[k * 64 + lane] <= target));
@@ -766,7 +858,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     } else {
 #pragma unroll 1
         for (int d = tid; d < a.D; d += NT) {
-            const unsigned long long target = target_of(u[d], mass);
+            const unsigned long long target = target_of(d == tid ? u_thread : u[d], mass);
             int lo = 0, hi = NT - 1;                           // the first thread that ends above the target
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
