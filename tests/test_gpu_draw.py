@@ -230,8 +230,8 @@ def test_rows_behind_the_last_are_left_alone():
         f = L.DrawFilterC(kappa=1.0, top_k=5, top_p=0.9, min_p=0.0)
         torch.cuda.synchronize()
         index2, weight2 = _draw(R, u, kappa=1.0, top_k=5, top_p=0.9)
-        from trajopt_amd.device import _draw_call
-        _draw_call(torch, R, L.F32, 3, K, K, 1, u, 2, f, index[3:], weight[3:])
+        L.check(L.lib().mppi_draw_from_returns(0, R.data_ptr(), L.F32, 3, K, K, 1, u.data_ptr(), 2, ctypes.byref(f), index[3:].data_ptr(),
+                                               weight[3:].data_ptr(), torch.cuda.current_stream().cuda_stream))
         torch.cuda.synchronize()
         assert (index[:3] == 77).all() and (index[9:] == 77).all() and (weight[:3] == 7).all() and (weight[9:] == 7).all()
         assert torch.equal(index[3:9].reshape(3, 2), index2) and torch.equal(weight[3:9].reshape(3, 2), weight2)

@@ -134,6 +134,27 @@ def lib():
     return _lib
 
 
+_tensors = None
+
+
+def tensors():
+    """The module that calls the library with torch tensors (csrc/tensors.cpp), bound to the loaded library."""
+    global _tensors
+    if _tensors is None:
+        L = lib()
+        import torch  # noqa: F401  (its libraries have to be loaded first)
+        try:
+            from . import _tensors as module
+        except ImportError as e:
+            raise MppiError("the tensor binding trajopt_amd/_tensors.so is missing or does not fit this torch (%s): build it with "
+                            "`python -c 'import __graft_entry__ as g; g.build()'` or `make -C trajopt_amd/csrc`" % e) from e
+        module.bind(MppiError, *[C.cast(getattr(L, n), _vp).value
+                                 for n in ("mppi_last_error", "mppi_draw_from_returns", "mppi_gradient_workspace",
+                                           "mppi_gradient_norm", "mppi_clip_gradients")])
+        _tensors = module
+    return _tensors
+
+
 def check(rc):
     if rc != 0:
         msg = lib().mppi_last_error()

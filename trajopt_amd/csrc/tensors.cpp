@@ -1,0 +1,237 @@
+// Python module `_tensors`: the entry points of the C ABI that work on torch tensors, called with the tensors themselves.
+// Reading the address, type, layout and device of a tensor from Python costs half a microsecond or more, which for lists of
+// hundreds of gradients is many times what the kernels take; here it costs nanoseconds.  The library is the one trajopt_amd._lib
+// has loaded: bind() receives the addresses of its functions.
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
+
+#include <vector>
+
+#include "../../include/mppi_hip.h"
+
+namespace {
+
+decltype(&mppi_last_error) last_error;
+decltype(&mppi_draw_from_returns) draw_from_returns;
+decltype(&mppi_gradient_workspace) gradient_workspace;
+decltype(&mppi_gradient_norm) gradient_norm;
+decltype(&mppi_clip_gradients) clip_gradients;
+PyObject* library_error;              // trajopt_amd._lib.MppiError
+
+struct Raised {};                     // a Python exception has been set
+
+[[noreturn]] void raise(PyObject* type, const std::string& message) {
+    PyErr_SetString(type, message.c_str());
+    throw Raised();
+}
+void check(int rc) {
+    if (rc == 0) return;
+    const char* m = last_error();
+    raise(library_error, "mppi_hip error " + std::to_string(rc) + ": " + (m ? m : "?"));
+}
+std::string text(at::IntArrayRef shape) {
+    std::string s = "(";
+    for (size_t i = 0; i < shape.size(); i++) s += (i ? ", " : "") + std::to_string(shape[i]);
+    return s + (shape.size() == 1 ? ",)" : ")");
+}
+std::string text(const at::Device& d) { return d.str(); }
+
+int element_type(const at::Tensor& t, bool doubles) {
+    switch (t.scalar_type()) {
+    case at::kFloat: return MPPI_F32;
+    case at::kHalf: return MPPI_F16;
+    case at::kBFloat16: return MPPI_BF16;
+    case at::kDouble: if (doubles) return MPPI_F64; break;
+    default: break;
+    }
+    raise(PyExc_TypeError, std::string("unsupported element type ") + c10::toString(t.scalar_type()));
+}
+void* stream_of(const at::Device& d) { return (void*)c10::hip::getCurrentHIPStream(d.index()).stream(); }
+
+bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
+const at::Tensor& tensor(PyObject* o) { return THPVariable_Unpack(o); }
+
+// a draw's parameter: a number, or a tensor of one value per row
+struct PerRow {
+    at::Tensor held;
+    const void* data = nullptr;
+    PerRow(PyObject* o, const char* name, int64_t rows, at::ScalarType type, const at::Device& device) {
+        if (!is_tensor(o)) return;
+        const at::Tensor& t = tensor(o);
+        if (t.device() != device) raise(PyExc_ValueError, std::string(name) + " lies on " + text(t.device()) + ", the returns on " + text(device));
+        if (t.dim() != 1 || t.size(0) != rows)
+            raise(PyExc_ValueError, std::string(name) + ": one value per row, shape (" + std::to_string(rows) + ",), got " + text(t.sizes()));
+        if (t.is_complex() || (type == at::kLong && t.is_floating_point()))
+            raise(PyExc_TypeError, std::string(name) + ": unsupported element type " + c10::toString(t.scalar_type()));
+        held = t.detach().to(type).contiguous();
+        data = held.const_data_ptr();
+    }
+};
+double number(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw Raised();
+    return v;
+}
+int64_t whole(PyObject* o) {
+    PyObject* i = PyNumber_Index(o);
+    if (!i) throw Raised();
+    const long long v = PyLong_AsLongLong(i);
+    Py_DECREF(i);
+    if (v == -1 && PyErr_Occurred()) throw Raised();
+    return v;
+}
+
+// draw(R, u, kappa, top_k, top_p, min_p) -> (index, weight)
+PyObject* draw(PyObject* const* args) {
+    if (!is_tensor(args[0]) || !is_tensor(args[1])) raise(PyExc_TypeError, "draw_from_returns works on CUDA tensors");
+    const at::Tensor &R = tensor(args[0]), &u = tensor(args[1]);
+    if (!R.is_cuda() || !u.is_cuda() || R.layout() != at::kStrided || u.layout() != at::kStrided)
+        raise(PyExc_TypeError, "draw_from_returns works on CUDA tensors");
+    if ((R.dim() != 1 && R.dim() != 2) || u.dim() != R.dim() || (R.dim() == 2 && u.size(0) != R.size(0)))
+        raise(PyExc_ValueError, "R is (K,) with u (D,), or (P, K) with u (P, D): got " + text(R.sizes()) + " and " + text(u.sizes()));
+    const at::Device device = R.device();
+    if (u.device() != device) raise(PyExc_ValueError, "u lies on " + text(u.device()) + ", the returns on " + text(device));
+    if (u.scalar_type() != at::kDouble && u.scalar_type() != at::kFloat)
+        raise(PyExc_TypeError, std::string("u must be float64 or float32, got ") + c10::toString(u.scalar_type()));
+    const int type = element_type(R, true);
+    const bool one = R.dim() == 1;
+    const int64_t rows = one ? 1 : R.size(0), K = R.size(one ? 0 : 1), D = u.size(one ? 0 : 1);
+    if (rows > INT32_MAX || K > INT32_MAX || D > INT32_MAX)
+        raise(PyExc_ValueError, "too many rows, samples or draws: " + std::to_string(rows) + ", " + std::to_string(K) + ", " + std::to_string(D));
+    const PerRow kappa(args[2], "kappa", rows, at::kDouble, device), top_k(args[3], "top_k", rows, at::kLong, device),
+        top_p(args[4], "top_p", rows, at::kDouble, device), min_p(args[5], "min_p", rows, at::kDouble, device);
+    mppi_draw_filter f;
+    f.kappa = kappa.data ? 0.0 : number(args[2]);
+    f.top_k = top_k.data ? 0 : whole(args[3]);
+    f.top_p = top_p.data ? 1.0 : number(args[4]);
+    f.min_p = min_p.data ? 0.0 : number(args[5]);
+    f.kappa_of = (const double*)kappa.data; f.top_k_of = (const int64_t*)top_k.data;
+    f.top_p_of = (const double*)top_p.data; f.min_p_of = (const double*)min_p.data;
+    at::Tensor u64 = u;
+    if (u.scalar_type() != at::kDouble || !u.is_contiguous()) u64 = u.detach().to(at::kDouble).contiguous();
+    at::Tensor index = at::empty(u.sizes(), at::TensorOptions().dtype(at::kLong).device(device));
+    at::Tensor weight = at::empty(u.sizes(), at::TensorOptions().dtype(at::kFloat).device(device));
+    check(draw_from_returns(device.index(), R.const_data_ptr(), type, (int32_t)rows, (int32_t)K, one ? 0 : R.stride(0), R.stride(one ? 0 : 1),
+                            (const double*)u64.const_data_ptr(), (int32_t)D, &f, (int64_t*)index.mutable_data_ptr(),
+                            (float*)weight.mutable_data_ptr(), stream_of(device)));
+    PyObject* out = PyTuple_New(2);
+    if (!out) throw Raised();
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(index)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(weight)));
+    return out;
+}
+
+std::vector<at::Tensor> tensors(PyObject* o, const char* what) {
+    std::vector<at::Tensor> list;
+    auto add = [&](PyObject* item) {
+        if (!is_tensor(item)) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
+        const at::Tensor& t = tensor(item);
+        if (!t.is_cuda() || t.layout() != at::kStrided) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
+        if (!t.is_non_overlapping_and_dense())
+            raise(PyExc_ValueError, std::string(what) + " must fill their memory without gaps or overlaps (a slice or an expanded tensor does not)");
+        list.push_back(t);
+    };
+    if (is_tensor(o)) {
+        add(o);
+        return list;
+    }
+    PyObject* seq = PySequence_Fast(o, "a list of tensors is needed");
+    if (!seq) throw Raised();
+    struct Owned { PyObject* o; ~Owned() { Py_DECREF(o); } } owned{seq};
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    list.reserve(n);
+    for (Py_ssize_t i = 0; i < n; i++) add(PySequence_Fast_GET_ITEM(seq, i));
+    return list;
+}
+
+// gradients(grads, out or None, norm type, max_norm or None) -> norm
+PyObject* gradients(PyObject* const* args) {
+    const std::vector<at::Tensor> grads = tensors(args[0], "gradients");
+    if (grads.empty()) raise(PyExc_ValueError, "no gradients");
+    if (grads.size() > INT32_MAX) raise(PyExc_ValueError, "too many gradients");
+    const bool clip = args[3] != Py_None, elsewhere = args[1] != Py_None;
+    const std::vector<at::Tensor> outs = elsewhere ? tensors(args[1], "outputs") : std::vector<at::Tensor>();
+    if (elsewhere && outs.size() != grads.size())
+        raise(PyExc_ValueError, std::to_string(grads.size()) + " gradients, " + std::to_string(outs.size()) + " outputs");
+    const at::Device device = grads[0].device();
+    const size_t n = grads.size();
+    std::vector<const void*> in(n);
+    std::vector<void*> out(n);
+    std::vector<int64_t> sizes(n);
+    std::vector<int32_t> types(n);
+    for (size_t i = 0; i < n; i++) {
+        const at::Tensor& g = grads[i];
+        if (g.device() != device) raise(PyExc_ValueError, "all tensors must lie on one device");
+        types[i] = element_type(g, false);
+        sizes[i] = g.numel();
+        in[i] = g.const_data_ptr();
+        if (!clip) continue;
+        const at::Tensor& o = elsewhere ? outs[i] : g;
+        if (elsewhere) {
+            if (o.device() != device) raise(PyExc_ValueError, "all tensors must lie on one device");
+            if (o.scalar_type() != g.scalar_type() || o.sizes() != g.sizes() || o.strides() != g.strides())
+                raise(PyExc_ValueError, "an output has another shape, type or layout than its gradient");
+        }
+        out[i] = o.mutable_data_ptr();
+    }
+    size_t bytes = 0;
+    check(gradient_workspace((int32_t)n, &bytes));
+    at::Tensor ws = at::empty({(int64_t)(bytes + 7) / 8}, at::TensorOptions().dtype(at::kDouble).device(device));
+    at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
+    const int32_t kind = (int32_t)whole(args[2]);
+    if (clip) {
+        const double most = number(args[3]);
+        check(clip_gradients(device.index(), (int32_t)n, in.data(), out.data(), sizes.data(), types.data(), kind, most,
+                             (float*)norm.mutable_data_ptr(), ws.mutable_data_ptr(), bytes, stream_of(device)));
+        for (const at::Tensor& o : elsewhere ? outs : grads)
+            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();        // written in place: autograd has to know
+    } else {
+        check(gradient_norm(device.index(), (int32_t)n, in.data(), sizes.data(), types.data(), kind, (float*)norm.mutable_data_ptr(),
+                            ws.mutable_data_ptr(), bytes, stream_of(device)));
+    }
+    return THPVariable_Wrap(std::move(norm));
+}
+
+// bind(MppiError, address of mppi_last_error, ..._draw_from_returns, ..._gradient_workspace, ..._gradient_norm, ..._clip_gradients)
+PyObject* bind(PyObject* const* args) {
+    void* address[5];
+    for (int i = 0; i < 5; i++) {
+        address[i] = PyLong_AsVoidPtr(args[1 + i]);
+        if (!address[i]) raise(PyExc_ValueError, "null function address");
+    }
+    Py_INCREF(args[0]);
+    Py_XDECREF(library_error);
+    library_error = args[0];
+    last_error = (decltype(last_error))address[0];
+    draw_from_returns = (decltype(draw_from_returns))address[1];
+    gradient_workspace = (decltype(gradient_workspace))address[2];
+    gradient_norm = (decltype(gradient_norm))address[3];
+    clip_gradients = (decltype(clip_gradients))address[4];
+    Py_RETURN_NONE;
+}
+
+template <PyObject* (*F)(PyObject* const*), int N> PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    try {
+        if (n != N) raise(PyExc_TypeError, "wrong number of arguments");
+        if (F != &bind && !library_error) raise(PyExc_RuntimeError, "bind() has not been called");
+        return F(args);
+    } catch (const Raised&) {
+        return nullptr;
+    }
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {
+    {"bind", (PyCFunction)(void (*)())&entry<bind, 6>, METH_FASTCALL, nullptr},
+    {"draw", (PyCFunction)(void (*)())&entry<draw, 6>, METH_FASTCALL, nullptr},
+    {"gradients", (PyCFunction)(void (*)())&entry<gradients, 4>, METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__tensors() { return PyModule_Create(&module); }

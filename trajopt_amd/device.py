@@ -70,32 +70,6 @@ def update_from_returns(actions, R, kappa, device=None):
     return out
 
 
-def _element_type(torch, t, types):
-    code = {torch.float32: L.F32, torch.float64: L.F64, torch.float16: L.F16, torch.bfloat16: L.BF16}.get(t.dtype)
-    if code not in types:
-        raise TypeError("unsupported element type %s" % t.dtype)
-    return code
-
-
-def _per_row(torch, value, name, rows, dtype, device):
-    """(number, None) or (0, tensor of one value per row on the device) of a draw's parameter."""
-    if not isinstance(value, torch.Tensor):
-        return value, None
-    if value.device != device:
-        raise ValueError("%s lies on %s, the returns on %s" % (name, value.device, device))
-    if value.shape != (rows,):
-        raise ValueError("%s: one value per row, shape (%d,), got %s" % (name, rows, tuple(value.shape)))
-    if value.is_complex() or (dtype == torch.int64 and value.is_floating_point()):
-        raise TypeError("%s: unsupported element type %s" % (name, value.dtype))
-    return 0, value.detach().to(dtype).contiguous()
-
-
-def _draw_call(torch, R, code, rows, K, row_stride, col_stride, u, D, f, index, weight):
-    L.check(L.lib().mppi_draw_from_returns(R.device.index, R.data_ptr(), code, rows, K, row_stride, col_stride, u.data_ptr(), D,
-                                           C.byref(f), index.data_ptr(), weight.data_ptr(),
-                                           torch.cuda.current_stream(R.device).cuda_stream))
-
-
 def draw_from_returns(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draws samples by their exponentiated returns, w = exp(kappa (R - max R)): the weights `update_from_returns` averages
     with, here as probabilities (kappa is the inverse of a temperature).
@@ -111,99 +85,19 @@ def draw_from_returns(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Returns (index, weight) of u's shape: index (int64) is the smallest one at which the running sum of the kept weights
     exceeds u times their sum, weight (float32) its share of that sum.  A row without samples gives -1 and 0.  Runs on
     the current stream of R's device, without synchronising; can be captured into a graph."""
-    import torch
-    if not (isinstance(R, torch.Tensor) and isinstance(u, torch.Tensor) and R.is_cuda and u.is_cuda):
-        raise TypeError("draw_from_returns works on CUDA tensors")
-    if R.dim() not in (1, 2) or u.dim() != R.dim() or (R.dim() == 2 and u.shape[0] != R.shape[0]):
-        raise ValueError("R is (K,) with u (D,), or (P, K) with u (P, D): got %s and %s" % (tuple(R.shape), tuple(u.shape)))
-    if u.device != R.device:
-        raise ValueError("u lies on %s, the returns on %s" % (u.device, R.device))
-    if u.dtype not in (torch.float64, torch.float32):
-        raise TypeError("u must be float64 or float32, got %s" % u.dtype)
-    code = _element_type(torch, R, (L.F32, L.F64, L.F16, L.BF16))
-    rows, K = (1, R.shape[0]) if R.dim() == 1 else R.shape
-    D = u.shape[-1]
-    if max(rows, K, D) >= 2 ** 31:
-        raise ValueError("too many rows, samples or draws: %d, %d, %d" % (rows, K, D))
-    f = L.DrawFilterC()
-    hold = []
-    for name, value, dtype in (("kappa", kappa, torch.float64), ("top_k", top_k, torch.int64),
-                               ("top_p", top_p, torch.float64), ("min_p", min_p, torch.float64)):
-        number, tensor = _per_row(torch, value, name, rows, dtype, R.device)
-        setattr(f, name, int(number) if name == "top_k" else float(number))
-        if tensor is not None:
-            hold.append(tensor)
-            setattr(f, name + "_of", tensor.data_ptr())
-    u64 = u.detach().to(torch.float64).contiguous()
-    index = torch.empty(u.shape, dtype=torch.int64, device=R.device)
-    weight = torch.empty(u.shape, dtype=torch.float32, device=R.device)
-    row_stride, col_stride = (0, R.stride(0)) if R.dim() == 1 else R.stride()
-    _draw_call(torch, R, code, rows, K, row_stride, col_stride, u64, D, f, index, weight)
-    return index, weight
+    return L.tensors().draw(R, u, kappa, top_k, top_p, min_p)
 
 
-def _fills_its_memory(t):
-    """True if the entries of t are numel() neighbouring ones, in whatever order of the dimensions."""
-    step = 1
-    for stride, size in sorted((stride, size) for stride, size in zip(t.stride(), t.shape) if size != 1):
-        if stride != step:
-            return False
-        step *= size
-    return True
-
-
-def _gradient_table(torch, tensors, what):
-    if isinstance(tensors, torch.Tensor):
-        tensors = [tensors]
-    tensors = list(tensors)
-    for t in tensors:
-        if not (isinstance(t, torch.Tensor) and t.is_cuda) or t.layout != torch.strided:
-            raise TypeError("%s must be dense CUDA tensors" % what)
-        if not t.is_contiguous() and not _fills_its_memory(t):
-            raise ValueError("%s must fill their memory without gaps or overlaps (a slice or an expanded tensor does not)" % what)
-    return tensors
-
-
-def _gradient_call(grads, norm, max_norm, out):
-    import torch
+def _norm_type(norm):
     if norm not in L.NORMS:
         raise ValueError("norm must be 'l2' or 'max', got %r" % (norm,))
-    grads = _gradient_table(torch, grads, "gradients")
-    if not grads:
-        raise ValueError("no gradients")
-    device = grads[0].device
-    outs = grads if out is None else _gradient_table(torch, out, "outputs")
-    if len(outs) != len(grads):
-        raise ValueError("%d gradients, %d outputs" % (len(grads), len(outs)))
-    for g, o in zip(grads, outs):
-        if g.device != device or o.device != device:
-            raise ValueError("all tensors must lie on one device")
-        if o is not g and (o.shape != g.shape or o.dtype != g.dtype or o.stride() != g.stride()):
-            raise ValueError("an output has another shape, type or layout than its gradient")
-    codes = [_element_type(torch, g, (L.F32, L.F16, L.BF16)) for g in grads]
-    n = len(grads)
-    ptrs = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
-    sizes = (C.c_int64 * n)(*[g.numel() for g in grads])
-    types = (C.c_int32 * n)(*codes)
-    need = C.c_size_t()
-    L.check(L.lib().mppi_gradient_workspace(n, C.byref(need)))
-    ws = torch.empty(need.value // 8, dtype=torch.float64, device=device)
-    result = torch.empty((), dtype=torch.float32, device=device)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if max_norm is None:
-        L.check(L.lib().mppi_gradient_norm(device.index, n, ptrs, sizes, types, L.NORMS[norm], result.data_ptr(),
-                                           ws.data_ptr(), need.value, stream))
-    else:
-        optrs = ptrs if out is None else (C.c_void_p * n)(*[o.data_ptr() for o in outs])
-        L.check(L.lib().mppi_clip_gradients(device.index, n, ptrs, optrs, sizes, types, L.NORMS[norm], float(max_norm),
-                                            result.data_ptr(), ws.data_ptr(), need.value, stream))
-    return result
+    return L.NORMS[norm]
 
 
 def gradient_norm(grads, norm="l2"):
     """Norm over all entries of a list of CUDA tensors (float32, float16, bfloat16, mixed freely): 'l2' or 'max', as a
     float32 scalar tensor.  Sums of squares are fp64.  Runs on the device's current stream, without synchronising."""
-    return _gradient_call(grads, norm, None, None)
+    return L.tensors().gradients(grads, None, _norm_type(norm), None)
 
 
 def clip_gradients(grads, max_norm, norm="l2", out=None):
@@ -211,7 +105,7 @@ def clip_gradients(grads, max_norm, norm="l2", out=None):
     of the same shapes, types and layouts), and returns the norm before as a float32 scalar tensor.  A norm that is not
     finite leaves the gradients as they are: the caller sees it in the result and can skip the step.  Runs on the device's
     current stream, without synchronising; can be captured into a graph, which then clips the same tensors."""
-    return _gradient_call(grads, norm, float(max_norm), out)
+    return L.tensors().gradients(grads, out, _norm_type(norm), float(max_norm))
 
 
 class DevicePlanner:
