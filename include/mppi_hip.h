@@ -326,12 +326,14 @@ typedef struct mppi_draw_filter {
  * outside are taken as the nearest end.  A row without samples gives index -1 and weight 0.  No counterpart in the reference,
  * whose update is the mean over the same weights (trajopt/algos/mppi.py:56-65).
  * All arrays are device memory: returns of type `dtype` (MPPI_F32, F64, F16, BF16), element k of row r at
- * r * row_stride + k * col_stride elements; u (rows, D), index (rows, D) and weight (rows, D) contiguous.  The work is
- * enqueued on `stream` (NULL: the default stream); nothing is allocated or synchronised, and it may be captured.  K up to
- * MPPI_DRAW_MAX_K (-6 beyond).  The current device of the calling thread is left as it was. */
+ * r * row_stride + k * col_stride elements; u (rows, D), index (rows, D) and weight (rows, D) contiguous; d_workspace of at
+ * least mppi_draw_workspace bytes (0 for rows of up to 128 KB), aligned to 256 bytes, that nothing else uses until the work
+ * on `stream` is done.  The work is enqueued on `stream` (NULL: the default stream); nothing is allocated or synchronised, and
+ * it may be captured.  K up to MPPI_DRAW_MAX_K (-6 beyond).  The current device of the calling thread is left as it was. */
+int mppi_draw_workspace(int32_t dtype, int32_t rows, int32_t K, size_t* bytes);
 int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32_t rows, int32_t K, int64_t row_stride,
                            int64_t col_stride, const double* d_u, int32_t D, const mppi_draw_filter* filter, int64_t* d_index,
-                           float* d_weight, void* stream);
+                           float* d_weight, void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* Norm of the gradients of a critic (or of any tensors) and clipping to a largest norm, for the training steps between
  * planning epochs (sandbox/examples/ac_reacher_7dof_mppi.py:146-229; the reference leaves them unclipped).

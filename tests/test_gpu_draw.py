@@ -230,8 +230,13 @@ def test_rows_behind_the_last_are_left_alone():
         f = L.DrawFilterC(kappa=1.0, top_k=5, top_p=0.9, min_p=0.0)
         torch.cuda.synchronize()
         index2, weight2 = _draw(R, u, kappa=1.0, top_k=5, top_p=0.9)
+        need = ctypes.c_size_t()
+        L.check(L.lib().mppi_draw_workspace(L.F32, 3, K, ctypes.byref(need)))
+        ws = torch.full((need.value + 64,), 0x5a, dtype=torch.uint8, device="cuda")
         L.check(L.lib().mppi_draw_from_returns(0, R.data_ptr(), L.F32, 3, K, K, 1, u.data_ptr(), 2, ctypes.byref(f), index[3:].data_ptr(),
-                                               weight[3:].data_ptr(), torch.cuda.current_stream().cuda_stream))
+                                               weight[3:].data_ptr(), ws.data_ptr() if need.value else None, need.value,
+                                               torch.cuda.current_stream().cuda_stream))
+        assert (ws[need.value:] == 0x5a).all()
         torch.cuda.synchronize()
         assert (index[:3] == 77).all() and (index[9:] == 77).all() and (weight[:3] == 7).all() and (weight[9:] == 7).all()
         assert torch.equal(index[3:9].reshape(3, 2), index2) and torch.equal(weight[3:9].reshape(3, 2), weight2)

@@ -10,11 +10,11 @@ from oracle import ref_learn
 def _draw(**kw):
     from trajopt_amd import _lib as L
     a = dict(device=0, R=0x1000, dtype=L.F32, rows=2, K=10, rs=10, cs=1, u=0x2000, D=1, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0,
-             index=0x3000, filter=True)
+             index=0x3000, filter=True, ws=None, ws_bytes=0)
     a.update(kw)
     f = L.DrawFilterC(kappa=a["kappa"], top_k=a["top_k"], top_p=a["top_p"], min_p=a["min_p"])
     return L.lib().mppi_draw_from_returns(a["device"], a["R"], a["dtype"], a["rows"], a["K"], a["rs"], a["cs"], a["u"], a["D"],
-                                          C.byref(f) if a["filter"] else None, a["index"], None, None)
+                                          C.byref(f) if a["filter"] else None, a["index"], None, a["ws"], a["ws_bytes"], None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -22,6 +22,7 @@ def _draw(**kw):
     (dict(dtype=4), -1), (dict(dtype=-1), -1), (dict(K=(1 << 24) + 1), -6), (dict(R=None), -1), (dict(u=None), -1), (dict(index=None), -1),
     (dict(kappa=-0.5), -1), (dict(kappa=float("nan")), -1), (dict(kappa=float("inf")), -1), (dict(top_k=-1), -1), (dict(top_p=0.0), -1),
     (dict(top_p=1.5), -1), (dict(top_p=float("nan")), -1), (dict(min_p=-0.1), -1), (dict(min_p=1.1), -1), (dict(min_p=float("nan")), -1),
+    (dict(K=100000), -1), (dict(K=100000, ws=0x10000, ws_bytes=4096), -1), (dict(K=100000, ws=0x10010, ws_bytes=1 << 40), -1),
     (dict(rows=0), 0), (dict(D=0), 0), (dict(rows=0, R=None, index=None, u=None), 0)])
 def test_draw_refuses(kw, code):
     from trajopt_amd import _lib as L
@@ -71,6 +72,13 @@ def test_clip_refuses(args, kw):
 def test_workspace_query():
     from trajopt_amd import _lib as L
     need = C.c_size_t()
+    for dtype, most in ((L.F32, 32768), (L.F64, 16384), (L.F16, 65536), (L.BF16, 65536)):
+        assert L.lib().mppi_draw_workspace(dtype, 1000, most, C.byref(need)) == 0 and need.value == 0
+        assert L.lib().mppi_draw_workspace(dtype, 3, most + 1, C.byref(need)) == 0
+        assert 3 * (most + 1) * 8 <= need.value < 3 * (most + 1) * 14 + 100000
+    for bad in ((L.F32, -1, 5), (L.F32, 1, 0), (9, 1, 5), (L.F32, 1, (1 << 24) + 1)):
+        assert L.lib().mppi_draw_workspace(*bad, C.byref(need)) < 0
+    assert L.lib().mppi_draw_workspace(L.F32, 1, 5, None) == -1
     assert L.lib().mppi_gradient_workspace(-1, C.byref(need)) == -1 and L.lib().mppi_gradient_workspace(1, None) == -1
     assert L.lib().mppi_gradient_workspace(100000, C.byref(need)) == 0 and 0 < need.value < 1 << 20
 

@@ -99,7 +99,8 @@ _PROTOS = {
     "mppi_update_from_returns": (C.c_int, [_i32, _vp, _vp, _i32, _i32, _d, _vp]),
     "mppi_update_from_returns_noalloc": (C.c_int, [_i32, _vp, _vp, _i32, _i32, _d, _vp, _vp]),
     "mppi_draw_from_returns": (C.c_int, [_i32, _vp, _i32, _i32, _i32, C.c_int64, C.c_int64, _vp, _i32,
-                                         C.POINTER(DrawFilterC), _vp, _vp, _vp]),
+                                         C.POINTER(DrawFilterC), _vp, _vp, _vp, C.c_size_t, _vp]),
+    "mppi_draw_workspace": (C.c_int, [_i32, _i32, _i32, C.POINTER(C.c_size_t)]),
     "mppi_gradient_workspace": (C.c_int, [_i32, C.POINTER(C.c_size_t)]),
     "mppi_gradient_norm": (C.c_int, [_i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, C.c_size_t, _vp]),
     "mppi_clip_gradients": (C.c_int, [_i32, _i32, _vp, _vp, _vp, _vp, _i32, _d, _vp, _vp, C.c_size_t, _vp]),
@@ -149,7 +150,7 @@ def tensors():
             raise MppiError("the tensor binding trajopt_amd/_tensors.so is missing or does not fit this torch (%s): build it with "
                             "`python -c 'import __graft_entry__ as g; g.build()'` or `make -C trajopt_amd/csrc`" % e) from e
         module.bind(MppiError, *[C.cast(getattr(L, n), _vp).value
-                                 for n in ("mppi_last_error", "mppi_draw_from_returns", "mppi_gradient_workspace",
+                                 for n in ("mppi_last_error", "mppi_draw_workspace", "mppi_draw_from_returns", "mppi_gradient_workspace",
                                            "mppi_gradient_norm", "mppi_clip_gradients")])
         _tensors = module
     return _tensors

@@ -16,6 +16,7 @@
 #include "abi_common.hpp"
 #include "../../include/mppi_hip.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -53,11 +54,6 @@ __device__ __forceinline__ uint64_t key_of(double x) {
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
 }
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
-__device__ __forceinline__ double of_key(uint64_t k) {
-    return __longlong_as_double((long long)((k & 0x8000000000000000ull) ? k ^ 0x8000000000000000ull : ~k));
-}
-
 struct DrawArgs {
     const void* R;
     long long row_stride, col_stride;
@@ -130,309 +126,6 @@ template <int NT, class X> __device__ __forceinline__ X group_scan(X v, X* s_tot
     return lane_value(tot - own, __builtin_amdgcn_readfirstlane(wave)) + inc - v;
 }
 
-// ------------------------------------------------------------------------------------------
-// one row per workgroup, read from memory in every pass
-// ------------------------------------------------------------------------------------------
-template <class T, int NT> struct Row {
-    using V = typename Traits<T>::V;
-    using U = typename Traits<T>::U;
-    static constexpr int VEC = 16 / sizeof(T);          // samples a thread takes at a time: 16 bytes
-    static constexpr int BINS = NT, LIST = 256;
-    struct Shared {
-        unsigned cnt[BINS];
-        unsigned long long mass[BINS];
-        unsigned long long tot[NT / 64 + 1];
-        U list_key[LIST];
-        unsigned list_idx[LIST];
-        unsigned long long list_q[LIST], list_before[LIST];
-        unsigned list_rank[LIST], list_ties[LIST];
-        unsigned n_list;
-        unsigned long long pick_before;
-        unsigned pick_bin, pick_n;
-        U border_key;
-        unsigned border_keep, border_all;
-    };
-    const T* R;
-    long long cs;
-    int K, S;
-    double kappa, best, cut;          // cut: kappa (best - R) beyond which a sample is left out
-    Shared& s;
-
-    __device__ Row(Shared& s_) : s(s_) {}
-
-    __device__ double distance(V x) const { return kappa > 0.0 ? kappa * (best - (double)x) : 0.0; }
-    __device__ unsigned long long mass_of(V x) const { return (unsigned long long)__double2ull_rn(ldexp(exp(-distance(x)), S)); }
-
-    // f(x, i): every sample in reach; those left out come as -inf
-    template <class F> __device__ void each(F f) const {
-        for (long long i0 = (long long)threadIdx.x * VEC; i0 < K; i0 += (long long)NT * VEC) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if (i0 + j < K) f(load(i0 + j), (int)(i0 + j));
-        }
-    }
-    __device__ V load(long long i) const {
-        const V x = value_of(R[i * cs]);
-        if (!isfinite(x)) return (V)-INFINITY;
-        return distance(x) > cut ? (V)-INFINITY : x;
-    }
-
-    // Border of a prefix of the order: `target` counts samples (MASS false: the border is the target-th sample) or mass (the
-    // last sample with less than the target before it).  Only samples with keys >= from take part.  A target beyond what
-    // there is leaves no border (false).
-    template <bool MASS> __device__ bool border(unsigned long long target, U from) {
-        // range of kappa (best - R) over the samples in reach
-        double far = 0.0;
-        each([&](V x, int) {
-            if (x > (V)-INFINITY && key_of(x) >= from) far = fmax(far, distance(x));
-        });
-        far = group_reduce<NT>(far, 0.0, (double*)s.tot, Max());
-        const double per = far > 0.0 ? BINS / far : 0.0;
-        U lo = from, hi = ~(U)0;
-        int shift = -1;                                  // -1: bins linear in the distance; else bits of hi - key
-        unsigned long long before = 0;
-        unsigned n = 0;
-        auto bin_of = [&](V x, U key) -> int {
-            if (shift >= 0) return (int)((hi - key) >> shift);
-            const int b = (int)(distance(x) * per);
-            return b < BINS ? b : BINS - 1;
-        };
-        while (true) {
-            s.cnt[threadIdx.x] = 0;
-            s.mass[threadIdx.x] = 0;
-            __syncthreads();
-            each([&](V x, int) {
-                const U key = key_of(x);
-                if (x > (V)-INFINITY && key >= lo && key <= hi) {
-                    const int b = bin_of(x, key);
-                    atomicAdd(&s.cnt[b], 1u);
-                    if (MASS) atomicAdd(&s.mass[b], mass_of(x));
-                }
-            });
-            __syncthreads();
-            const unsigned long long v = MASS ? s.mass[threadIdx.x] : (unsigned long long)s.cnt[threadIdx.x];
-            unsigned long long total;
-            const unsigned long long at = before + group_scan<NT>(v, s.tot, total);
-            if (before + total < target) return false;   // (first pass only: later ones hold the border)
-            if (at < target && target <= at + v) {
-                s.pick_bin = threadIdx.x;
-                s.pick_n = s.cnt[threadIdx.x];
-                s.pick_before = at;
-            }
-            __syncthreads();
-            const int b = (int)s.pick_bin;
-            n = s.pick_n;
-            before = s.pick_before;
-            // keys of that bin
-            if (shift < 0) {
-                U klo = ~(U)0, khi = 0;
-                each([&](V x, int) {
-                    const U key = key_of(x);
-                    if (x > (V)-INFINITY && key >= lo && bin_of(x, key) == b) { klo = key < klo ? key : klo; khi = key > khi ? key : khi; }
-                });
-                klo = group_reduce<NT>(klo, ~(U)0, (U*)s.tot, Min());
-                khi = group_reduce<NT>(khi, (U)0, (U*)s.tot, Max());
-                lo = klo;
-                hi = khi;
-            } else {
-                const U top = hi - ((U)b << shift), width = ((U)1 << shift) - 1;
-                lo = top - lo > width ? top - width : lo;
-                hi = top;
-            }
-            if (n <= LIST || lo == hi) break;
-            shift = 0;
-            while (((hi - lo) >> shift) >= (U)BINS) shift++;
-        }
-        if (lo == hi) {                                  // all n of one return
-            if (threadIdx.x == 0) {
-                s.border_key = lo;
-                s.border_all = n;
-                if (MASS) {
-                    const unsigned long long q = mass_of(of_key(lo));
-                    s.border_keep = (unsigned)((target - before + q - 1) / q);
-                } else {
-                    s.border_keep = (unsigned)(target - before);
-                }
-            }
-            __syncthreads();
-            return true;
-        }
-        if (threadIdx.x == 0) s.n_list = 0;
-        if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
-        __syncthreads();
-        each([&](V x, int i) {
-            const U key = key_of(x);
-            if (x > (V)-INFINITY && key >= lo && key <= hi) {
-                const unsigned at = atomicAdd(&s.n_list, 1u);
-                s.list_key[at] = key;
-                s.list_idx[at] = (unsigned)i;
-                s.list_q[at] = MASS ? mass_of(x) : 0;
-            }
-        });
-        __syncthreads();
-        // rank of every candidate: the threads share the comparisons
-        const unsigned parts = NT / n;                   // n <= LIST <= NT
-        const unsigned e = threadIdx.x / parts, part = threadIdx.x % parts;
-        if (e < n) {
-            const U key = s.list_key[e];
-            const unsigned idx = s.list_idx[e];
-            unsigned rank = 0, ties = 0;
-            unsigned long long ahead = 0;
-            for (unsigned o = part; o < n; o += parts) {
-                const U ok = s.list_key[o];
-                const bool first = ok > key || (ok == key && s.list_idx[o] < idx);
-                rank += first ? 1u : 0u;
-                ties += ok == key ? (first ? 0x10001u : 0x1u) : 0u;        // low half: all equal ones, high half: those ahead
-                if (MASS) ahead += first ? s.list_q[o] : 0ull;
-            }
-            atomicAdd(&s.list_rank[e], rank);
-            atomicAdd(&s.list_ties[e], ties);
-            if (MASS) atomicAdd(&s.list_before[e], ahead);
-        }
-        __syncthreads();
-        if (threadIdx.x < n) {
-            const unsigned long long at = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
-            const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
-            if (at < target && target <= at + own) {
-                s.border_key = s.list_key[threadIdx.x];
-                s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
-                s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
-            }
-        }
-        __syncthreads();
-        return true;
-    }
-};
-
-template <class T, int NT> __global__ void __launch_bounds__(NT) draw_rows_kernel(DrawArgs a) {
-    using W = Row<T, NT>;
-    using V = typename W::V;
-    using U = typename W::U;
-    __shared__ typename W::Shared s;
-    W r(s);
-    const long long row = blockIdx.x;
-    r.R = (const T*)a.R + row * a.row_stride;
-    r.cs = a.col_stride;
-    r.K = a.K;
-    r.kappa = a.f.kappa_of ? a.f.kappa_of[row] : a.f.kappa;
-    const double top_p = a.f.top_p_of ? a.f.top_p_of[row] : a.f.top_p;
-    const double min_p = a.f.min_p_of ? a.f.min_p_of[row] : a.f.min_p;
-    const long long top_k = a.f.top_k_of ? a.f.top_k_of[row] : a.f.top_k;
-    long long* index = a.index + row * a.D;
-    float* weight = a.weight ? a.weight + row * a.D : nullptr;
-    const double* u = a.u + row * a.D;
-
-    auto nothing = [&]() {
-        for (int d = threadIdx.x; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
-    };
-    if (!(r.kappa >= 0.0 && r.kappa < INFINITY)) return nothing();
-
-    // best return, then the scale from the mass
-    r.best = 0.0;
-    r.cut = INFINITY;
-    V best = (V)-INFINITY;
-    r.each([&](V x, int) { best = x > best ? x : best; });
-    best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.tot, Max());
-    if (!(best > (V)-INFINITY)) return nothing();
-    r.best = (double)best;
-    double mass = 0.0;
-    r.each([&](V x, int) { if (x > (V)-INFINITY) mass += exp(-r.distance(x)); });
-    mass = group_reduce<NT>(mass, 0.0, (double*)s.tot, Add());
-    int e;
-    (void)frexp(mass, &e);                                // mass < 2^e
-    r.S = 62 - e;
-    r.cut = (r.S + 1) * 0.6931471805599453;
-
-    U from = 0;                                           // border: keys above it, and the first `keep` samples that equal it
-    unsigned keep = UINT_MAX, ties = 0;
-    if (top_k > 0 && top_k < a.K && r.template border<false>((unsigned long long)top_k, 0)) {
-        from = s.border_key; keep = s.border_keep; ties = s.border_all;
-    }
-    __syncthreads();
-    auto kept_mass = [&](double least) {                  // of the samples with w >= least inside the border
-        unsigned long long sum = 0;
-        r.each([&](V x, int) {
-            if (x > (V)-INFINITY) {
-                const U key = key_of(x);
-                if (key > from || (key == from && keep >= ties)) {
-                    const double w = exp(-r.distance(x));
-                    if (w >= least) sum += __double2ull_rn(ldexp(w, r.S));
-                }
-            }
-        });
-        sum = group_reduce<NT>(sum, 0ull, s.tot, Add());
-        if (keep < ties && exp(-r.distance(of_key(from))) >= least) sum += keep * r.mass_of(of_key(from));
-        return sum;
-    };
-    if (!(top_p >= 1.0)) {
-        const unsigned long long all = kept_mass(0.0);
-        const double part = ceil(top_p * (double)all);    // a whole number: "mass before < top_p W" is "mass before < part"
-        if (!(part >= 1.0)) return nothing();
-        const unsigned long long target = part < (double)all ? (unsigned long long)part : all;
-        if (r.template border<true>(target, from)) {
-            // inside the samples that top-k kept: its own border never lies behind theirs
-            if (s.border_key != from || s.border_keep < keep) { from = s.border_key; keep = s.border_keep; ties = s.border_all; }
-        }
-        __syncthreads();
-    }
-    const unsigned long long all = kept_mass(min_p);
-    if (all == 0) return nothing();
-
-    // running mass in the order of the samples, a tile of NT VEC samples at a time
-    unsigned long long running = 0;
-    unsigned equal = 0;
-    for (long long t0 = 0; t0 < a.K; t0 += (long long)NT * W::VEC) {
-        V x[W::VEC];
-        unsigned mine = 0;
-#pragma unroll
-        for (int j = 0; j < W::VEC; j++) {
-            const long long i = t0 + (long long)threadIdx.x * W::VEC + j;
-            x[j] = i < a.K ? r.load(i) : (V)-INFINITY;
-            mine += x[j] > (V)-INFINITY && key_of(x[j]) == from ? 1u : 0u;
-        }
-        unsigned tile_equal;
-        unsigned rank = equal + group_scan<NT>(mine, (unsigned*)s.tot, tile_equal);
-        unsigned long long q[W::VEC], sum = 0;
-#pragma unroll
-        for (int j = 0; j < W::VEC; j++) {
-            q[j] = 0;
-            if (x[j] > (V)-INFINITY) {
-                const U key = key_of(x[j]);
-                const bool in = key > from || (key == from && rank < keep);
-                rank += key == from ? 1u : 0u;
-                if (in) {
-                    const double w = exp(-r.distance(x[j]));
-                    q[j] = w >= min_p ? __double2ull_rn(ldexp(w, r.S)) : 0ull;
-                }
-            }
-            sum += q[j];
-        }
-        unsigned long long tile;
-        const unsigned long long at = running + group_scan<NT>(sum, s.tot, tile);
-        for (int d = 0; d < a.D; d++) {
-            const double want = u[d] * (double)all;
-            unsigned long long target = want > 0.0 ? (want < (double)all ? (unsigned long long)want : all) : 0ull;
-            target = target < all ? target : all - 1;
-            if (target >= at && target < at + sum) {
-                unsigned long long c = at;
-#pragma unroll
-                for (int j = 0; j < W::VEC; j++) {
-                    if (target >= c && target < c + q[j]) {
-                        index[d] = t0 + (long long)threadIdx.x * W::VEC + j;
-                        if (weight) weight[d] = (float)(ldexp(exp(-r.distance(x[j])), r.S) / (double)all);
-                    }
-                    c += q[j];
-                }
-            }
-        }
-        running += tile;
-        equal += tile_equal;
-    }
-}
-
-// ------------------------------------------------------------------------------------------
-// one row per workgroup, held in registers
-// ------------------------------------------------------------------------------------------
 struct Param {
     double kappa, top_p, min_p;
     long long top_k;
@@ -448,46 +141,273 @@ __device__ __forceinline__ unsigned long long target_of(double u, unsigned long 
     return t < mass ? t : mass - 1;
 }
 
+// ------------------------------------------------------------------------------------------
+// weights and masses of one row
+// ------------------------------------------------------------------------------------------
+// exp(-d) for 0 <= d < 700: 2^n e^r with r = -d - n ln 2, |r| <= ln 2 / 2, and the series of e^r up to r^12 / 12!, whose next term
+// is below 2^-52.  ln 2 is split into a part of 32 bits, whose product with n is exact, and the rest.
+__device__ __forceinline__ double exp_minus(double d) {
+    const double n = rint(d * -1.4426950408889634);
+    double r = fma(n, -6.9314718036912382e-01, -d);
+    r = fma(n, -1.9082149292705877e-10, r);
+    double p = 1.0 / 479001600.0;
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+// x in [0, 2^51] to the nearest whole number: added to 2^52, it lies in the low bits of the sum
+__device__ __forceinline__ unsigned long long whole(double x) {
+    return (unsigned long long)__double_as_longlong(x + 4503599627370496.0) & 0xfffffffffffffull;
+}
+
+template <class V> struct Weights {
+    double kappa, scale;              // scale: 2^S
+    V best, from;                     // highest value of the row, lowest that takes part
+
+    // Samples further behind than (S + 1) ln 2 / kappa have masses below half a unit.  (A margin covers the rounding of this
+    // bound, and rounding to the type of the values cannot pass one of them.)
+    __device__ __forceinline__ void set(double kappa_, V best_, V worst, int S) {
+        kappa = kappa_;
+        best = best_;
+        scale = __longlong_as_double((long long)(1023 + S) << 52);
+        const V bound = (V)((double)best - (S + 1.01) * 0.6931471805599453 / kappa * (1.0 + 1e-6));
+        from = worst > bound ? worst : bound;
+    }
+    // kappa (best - v) of a sample that takes part (of one that does not: that of the last that does).  Both ends of fp64 may be
+    // apart by more than its range, and 0 times that is 0.
+    __device__ __forceinline__ double distance(V v) const {
+        const double d = (double)best - (double)(v > from ? v : from);
+        return kappa * (sizeof(V) == 8 ? fmin(d, 1.7976931348623157e308) : d);
+    }
+    __device__ __forceinline__ double weight(V v) const { return exp_minus(distance(v)); }
+    __device__ __forceinline__ unsigned long long mass_of(V v) const { return whole(weight(v) * scale); }
+    // masses of several samples side by side (their exponentials are long chains of dependent operations); live: bit j for v[j]
+    template <int N> __device__ __forceinline__ void masses(const V (&v)[N], unsigned live, double least, unsigned long long (&q)[N]) const {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const double w = weight(v[j]);
+            q[j] = (live >> j & 1u) && w >= least ? whole(w * scale) : 0ull;
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) asm volatile("" : "+v"(q[j]));         // (or each would be moved behind the test of its bit)
+    }
+};
+
+// VEC samples from sample i on, those behind the end of the row as -inf
+template <class T, int VEC> __device__ __forceinline__ void load_piece(const T* R, long long col_stride, long long i, int K, T (&v)[VEC]) {
+    if (col_stride == 1 && i + VEC <= K) {
+        __builtin_memcpy(v, R + i, sizeof(v));
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = i + j < K ? R[(i + j) * col_stride] : minus_infinity((T*)nullptr);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// the border of a prefix of the order
+// ------------------------------------------------------------------------------------------
+template <class V, int NT> struct BorderArea {
+    static constexpr int BINS = NT == 64 ? 256 : 1024, LIST = NT == 64 ? 64 : 128;
+    unsigned long long mass[BINS], tot[32], list_q[LIST], list_before[LIST], pick_before;
+    V list_v[LIST], border;
+    unsigned cnt[BINS], list_idx[LIST], list_rank[LIST], list_ties[LIST], n_list, pick_bin, pick_n;
+    unsigned border_keep, border_all;                // of the border_all samples equal to the border, this many are kept
+    unsigned border_idx;                             // the last of those that are kept; UINT_MAX: not known
+};
+
+// Among the samples of `src` in [low, high]: BY_COUNT: sample number `target` of the order.  BY_MASS: the last sample with less than
+// `target` of the mass before it.  BY_SHARE: the same with `share` (< 1) of their whole mass for a target.  False: there is no such
+// sample (too few of them; a share so small that nothing is kept, then src.from is raised to infinity).  Every thread has to call.
+enum Aim { BY_COUNT, BY_MASS, BY_SHARE };
+template <Aim AIM, int NT, class Src, class V>
+__device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long target, double share, V low, V high) {
+    using U = typename Traits<V>::U;
+    using Area = BorderArea<V, NT>;
+    constexpr bool MASS = AIM != BY_COUNT;
+    constexpr int BINS = Area::BINS, PER = BINS / NT, LIST = Area::LIST, VEC = Src::VEC;
+    // bins linear in high - v first (monotone: every step rounds monotonically); per = 0 where that range overflows
+    const V per = high > low ? (V)BINS / (high - low) : (V)0, high0 = high;
+    V lo = low, hi = high;
+    int shift = -1, bin = 0;                         // -1: linear bins; else bits of key(hi) - key(v)
+    U top = key_of(hi);
+    unsigned long long before = 0;
+    unsigned n = 0;
+    auto bin_of = [&](V v) -> int {
+        if (shift >= 0) return (int)((top - key_of(v)) >> shift);
+        const int b = (int)((high0 - v) * per);
+        return b < BINS ? b : BINS - 1;
+    };
+#pragma unroll 1
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            s.cnt[threadIdx.x + i * NT] = 0;
+            if (MASS) s.mass[threadIdx.x + i * NT] = 0;
+        }
+        if (threadIdx.x == 0) s.n_list = 0;
+        if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
+        __syncthreads();
+        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
+            unsigned long long q[VEC];
+            if (MASS) src.w.masses(v, live, 0.0, q);
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (live >> j & 1u) {
+                    const int b = bin_of(v[j]);
+                    atomicAdd(&s.cnt[b], 1u);
+                    if (MASS) atomicAdd(&s.mass[b], q[j]);
+                }
+        });
+        __syncthreads();
+        unsigned long long own[PER], sum = 0, total;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int b = threadIdx.x * PER + i;
+            own[i] = MASS ? s.mass[b] : (unsigned long long)s.cnt[b];
+            sum += own[i];
+        }
+        unsigned long long run = before + group_scan<NT>(sum, s.tot, total);
+        if (shift < 0) {
+            if (AIM == BY_SHARE) {
+                // a whole number: "mass before < share W" is "mass before < ceil(share W)"
+                const double want = ceil(share * (double)total);
+                if (!(want >= 1.0)) { src.w.from = (V)INFINITY; return false; }
+                target = want < (double)total ? (unsigned long long)want : total;
+            }
+            if (total < target) return false;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if (run < target && target <= run + own[i]) {
+                s.pick_bin = threadIdx.x * PER + i;
+                s.pick_n = s.cnt[threadIdx.x * PER + i];
+                s.pick_before = run;
+            }
+            run += own[i];
+        }
+        __syncthreads();
+        bin = (int)s.pick_bin;
+        n = s.pick_n;
+        before = s.pick_before;
+        if (n <= LIST) break;
+        // the values of that bin, from its lowest to its highest
+        V least = (V)INFINITY, most = (V)-INFINITY;
+        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if ((live >> j & 1u) && bin_of(v[j]) == bin) { least = v[j] < least ? v[j] : least; most = v[j] > most ? v[j] : most; }
+        });
+        lo = group_reduce<NT>(least, (V)INFINITY, (V*)s.tot, Min());
+        hi = group_reduce<NT>(most, (V)-INFINITY, (V*)s.tot, Max());
+        if (lo == hi) break;
+        top = key_of(hi);
+        shift = 0;
+        while (((top - key_of(lo)) >> shift) >= (U)BINS) shift++;
+    }
+    if (n > LIST) {                                  // all n of one return
+        if (threadIdx.x == 0) {
+            s.border = lo;
+            s.border_all = n;
+            const unsigned long long one = MASS ? src.w.mass_of(lo) : 1ull;
+            s.border_keep = (unsigned)((target - before + one - 1) / one);
+            s.border_idx = UINT_MAX;
+        }
+    } else {
+        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int i) {
+            unsigned hit = 0;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
+            if (hit) {
+#pragma unroll 1
+                for (int j = 0; j < VEC; j++)
+                    if (hit >> j & 1u) {
+                        const unsigned e = atomicAdd(&s.n_list, 1u);
+                        s.list_v[e] = src.value(i, j);
+                        s.list_idx[e] = src.index(i, j);
+                    }
+            }
+        });
+        __syncthreads();
+        if (MASS) {
+            if (threadIdx.x < n) s.list_q[threadIdx.x] = src.w.mass_of(s.list_v[threadIdx.x]);
+            __syncthreads();
+        }
+        // rank of every candidate: the threads share the comparisons
+        const unsigned parts = NT / n;               // 1 <= n <= LIST <= NT
+        const unsigned e = threadIdx.x / parts, first = threadIdx.x - e * parts;
+        if (e < n) {
+            const V v = s.list_v[e];
+            const unsigned idx = s.list_idx[e];
+            unsigned rank = 0, ties = 0;
+            unsigned long long ahead = 0;
+            for (unsigned o = first; o < n; o += parts) {
+                const V ov = s.list_v[o];
+                const bool lead = ov > v || (ov == v && s.list_idx[o] < idx);
+                rank += lead ? 1u : 0u;
+                ties += ov == v ? (lead ? 0x10001u : 0x1u) : 0u;           // low half: all equal ones, high half: those ahead
+                if (MASS) ahead += lead ? s.list_q[o] : 0ull;
+            }
+            atomicAdd(&s.list_rank[e], rank);
+            atomicAdd(&s.list_ties[e], ties);
+            if (MASS) atomicAdd(&s.list_before[e], ahead);
+        }
+        __syncthreads();
+        if (threadIdx.x < n) {
+            const unsigned long long run = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
+            const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
+            if (run < target && target <= run + own) {
+                s.border = s.list_v[threadIdx.x];
+                s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
+                s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
+                s.border_idx = s.list_idx[threadIdx.x];
+            }
+        }
+    }
+    __syncthreads();
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------
+// rows of up to 128 KB: one workgroup each
+// ------------------------------------------------------------------------------------------
 // The row lies in LDS as it came (what takes no part as -inf of its type).  Thread t owns the C samples from t C on, in GP
 // pieces of 16 bytes; it visits them from piece t mod GP on, so that the lanes of a wave read from all banks.  All loops over
 // samples stay rolled: unrolled, a kernel of this many passes is larger than the instruction cache.  A pass tests values
 // against the lowest one that takes part, in the type of the row (fp32 or fp64); exponentials, in fp64, are evaluated only for
-// samples that pass.
+// pieces with a sample that passes.
 template <class T, int NT, int BYTES> struct Shelf {
     using V = typename Traits<T>::V;
-    using U = typename Traits<T>::U;
     static constexpr int VEC = 16 / sizeof(T);
-    static constexpr int BINS = NT == 64 ? 256 : 1024, PER = BINS / NT, LIST = NT == 64 ? 64 : 128;
     static constexpr int FEW = BYTES >= 131072 ? 1024 : 0;     // up to this many samples that take part move together
     struct alignas(16) Piece { T v[VEC]; };
+    using Area = BorderArea<V, NT>;
     struct Shared {
         Piece row[(BYTES / (int)sizeof(T) + FEW) / VEC];
         unsigned few_idx[FEW ? FEW : 1];
-        union {
-            unsigned long long mass[BINS];
-            unsigned long long ends[NT];             // (once the borders are found)
-        };
-        unsigned long long tot[32], list_q[LIST], list_before[LIST], pick_before;
-        V list_v[LIST], border;
-        unsigned cnt[BINS], list_idx[LIST], list_rank[LIST], list_ties[LIST], n_list, pick_bin, pick_n, border_keep, border_all;
+        Area b;
+        __device__ unsigned long long* ends() { return b.mass; }           // (once the borders are found; NT <= BINS)
     };
     Shared& s;
+    Weights<V> w;
     int GP, start, base;              // pieces of this thread, the one it begins with, the row's first piece
     int C;                            // samples per thread
-    double kappa, scale;
-    V best, from;                     // from: the lowest value that takes part
 
     __device__ Shelf(Shared& s_) : s(s_) {}
     __device__ __forceinline__ static V at(const Piece& p, int j) { return value_of(p.v[j]); }
-    // kappa (best - v); both ends of fp64 may be apart by more than its range, and 0 times that is 0
-    __device__ __forceinline__ double distance(V v) const {
-        const double d = (double)best - (double)v;
-        return kappa * (sizeof(V) == 8 ? fmin(d, 1.7976931348623157e308) : d);
-    }
-    __device__ __forceinline__ double weight(V v) const { return exp(-distance(v)); }
-    __device__ __forceinline__ unsigned long long mass_of(V v) const { return __double2ull_rn(weight(v) * scale); }
+    __device__ __forceinline__ V value(int i, int j) const { return at(s.row[base + i / VEC], j); }
+    __device__ __forceinline__ unsigned index(int i, int j) const { return (unsigned)(i + j); }
 
-    // f(v, live, i): the pieces with samples that take part; live: bit j for sample v[j], whose index is i + j
+    // f(v, live, i): the pieces with samples in [low, high]; live: bit j for sample v[j], whose index is i + j
     template <class F> __device__ __forceinline__ void each(V low, V high, F f) {
         const int own = (int)threadIdx.x * GP;
         int g = start;
@@ -505,185 +425,32 @@ template <class T, int NT, int BYTES> struct Shelf {
             g = g + 1 == GP ? 0 : g + 1;
         }
     }
-    // masses of a piece side by side: their exponentials are long chains of dependent operations
-    __device__ __forceinline__ void masses(const V (&v)[VEC], unsigned live, double least, unsigned long long (&q)[VEC]) const {
-#pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            const double w = weight(v[j]);
-            q[j] = (live >> j & 1u) && w >= least ? __double2ull_rn(w * scale) : 0ull;
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; j++) asm volatile("" : "+v"(q[j]));       // (or each would be moved behind the test of its bit)
-    }
 
-    // Border of a prefix of the order among the samples that take part (none below `low`).  MASS false: the border is sample
-    // number `count` of the order; there is none (false) if there are fewer.  MASS true: it is the last sample with less
-    // than `part` of the mass before it (part < 1).
-    template <bool MASS> __device__ bool border(unsigned long long count, double part, V low) {
-        // bins linear in best - v first (monotone: every step rounds monotonically); per = 0 where that range overflows
-        const V per = best > low ? (V)BINS / (best - low) : (V)0;
-        V lo = from, hi = best;
-        int shift = -1, bin = 0;                     // -1: linear bins; else bits of key(hi) - key(v)
-        U top = key_of(hi);
-        unsigned long long before = 0, target = count;
-        unsigned n = 0;
-        auto bin_of = [&](V v) -> int {
-            if (shift >= 0) return (int)((top - key_of(v)) >> shift);
-            const int b = (int)((best - v) * per);
-            return b < BINS ? b : BINS - 1;
-        };
-#pragma unroll 1
-        while (true) {
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                s.cnt[threadIdx.x + i * NT] = 0;
-                if (MASS) s.mass[threadIdx.x + i * NT] = 0;
-            }
-            if (threadIdx.x == 0) s.n_list = 0;
-            if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
-            __syncthreads();
-            each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
-                unsigned long long q[VEC];
-                if (MASS) masses(v, live, 0.0, q);
-#pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    if (live >> j & 1u) {
-                        const int b = bin_of(v[j]);
-                        atomicAdd(&s.cnt[b], 1u);
-                        if (MASS) atomicAdd(&s.mass[b], q[j]);
-                    }
-            });
-            __syncthreads();
-            unsigned long long own[PER], sum = 0, total;
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const int b = threadIdx.x * PER + i;
-                own[i] = MASS ? s.mass[b] : (unsigned long long)s.cnt[b];
-                sum += own[i];
-            }
-            unsigned long long run = before + group_scan<NT>(sum, s.tot, total);
-            if (shift < 0) {
-                if (MASS) {
-                    // a whole number: "mass before < part W" is "mass before < ceil(part W)"
-                    const double want = ceil(part * (double)total);
-                    if (!(want >= 1.0)) { from = (V)INFINITY; return false; }     // nothing is kept
-                    target = want < (double)total ? (unsigned long long)want : total;
-                }
-                if (total < target) return false;
-            }
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                if (run < target && target <= run + own[i]) {
-                    s.pick_bin = threadIdx.x * PER + i;
-                    s.pick_n = s.cnt[threadIdx.x * PER + i];
-                    s.pick_before = run;
-                }
-                run += own[i];
-            }
-            __syncthreads();
-            bin = (int)s.pick_bin;
-            n = s.pick_n;
-            before = s.pick_before;
-            if (n <= LIST) break;
-            // the values of that bin, from its lowest to its highest
-            V least = (V)INFINITY, most = (V)-INFINITY;
-            each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
-#pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    if ((live >> j & 1u) && bin_of(v[j]) == bin) { least = v[j] < least ? v[j] : least; most = v[j] > most ? v[j] : most; }
-            });
-            lo = group_reduce<NT>(least, (V)INFINITY, (V*)s.tot, Min());
-            hi = group_reduce<NT>(most, (V)-INFINITY, (V*)s.tot, Max());
-            if (lo == hi) break;
-            top = key_of(hi);
-            shift = 0;
-            while (((top - key_of(lo)) >> shift) >= (U)BINS) shift++;
-        }
-        if (n > LIST) {                              // all n of one return
-            if (threadIdx.x == 0) {
-                s.border = lo;
-                s.border_all = n;
-                const unsigned long long one = MASS ? mass_of(lo) : 1ull;
-                s.border_keep = (unsigned)((target - before + one - 1) / one);
-            }
-        } else {
-            each(lo, hi, [&](const V (&v)[VEC], unsigned live, int i) {
-                unsigned hit = 0;
-#pragma unroll
-                for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
-                if (hit) {
-#pragma unroll 1
-                    for (int j = 0; j < VEC; j++)
-                        if (hit >> j & 1u) {
-                            const unsigned e = atomicAdd(&s.n_list, 1u);
-                            s.list_v[e] = at(s.row[base + i / VEC], j);
-                            s.list_idx[e] = (unsigned)(i + j);
-                        }
-                }
-            });
-            __syncthreads();
-            if (MASS) {
-                if (threadIdx.x < n) s.list_q[threadIdx.x] = mass_of(s.list_v[threadIdx.x]);
-                __syncthreads();
-            }
-            // rank of every candidate: the threads share the comparisons
-            const unsigned parts = NT / n;           // 1 <= n <= LIST <= NT
-            const unsigned e = threadIdx.x / parts, first = threadIdx.x - e * parts;
-            if (e < n) {
-                const V v = s.list_v[e];
-                const unsigned idx = s.list_idx[e];
-                unsigned rank = 0, ties = 0;
-                unsigned long long ahead = 0;
-                for (unsigned o = first; o < n; o += parts) {
-                    const V ov = s.list_v[o];
-                    const bool lead = ov > v || (ov == v && s.list_idx[o] < idx);
-                    rank += lead ? 1u : 0u;
-                    ties += ov == v ? (lead ? 0x10001u : 0x1u) : 0u;       // low half: all equal ones, high half: those ahead
-                    if (MASS) ahead += lead ? s.list_q[o] : 0ull;
-                }
-                atomicAdd(&s.list_rank[e], rank);
-                atomicAdd(&s.list_ties[e], ties);
-                if (MASS) atomicAdd(&s.list_before[e], ahead);
-            }
-            __syncthreads();
-            if (threadIdx.x < n) {
-                const unsigned long long run = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
-                const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
-                if (run < target && target <= run + own) {
-                    s.border = s.list_v[threadIdx.x];
-                    s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
-                    s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
-                }
-            }
-        }
-        __syncthreads();
-        return true;
-    }
-
-    // raises `from` to a value that at least k threads' own values `mine` reach (one per thread), near the highest such
+    // raises w.from to a value that at least k threads' own values `mine` reach (one per thread), near the highest such
     __device__ void raise(V mine, unsigned k) {
-        const V per = best > from ? (V)BINS / (best - from) : (V)0;
-        const bool in = mine >= from;
-        int b = in ? (int)((best - mine) * per) : 0;
+        constexpr int BINS = Area::BINS, PER = BINS / NT;
+        const V per = w.best > w.from ? (V)BINS / (w.best - w.from) : (V)0;
+        const bool in = mine >= w.from;
+        int b = in ? (int)((w.best - mine) * per) : 0;
         b = b < BINS ? b : BINS - 1;
 #pragma unroll
-        for (int i = 0; i < PER; i++) s.cnt[threadIdx.x + i * NT] = 0;
+        for (int i = 0; i < PER; i++) s.b.cnt[threadIdx.x + i * NT] = 0;
         __syncthreads();
-        if (in) atomicAdd(&s.cnt[b], 1u);
+        if (in) atomicAdd(&s.b.cnt[b], 1u);
         __syncthreads();
         unsigned own[PER], sum = 0, total;
 #pragma unroll
-        for (int i = 0; i < PER; i++) { own[i] = s.cnt[threadIdx.x * PER + i]; sum += own[i]; }
-        unsigned run = group_scan<NT>(sum, (unsigned*)s.tot, total);
+        for (int i = 0; i < PER; i++) { own[i] = s.b.cnt[threadIdx.x * PER + i]; sum += own[i]; }
+        unsigned run = group_scan<NT>(sum, (unsigned*)s.b.tot, total);
         if (total < k) return;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            if (run < k && k <= run + own[i]) s.pick_bin = threadIdx.x * PER + i;
+            if (run < k && k <= run + own[i]) s.b.pick_bin = threadIdx.x * PER + i;
             run += own[i];
         }
         __syncthreads();
-        const V low = in && b <= (int)s.pick_bin ? mine : (V)INFINITY;
-        from = group_reduce<NT>(low, (V)INFINITY, (V*)s.tot, Min());
+        const V low = in && b <= (int)s.b.pick_bin ? mine : (V)INFINITY;
+        w.from = group_reduce<NT>(low, (V)INFINITY, (V*)s.b.tot, Min());
     }
 
     // If few samples take part, they move together (in their order, with their indices), and the passes that follow go over
@@ -691,11 +458,11 @@ template <class T, int NT, int BYTES> struct Shelf {
     __device__ void gather_few() {
         unsigned mine = 0, pieces = 0, total;
         const int own = (int)threadIdx.x * GP;
-        each(from, best, [&](const V (&)[VEC], unsigned live, int i) {
+        each(w.from, w.best, [&](const V (&)[VEC], unsigned live, int i) {
             mine += (unsigned)__popc(live);
             pieces |= 1u << (i / VEC - own);
         });
-        unsigned to = group_scan<NT>(mine, (unsigned*)s.tot, total);
+        unsigned to = group_scan<NT>(mine, (unsigned*)s.b.tot, total);
         if (total > FEW) return;
         constexpr int first = BYTES / 16;
         if (threadIdx.x < FEW / VEC) {
@@ -708,7 +475,7 @@ template <class T, int NT, int BYTES> struct Shelf {
             const int p = own + __ffs(pieces) - 1;
 #pragma unroll 1
             for (int j = 0; j < VEC; j++)
-                if (at(s.row[p], j) >= from) {
+                if (at(s.row[p], j) >= w.from) {
                     s.row[first + to / VEC].v[to % VEC] = s.row[p].v[j];
                     s.few_idx[to] = (unsigned)(p * VEC + j);
                     to++;
@@ -723,21 +490,21 @@ template <class T, int NT, int BYTES> struct Shelf {
 
     // leaves out what lies behind the border that was found
     __device__ void cut_behind() {
-        from = s.border;
-        const unsigned keep = s.border_keep;
-        if (keep < s.border_all) {                   // of the equal ones, the first in the order of the samples stay
+        w.from = s.b.border;
+        const unsigned keep = s.b.border_keep;
+        if (keep < s.b.border_all) {                 // of the equal ones, the first in the order of the samples stay
             unsigned mine = 0, total;
-            each(from, from, [&](const V (&)[VEC], unsigned live, int) { mine += (unsigned)__popc(live); });
-            unsigned rank = group_scan<NT>(mine, (unsigned*)s.tot, total);
+            each(w.from, w.from, [&](const V (&)[VEC], unsigned live, int) { mine += (unsigned)__popc(live); });
+            unsigned rank = group_scan<NT>(mine, (unsigned*)s.b.tot, total);
 #pragma unroll 1
             for (int g = 0; g < GP && mine > 0; g++) {
                 Piece& p = s.row[base + (int)threadIdx.x * GP + g];
 #pragma unroll
                 for (int j = 0; j < VEC; j++)
-                    if (at(p, j) == from && rank++ >= keep) p.v[j] = minus_infinity((T*)nullptr);
+                    if (at(p, j) == w.from && rank++ >= keep) p.v[j] = minus_infinity((T*)nullptr);
             }
         }
-        __syncthreads();                             // s.border may be written again
+        __syncthreads();                             // the border may be written again
     }
 };
 
@@ -745,7 +512,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     using H = Shelf<T, NT, BYTES>;
     using V = typename H::V;
     using Piece = typename H::Piece;
-    constexpr int VEC = H::VEC;
+    constexpr int VEC = H::VEC, NW = NT / 64;
     __shared__ typename H::Shared s;
     H h(s);
     const long long row = blockIdx.x;
@@ -771,15 +538,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {
         Piece in[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) {
-            const int i = ((p0 + k) * NT + tid) * VEC;
-            if (a.col_stride == 1 && i + VEC <= a.K) {
-                __builtin_memcpy(&in[k], R + i, 16);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; j++) in[k].v[j] = i + j < a.K ? R[(long long)(i + j) * a.col_stride] : minus_infinity((T*)nullptr);
-            }
-        }
+        for (int k = 0; k < AHEAD; k++) load_piece(R, a.col_stride, (long long)((p0 + k) * NT + tid) * VEC, a.K, in[k].v);
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             if (p0 + k >= h.GP) break;
@@ -797,63 +556,54 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         }
     }
     const V mine = best;                                                  // best of what this thread loaded
-    best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.tot, Max());
-    worst = group_reduce<NT>(worst, (V)INFINITY, (V*)s.tot, Min());
+    best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.b.tot, Max());
+    worst = group_reduce<NT>(worst, (V)INFINITY, (V*)s.b.tot, Min());
     __syncthreads();
     if (!par.valid() || !(best > (V)-INFINITY)) return nothing();
-    h.kappa = par.kappa;
-    h.best = best;
-    h.scale = __longlong_as_double((long long)(1023 + S) << 52);          // 2^S
-    // samples this far behind have masses below half a unit, with a margin for the rounding of the bound itself
-    h.from = fmax(worst, (V)((double)best - (S + 1.01) * 0.6931471805599453 / h.kappa * (1.0 + 1e-6)));
+    h.w.set(par.kappa, best, worst, S);
     // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
     // thread next to nothing else passes that bound.
     if (BYTES >= 131072 && par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
     if (H::FEW && h.GP > 1) h.gather_few();
-    if (par.top_k > 0 && par.top_k < a.K && h.template border<false>((unsigned long long)par.top_k, 0.0, h.from)) h.cut_behind();
-    if (!(par.top_p >= 1.0) && h.template border<true>(0, par.top_p, h.from)) h.cut_behind();
+    if (par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, (unsigned long long)par.top_k, 0.0, h.w.from, best)) h.cut_behind();
+    if (!(par.top_p >= 1.0) && find_border<BY_SHARE>(h, s.b, 0, par.top_p, h.w.from, best)) h.cut_behind();
 
     unsigned long long sum = 0, mass;
-    h.each(h.from, h.best, [&](const V (&v)[VEC], unsigned live, int) {
+    h.each(h.w.from, best, [&](const V (&v)[VEC], unsigned live, int) {
         unsigned long long q[VEC];
-        h.masses(v, live, par.min_p, q);
+        h.w.masses(v, live, par.min_p, q);
 #pragma unroll
         for (int j = 0; j < VEC; j++) sum += q[j];
     });
-    const unsigned long long base = group_scan<NT>(sum, s.tot, mass);
+    const unsigned long long base = group_scan<NT>(sum, s.b.tot, mass);
     if (mass == 0) return nothing();
-    s.ends[tid] = base + sum;
+    unsigned long long* ends = s.ends();
+    ends[tid] = base + sum;
     __syncthreads();
     // mass of sample i of the row, zero if it may not be drawn
     auto mass_of_sample = [&](int i, double& w) -> unsigned long long {
         const V v = H::at(s.row[h.base + i / VEC], i % VEC);
-        w = h.weight(v);
-        return v >= h.from && w >= par.min_p ? __double2ull_rn(w * h.scale) : 0ull;
+        w = h.w.weight(v);
+        return v >= h.w.from && w >= par.min_p ? whole(w * h.w.scale) : 0ull;
     };
     auto answer = [&](int d, int i, double w) {
         index[d] = h.base ? (long long)s.few_idx[i] : i;
-        if (weight) weight[d] = (float)(w * h.scale / (double)mass);
+        if (weight) weight[d] = (float)(w * h.w.scale / (double)mass);
     };
     const int C = h.C;
     // A wave for every draw (about 500 cycles each) or a thread for every draw (about 150 cycles for every sample it walks over)
-    if ((long long)(a.D + NT / 64 - 1) / (NT / 64) * 500 <= (long long)((a.D + NT - 1) / NT) * C * 150) {
+    if ((long long)((a.D + NW - 1) / NW) * 500 <= (long long)((a.D + NT - 1) / NT) * C * 150) {
 #pragma unroll 1
-        for (int d = wave; d < a.D; d += NT / 64) {
+        for (int d = wave; d < a.D; d += NW) {
             const unsigned long long target = target_of(d == wave ? u_wave : u[d], mass);
             int owner = 0;                                     // number of threads that end at or below the target
 #pragma unroll
-            for (int k = 0; k < NT / 64; k++) owner += __popcll(__ballot(s.ends[k * 64 + lane] <= target));
-            const unsigned long long ahead = owner > 0 ? s.ends[owner - 1] : 0ull;
-            unsigned long long m[(BYTES / (int)sizeof(T) / NT + 63) / 64], run = ahead;
-            double w;
-#pragma unroll
-            for (int k = 0; k < (int)(sizeof(m) / sizeof(m[0])); k++) {
-                const int j = k * 64 + lane;
-                m[k] = j < C ? mass_of_sample(owner * C + j, w) : 0ull;
-                const unsigned long long inc = wave_scan(m[k], 0ull, Add());
-                if (target - (run + inc - m[k]) < m[k]) answer(d, owner * C + j, w);
-                run += lane_value(inc, 63);
-            }
+            for (int k = 0; k < NW; k++) owner += __popcll(__ballot(ends[k * 64 + lane] <= target));
+            const unsigned long long ahead = owner > 0 ? ends[owner - 1] : 0ull;
+            double w = 0.0;
+            const unsigned long long m = lane < C ? mass_of_sample(owner * C + lane, w) : 0ull;      // C <= 64
+            const unsigned long long at = ahead + wave_scan(m, 0ull, Add()) - m;
+            if (target - at < m) answer(d, owner * C + lane, w);
         }
     } else {
 #pragma unroll 1
@@ -862,9 +612,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             int lo = 0, hi = NT - 1;                           // the first thread that ends above the target
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                if (s.ends[mid] > target) hi = mid; else lo = mid + 1;
+                if (ends[mid] > target) hi = mid; else lo = mid + 1;
             }
-            unsigned long long c = lo > 0 ? s.ends[lo - 1] : 0ull;
+            unsigned long long c = lo > 0 ? ends[lo - 1] : 0ull;
 #pragma unroll 1
             for (int i = lo * C; i < (lo + 1) * C; i++) {
                 double w;
@@ -876,24 +626,596 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// longer rows: a workgroup for every chunk of CHUNK samples, five launches
+// ------------------------------------------------------------------------------------------
+//   chunk_best    highest, lowest and summed weight of every chunk; clears what the next ones add to
+//   chunk_bins    counts and masses over bins linear in best - v, a histogram per row
+//   chunk_split   the bins in which the borders can lie follow from the histogram: mass of what lies before them by chunk, and a
+//                 list of the samples in them
+//   row_border    the borders among the listed samples; their masses join those of their chunks
+//   long_draw     for every draw: the chunk, then the sample
+// Rows without top-k and top-p need no list: chunk_split and row_border leave their chunks' masses as chunk_bins wrote them.
+constexpr int LT = 512, CHUNK = 8192, HELD = CHUNK / LT, LONG_BINS = 1024, BT = 1024;
+
+template <class V> struct LongRow {                  // what is known of a row (written by its first workgroup of chunk_bins)
+    Weights<V> w;
+    V border;                                        // kept: above the border, or equal to it with an index up to last
+    unsigned last, listed;
+    int state;                                       // 0: nothing to draw, 1: every sample that takes part is kept, 2: borders
+};
+template <class V> struct LongArea {                 // the workspace, of all rows
+    V *best, *worst;                                 // [rows][chunks]
+    double* sum;
+    unsigned long long *kept, *mass;                 // [rows][chunks] mass of a chunk, [rows][LONG_BINS]
+    unsigned* cnt;
+    LongRow<V>* row;
+    V* list_v;                                       // [rows][K]
+    unsigned* list_i;
+    int chunks;
+    static size_t carve(LongArea* a, char* p, size_t rows, size_t K) {
+        const size_t chunks = (K + CHUNK - 1) / CHUNK;
+        size_t at = 0;
+        auto take = [&](size_t bytes) { char* r = p + at; at += (bytes + 255) & ~(size_t)255; return r; };
+        LongArea local;
+        if (!a) a = &local;
+        a->best = (V*)take(rows * chunks * sizeof(V));
+        a->worst = (V*)take(rows * chunks * sizeof(V));
+        a->sum = (double*)take(rows * chunks * 8);
+        a->kept = (unsigned long long*)take(rows * chunks * 8);
+        a->mass = (unsigned long long*)take(rows * LONG_BINS * 8);
+        a->cnt = (unsigned*)take(rows * LONG_BINS * 4);
+        a->row = (LongRow<V>*)take(rows * sizeof(LongRow<V>));
+        a->list_v = (V*)take(rows * K * sizeof(V));
+        a->list_i = (unsigned*)take(rows * K * 4);
+        a->chunks = (int)chunks;
+        return at;
+    }
+};
+
+// the chunk of this workgroup, HELD samples per thread, in pieces of VEC neighbours
+template <class T> struct Chunk {
+    using V = typename Traits<T>::V;
+    static constexpr int VEC = 16 / sizeof(T), PIECES = HELD / VEC;
+    V x[PIECES][VEC];
+    int first;                                       // index of x[0][0]
+    __device__ __forceinline__ int index(int p, int j) const { return first + p * LT * VEC + j; }
+    __device__ __forceinline__ void load(const DrawArgs& a, long long row, int chunk) {
+        const T* R = (const T*)a.R + row * a.row_stride;
+        T raw[PIECES][VEC];
+        first = chunk * CHUNK + (int)threadIdx.x * VEC;
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) load_piece(R, a.col_stride, index(p, 0), a.K, raw[p]);
+#pragma unroll
+        for (int p = 0; p < PIECES; p++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                x[p][j] = value_of(raw[p][j]);
+                x[p][j] = isfinite(x[p][j]) ? x[p][j] : (V)-INFINITY;
+            }
+    }
+    __device__ __forceinline__ unsigned live(int p, V low) const {
+        unsigned bits = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) bits |= x[p][j] >= low ? 1u << j : 0u;
+        return bits;
+    }
+};
+
+__device__ __forceinline__ bool wants_border(const Param& par, int K) { return (par.top_k > 0 && par.top_k < K) || !(par.top_p >= 1.0); }
+
+template <class T> __global__ void __launch_bounds__(LT) chunk_best_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    using V = typename Traits<T>::V;
+    __shared__ unsigned long long s_tot[LT / 64];
+    const long long row = blockIdx.x / l.chunks;
+    const int chunk = (int)(blockIdx.x - row * l.chunks);
+    Chunk<T> c;
+    c.load(a, row, chunk);
+    const Param par(a.f, row);
+    for (int i = chunk * LT + (int)threadIdx.x; i < LONG_BINS; i += l.chunks * LT) {
+        l.mass[row * LONG_BINS + i] = 0;
+        l.cnt[row * LONG_BINS + i] = 0;
+    }
+    if (chunk == 0 && threadIdx.x == 0) l.row[row].listed = 0;
+    V best = (V)-INFINITY, worst = (V)INFINITY;
+#pragma unroll
+    for (int p = 0; p < c.PIECES; p++)
+#pragma unroll
+        for (int j = 0; j < c.VEC; j++) {
+            const V v = c.x[p][j];
+            best = v > best ? v : best;
+            worst = v > (V)-INFINITY && v < worst ? v : worst;
+        }
+    best = group_reduce<LT>(best, (V)-INFINITY, (V*)s_tot, Max());
+    worst = group_reduce<LT>(worst, (V)INFINITY, (V*)s_tot, Min());
+    double sum = 0.0;
+    if (par.valid() && best > (V)-INFINITY) {
+        Weights<V> w;
+        w.set(par.kappa, best, worst, 51);
+#pragma unroll
+        for (int p = 0; p < c.PIECES; p++)
+#pragma unroll
+            for (int j = 0; j < c.VEC; j++) sum += c.x[p][j] >= w.from ? w.weight(c.x[p][j]) : 0.0;
+    }
+    sum = group_reduce<LT>(sum, 0.0, (double*)s_tot, Add());
+    if (threadIdx.x == 0) {
+        l.best[blockIdx.x] = best;
+        l.worst[blockIdx.x] = worst;
+        l.sum[blockIdx.x] = sum;
+    }
+}
+
+// bins of a long row
+template <class V> struct LongBins {
+    V best, per;
+    __device__ LongBins(const Weights<V>& w) : best(w.best), per(w.best > w.from ? (V)LONG_BINS / (w.best - w.from) : (V)0) {}
+    __device__ __forceinline__ int of(V v) const {
+        const int b = (int)((best - v) * per);
+        return b < LONG_BINS ? b : LONG_BINS - 1;
+    }
+};
+
+template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    using V = typename Traits<T>::V;
+    __shared__ unsigned long long s_tot[LT / 64], s_mass[LONG_BINS];
+    __shared__ unsigned s_cnt[LONG_BINS];
+    const long long row = blockIdx.x / l.chunks;
+    const int chunk = (int)(blockIdx.x - row * l.chunks);
+    Chunk<T> c;
+    c.load(a, row, chunk);
+    const Param par(a.f, row);
+    // the row's best, worst and mass from those of its chunks
+    V best = (V)-INFINITY, worst = (V)INFINITY;
+    for (int i = threadIdx.x; i < l.chunks; i += LT) {
+        const V b = l.best[row * l.chunks + i], w = l.worst[row * l.chunks + i];
+        best = b > best ? b : best;
+        worst = w < worst ? w : worst;
+    }
+    best = group_reduce<LT>(best, (V)-INFINITY, (V*)s_tot, Max());
+    worst = group_reduce<LT>(worst, (V)INFINITY, (V*)s_tot, Min());
+    const bool some = par.valid() && best > (V)-INFINITY;
+    Weights<V> w;
+    int state = 0;
+    if (some) {
+        w.set(par.kappa, best, worst, 51);
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < l.chunks; i += LT) {
+            const V b = l.best[row * l.chunks + i];
+            if (b >= w.from) sum += l.sum[row * l.chunks + i] * w.weight(b);
+        }
+        sum = group_reduce<LT>(sum, 0.0, (double*)s_tot, Add());
+        int e;
+        (void)frexp(sum, &e);                         // sum < 2^e
+        const int S = 62 - e < 51 ? 62 - e : 51;
+        w.set(par.kappa, best, worst, S);
+        state = wants_border(par, a.K) ? 2 : 1;
+    }
+    if (chunk == 0 && threadIdx.x == 0) {
+        LongRow<V>& r = l.row[row];
+        r.w = w;
+        r.border = w.from;
+        r.last = UINT_MAX;
+        r.state = state;
+    }
+    if (state == 2) {
+        for (int i = threadIdx.x; i < LONG_BINS; i += LT) { s_cnt[i] = 0; s_mass[i] = 0; }
+        __syncthreads();
+    }
+    const LongBins<V> bins(w);
+    unsigned long long kept = 0;
+    if (state != 0) {
+#pragma unroll
+        for (int p = 0; p < c.PIECES; p++) {
+            const unsigned live = c.live(p, w.from);
+            if (live) {
+                unsigned long long q[c.VEC];
+                w.masses(c.x[p], live, state == 1 ? par.min_p : 0.0, q);
+#pragma unroll
+                for (int j = 0; j < c.VEC; j++) {
+                    kept += q[j];
+                    if (state == 2 && (live >> j & 1u)) {
+                        const int b = bins.of(c.x[p][j]);
+                        atomicAdd(&s_cnt[b], 1u);
+                        atomicAdd(&s_mass[b], q[j]);
+                    }
+                }
+            }
+        }
+    }
+    if (state != 2) {
+        kept = group_reduce<LT>(kept, 0ull, s_tot, Add());
+        if (threadIdx.x == 0) l.kept[blockIdx.x] = kept;
+        return;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < LONG_BINS; i += LT)
+        if (s_cnt[i]) {
+            atomicAdd(&l.cnt[row * LONG_BINS + i], s_cnt[i]);
+            atomicAdd(&l.mass[row * LONG_BINS + i], s_mass[i]);
+        }
+}
+
+// Where the borders can lie: the count border in bin k (-1: none) with so many samples and so much mass before it, the mass border in
+// bins p_first ... p_last (none: p_first > p_last)
+struct Where {
+    int k, p_first, p_last;
+    unsigned k_before;
+    unsigned long long k_mass_before, mass_before;   // mass_before: before p_first
+    bool nothing;
+};
+template <int NT> struct WhereArea {
+    unsigned long long tot[NT / 64], total, k_mass_before, k_mass, p_before;
+    unsigned utot[NT / 64], k_before;
+    int k, first, last;
+};
+// whole number above the mass that lies before what top-p keeps
+__device__ __forceinline__ unsigned long long share_of(double share, unsigned long long mass) {
+    const double want = ceil(share * (double)mass);
+    return want >= 1.0 ? (want < (double)mass ? (unsigned long long)want : mass) : 0ull;
+}
+template <int NT> __device__ Where where(const Param& par, int K, const unsigned* cnt, const unsigned long long* mass, WhereArea<NT>& s) {
+    constexpr int PER = LONG_BINS / NT;
+    unsigned c[PER], csum = 0, ctotal;
+    unsigned long long m[PER], msum = 0, mtotal;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        c[i] = cnt[threadIdx.x * PER + i];
+        m[i] = mass[threadIdx.x * PER + i];
+        csum += c[i];
+        msum += m[i];
+    }
+    const unsigned crun0 = group_scan<NT>(csum, s.utot, ctotal);
+    const unsigned long long mrun0 = group_scan<NT>(msum, s.tot, mtotal);
+    Where r;
+    r.k = -1;
+    r.p_first = 1; r.p_last = 0;
+    r.k_before = 0;
+    r.k_mass_before = r.mass_before = 0;
+    r.nothing = false;
+    unsigned long long least = mtotal, most = mtotal;          // bounds of the mass that top-k keeps
+    if (par.top_k > 0 && par.top_k < K && (unsigned long long)par.top_k <= ctotal) {
+        const unsigned k = (unsigned)par.top_k;
+        unsigned crun = crun0;
+        unsigned long long mrun = mrun0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if (crun < k && k <= crun + c[i]) { s.k = threadIdx.x * PER + i; s.k_before = crun; s.k_mass_before = mrun; s.k_mass = m[i]; }
+            crun += c[i];
+            mrun += m[i];
+        }
+        __syncthreads();
+        r.k = s.k;
+        r.k_before = s.k_before;
+        r.k_mass_before = least = s.k_mass_before;
+        most = least + s.k_mass;
+    }
+    if (!(par.top_p >= 1.0)) {
+        const unsigned long long to = share_of(par.top_p, most);
+        unsigned long long from = share_of(par.top_p, least);
+        if (to == 0) { r.nothing = true; return r; }
+        from = from > 0 ? from : 1;
+        unsigned long long mrun = mrun0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if (mrun < from && from <= mrun + m[i]) { s.first = threadIdx.x * PER + i; s.p_before = mrun; }
+            if (mrun < to && to <= mrun + m[i]) s.last = threadIdx.x * PER + i;
+            mrun += m[i];
+        }
+        __syncthreads();
+        r.p_first = s.first;
+        r.p_last = s.last;
+        r.mass_before = s.p_before;
+    }
+    return r;
+}
+
+template <class T> __global__ void __launch_bounds__(LT) chunk_split_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    using V = typename Traits<T>::V;
+    __shared__ WhereArea<LT> s;
+    __shared__ unsigned s_listed, s_at;
+    const long long row = blockIdx.x / l.chunks;
+    const int chunk = (int)(blockIdx.x - row * l.chunks);
+    if (l.row[row].state != 2) return;
+    Chunk<T> c;
+    c.load(a, row, chunk);
+    const Param par(a.f, row);
+    const Weights<V> w = l.row[row].w;
+    const LongBins<V> bins(w);
+    if (threadIdx.x == 0) s_listed = 0;
+    const Where at = where<LT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, s);
+    // before `first` everything is kept; with neither border (top-k of more samples than there are) that is all of it
+    const int first = at.nothing ? 0 : at.p_first <= at.p_last ? at.p_first : at.k >= 0 ? at.k : LONG_BINS;
+    unsigned long long kept = 0;
+    unsigned mine = 0;
+    unsigned hits[c.PIECES];
+#pragma unroll
+    for (int p = 0; p < c.PIECES; p++) {
+        hits[p] = 0;
+        const unsigned live = at.nothing ? 0u : c.live(p, w.from);
+        if (live) {
+            unsigned sure = 0;
+#pragma unroll
+            for (int j = 0; j < c.VEC; j++) {
+                const int b = bins.of(c.x[p][j]);
+                const unsigned bit = live & 1u << j;
+                sure |= b < first ? bit : 0u;
+                hits[p] |= (b >= at.p_first && b <= at.p_last) || b == at.k ? bit : 0u;
+            }
+            mine += (unsigned)__popc(hits[p]);
+            if (sure) {
+                unsigned long long q[c.VEC];
+                w.masses(c.x[p], sure, par.min_p, q);
+#pragma unroll
+                for (int j = 0; j < c.VEC; j++) kept += q[j];
+            }
+        }
+    }
+    __syncthreads();                                  // (s_listed)
+    unsigned to = mine ? atomicAdd(&s_listed, mine) : 0u;
+    kept = group_reduce<LT>(kept, 0ull, s.tot, Add());
+    if (threadIdx.x == 0) {
+        l.kept[blockIdx.x] = kept;
+        s_at = s_listed ? atomicAdd(&l.row[row].listed, s_listed) : 0u;
+    }
+    __syncthreads();
+    to += s_at;
+    if (mine) {
+#pragma unroll
+        for (int p = 0; p < c.PIECES; p++)
+#pragma unroll
+            for (int j = 0; j < c.VEC; j++)
+                if (hits[p] >> j & 1u) {
+                    l.list_v[row * a.K + to] = c.x[p][j];
+                    l.list_i[row * a.K + to] = (unsigned)c.index(p, j);
+                    to++;
+                }
+    }
+}
+
+// The listed samples of a row as a source of find_border.  BY_INDEX: only those equal to `only`, ordered by their index alone (an index
+// below 2^24 is exact as a float).
+template <class V, bool BY_INDEX> struct Listed {
+    static constexpr int VEC = 4;
+    const V* v;
+    const unsigned* i;
+    unsigned n;
+    V only;
+    Weights<V> w;
+    __device__ __forceinline__ V value(int e, int j) const { return BY_INDEX ? -(V)i[e + j * BT] : v[e + j * BT]; }
+    __device__ __forceinline__ unsigned index(int e, int j) const { return i[e + j * BT]; }
+    template <class F> __device__ __forceinline__ void each(V low, V high, F f) {
+#pragma unroll 1
+        for (unsigned e = threadIdx.x; e < n; e += BT * VEC) {
+            V x[VEC];
+            unsigned live = 0;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const unsigned at = e + j * BT < n ? e + j * BT : e;
+                x[j] = v[at];
+                const bool in = e + j * BT < n && (!BY_INDEX || x[j] == only);
+                if (BY_INDEX) x[j] = -(V)i[at];
+                live |= in && x[j] >= low && x[j] <= high ? 1u << j : 0u;
+            }
+            if (live) f(x, live, (int)e);
+        }
+    }
+};
+
+template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    using V = typename Traits<T>::V;
+    __shared__ BorderArea<V, BT> s;
+    __shared__ WhereArea<BT> sw;
+    const long long row = blockIdx.x;
+    LongRow<V>& r = l.row[row];
+    if (r.state != 2) return;
+    const Param par(a.f, row);
+    const Where at = where<BT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, sw);
+    if (at.nothing) {
+        __syncthreads();
+        if (threadIdx.x == 0) r.state = 0;
+        return;
+    }
+    if (at.k < 0 && at.p_first > at.p_last) return;  // all of them are kept
+    const Weights<V> w = r.w;
+    const LongBins<V> bins(w);
+    Listed<V, false> list{l.list_v + row * a.K, l.list_i + row * a.K, r.listed, (V)0, w};
+    // values of the listed samples in bins first ... last
+    auto range = [&](int first, int last, V low, V& lo, V& hi) {
+        V least = (V)INFINITY, most = (V)-INFINITY;
+        list.each(low, w.best, [&](const V (&x)[4], unsigned live, int) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int b = bins.of(x[j]);
+                if ((live >> j & 1u) && b >= first && b <= last) { least = x[j] < least ? x[j] : least; most = x[j] > most ? x[j] : most; }
+            }
+        });
+        lo = group_reduce<BT>(least, (V)INFINITY, (V*)s.tot, Min());
+        hi = group_reduce<BT>(most, (V)-INFINITY, (V*)s.tot, Max());
+    };
+    V border = w.from, lo, hi;
+    unsigned keep = 0, all = 0, last = UINT_MAX;
+    auto found = [&]() { border = s.border; keep = s.border_keep; all = s.border_all; last = s.border_idx; __syncthreads(); };
+    unsigned long long mass = 0;                      // of what top-k keeps, where top-p asks
+    const bool share = at.p_first <= at.p_last;
+    if (at.k >= 0) {
+        range(at.k, at.k, w.from, lo, hi);
+        (void)find_border<BY_COUNT>(list, s, (unsigned long long)par.top_k - at.k_before, 0.0, lo, hi);
+        found();
+        if (share) {
+            unsigned long long sum = 0;
+            list.each(border, hi, [&](const V (&x)[4], unsigned live, int) {
+                unsigned above = 0;
+                unsigned long long q[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) above |= x[j] > border ? live & 1u << j : 0u;
+                w.masses(x, above, 0.0, q);
+#pragma unroll
+                for (int j = 0; j < 4; j++) sum += q[j];
+            });
+            mass = at.k_mass_before + group_reduce<BT>(sum, 0ull, s.tot, Add()) + keep * w.mass_of(border);
+        }
+    } else {
+        unsigned long long m = 0;
+        for (int i = threadIdx.x; i < LONG_BINS; i += BT) m += l.mass[row * LONG_BINS + i];
+        mass = group_reduce<BT>(m, 0ull, s.tot, Add());
+    }
+    if (share) {
+        const unsigned long long target = share_of(par.top_p, mass);
+        if (target == 0) {
+            if (threadIdx.x == 0) r.state = 0;
+            return;
+        }
+        range(at.p_first, at.p_last, border, lo, hi);
+        if (find_border<BY_MASS>(list, s, target - at.mass_before, 0.0, lo, hi)) found();
+    }
+    if (keep >= all) {
+        last = UINT_MAX;
+    } else if (last == UINT_MAX) {
+        // more equal ones than a list of candidates holds: the keep-th of them by index
+        Listed<V, true> equal{list.v, list.i, list.n, border, w};
+        (void)find_border<BY_COUNT>(equal, s, keep, 0.0, -(V)a.K, (V)0);
+        last = s.border_idx;
+    }
+    if (threadIdx.x == 0) { r.border = border; r.last = last; }
+    // what the list keeps joins the chunks
+    list.each(border, w.best, [&](const V (&x)[4], unsigned live, int e) {
+        unsigned in = 0;
+        unsigned idx[4];
+        unsigned long long q[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            idx[j] = live >> j & 1u ? list.index(e, j) : 0u;
+            in |= x[j] > border || idx[j] <= last ? live & 1u << j : 0u;
+        }
+        w.masses(x, in, par.min_p, q);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (q[j]) atomicAdd(&l.kept[row * l.chunks + idx[j] / CHUNK], q[j]);
+    });
+}
+
+template <class T> __global__ void __launch_bounds__(LT) long_draw_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    using V = typename Traits<T>::V;
+    __shared__ unsigned long long s_tot[LT / 64], s_ends[Chunk<T>::PIECES * LT / 64], s_before;
+    __shared__ int s_chunk;
+    const long long row = blockIdx.x / a.D;
+    const long long at = blockIdx.x;
+    const LongRow<V>& r = l.row[row];
+    const Param par(a.f, row);
+    unsigned long long mass = 0, target = 0;
+    if (r.state != 0) {
+        // the chunk: each thread sums PER neighbours
+        const int PER = (l.chunks + LT - 1) / LT;
+        unsigned long long sum = 0;
+        for (int i = 0; i < PER; i++) {
+            const int c = (int)threadIdx.x * PER + i;
+            sum += c < l.chunks ? l.kept[row * l.chunks + c] : 0ull;
+        }
+        unsigned long long run = group_scan<LT>(sum, s_tot, mass);
+        if (mass != 0) {
+            target = target_of(a.u[at], mass);
+            if (target - run < sum)
+                for (int i = 0; i < PER; i++) {
+                    const int c = (int)threadIdx.x * PER + i;
+                    const unsigned long long m = c < l.chunks ? l.kept[row * l.chunks + c] : 0ull;
+                    if (target - run < m) { s_chunk = c; s_before = run; }
+                    run += m;
+                }
+        }
+    }
+    if (mass == 0) {
+        if (threadIdx.x == 0) { a.index[at] = -1; if (a.weight) a.weight[at] = 0.0f; }
+        return;
+    }
+    __syncthreads();
+    const Weights<V> w = r.w;
+    const V border = r.border;
+    const unsigned last = r.last;
+    Chunk<T> c;
+    c.load(a, row, s_chunk);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    unsigned long long q[c.PIECES][c.VEC], base[c.PIECES], sum[c.PIECES];
+#pragma unroll
+    for (int p = 0; p < c.PIECES; p++) {
+        unsigned live = 0;
+#pragma unroll
+        for (int j = 0; j < c.VEC; j++) {
+            const V v = c.x[p][j];
+            live |= v > border || (v == border && (unsigned)c.index(p, j) <= last) ? 1u << j : 0u;
+        }
+        sum[p] = 0;
+        w.masses(c.x[p], live, par.min_p, q[p]);
+#pragma unroll
+        for (int j = 0; j < c.VEC; j++) sum[p] += q[p][j];
+        const unsigned long long inc = wave_scan(sum[p], 0ull, Add());
+        base[p] = inc - sum[p];
+        if (lane == 63) s_ends[p * (LT / 64) + wave] = inc;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < c.PIECES; p++) {
+        unsigned long long run = s_before + base[p];
+        for (int k = 0; k < p * (LT / 64) + wave; k++) run += s_ends[k];
+        if (target - run < sum[p]) {
+#pragma unroll
+            for (int j = 0; j < c.VEC; j++) {
+                if (target - run < q[p][j]) {
+                    a.index[at] = c.index(p, j);
+                    if (a.weight) a.weight[at] = (float)(w.weight(c.x[p][j]) * w.scale / (double)mass);
+                }
+                run += q[p][j];
+            }
+        }
+    }
+}
+
 int ceil_log2(int n) {
     int e = 0;
     while ((1ll << e) < n) e++;
     return e;
 }
 
-template <class T> hipError_t launch(const DrawArgs& a, hipStream_t s) {
-    const int S = 62 - ceil_log2(a.K);
-    const size_t bytes = (size_t)a.K * sizeof(T);
-    if (a.K <= 512)
-        hipLaunchKernelGGL((draw_row_kernel<T, 64, 512 * sizeof(T)>), dim3(a.rows), dim3(64), 0, s, a, S);
-    else if (a.K <= 4096)
-        hipLaunchKernelGGL((draw_row_kernel<T, 256, 4096 * sizeof(T)>), dim3(a.rows), dim3(256), 0, s, a, S);
-    else if (bytes <= 131072)
-        hipLaunchKernelGGL((draw_row_kernel<T, 1024, 131072>), dim3(a.rows), dim3(1024), 0, s, a, S);
-    else
-        hipLaunchKernelGGL((draw_rows_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a);
-    return hipGetLastError();
+constexpr size_t SHELF = 131072;                     // bytes of the longest row that one workgroup holds in LDS
+
+template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+    using V = typename Traits<T>::V;
+    if ((size_t)a.K * sizeof(T) <= SHELF) {
+        // K units of half 2^-S at most in error, and sums below 2^62
+        const int S = std::min(51, 62 - ceil_log2(a.K));
+        if (a.K <= 512)
+            hipLaunchKernelGGL((draw_row_kernel<T, 64, 512 * sizeof(T)>), dim3(a.rows), dim3(64), 0, s, a, S);
+        else if (a.K <= 4096)
+            hipLaunchKernelGGL((draw_row_kernel<T, 256, 4096 * sizeof(T)>), dim3(a.rows), dim3(256), 0, s, a, S);
+        else
+            hipLaunchKernelGGL((draw_row_kernel<T, 1024, SHELF>), dim3(a.rows), dim3(1024), 0, s, a, S);
+        HIP_OK(hipGetLastError());
+        return 0;
+    }
+    LongArea<V> l;
+    if (!workspace || workspace_bytes < LongArea<V>::carve(&l, (char*)workspace, a.rows, a.K))
+        return fail(-1, "workspace too small (mppi_draw_workspace)");
+    if ((long long)a.rows * l.chunks > INT_MAX || (long long)a.rows * a.D > INT_MAX)
+        return fail(-6, "more than 2^31 - 1 chunks or draws in one call of long rows");
+    const dim3 chunks((unsigned)(a.rows * l.chunks));
+    hipLaunchKernelGGL((chunk_best_kernel<T>), chunks, dim3(LT), 0, s, a, l);
+    HIP_OK(hipGetLastError());
+    hipLaunchKernelGGL((chunk_bins_kernel<T>), chunks, dim3(LT), 0, s, a, l);
+    HIP_OK(hipGetLastError());
+    if (a.f.top_k_of || a.f.top_p_of || (a.f.top_k > 0 && a.f.top_k < a.K) || a.f.top_p < 1.0) {
+        hipLaunchKernelGGL((chunk_split_kernel<T>), chunks, dim3(LT), 0, s, a, l);
+        HIP_OK(hipGetLastError());
+        hipLaunchKernelGGL((row_border_kernel<T>), dim3(a.rows), dim3(BT), 0, s, a, l);
+        HIP_OK(hipGetLastError());
+    }
+    hipLaunchKernelGGL((long_draw_kernel<T>), dim3((unsigned)(a.rows * a.D)), dim3(LT), 0, s, a, l);
+    HIP_OK(hipGetLastError());
+    return 0;
+}
+
+size_t workspace_of(int dtype, size_t rows, size_t K) {
+    const size_t size = dtype == MPPI_F64 ? 8 : dtype == MPPI_F32 ? 4 : 2;
+    if (K * size <= SHELF) return 0;
+    return dtype == MPPI_F64 ? LongArea<double>::carve(nullptr, nullptr, rows, K) : LongArea<float>::carve(nullptr, nullptr, rows, K);
 }
 
 int check_filter(const mppi_draw_filter* f) {
@@ -908,9 +1230,20 @@ int check_filter(const mppi_draw_filter* f) {
 
 extern "C" {
 
+int mppi_draw_workspace(int32_t dtype, int32_t rows, int32_t K, size_t* bytes) try {
+    if (!bytes) return fail(-1, "null argument");
+    if (rows < 0 || K < 1) return fail(-1, "rows must not be negative, K must be positive");
+    if (dtype < MPPI_F32 || dtype > MPPI_BF16) return fail(-1, "dtype must be MPPI_F32, MPPI_F64, MPPI_F16 or MPPI_BF16");
+    if (K > MPPI_DRAW_MAX_K) return fail(-6, "K = " + std::to_string(K) + " exceeds " + std::to_string(MPPI_DRAW_MAX_K) + " samples");
+    *bytes = workspace_of(dtype, (size_t)rows, (size_t)K);
+    return 0;
+} catch (const std::exception& e) {
+    return fail(-8, std::string("host exception: ") + e.what());
+}
+
 int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32_t rows, int32_t K, int64_t row_stride,
                            int64_t col_stride, const double* d_u, int32_t D, const mppi_draw_filter* filter, int64_t* d_index,
-                           float* d_weight, void* stream) try {
+                           float* d_weight, void* d_workspace, size_t workspace_bytes, void* stream) try {
     if (!filter) return fail(-1, "null argument");
     if (rows < 0 || K < 1 || D < 0) return fail(-1, "rows and D must not be negative, K must be positive");
     if (K > MPPI_DRAW_MAX_K)
@@ -921,6 +1254,8 @@ int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32
     if (rc) return rc;
     if (rows == 0 || D == 0) return 0;
     if (!d_R || !d_u || !d_index) return fail(-1, "null argument");
+    if (workspace_bytes < workspace_of(dtype, (size_t)rows, (size_t)K) || ((uintptr_t)d_workspace & 255))
+        return fail(-1, "workspace too small (mppi_draw_workspace) or not aligned to 256 bytes");
     mppi::DeviceGuard guard;
     HIP_OK(guard.enter(device));
     DrawArgs a;
@@ -930,12 +1265,11 @@ int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32
     a.index = (long long*)d_index; a.weight = d_weight;
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
-    case MPPI_F32: HIP_OK(launch<float>(a, s)); break;
-    case MPPI_F64: HIP_OK(launch<double>(a, s)); break;
-    case MPPI_F16: HIP_OK(launch<Half>(a, s)); break;
-    default: HIP_OK(launch<Bfloat>(a, s)); break;
+    case MPPI_F32: return launch<float>(a, d_workspace, workspace_bytes, s);
+    case MPPI_F64: return launch<double>(a, d_workspace, workspace_bytes, s);
+    case MPPI_F16: return launch<Half>(a, d_workspace, workspace_bytes, s);
+    default: return launch<Bfloat>(a, d_workspace, workspace_bytes, s);
     }
-    return 0;
 } catch (const std::exception& e) {
     return fail(-8, std::string("host exception: ") + e.what());
 }

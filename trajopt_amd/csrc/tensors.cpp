@@ -15,6 +15,7 @@
 namespace {
 
 decltype(&mppi_last_error) last_error;
+decltype(&mppi_draw_workspace) draw_workspace;
 decltype(&mppi_draw_from_returns) draw_from_returns;
 decltype(&mppi_gradient_workspace) gradient_workspace;
 decltype(&mppi_gradient_norm) gradient_norm;
@@ -114,9 +115,13 @@ PyObject* draw(PyObject* const* args) {
     if (u.scalar_type() != at::kDouble || !u.is_contiguous()) u64 = u.detach().to(at::kDouble).contiguous();
     at::Tensor index = at::empty(u.sizes(), at::TensorOptions().dtype(at::kLong).device(device));
     at::Tensor weight = at::empty(u.sizes(), at::TensorOptions().dtype(at::kFloat).device(device));
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (rows > 0 && K > 0 && D > 0) check(draw_workspace(type, (int32_t)rows, (int32_t)K, &bytes));
+    if (bytes) ws = at::empty({(int64_t)(bytes + 7) / 8}, at::TensorOptions().dtype(at::kDouble).device(device));
     check(draw_from_returns(device.index(), R.const_data_ptr(), type, (int32_t)rows, (int32_t)K, one ? 0 : R.stride(0), R.stride(one ? 0 : 1),
                             (const double*)u64.const_data_ptr(), (int32_t)D, &f, (int64_t*)index.mutable_data_ptr(),
-                            (float*)weight.mutable_data_ptr(), stream_of(device)));
+                            (float*)weight.mutable_data_ptr(), bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(device)));
     PyObject* out = PyTuple_New(2);
     if (!out) throw Raised();
     PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(index)));
@@ -195,10 +200,11 @@ PyObject* gradients(PyObject* const* args) {
     return THPVariable_Wrap(std::move(norm));
 }
 
-// bind(MppiError, address of mppi_last_error, ..._draw_from_returns, ..._gradient_workspace, ..._gradient_norm, ..._clip_gradients)
+// bind(MppiError, addresses of mppi_last_error, ..._draw_workspace, ..._draw_from_returns, ..._gradient_workspace, ..._gradient_norm,
+// ..._clip_gradients)
 PyObject* bind(PyObject* const* args) {
-    void* address[5];
-    for (int i = 0; i < 5; i++) {
+    void* address[6];
+    for (int i = 0; i < 6; i++) {
         address[i] = PyLong_AsVoidPtr(args[1 + i]);
         if (!address[i]) raise(PyExc_ValueError, "null function address");
     }
@@ -206,10 +212,11 @@ PyObject* bind(PyObject* const* args) {
     Py_XDECREF(library_error);
     library_error = args[0];
     last_error = (decltype(last_error))address[0];
-    draw_from_returns = (decltype(draw_from_returns))address[1];
-    gradient_workspace = (decltype(gradient_workspace))address[2];
-    gradient_norm = (decltype(gradient_norm))address[3];
-    clip_gradients = (decltype(clip_gradients))address[4];
+    draw_workspace = (decltype(draw_workspace))address[1];
+    draw_from_returns = (decltype(draw_from_returns))address[2];
+    gradient_workspace = (decltype(gradient_workspace))address[3];
+    gradient_norm = (decltype(gradient_norm))address[4];
+    clip_gradients = (decltype(clip_gradients))address[5];
     Py_RETURN_NONE;
 }
 
@@ -226,7 +233,7 @@ template <PyObject* (*F)(PyObject* const*), int N> PyObject* entry(PyObject*, Py
 }
 
 PyMethodDef methods[] = {
-    {"bind", (PyCFunction)(void (*)())&entry<bind, 6>, METH_FASTCALL, nullptr},
+    {"bind", (PyCFunction)(void (*)())&entry<bind, 7>, METH_FASTCALL, nullptr},
     {"draw", (PyCFunction)(void (*)())&entry<draw, 6>, METH_FASTCALL, nullptr},
     {"gradients", (PyCFunction)(void (*)())&entry<gradients, 4>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
