@@ -144,26 +144,27 @@ __device__ __forceinline__ unsigned long long target_of(double u, unsigned long 
 // ------------------------------------------------------------------------------------------
 // weights and masses of one row
 // ------------------------------------------------------------------------------------------
-// exp(-d) for 0 <= d < 700: 2^n e^r with r = -d - n ln 2, |r| <= ln 2 / 2, and the series of e^r up to r^12 / 12!, whose next term
-// is below 2^-52.  ln 2 is split into a part of 32 bits, whose product with n is exact, and the rest.
-__device__ __forceinline__ double exp_minus(double d) {
-    const double n = rint(d * -1.4426950408889634);
-    double r = fma(n, -6.9314718036912382e-01, -d);
-    r = fma(n, -1.9082149292705877e-10, r);
-    double p = 1.0 / 479001600.0;
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n);
+// w[j] = exp(-d[j]) for 0 <= d < 700: 2^n e^r with r = -d - n ln 2, |r| <= ln 2 / 2 (ln 2 split into a part of 32 bits, whose product
+// with n is exact, and the rest, as Cody and Waite do it), and the series of e^r up to r^12 / 12!, whose next term is below 2^-52.
+// N of them side by side: one alone is a chain of dependent operations.
+template <int N> __device__ __forceinline__ void exp_minus(const double (&d)[N], double (&w)[N]) {
+    constexpr double C[13] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0,
+                              1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+    double n[N], r[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) n[j] = rint(d[j] * -1.4426950408889634);
+#pragma unroll
+    for (int j = 0; j < N; j++) r[j] = fma(n[j], -6.9314718036912382e-01, -d[j]);
+#pragma unroll
+    for (int j = 0; j < N; j++) { r[j] = fma(n[j], -1.9082149292705877e-10, r[j]); w[j] = C[0]; }
+#pragma unroll
+    for (int i = 1; i < 13; i++) {
+#pragma unroll
+        for (int j = 0; j < N; j++) w[j] = fma(w[j], r[j], C[i]);
+        __builtin_amdgcn_sched_barrier(0);           // (the scheduler would line the chains up one behind the other)
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) w[j] = ldexp(w[j], (int)n[j]);
 }
 // x in [0, 2^51] to the nearest whole number: added to 2^52, it lies in the low bits of the sum
 __device__ __forceinline__ unsigned long long whole(double x) {
@@ -189,15 +190,21 @@ template <class V> struct Weights {
         const double d = (double)best - (double)(v > from ? v : from);
         return kappa * (sizeof(V) == 8 ? fmin(d, 1.7976931348623157e308) : d);
     }
-    __device__ __forceinline__ double weight(V v) const { return exp_minus(distance(v)); }
+    __device__ __forceinline__ double weight(V v) const {
+        const double d[1] = {distance(v)};
+        double w[1];
+        exp_minus(d, w);
+        return w[0];
+    }
     __device__ __forceinline__ unsigned long long mass_of(V v) const { return whole(weight(v) * scale); }
-    // masses of several samples side by side (their exponentials are long chains of dependent operations); live: bit j for v[j]
+    // masses of several samples, zero where bit j of live is not set or the weight is below `least`
     template <int N> __device__ __forceinline__ void masses(const V (&v)[N], unsigned live, double least, unsigned long long (&q)[N]) const {
+        double d[N], w[N];
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const double w = weight(v[j]);
-            q[j] = (live >> j & 1u) && w >= least ? whole(w * scale) : 0ull;
-        }
+        for (int j = 0; j < N; j++) d[j] = distance(v[j]);
+        exp_minus(d, w);
+#pragma unroll
+        for (int j = 0; j < N; j++) q[j] = (live >> j & 1u) && w[j] >= least ? whole(w[j] * scale) : 0ull;
 #pragma unroll
         for (int j = 0; j < N; j++) asm volatile("" : "+v"(q[j]));         // (or each would be moved behind the test of its bit)
     }
@@ -242,21 +249,12 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long t
     U top = key_of(hi);
     unsigned long long before = 0;
     unsigned n = 0;
-    auto bin_of = [&](V v) -> int {
-        if (shift >= 0) return (int)((top - key_of(v)) >> shift);
+    const auto linear = [&](V v) -> int {
         const int b = (int)((high0 - v) * per);
         return b < BINS ? b : BINS - 1;
     };
-#pragma unroll 1
-    while (true) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            s.cnt[threadIdx.x + i * NT] = 0;
-            if (MASS) s.mass[threadIdx.x + i * NT] = 0;
-        }
-        if (threadIdx.x == 0) s.n_list = 0;
-        if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
-        __syncthreads();
+    const auto keyed = [&](V v) -> int { return (int)((top - key_of(v)) >> shift); };
+    const auto fill = [&](auto bin_of) {
         src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
             unsigned long long q[VEC];
             if (MASS) src.w.masses(v, live, 0.0, q);
@@ -268,6 +266,44 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long t
                     if (MASS) atomicAdd(&s.mass[b], q[j]);
                 }
         });
+    };
+    const auto ends = [&](auto bin_of) {             // the values of the bin, from its lowest to its highest
+        V least = (V)INFINITY, most = (V)-INFINITY;
+        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if ((live >> j & 1u) && bin_of(v[j]) == bin) { least = v[j] < least ? v[j] : least; most = v[j] > most ? v[j] : most; }
+        });
+        lo = group_reduce<NT>(least, (V)INFINITY, (V*)s.tot, Min());
+        hi = group_reduce<NT>(most, (V)-INFINITY, (V*)s.tot, Max());
+    };
+    const auto gather = [&](auto bin_of) {
+        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int i) {
+            unsigned hit = 0;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
+            if (hit) {
+#pragma unroll 1
+                for (int j = 0; j < VEC; j++)
+                    if (hit >> j & 1u) {
+                        const unsigned e = atomicAdd(&s.n_list, 1u);
+                        s.list_v[e] = src.value(i, j);
+                        s.list_idx[e] = src.index(i, j);
+                    }
+            }
+        });
+    };
+#pragma unroll 1
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            s.cnt[threadIdx.x + i * NT] = 0;
+            if (MASS) s.mass[threadIdx.x + i * NT] = 0;
+        }
+        if (threadIdx.x == 0) s.n_list = 0;
+        if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
+        __syncthreads();
+        if (shift < 0) fill(linear); else fill(keyed);
         __syncthreads();
         unsigned long long own[PER], sum = 0, total;
 #pragma unroll
@@ -300,15 +336,7 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long t
         n = s.pick_n;
         before = s.pick_before;
         if (n <= LIST) break;
-        // the values of that bin, from its lowest to its highest
-        V least = (V)INFINITY, most = (V)-INFINITY;
-        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if ((live >> j & 1u) && bin_of(v[j]) == bin) { least = v[j] < least ? v[j] : least; most = v[j] > most ? v[j] : most; }
-        });
-        lo = group_reduce<NT>(least, (V)INFINITY, (V*)s.tot, Min());
-        hi = group_reduce<NT>(most, (V)-INFINITY, (V*)s.tot, Max());
+        if (shift < 0) ends(linear); else ends(keyed);
         if (lo == hi) break;
         top = key_of(hi);
         shift = 0;
@@ -323,20 +351,7 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long t
             s.border_idx = UINT_MAX;
         }
     } else {
-        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int i) {
-            unsigned hit = 0;
-#pragma unroll
-            for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
-            if (hit) {
-#pragma unroll 1
-                for (int j = 0; j < VEC; j++)
-                    if (hit >> j & 1u) {
-                        const unsigned e = atomicAdd(&s.n_list, 1u);
-                        s.list_v[e] = src.value(i, j);
-                        s.list_idx[e] = src.index(i, j);
-                    }
-            }
-        });
+        if (shift < 0) gather(linear); else gather(keyed);
         __syncthreads();
         if (MASS) {
             if (threadIdx.x < n) s.list_q[threadIdx.x] = src.w.mass_of(s.list_v[threadIdx.x]);
