@@ -101,31 +101,43 @@ struct Add { template <class X> __device__ __forceinline__ X operator()(X a, X b
 struct Max { template <class X> __device__ __forceinline__ X operator()(X a, X b) const { return a > b ? a : b; } };
 struct Min { template <class X> __device__ __forceinline__ X operator()(X a, X b) const { return a < b ? a : b; } };
 
-// over the NT threads of a workgroup; s_tot: NT / 64 values nobody else uses before the next barrier
-template <int NT, class X, class Op> __device__ __forceinline__ X group_reduce(X v, X none, X* s_tot, Op op) {
-    v = wave_scan(v, none, op);
-    if (NT == 64) return lane_value(v, 63);
-    const int lane = threadIdx.x & 63;
-    if (lane == 63) s_tot[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = wave_scan(lane < NT / 64 ? s_tot[lane] : none, none, op);       // (the lanes behind the totals add nothing)
-    __syncthreads();
-    return lane_value(v, 63);
-}
-template <int NT, class X> __device__ __forceinline__ X group_scan(X v, X* s_tot, X& total) {        // exclusive sums
-    const int wave = threadIdx.x >> 6;
-    const X inc = wave_scan(v, (X)0, Add());
-    if (NT == 64) { total = lane_value(inc, 63); return inc - v; }
-    const int lane = threadIdx.x & 63;
-    if (lane == 63) s_tot[wave] = inc;
-    __syncthreads();
-    const X own = lane < NT / 64 ? s_tot[lane] : (X)0;
-    const X tot = wave_scan(own, (X)0, Add());
-    __syncthreads();
-    total = lane_value(tot, 63);
-    return lane_value(tot - own, __builtin_amdgcn_readfirstlane(wave)) + inc - v;
-}
+// Over the NT threads of a workgroup.  Two sets of slots in LDS are used in turn, so that one barrier is enough: who writes to a set
+// again has passed the barrier of the other set, and with it everybody who had to read the first.
+template <int NT> struct Group {
+    unsigned long long* slots;                       // 2 NT / 64
+    int flip = 0;
+    __device__ Group(unsigned long long* s) : slots(s) {}
+    template <class X> __device__ __forceinline__ X* next() {
+        X* p = (X*)(slots + flip);
+        flip = NT / 64 - flip;
+        return p;
+    }
+    template <class X, class Op> __device__ __forceinline__ X reduce(X v, X none, Op op) {
+        v = wave_scan(v, none, op);
+        if (NT == 64) return lane_value(v, 63);
+        const int lane = threadIdx.x & 63;
+        X* tot = next<X>();
+        if (lane == 63) tot[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return lane_value(wave_scan(lane < NT / 64 ? tot[lane] : none, none, op), 63);      // (lanes behind the totals add nothing)
+    }
+    template <class X> __device__ __forceinline__ X scan(X v, X& total) {                   // exclusive sums
+        const X inc = wave_scan(v, (X)0, Add());
+        if (NT == 64) { total = lane_value(inc, 63); return inc - v; }
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        X* tot = next<X>();
+        if (lane == 63) tot[wave] = inc;
+        __syncthreads();
+        const X own = lane < NT / 64 ? tot[lane] : (X)0;
+        const X all = wave_scan(own, (X)0, Add());
+        total = lane_value(all, 63);
+        return lane_value(all - own, __builtin_amdgcn_readfirstlane(wave)) + inc - v;
+    }
+};
 
+// ------------------------------------------------------------------------------------------
+// parameters and targets
+// ------------------------------------------------------------------------------------------
 struct Param {
     double kappa, top_p, min_p;
     long long top_k;
@@ -141,6 +153,11 @@ __device__ __forceinline__ unsigned long long target_of(double u, unsigned long 
     return t < mass ? t : mass - 1;
 }
 
+// top-p keeps the samples with less than share W of the mass W before them: less than this whole number; 0: none is kept
+__device__ __forceinline__ unsigned long long share_of(double share, unsigned long long mass) {
+    const double want = ceil(share * (double)mass);
+    return want >= 1.0 ? (want < (double)mass ? (unsigned long long)want : mass) : 0ull;
+}
 // ------------------------------------------------------------------------------------------
 // weights and masses of one row
 // ------------------------------------------------------------------------------------------
@@ -224,33 +241,34 @@ template <class T, int VEC> __device__ __forceinline__ void load_piece(const T* 
 // the border of a prefix of the order
 // ------------------------------------------------------------------------------------------
 template <class V, int NT> struct BorderArea {
-    static constexpr int BINS = NT == 64 ? 256 : 1024, LIST = NT == 64 ? 64 : 128;
-    unsigned long long mass[BINS], tot[32], list_q[LIST], list_before[LIST], pick_before;
+    static constexpr int BINS = NT == 64 ? 256 : 1024, LIST = NT >= 1024 ? 128 : 64;
+    unsigned long long mass[BINS], slots[NT / 32], list_q[LIST], pick_before;
     V list_v[LIST], border;
-    unsigned cnt[BINS], list_idx[LIST], list_rank[LIST], list_ties[LIST], n_list, pick_bin, pick_n;
+    unsigned cnt[BINS], list_idx[LIST], n_list, pick_bin, pick_n;
     unsigned border_keep, border_all;                // of the border_all samples equal to the border, this many are kept
     unsigned border_idx;                             // the last of those that are kept; UINT_MAX: not known
 };
 
 // Among the samples of `src` in [low, high]: BY_COUNT: sample number `target` of the order.  BY_MASS: the last sample with less than
 // `target` of the mass before it.  BY_SHARE: the same with `share` (< 1) of their whole mass for a target.  False: there is no such
-// sample (too few of them; a share so small that nothing is kept, then src.from is raised to infinity).  Every thread has to call.
+// sample (too few of them; a share so small that nothing is kept, then src.from is raised to infinity).  `most`: as many samples as
+// there can be.  Every thread has to call.
 enum Aim { BY_COUNT, BY_MASS, BY_SHARE };
 template <Aim AIM, int NT, class Src, class V>
-__device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long target, double share, V low, V high) {
+__device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, unsigned long long target, double share, V low, V high, unsigned most) {
     using U = typename Traits<V>::U;
     using Area = BorderArea<V, NT>;
     constexpr bool MASS = AIM != BY_COUNT;
     constexpr int BINS = Area::BINS, PER = BINS / NT, LIST = Area::LIST, VEC = Src::VEC;
     // bins linear in high - v first (monotone: every step rounds monotonically); per = 0 where that range overflows
-    const V per = high > low ? (V)BINS / (high - low) : (V)0, high0 = high;
+    const V per = high > low ? (V)BINS / (high - low) : (V)0;
     V lo = low, hi = high;
     int shift = -1, bin = 0;                         // -1: linear bins; else bits of key(hi) - key(v)
-    U top = key_of(hi);
+    U top = 0;
     unsigned long long before = 0;
-    unsigned n = 0;
+    unsigned n = most;
     const auto linear = [&](V v) -> int {
-        const int b = (int)((high0 - v) * per);
+        const int b = (int)((high - v) * per);
         return b < BINS ? b : BINS - 1;
     };
     const auto keyed = [&](V v) -> int { return (int)((top - key_of(v)) >> shift); };
@@ -268,79 +286,90 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long t
         });
     };
     const auto ends = [&](auto bin_of) {             // the values of the bin, from its lowest to its highest
-        V least = (V)INFINITY, most = (V)-INFINITY;
+        V first = (V)-INFINITY, last = (V)INFINITY;
         src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
 #pragma unroll
             for (int j = 0; j < VEC; j++)
-                if ((live >> j & 1u) && bin_of(v[j]) == bin) { least = v[j] < least ? v[j] : least; most = v[j] > most ? v[j] : most; }
+                if ((live >> j & 1u) && bin_of(v[j]) == bin) { first = v[j] > first ? v[j] : first; last = v[j] < last ? v[j] : last; }
         });
-        lo = group_reduce<NT>(least, (V)INFINITY, (V*)s.tot, Min());
-        hi = group_reduce<NT>(most, (V)-INFINITY, (V*)s.tot, Max());
+        lo = group.reduce(last, (V)INFINITY, Min());
+        hi = group.reduce(first, (V)-INFINITY, Max());
     };
-    const auto gather = [&](auto bin_of) {
-        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int i) {
+    const auto enlist = [&](int o, int j) {          // sample j of the thread's piece o
+        const unsigned e = atomicAdd(&s.n_list, 1u);
+        s.list_v[e] = src.value(o, j);
+        s.list_idx[e] = src.index(o, j);
+    };
+    const auto gather = [&](auto bin_of) {           // (few samples per thread: their places first, then one after the other)
+        unsigned long long hits = 0;
+        src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int o) {
             unsigned hit = 0;
 #pragma unroll
             for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
-            if (hit) {
-#pragma unroll 1
-                for (int j = 0; j < VEC; j++)
-                    if (hit >> j & 1u) {
-                        const unsigned e = atomicAdd(&s.n_list, 1u);
-                        s.list_v[e] = src.value(i, j);
-                        s.list_idx[e] = src.index(i, j);
-                    }
+            if (o < 64 / VEC) {
+                hits |= (unsigned long long)hit << (o * VEC);
+            } else {
+                for (; hit; hit &= hit - 1) enlist(o, __ffs(hit) - 1);
             }
         });
+        for (; hits; hits &= hits - 1) {
+            const int at = __ffsll((long long)hits) - 1;
+            enlist(at / VEC, at % VEC);
+        }
     };
+    if (NT == 64) __syncthreads();                   // (larger groups have just met at a barrier)
+    if (threadIdx.x == 0) s.n_list = 0;
+    if (most > LIST) {
 #pragma unroll 1
-    while (true) {
+        while (true) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            s.cnt[threadIdx.x + i * NT] = 0;
-            if (MASS) s.mass[threadIdx.x + i * NT] = 0;
-        }
-        if (threadIdx.x == 0) s.n_list = 0;
-        if (threadIdx.x < LIST) { s.list_rank[threadIdx.x] = 0; s.list_before[threadIdx.x] = 0; s.list_ties[threadIdx.x] = 0; }
-        __syncthreads();
-        if (shift < 0) fill(linear); else fill(keyed);
-        __syncthreads();
-        unsigned long long own[PER], sum = 0, total;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int b = threadIdx.x * PER + i;
-            own[i] = MASS ? s.mass[b] : (unsigned long long)s.cnt[b];
-            sum += own[i];
-        }
-        unsigned long long run = before + group_scan<NT>(sum, s.tot, total);
-        if (shift < 0) {
-            if (AIM == BY_SHARE) {
-                // a whole number: "mass before < share W" is "mass before < ceil(share W)"
-                const double want = ceil(share * (double)total);
-                if (!(want >= 1.0)) { src.w.from = (V)INFINITY; return false; }
-                target = want < (double)total ? (unsigned long long)want : total;
+            for (int i = 0; i < PER; i++) {
+                s.cnt[threadIdx.x + i * NT] = 0;
+                if (MASS) s.mass[threadIdx.x + i * NT] = 0;
             }
-            if (total < target) return false;
-        }
+            __syncthreads();
+            if (shift < 0) fill(linear); else fill(keyed);
+            __syncthreads();
+            unsigned long long own[PER], sum = 0, total;
+            unsigned c[PER];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            if (run < target && target <= run + own[i]) {
-                s.pick_bin = threadIdx.x * PER + i;
-                s.pick_n = s.cnt[threadIdx.x * PER + i];
-                s.pick_before = run;
+            for (int i = 0; i < PER; i++) {
+                const int b = threadIdx.x * PER + i;
+                c[i] = s.cnt[b];
+                own[i] = MASS ? s.mass[b] : (unsigned long long)c[i];
+                sum += own[i];
             }
-            run += own[i];
+            unsigned long long run = before + group.scan(sum, total);
+            if (shift < 0) {
+                if (AIM == BY_SHARE) {
+                    target = share_of(share, total);
+                    if (target == 0) { src.w.from = (V)INFINITY; return false; }
+                }
+                if (total < target) return false;
+            }
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (run < target && target <= run + own[i]) {
+                    s.pick_bin = threadIdx.x * PER + i;
+                    s.pick_n = c[i];
+                    s.pick_before = run;
+                }
+                run += own[i];
+            }
+            __syncthreads();
+            bin = (int)s.pick_bin;
+            n = s.pick_n;
+            before = s.pick_before;
+            if (n <= LIST) break;
+            if (shift < 0) ends(linear); else ends(keyed);
+            if (lo == hi) break;
+            top = key_of(hi);
+            shift = 0;
+            while (((top - key_of(lo)) >> shift) >= (U)BINS) shift++;
         }
+    } else {
+        bin = -1;                                    // (no binning: all of them are candidates)
         __syncthreads();
-        bin = (int)s.pick_bin;
-        n = s.pick_n;
-        before = s.pick_before;
-        if (n <= LIST) break;
-        if (shift < 0) ends(linear); else ends(keyed);
-        if (lo == hi) break;
-        top = key_of(hi);
-        shift = 0;
-        while (((top - key_of(lo)) >> shift) >= (U)BINS) shift++;
     }
     if (n > LIST) {                                  // all n of one return
         if (threadIdx.x == 0) {
@@ -350,45 +379,71 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, unsigned long long t
             s.border_keep = (unsigned)((target - before + one - 1) / one);
             s.border_idx = UINT_MAX;
         }
-    } else {
-        if (shift < 0) gather(linear); else gather(keyed);
         __syncthreads();
-        if (MASS) {
-            if (threadIdx.x < n) s.list_q[threadIdx.x] = src.w.mass_of(s.list_v[threadIdx.x]);
-            __syncthreads();
+        return true;
+    }
+    if (bin < 0) gather([](V) { return -1; });
+    else if (shift < 0) gather(linear);
+    else gather(keyed);
+    __syncthreads();
+    // The first wave compares each candidate with each: lane l holds candidates l, l + 64, ...
+    if (threadIdx.x < 64) {
+        constexpr int E = LIST / 64;
+        n = s.n_list;
+        V v[E];
+        unsigned idx[E], lead[E], ties[E];
+        unsigned long long q[E], ahead[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const unsigned at = threadIdx.x + e * 64;
+            v[e] = at < n ? s.list_v[at] : (V)-INFINITY;
+            idx[e] = at < n ? s.list_idx[at] : UINT_MAX;
+            q[e] = MASS ? (at < n ? src.w.mass_of(v[e]) : 0ull) : 1ull;
+            if (MASS && at < n) s.list_q[at] = q[e];
+            lead[e] = ties[e] = 0;
+            ahead[e] = 0;
         }
-        // rank of every candidate: the threads share the comparisons
-        const unsigned parts = NT / n;               // 1 <= n <= LIST <= NT
-        const unsigned e = threadIdx.x / parts, first = threadIdx.x - e * parts;
-        if (e < n) {
-            const V v = s.list_v[e];
-            const unsigned idx = s.list_idx[e];
-            unsigned rank = 0, ties = 0;
-            unsigned long long ahead = 0;
-            for (unsigned o = first; o < n; o += parts) {
-                const V ov = s.list_v[o];
-                const bool lead = ov > v || (ov == v && s.list_idx[o] < idx);
-                rank += lead ? 1u : 0u;
-                ties += ov == v ? (lead ? 0x10001u : 0x1u) : 0u;           // low half: all equal ones, high half: those ahead
-                if (MASS) ahead += lead ? s.list_q[o] : 0ull;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        unsigned long long all = 0;
+#pragma unroll 4
+        for (unsigned o = 0; o < n; o++) {
+            const V ov = s.list_v[o];
+            const unsigned oi = s.list_idx[o];
+            const unsigned long long oq = MASS ? s.list_q[o] : 1ull;
+            all += oq;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const bool same = ov == v[e], first = ov > v[e] || (same && oi < idx[e]);
+                ahead[e] += first ? oq : 0ull;
+                ties[e] += same ? 1u : 0u;
+                lead[e] += same && first ? 1u : 0u;
             }
-            atomicAdd(&s.list_rank[e], rank);
-            atomicAdd(&s.list_ties[e], ties);
-            if (MASS) atomicAdd(&s.list_before[e], ahead);
         }
-        __syncthreads();
-        if (threadIdx.x < n) {
-            const unsigned long long run = before + (MASS ? s.list_before[threadIdx.x] : (unsigned long long)s.list_rank[threadIdx.x]);
-            const unsigned long long own = MASS ? s.list_q[threadIdx.x] : 1ull;
-            if (run < target && target <= run + own) {
-                s.border = s.list_v[threadIdx.x];
-                s.border_all = s.list_ties[threadIdx.x] & 0xffffu;
-                s.border_keep = (s.list_ties[threadIdx.x] >> 16) + 1;
-                s.border_idx = s.list_idx[threadIdx.x];
+        bool some = true;
+        if (bin < 0) {                               // what the histogram would have said
+            if (AIM == BY_SHARE) target = share_of(share, all);
+            some = target > 0 && all >= target;
+            if (threadIdx.x == 0) s.pick_n = some ? 1u : target == 0 ? 2u : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const unsigned long long run = before + ahead[e];
+            if (some && threadIdx.x + e * 64 < n && run < target && target <= run + q[e]) {
+                s.border = v[e];
+                s.border_all = ties[e];
+                s.border_keep = lead[e] + 1;
+                s.border_idx = idx[e];
             }
         }
     }
     __syncthreads();
+    if (bin < 0) {
+        const unsigned said = s.pick_n;
+        if (said == 2u) src.w.from = (V)INFINITY;
+        if (said != 1u) { __syncthreads(); return false; }
+    }
     return true;
 }
 
@@ -417,18 +472,23 @@ template <class T, int NT, int BYTES> struct Shelf {
     int GP, start, base;              // pieces of this thread, the one it begins with, the row's first piece
     int C;                            // samples per thread
 
-    __device__ Shelf(Shared& s_) : s(s_) {}
-    __device__ __forceinline__ static V at(const Piece& p, int j) { return value_of(p.v[j]); }
-    __device__ __forceinline__ V value(int i, int j) const { return at(s.row[base + i / VEC], j); }
-    __device__ __forceinline__ unsigned index(int i, int j) const { return (unsigned)(i + j); }
+    Group<NT> group;
+    unsigned most;                    // samples that can take part
 
-    // f(v, live, i): the pieces with samples in [low, high]; live: bit j for sample v[j], whose index is i + j
+    __device__ Shelf(Shared& s_) : s(s_), group(s_.b.slots) {}
+    __device__ __forceinline__ static V at(const Piece& p, int j) { return value_of(p.v[j]); }
+    // the thread's pieces in the order in which it visits them
+    __device__ __forceinline__ int piece(int o) const { const int g = start + o; return (int)threadIdx.x * GP + (g < GP ? g : g - GP); }
+    __device__ __forceinline__ V value(int o, int j) const { return at(s.row[base + piece(o)], j); }
+    __device__ __forceinline__ unsigned index(int o, int j) const { return (unsigned)(piece(o) * VEC + j); }
+
+    // f(v, live, o): the pieces with samples in [low, high]; live: bit j for sample v[j] of the o-th piece visited
     template <class F> __device__ __forceinline__ void each(V low, V high, F f) {
-        const int own = (int)threadIdx.x * GP;
+        const int own = base + (int)threadIdx.x * GP;
         int g = start;
 #pragma unroll 1
-        for (int n = 0; n < GP; n++) {
-            const Piece p = s.row[base + own + g];
+        for (int o = 0; o < GP; o++) {
+            const Piece p = s.row[own + g];
             V v[VEC];
             unsigned live = 0;
 #pragma unroll
@@ -436,7 +496,7 @@ template <class T, int NT, int BYTES> struct Shelf {
                 v[j] = at(p, j);
                 live |= v[j] >= low && v[j] <= high ? 1u << j : 0u;
             }
-            if (live) f(v, live, (own + g) * VEC);
+            if (live) f(v, live, o);
             g = g + 1 == GP ? 0 : g + 1;
         }
     }
@@ -456,7 +516,7 @@ template <class T, int NT, int BYTES> struct Shelf {
         unsigned own[PER], sum = 0, total;
 #pragma unroll
         for (int i = 0; i < PER; i++) { own[i] = s.b.cnt[threadIdx.x * PER + i]; sum += own[i]; }
-        unsigned run = group_scan<NT>(sum, (unsigned*)s.b.tot, total);
+        unsigned run = group.scan(sum, total);
         if (total < k) return;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
@@ -465,7 +525,7 @@ template <class T, int NT, int BYTES> struct Shelf {
         }
         __syncthreads();
         const V low = in && b <= (int)s.b.pick_bin ? mine : (V)INFINITY;
-        w.from = group_reduce<NT>(low, (V)INFINITY, (V*)s.b.tot, Min());
+        w.from = group.reduce(low, (V)INFINITY, Min());
     }
 
     // If few samples take part, they move together (in their order, with their indices), and the passes that follow go over
@@ -473,11 +533,12 @@ template <class T, int NT, int BYTES> struct Shelf {
     __device__ void gather_few() {
         unsigned mine = 0, pieces = 0, total;
         const int own = (int)threadIdx.x * GP;
-        each(w.from, w.best, [&](const V (&)[VEC], unsigned live, int i) {
+        each(w.from, w.best, [&](const V (&)[VEC], unsigned live, int o) {
             mine += (unsigned)__popc(live);
-            pieces |= 1u << (i / VEC - own);
+            pieces |= 1u << (piece(o) - own);
         });
-        unsigned to = group_scan<NT>(mine, (unsigned*)s.b.tot, total);
+        unsigned to = group.scan(mine, total);
+        most = total;
         if (total > FEW) return;
         constexpr int first = BYTES / 16;
         if (threadIdx.x < FEW / VEC) {
@@ -510,7 +571,7 @@ template <class T, int NT, int BYTES> struct Shelf {
         if (keep < s.b.border_all) {                 // of the equal ones, the first in the order of the samples stay
             unsigned mine = 0, total;
             each(w.from, w.from, [&](const V (&)[VEC], unsigned live, int) { mine += (unsigned)__popc(live); });
-            unsigned rank = group_scan<NT>(mine, (unsigned*)s.b.tot, total);
+            unsigned rank = group.scan(mine, total);
 #pragma unroll 1
             for (int g = 0; g < GP && mine > 0; g++) {
                 Piece& p = s.row[base + (int)threadIdx.x * GP + g];
@@ -537,6 +598,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     h.C = h.GP * VEC;
     h.start = tid % h.GP;
     h.base = 0;
+    h.most = (unsigned)a.K;
     const Param par(a.f, row);
     long long* index = a.index + row * a.D;
     float* weight = a.weight ? a.weight + row * a.D : nullptr;
@@ -571,17 +633,20 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         }
     }
     const V mine = best;                                                  // best of what this thread loaded
-    best = group_reduce<NT>(best, (V)-INFINITY, (V*)s.b.tot, Max());
-    worst = group_reduce<NT>(worst, (V)INFINITY, (V*)s.b.tot, Min());
-    __syncthreads();
+    best = h.group.reduce(best, (V)-INFINITY, Max());
+    worst = h.group.reduce(worst, (V)INFINITY, Min());
+    if (NT == 64) __syncthreads();                                        // (the row is there; larger groups have just waited)
     if (!par.valid() || !(best > (V)-INFINITY)) return nothing();
     h.w.set(par.kappa, best, worst, S);
     // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
     // thread next to nothing else passes that bound.
     if (BYTES >= 131072 && par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
     if (H::FEW && h.GP > 1) h.gather_few();
-    if (par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, (unsigned long long)par.top_k, 0.0, h.w.from, best)) h.cut_behind();
-    if (!(par.top_p >= 1.0) && find_border<BY_SHARE>(h, s.b, 0, par.top_p, h.w.from, best)) h.cut_behind();
+    if (par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, h.group, (unsigned long long)par.top_k, 0.0, h.w.from, best, h.most)) {
+        h.cut_behind();
+        h.most = h.most < par.top_k ? h.most : (unsigned)par.top_k;
+    }
+    if (!(par.top_p >= 1.0) && find_border<BY_SHARE>(h, s.b, h.group, 0, par.top_p, h.w.from, best, h.most)) h.cut_behind();
 
     unsigned long long sum = 0, mass;
     h.each(h.w.from, best, [&](const V (&v)[VEC], unsigned live, int) {
@@ -590,7 +655,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 #pragma unroll
         for (int j = 0; j < VEC; j++) sum += q[j];
     });
-    const unsigned long long base = group_scan<NT>(sum, s.b.tot, mass);
+    const unsigned long long base = h.group.scan(sum, mass);
     if (mass == 0) return nothing();
     unsigned long long* ends = s.ends();
     ends[tid] = base + sum;
@@ -651,7 +716,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 //   row_border    the borders among the listed samples; their masses join those of their chunks
 //   long_draw     for every draw: the chunk, then the sample
 // Rows without top-k and top-p need no list: chunk_split and row_border leave their chunks' masses as chunk_bins wrote them.
-constexpr int LT = 512, CHUNK = 8192, HELD = CHUNK / LT, LONG_BINS = 1024, BT = 1024;
+//                 (segment: the 64 VEC samples that one wave holds in one piece each)
+constexpr int MOST_SEGS = 64, LT = 512, CHUNK = 8192, HELD = CHUNK / LT, LONG_BINS = 1024, BT = 256;
 
 template <class V> struct LongRow {                  // what is known of a row (written by its first workgroup of chunk_bins)
     Weights<V> w;
@@ -662,7 +728,7 @@ template <class V> struct LongRow {                  // what is known of a row (
 template <class V> struct LongArea {                 // the workspace, of all rows
     V *best, *worst;                                 // [rows][chunks]
     double* sum;
-    unsigned long long *kept, *mass;                 // [rows][chunks] mass of a chunk, [rows][LONG_BINS]
+    unsigned long long *kept, *seg, *mass;           // mass of a chunk, [rows][chunks], and of its segments; [rows][LONG_BINS]
     unsigned* cnt;
     LongRow<V>* row;
     V* list_v;                                       // [rows][K]
@@ -678,6 +744,7 @@ template <class V> struct LongArea {                 // the workspace, of all ro
         a->worst = (V*)take(rows * chunks * sizeof(V));
         a->sum = (double*)take(rows * chunks * 8);
         a->kept = (unsigned long long*)take(rows * chunks * 8);
+        a->seg = (unsigned long long*)take(rows * chunks * MOST_SEGS * 8);
         a->mass = (unsigned long long*)take(rows * LONG_BINS * 8);
         a->cnt = (unsigned*)take(rows * LONG_BINS * 4);
         a->row = (LongRow<V>*)take(rows * sizeof(LongRow<V>));
@@ -691,7 +758,8 @@ template <class V> struct LongArea {                 // the workspace, of all ro
 // the chunk of this workgroup, HELD samples per thread, in pieces of VEC neighbours
 template <class T> struct Chunk {
     using V = typename Traits<T>::V;
-    static constexpr int VEC = 16 / sizeof(T), PIECES = HELD / VEC;
+    static constexpr int VEC = 16 / sizeof(T), PIECES = HELD / VEC, SEG = 64 * VEC, SEGS = CHUNK / SEG;
+    static_assert(SEGS <= MOST_SEGS, "");
     V x[PIECES][VEC];
     int first;                                       // index of x[0][0]
     __device__ __forceinline__ int index(int p, int j) const { return first + p * LT * VEC + j; }
@@ -709,6 +777,18 @@ template <class T> struct Chunk {
                 x[p][j] = isfinite(x[p][j]) ? x[p][j] : (V)-INFINITY;
             }
     }
+    // mass of every segment and of the chunk from those of the thread's pieces
+    __device__ __forceinline__ static void store(const unsigned long long (&sum)[PIECES], Group<LT>& group, unsigned long long* seg, unsigned long long* kept) {
+        unsigned long long all = 0;
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+            const unsigned long long inc = wave_scan(sum[p], 0ull, Add());
+            if ((threadIdx.x & 63) == 63) seg[p * (LT / 64) + (threadIdx.x >> 6)] = inc;
+            all += sum[p];
+        }
+        all = group.reduce(all, 0ull, Add());
+        if (threadIdx.x == 0) *kept = all;
+    }
     __device__ __forceinline__ unsigned live(int p, V low) const {
         unsigned bits = 0;
 #pragma unroll
@@ -721,7 +801,8 @@ __device__ __forceinline__ bool wants_border(const Param& par, int K) { return (
 
 template <class T> __global__ void __launch_bounds__(LT) chunk_best_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
-    __shared__ unsigned long long s_tot[LT / 64];
+    __shared__ unsigned long long s_slots[LT / 32];
+    Group<LT> group(s_slots);
     const long long row = blockIdx.x / l.chunks;
     const int chunk = (int)(blockIdx.x - row * l.chunks);
     Chunk<T> c;
@@ -741,8 +822,8 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_best_kernel(DrawA
             best = v > best ? v : best;
             worst = v > (V)-INFINITY && v < worst ? v : worst;
         }
-    best = group_reduce<LT>(best, (V)-INFINITY, (V*)s_tot, Max());
-    worst = group_reduce<LT>(worst, (V)INFINITY, (V*)s_tot, Min());
+    best = group.reduce(best, (V)-INFINITY, Max());
+    worst = group.reduce(worst, (V)INFINITY, Min());
     double sum = 0.0;
     if (par.valid() && best > (V)-INFINITY) {
         Weights<V> w;
@@ -752,7 +833,7 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_best_kernel(DrawA
 #pragma unroll
             for (int j = 0; j < c.VEC; j++) sum += c.x[p][j] >= w.from ? w.weight(c.x[p][j]) : 0.0;
     }
-    sum = group_reduce<LT>(sum, 0.0, (double*)s_tot, Add());
+    sum = group.reduce(sum, 0.0, Add());
     if (threadIdx.x == 0) {
         l.best[blockIdx.x] = best;
         l.worst[blockIdx.x] = worst;
@@ -772,7 +853,8 @@ template <class V> struct LongBins {
 
 template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
-    __shared__ unsigned long long s_tot[LT / 64], s_mass[LONG_BINS];
+    __shared__ unsigned long long s_slots[LT / 32], s_mass[LONG_BINS];
+    Group<LT> group(s_slots);
     __shared__ unsigned s_cnt[LONG_BINS];
     const long long row = blockIdx.x / l.chunks;
     const int chunk = (int)(blockIdx.x - row * l.chunks);
@@ -786,8 +868,8 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawA
         best = b > best ? b : best;
         worst = w < worst ? w : worst;
     }
-    best = group_reduce<LT>(best, (V)-INFINITY, (V*)s_tot, Max());
-    worst = group_reduce<LT>(worst, (V)INFINITY, (V*)s_tot, Min());
+    best = group.reduce(best, (V)-INFINITY, Max());
+    worst = group.reduce(worst, (V)INFINITY, Min());
     const bool some = par.valid() && best > (V)-INFINITY;
     Weights<V> w;
     int state = 0;
@@ -798,7 +880,7 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawA
             const V b = l.best[row * l.chunks + i];
             if (b >= w.from) sum += l.sum[row * l.chunks + i] * w.weight(b);
         }
-        sum = group_reduce<LT>(sum, 0.0, (double*)s_tot, Add());
+        sum = group.reduce(sum, 0.0, Add());
         int e;
         (void)frexp(sum, &e);                         // sum < 2^e
         const int S = 62 - e < 51 ? 62 - e : 51;
@@ -817,7 +899,9 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawA
         __syncthreads();
     }
     const LongBins<V> bins(w);
-    unsigned long long kept = 0;
+    unsigned long long kept[c.PIECES];
+#pragma unroll
+    for (int p = 0; p < c.PIECES; p++) kept[p] = 0;
     if (state != 0) {
 #pragma unroll
         for (int p = 0; p < c.PIECES; p++) {
@@ -827,7 +911,7 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawA
                 w.masses(c.x[p], live, state == 1 ? par.min_p : 0.0, q);
 #pragma unroll
                 for (int j = 0; j < c.VEC; j++) {
-                    kept += q[j];
+                    kept[p] += q[j];
                     if (state == 2 && (live >> j & 1u)) {
                         const int b = bins.of(c.x[p][j]);
                         atomicAdd(&s_cnt[b], 1u);
@@ -838,8 +922,7 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawA
         }
     }
     if (state != 2) {
-        kept = group_reduce<LT>(kept, 0ull, s_tot, Add());
-        if (threadIdx.x == 0) l.kept[blockIdx.x] = kept;
+        Chunk<T>::store(kept, group, l.seg + (size_t)blockIdx.x * c.SEGS, l.kept + blockIdx.x);
         return;
     }
     __syncthreads();
@@ -858,17 +941,12 @@ struct Where {
     unsigned long long k_mass_before, mass_before;   // mass_before: before p_first
     bool nothing;
 };
-template <int NT> struct WhereArea {
-    unsigned long long tot[NT / 64], total, k_mass_before, k_mass, p_before;
-    unsigned utot[NT / 64], k_before;
+struct WhereArea {
+    unsigned long long k_mass_before, k_mass, p_before;
+    unsigned k_before;
     int k, first, last;
 };
-// whole number above the mass that lies before what top-p keeps
-__device__ __forceinline__ unsigned long long share_of(double share, unsigned long long mass) {
-    const double want = ceil(share * (double)mass);
-    return want >= 1.0 ? (want < (double)mass ? (unsigned long long)want : mass) : 0ull;
-}
-template <int NT> __device__ Where where(const Param& par, int K, const unsigned* cnt, const unsigned long long* mass, WhereArea<NT>& s) {
+template <int NT> __device__ Where where(const Param& par, int K, const unsigned* cnt, const unsigned long long* mass, WhereArea& s, Group<NT>& group) {
     constexpr int PER = LONG_BINS / NT;
     unsigned c[PER], csum = 0, ctotal;
     unsigned long long m[PER], msum = 0, mtotal;
@@ -879,8 +957,8 @@ template <int NT> __device__ Where where(const Param& par, int K, const unsigned
         csum += c[i];
         msum += m[i];
     }
-    const unsigned crun0 = group_scan<NT>(csum, s.utot, ctotal);
-    const unsigned long long mrun0 = group_scan<NT>(msum, s.tot, mtotal);
+    const unsigned crun0 = group.scan(csum, ctotal);
+    const unsigned long long mrun0 = group.scan(msum, mtotal);
     Where r;
     r.k = -1;
     r.p_first = 1; r.p_last = 0;
@@ -926,8 +1004,10 @@ template <int NT> __device__ Where where(const Param& par, int K, const unsigned
 
 template <class T> __global__ void __launch_bounds__(LT) chunk_split_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
-    __shared__ WhereArea<LT> s;
+    __shared__ WhereArea s;
+    __shared__ unsigned long long s_slots[LT / 32];
     __shared__ unsigned s_listed, s_at;
+    Group<LT> group(s_slots);
     const long long row = blockIdx.x / l.chunks;
     const int chunk = (int)(blockIdx.x - row * l.chunks);
     if (l.row[row].state != 2) return;
@@ -937,15 +1017,16 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_split_kernel(Draw
     const Weights<V> w = l.row[row].w;
     const LongBins<V> bins(w);
     if (threadIdx.x == 0) s_listed = 0;
-    const Where at = where<LT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, s);
+    const Where at = where<LT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, s, group);
     // before `first` everything is kept; with neither border (top-k of more samples than there are) that is all of it
     const int first = at.nothing ? 0 : at.p_first <= at.p_last ? at.p_first : at.k >= 0 ? at.k : LONG_BINS;
-    unsigned long long kept = 0;
+    unsigned long long kept[c.PIECES];
     unsigned mine = 0;
     unsigned hits[c.PIECES];
 #pragma unroll
     for (int p = 0; p < c.PIECES; p++) {
         hits[p] = 0;
+        kept[p] = 0;
         const unsigned live = at.nothing ? 0u : c.live(p, w.from);
         if (live) {
             unsigned sure = 0;
@@ -961,15 +1042,14 @@ template <class T> __global__ void __launch_bounds__(LT) chunk_split_kernel(Draw
                 unsigned long long q[c.VEC];
                 w.masses(c.x[p], sure, par.min_p, q);
 #pragma unroll
-                for (int j = 0; j < c.VEC; j++) kept += q[j];
+                for (int j = 0; j < c.VEC; j++) kept[p] += q[j];
             }
         }
     }
     __syncthreads();                                  // (s_listed)
     unsigned to = mine ? atomicAdd(&s_listed, mine) : 0u;
-    kept = group_reduce<LT>(kept, 0ull, s.tot, Add());
+    Chunk<T>::store(kept, group, l.seg + (size_t)blockIdx.x * c.SEGS, l.kept + blockIdx.x);
     if (threadIdx.x == 0) {
-        l.kept[blockIdx.x] = kept;
         s_at = s_listed ? atomicAdd(&l.row[row].listed, s_listed) : 0u;
     }
     __syncthreads();
@@ -996,11 +1076,13 @@ template <class V, bool BY_INDEX> struct Listed {
     unsigned n;
     V only;
     Weights<V> w;
-    __device__ __forceinline__ V value(int e, int j) const { return BY_INDEX ? -(V)i[e + j * BT] : v[e + j * BT]; }
-    __device__ __forceinline__ unsigned index(int e, int j) const { return i[e + j * BT]; }
+    __device__ __forceinline__ static unsigned place(int o, int j) { return threadIdx.x + (o * VEC + j) * BT; }
+    __device__ __forceinline__ V value(int o, int j) const { return BY_INDEX ? -(V)i[place(o, j)] : v[place(o, j)]; }
+    __device__ __forceinline__ unsigned index(int o, int j) const { return i[place(o, j)]; }
     template <class F> __device__ __forceinline__ void each(V low, V high, F f) {
 #pragma unroll 1
-        for (unsigned e = threadIdx.x; e < n; e += BT * VEC) {
+        for (int o = 0; place(o, 0) < n; o++) {
+            const unsigned e = place(o, 0);
             V x[VEC];
             unsigned live = 0;
 #pragma unroll
@@ -1011,7 +1093,7 @@ template <class V, bool BY_INDEX> struct Listed {
                 if (BY_INDEX) x[j] = -(V)i[at];
                 live |= in && x[j] >= low && x[j] <= high ? 1u << j : 0u;
             }
-            if (live) f(x, live, (int)e);
+            if (live) f(x, live, o);
         }
     }
 };
@@ -1019,12 +1101,13 @@ template <class V, bool BY_INDEX> struct Listed {
 template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ BorderArea<V, BT> s;
-    __shared__ WhereArea<BT> sw;
+    __shared__ WhereArea sw;
+    Group<BT> group(s.slots);
     const long long row = blockIdx.x;
     LongRow<V>& r = l.row[row];
     if (r.state != 2) return;
     const Param par(a.f, row);
-    const Where at = where<BT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, sw);
+    const Where at = where<BT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, sw, group);
     if (at.nothing) {
         __syncthreads();
         if (threadIdx.x == 0) r.state = 0;
@@ -1044,8 +1127,8 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
                 if ((live >> j & 1u) && b >= first && b <= last) { least = x[j] < least ? x[j] : least; most = x[j] > most ? x[j] : most; }
             }
         });
-        lo = group_reduce<BT>(least, (V)INFINITY, (V*)s.tot, Min());
-        hi = group_reduce<BT>(most, (V)-INFINITY, (V*)s.tot, Max());
+        lo = group.reduce(least, (V)INFINITY, Min());
+        hi = group.reduce(most, (V)-INFINITY, Max());
     };
     V border = w.from, lo, hi;
     unsigned keep = 0, all = 0, last = UINT_MAX;
@@ -1054,7 +1137,7 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
     const bool share = at.p_first <= at.p_last;
     if (at.k >= 0) {
         range(at.k, at.k, w.from, lo, hi);
-        (void)find_border<BY_COUNT>(list, s, (unsigned long long)par.top_k - at.k_before, 0.0, lo, hi);
+        (void)find_border<BY_COUNT>(list, s, group, (unsigned long long)par.top_k - at.k_before, 0.0, lo, hi, list.n);
         found();
         if (share) {
             unsigned long long sum = 0;
@@ -1067,12 +1150,12 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
 #pragma unroll
                 for (int j = 0; j < 4; j++) sum += q[j];
             });
-            mass = at.k_mass_before + group_reduce<BT>(sum, 0ull, s.tot, Add()) + keep * w.mass_of(border);
+            mass = at.k_mass_before + group.reduce(sum, 0ull, Add()) + keep * w.mass_of(border);
         }
     } else {
         unsigned long long m = 0;
         for (int i = threadIdx.x; i < LONG_BINS; i += BT) m += l.mass[row * LONG_BINS + i];
-        mass = group_reduce<BT>(m, 0ull, s.tot, Add());
+        mass = group.reduce(m, 0ull, Add());
     }
     if (share) {
         const unsigned long long target = share_of(par.top_p, mass);
@@ -1081,105 +1164,106 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
             return;
         }
         range(at.p_first, at.p_last, border, lo, hi);
-        if (find_border<BY_MASS>(list, s, target - at.mass_before, 0.0, lo, hi)) found();
+        if (find_border<BY_MASS>(list, s, group, target - at.mass_before, 0.0, lo, hi, list.n)) found();
     }
     if (keep >= all) {
         last = UINT_MAX;
     } else if (last == UINT_MAX) {
         // more equal ones than a list of candidates holds: the keep-th of them by index
         Listed<V, true> equal{list.v, list.i, list.n, border, w};
-        (void)find_border<BY_COUNT>(equal, s, keep, 0.0, -(V)a.K, (V)0);
+        (void)find_border<BY_COUNT>(equal, s, group, keep, 0.0, -(V)a.K, (V)0, list.n);
         last = s.border_idx;
     }
     if (threadIdx.x == 0) { r.border = border; r.last = last; }
     // what the list keeps joins the chunks
-    list.each(border, w.best, [&](const V (&x)[4], unsigned live, int e) {
+    list.each(border, w.best, [&](const V (&x)[4], unsigned live, int o) {
         unsigned in = 0;
         unsigned idx[4];
         unsigned long long q[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            idx[j] = live >> j & 1u ? list.index(e, j) : 0u;
+            idx[j] = live >> j & 1u ? list.index(o, j) : 0u;
             in |= x[j] > border || idx[j] <= last ? live & 1u << j : 0u;
         }
         w.masses(x, in, par.min_p, q);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (q[j]) atomicAdd(&l.kept[row * l.chunks + idx[j] / CHUNK], q[j]);
+            if (q[j]) {
+                const long long chunk = row * l.chunks + idx[j] / CHUNK;
+                atomicAdd(&l.kept[chunk], q[j]);
+                atomicAdd(&l.seg[chunk * Chunk<T>::SEGS + idx[j] % CHUNK / Chunk<T>::SEG], q[j]);
+            }
     });
 }
 
-template <class T> __global__ void __launch_bounds__(LT) long_draw_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+// A wave for every draw: the chunk, its segment, the sample
+template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
-    __shared__ unsigned long long s_tot[LT / 64], s_ends[Chunk<T>::PIECES * LT / 64], s_before;
-    __shared__ int s_chunk;
-    const long long row = blockIdx.x / a.D;
-    const long long at = blockIdx.x;
+    using C = Chunk<T>;
+    constexpr int VEC = C::VEC;
+    const long long row = blockIdx.x / a.D, at = blockIdx.x;
     const LongRow<V>& r = l.row[row];
     const Param par(a.f, row);
-    unsigned long long mass = 0, target = 0;
+    const int lane = threadIdx.x;
+    const unsigned long long* kept = l.kept + row * l.chunks;
+    unsigned long long mass = 0, target = 0, run = 0;
+    int chunk = 0;
     if (r.state != 0) {
-        // the chunk: each thread sums PER neighbours
-        const int PER = (l.chunks + LT - 1) / LT;
+        const int PER = (l.chunks + 63) / 64;                   // neighbouring chunks of a lane
         unsigned long long sum = 0;
         for (int i = 0; i < PER; i++) {
-            const int c = (int)threadIdx.x * PER + i;
-            sum += c < l.chunks ? l.kept[row * l.chunks + c] : 0ull;
+            const int c = lane * PER + i;
+            sum += c < l.chunks ? kept[c] : 0ull;
         }
-        unsigned long long run = group_scan<LT>(sum, s_tot, mass);
+        const unsigned long long inc = wave_scan(sum, 0ull, Add());
+        mass = lane_value(inc, 63);
         if (mass != 0) {
             target = target_of(a.u[at], mass);
-            if (target - run < sum)
-                for (int i = 0; i < PER; i++) {
-                    const int c = (int)threadIdx.x * PER + i;
-                    const unsigned long long m = c < l.chunks ? l.kept[row * l.chunks + c] : 0ull;
-                    if (target - run < m) { s_chunk = c; s_before = run; }
-                    run += m;
-                }
+            run = inc - sum;
+            const int owner = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(target - run < sum)) - 1);
+            run = lane_value(run, owner);
+            chunk = owner * PER;
+            for (int i = 0; i < PER - 1; i++) {                  // (the same in every lane)
+                const unsigned long long m = kept[chunk];
+                if (target - run < m) break;
+                run += m;
+                chunk++;
+            }
         }
     }
     if (mass == 0) {
-        if (threadIdx.x == 0) { a.index[at] = -1; if (a.weight) a.weight[at] = 0.0f; }
+        if (lane == 0) { a.index[at] = -1; if (a.weight) a.weight[at] = 0.0f; }
         return;
     }
-    __syncthreads();
+    const unsigned long long m = lane < C::SEGS ? l.seg[(row * l.chunks + chunk) * C::SEGS + lane] : 0ull;
+    const unsigned long long inc = wave_scan(m, 0ull, Add());
+    const int seg = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(target - (run + inc - m) < m)) - 1);
+    run += lane_value(inc - m, seg);
+
     const Weights<V> w = r.w;
-    const V border = r.border;
-    const unsigned last = r.last;
-    Chunk<T> c;
-    c.load(a, row, s_chunk);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    unsigned long long q[c.PIECES][c.VEC], base[c.PIECES], sum[c.PIECES];
+    const int first = chunk * CHUNK + seg * C::SEG + lane * VEC;
+    T raw[VEC];
+    load_piece((const T*)a.R + row * a.row_stride, a.col_stride, (long long)first, a.K, raw);
+    V v[VEC];
+    unsigned live = 0;
 #pragma unroll
-    for (int p = 0; p < c.PIECES; p++) {
-        unsigned live = 0;
-#pragma unroll
-        for (int j = 0; j < c.VEC; j++) {
-            const V v = c.x[p][j];
-            live |= v > border || (v == border && (unsigned)c.index(p, j) <= last) ? 1u << j : 0u;
-        }
-        sum[p] = 0;
-        w.masses(c.x[p], live, par.min_p, q[p]);
-#pragma unroll
-        for (int j = 0; j < c.VEC; j++) sum[p] += q[p][j];
-        const unsigned long long inc = wave_scan(sum[p], 0ull, Add());
-        base[p] = inc - sum[p];
-        if (lane == 63) s_ends[p * (LT / 64) + wave] = inc;
+    for (int j = 0; j < VEC; j++) {
+        v[j] = value_of(raw[j]);
+        live |= v[j] < (V)INFINITY && (v[j] > r.border || (v[j] == r.border && (unsigned)(first + j) <= r.last)) ? 1u << j : 0u;
     }
-    __syncthreads();
+    unsigned long long q[VEC], sum = 0;
+    w.masses(v, live, par.min_p, q);
 #pragma unroll
-    for (int p = 0; p < c.PIECES; p++) {
-        unsigned long long run = s_before + base[p];
-        for (int k = 0; k < p * (LT / 64) + wave; k++) run += s_ends[k];
-        if (target - run < sum[p]) {
+    for (int j = 0; j < VEC; j++) sum += q[j];
+    run += wave_scan(sum, 0ull, Add()) - sum;
+    if (target - run < sum) {
 #pragma unroll
-            for (int j = 0; j < c.VEC; j++) {
-                if (target - run < q[p][j]) {
-                    a.index[at] = c.index(p, j);
-                    if (a.weight) a.weight[at] = (float)(w.weight(c.x[p][j]) * w.scale / (double)mass);
-                }
-                run += q[p][j];
+        for (int j = 0; j < VEC; j++) {
+            if (target - run < q[j]) {
+                a.index[at] = first + j;
+                if (a.weight) a.weight[at] = (float)(w.weight(v[j]) * w.scale / (double)mass);
             }
+            run += q[j];
         }
     }
 }
@@ -1211,7 +1295,7 @@ template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspa
         return fail(-1, "workspace too small (mppi_draw_workspace)");
     if ((long long)a.rows * l.chunks > INT_MAX || (long long)a.rows * a.D > INT_MAX)
         return fail(-6, "more than 2^31 - 1 chunks or draws in one call of long rows");
-    const dim3 chunks((unsigned)(a.rows * l.chunks));
+    const dim3 chunks((unsigned)((long long)a.rows * l.chunks));
     hipLaunchKernelGGL((chunk_best_kernel<T>), chunks, dim3(LT), 0, s, a, l);
     HIP_OK(hipGetLastError());
     hipLaunchKernelGGL((chunk_bins_kernel<T>), chunks, dim3(LT), 0, s, a, l);
@@ -1222,7 +1306,7 @@ template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspa
         hipLaunchKernelGGL((row_border_kernel<T>), dim3(a.rows), dim3(BT), 0, s, a, l);
         HIP_OK(hipGetLastError());
     }
-    hipLaunchKernelGGL((long_draw_kernel<T>), dim3((unsigned)(a.rows * a.D)), dim3(LT), 0, s, a, l);
+    hipLaunchKernelGGL((long_draw_kernel<T>), dim3((unsigned)((long long)a.rows * a.D)), dim3(64), 0, s, a, l);
     HIP_OK(hipGetLastError());
     return 0;
 }
