@@ -241,8 +241,8 @@ template <class T, int VEC> __device__ __forceinline__ void load_piece(const T* 
 // the border of a prefix of the order
 // ------------------------------------------------------------------------------------------
 template <class V, int NT> struct BorderArea {
-    static constexpr int BINS = NT == 64 ? 256 : 1024, LIST = NT >= 1024 ? 128 : 64;
-    unsigned long long mass[BINS], slots[NT / 32], list_q[LIST], pick_before;
+    static constexpr int BINS = NT == 64 ? 256 : 1024, LIST = 64;
+    unsigned long long mass[BINS], slots[NT / 32], pick_before;
     V list_v[LIST], border;
     unsigned cnt[BINS], list_idx[LIST], n_list, pick_bin, pick_n;
     unsigned border_keep, border_all;                // of the border_all samples equal to the border, this many are kept
@@ -295,31 +295,30 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
         lo = group.reduce(last, (V)INFINITY, Min());
         hi = group.reduce(first, (V)-INFINITY, Max());
     };
-    const auto enlist = [&](int o, int j) {          // sample j of the thread's piece o
-        const unsigned e = atomicAdd(&s.n_list, 1u);
-        s.list_v[e] = src.value(o, j);
-        s.list_idx[e] = src.index(o, j);
-    };
-    const auto gather = [&](auto bin_of) {           // (few samples per thread: their places first, then one after the other)
+    const auto gather = [&](auto bin_of) {           // the places first, then room for all of the thread's at once
         unsigned long long hits = 0;
+        const auto enlist = [&](unsigned long long bits, int first) {
+            unsigned e = atomicAdd(&s.n_list, (unsigned)__popcll(bits));
+#pragma unroll 1
+            for (; bits; bits &= bits - 1) {
+                const int at = first + __ffsll((long long)bits) - 1;
+                s.list_v[e] = src.value(at / VEC, at % VEC);
+                s.list_idx[e] = src.index(at / VEC, at % VEC);
+                e++;
+            }
+        };
         src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int o) {
             unsigned hit = 0;
 #pragma unroll
             for (int j = 0; j < VEC; j++) hit |= (live >> j & 1u) && bin_of(v[j]) == bin ? 1u << j : 0u;
-            if (o < 64 / VEC) {
-                hits |= (unsigned long long)hit << (o * VEC);
-            } else {
-                for (; hit; hit &= hit - 1) enlist(o, __ffs(hit) - 1);
-            }
+            if (o < 64 / VEC) hits |= (unsigned long long)hit << (o * VEC);
+            else if (hit) enlist(hit, o * VEC);      // (sources of more than 64 samples per thread)
         });
-        for (; hits; hits &= hits - 1) {
-            const int at = __ffsll((long long)hits) - 1;
-            enlist(at / VEC, at % VEC);
-        }
+        if (hits) enlist(hits, 0);
     };
     if (NT == 64) __syncthreads();                   // (larger groups have just met at a barrier)
     if (threadIdx.x == 0) s.n_list = 0;
-    if (most > LIST) {
+    if (most > 16) {                                 // (the histogram costs less than comparing as few as 32 with each other)
 #pragma unroll 1
         while (true) {
 #pragma unroll
@@ -386,55 +385,51 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
     else if (shift < 0) gather(linear);
     else gather(keyed);
     __syncthreads();
-    // The first wave compares each candidate with each: lane l holds candidates l, l + 64, ...
-    if (threadIdx.x < 64) {
-        constexpr int E = LIST / 64;
-        n = s.n_list;
-        V v[E];
-        unsigned idx[E], lead[E], ties[E];
-        unsigned long long q[E], ahead[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const unsigned at = threadIdx.x + e * 64;
-            v[e] = at < n ? s.list_v[at] : (V)-INFINITY;
-            idx[e] = at < n ? s.list_idx[at] : UINT_MAX;
-            q[e] = MASS ? (at < n ? src.w.mass_of(v[e]) : 0ull) : 1ull;
-            if (MASS && at < n) s.list_q[at] = q[e];
-            lead[e] = ties[e] = 0;
-            ahead[e] = 0;
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        unsigned long long all = 0;
-#pragma unroll 4
+    if (threadIdx.x < 64) {                          // the first wave compares each with each
+        static_assert(LIST == 64, "a candidate per lane");
+        const int lane = threadIdx.x;
+        n = __builtin_amdgcn_readfirstlane(s.n_list);
+        const bool in = lane < (int)n;
+        const V v = in ? s.list_v[lane] : (V)-INFINITY;
+        const unsigned idx = in ? s.list_idx[lane] : UINT_MAX;
+        const unsigned long long q = in ? (MASS ? src.w.mass_of(v) : 1ull) : 0ull;
+        unsigned long long run = before, all = 0;    // run: what lies before this lane's candidate in the order
+        unsigned rank = 0;
+        const unsigned long long place = (unsigned long long)(sizeof(V) == 4 ? (U)key_of(v) : (U)0) << 32 | (unsigned)~idx;
         for (unsigned o = 0; o < n; o++) {
-            const V ov = s.list_v[o];
-            const unsigned oi = s.list_idx[o];
-            const unsigned long long oq = MASS ? s.list_q[o] : 1ull;
-            all += oq;
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool same = ov == v[e], first = ov > v[e] || (same && oi < idx[e]);
-                ahead[e] += first ? oq : 0ull;
-                ties[e] += same ? 1u : 0u;
-                lead[e] += same && first ? 1u : 0u;
+            bool first;
+            if constexpr (sizeof(V) == 4) {          // value and index in one number
+                first = lane_value(place, o) > place;
+            } else {
+                const V ov = lane_value(v, o);
+                first = ov > v || (ov == v && lane_value(idx, o) < idx);
+            }
+            if (MASS) {
+                const unsigned long long oq = lane_value(q, o);
+                all += oq;
+                run += first ? oq : 0ull;
+            } else {
+                rank += first ? 1u : 0u;
             }
         }
+        if (!MASS) { run += rank; all = n; }
         bool some = true;
         if (bin < 0) {                               // what the histogram would have said
             if (AIM == BY_SHARE) target = share_of(share, all);
             some = target > 0 && all >= target;
-            if (threadIdx.x == 0) s.pick_n = some ? 1u : target == 0 ? 2u : 0u;
+            if (lane == 0) s.pick_n = some ? 1u : target == 0 ? 2u : 0u;
         }
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const unsigned long long run = before + ahead[e];
-            if (some && threadIdx.x + e * 64 < n && run < target && target <= run + q[e]) {
-                s.border = v[e];
-                s.border_all = ties[e];
-                s.border_keep = lead[e] + 1;
-                s.border_idx = idx[e];
+        const unsigned long long here = __ballot(some && run < target && target <= run + q);
+        if (here) {
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll((long long)here) - 1);
+            const V border = lane_value(v, at);
+            const unsigned last = lane_value(idx, at);
+            const unsigned long long same = __ballot(in && v == border), kept = __ballot(in && v == border && idx <= last);
+            if (lane == 0) {
+                s.border = border;
+                s.border_all = (unsigned)__popcll(same);
+                s.border_keep = (unsigned)__popcll(kept);
+                s.border_idx = last;
             }
         }
     }
@@ -529,17 +524,30 @@ template <class T, int NT, int BYTES> struct Shelf {
     }
 
     // If few samples take part, they move together (in their order, with their indices), and the passes that follow go over
-    // them alone.
-    __device__ void gather_few() {
-        unsigned mine = 0, pieces = 0, total;
-        const int own = (int)threadIdx.x * GP;
-        each(w.from, w.best, [&](const V (&)[VEC], unsigned live, int o) {
-            mine += (unsigned)__popc(live);
-            pieces |= 1u << (piece(o) - own);
-        });
-        unsigned to = group.scan(mine, total);
-        most = total;
-        if (total > FEW) return;
+    // them alone.  top[p]: highest value of piece p NT + t, as thread t loaded them, so that most pieces need not be looked at again.
+    template <int P> __device__ void gather_few(const V (&top)[P]) {
+        static_assert(P <= 8, "two words of four counts");
+        unsigned long long bits = 0, mine[2] = {0, 0}, total[2] = {0, 0};  // bit p VEC + j; samples by piece, 16 bits each
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            if (p < GP && top[p] >= w.from) {
+                const Piece x = s.row[p * NT + (int)threadIdx.x];
+                unsigned in = 0;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) in |= at(x, j) >= w.from ? 1u << j : 0u;
+                bits |= (unsigned long long)in << (p * VEC);
+                mine[p / 4] += (unsigned long long)__popc(in) << (p % 4 * 16);
+            }
+        }
+        unsigned long long to[2] = {group.scan(mine[0], total[0]), group.scan(mine[1], total[1])};
+        unsigned all = 0;                            // (at most 1024 threads of 8 samples: every count fits)
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            if (all <= FEW) to[p / 4] += (unsigned long long)all << (p % 4 * 16);
+            all += (unsigned)(total[p / 4] >> (p % 4 * 16) & 0xffffu);
+        }
+        most = all;
+        if (all > FEW) return;
         constexpr int first = BYTES / 16;
         if (threadIdx.x < FEW / VEC) {
 #pragma unroll
@@ -547,15 +555,13 @@ template <class T, int NT, int BYTES> struct Shelf {
         }
         __syncthreads();
 #pragma unroll 1
-        for (; pieces; pieces &= pieces - 1) {
-            const int p = own + __ffs(pieces) - 1;
-#pragma unroll 1
-            for (int j = 0; j < VEC; j++)
-                if (at(s.row[p], j) >= w.from) {
-                    s.row[first + to / VEC].v[to % VEC] = s.row[p].v[j];
-                    s.few_idx[to] = (unsigned)(p * VEC + j);
-                    to++;
-                }
+        for (; bits; bits &= bits - 1) {             // (in the order of the pieces, and in it within each)
+            const int at = __ffsll((long long)bits) - 1, p = at / VEC, j = at % VEC, from = p * NT + (int)threadIdx.x;
+            const int field = p % 4 * 16;
+            const unsigned e = (unsigned)((p < 4 ? to[0] : to[1]) >> field & 0xffffu);
+            if (p < 4) to[0] += 1ull << field; else to[1] += 1ull << field;
+            s.row[first + e / VEC].v[e % VEC] = s.row[from].v[j];
+            s.few_idx[e] = (unsigned)(from * VEC + j);
         }
         __syncthreads();
         base = first;
@@ -610,25 +616,27 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     const double u_wave = wave < a.D ? u[wave] : 0.0, u_thread = tid < a.D ? u[tid] : 0.0;      // asked for before anything waits
     // the row into LDS, AHEAD pieces requested at a time
     constexpr int AHEAD = BYTES >= 131072 ? 8 : 4;
-    V best = (V)-INFINITY, worst = (V)INFINITY;
+    V best = (V)-INFINITY, worst = (V)INFINITY, top[AHEAD];
 #pragma unroll 1
-    for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {
+    for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {                            // (once where few samples may move together)
         Piece in[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) load_piece(R, a.col_stride, (long long)((p0 + k) * NT + tid) * VEC, a.K, in[k].v);
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             if (p0 + k >= h.GP) break;
+            top[k] = (V)-INFINITY;
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 const V v = H::at(in[k], j);
                 if (!isfinite(v)) {
                     in[k].v[j] = minus_infinity((T*)nullptr);
                 } else {
-                    best = v > best ? v : best;
+                    top[k] = v > top[k] ? v : top[k];
                     worst = v < worst ? v : worst;
                 }
             }
+            best = top[k] > best ? top[k] : best;
             s.row[(p0 + k) * NT + tid] = in[k];
         }
     }
@@ -641,7 +649,10 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
     // thread next to nothing else passes that bound.
     if (BYTES >= 131072 && par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
-    if (H::FEW && h.GP > 1) h.gather_few();
+    if constexpr (H::FEW > 0) {
+        static_assert(AHEAD * NT * 16 >= BYTES, "the row is loaded in one go");
+        if (h.GP > 1) h.gather_few(top);
+    }
     if (par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, h.group, (unsigned long long)par.top_k, 0.0, h.w.from, best, h.most)) {
         h.cut_behind();
         h.most = h.most < par.top_k ? h.most : (unsigned)par.top_k;
@@ -671,8 +682,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         if (weight) weight[d] = (float)(w * h.w.scale / (double)mass);
     };
     const int C = h.C;
-    // A wave for every draw (about 500 cycles each) or a thread for every draw (about 150 cycles for every sample it walks over)
-    if ((long long)((a.D + NW - 1) / NW) * 500 <= (long long)((a.D + NT - 1) / NT) * C * 150) {
+    // A wave for every draw (about 500 cycles each) or a thread for every draw (about 500 cycles for every piece it walks over)
+    if ((a.D + NW - 1) / NW <= (a.D + NT - 1) / NT * (C / VEC)) {
 #pragma unroll 1
         for (int d = wave; d < a.D; d += NW) {
             const unsigned long long target = target_of(d == wave ? u_wave : u[d], mass);
@@ -686,9 +697,11 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             if (target - at < m) answer(d, owner * C + lane, w);
         }
     } else {
+        double next = u_thread;
 #pragma unroll 1
         for (int d = tid; d < a.D; d += NT) {
-            const unsigned long long target = target_of(d == tid ? u_thread : u[d], mass);
+            const unsigned long long target = target_of(next, mass);
+            next = d + NT < a.D ? u[d + NT] : 0.0;
             int lo = 0, hi = NT - 1;                           // the first thread that ends above the target
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
@@ -696,11 +709,31 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             }
             unsigned long long c = lo > 0 ? ends[lo - 1] : 0ull;
 #pragma unroll 1
-            for (int i = lo * C; i < (lo + 1) * C; i++) {
-                double w;
-                const unsigned long long m = mass_of_sample(i, w);
-                if (target - c < m) { answer(d, i, w); break; }
-                c += m;
+            for (int p = lo * C / VEC; p < (lo + 1) * C / VEC; p++) {
+                const Piece x = s.row[h.base + p];
+                V v[VEC];
+                unsigned live = 0;
+                unsigned long long q[VEC], sum = 0;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    v[j] = H::at(x, j);
+                    live |= v[j] >= h.w.from ? 1u << j : 0u;
+                }
+                h.w.masses(v, live, par.min_p, q);
+#pragma unroll
+                for (int j = 0; j < VEC; j++) sum += q[j];
+                if (target - c < sum) {
+                    V chosen = v[0];
+                    int at = 0;
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        if (target - c < q[j]) { chosen = v[j]; at = j; }
+                        c += q[j];
+                    }
+                    answer(d, p * VEC + at, h.w.weight(chosen));
+                    break;
+                }
+                c += sum;
             }
         }
     }
@@ -799,7 +832,7 @@ template <class T> struct Chunk {
 
 __device__ __forceinline__ bool wants_border(const Param& par, int K) { return (par.top_k > 0 && par.top_k < K) || !(par.top_p >= 1.0); }
 
-template <class T> __global__ void __launch_bounds__(LT) chunk_best_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+template <class T> __global__ void __launch_bounds__(LT, 4) chunk_best_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ unsigned long long s_slots[LT / 32];
     Group<LT> group(s_slots);
@@ -851,7 +884,7 @@ template <class V> struct LongBins {
     }
 };
 
-template <class T> __global__ void __launch_bounds__(LT) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+template <class T> __global__ void __launch_bounds__(LT, 4) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ unsigned long long s_slots[LT / 32], s_mass[LONG_BINS];
     Group<LT> group(s_slots);
@@ -1002,7 +1035,7 @@ template <int NT> __device__ Where where(const Param& par, int K, const unsigned
     return r;
 }
 
-template <class T> __global__ void __launch_bounds__(LT) chunk_split_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+template <class T> __global__ void __launch_bounds__(LT, 4) chunk_split_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ WhereArea s;
     __shared__ unsigned long long s_slots[LT / 32];
@@ -1281,7 +1314,7 @@ template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspa
     if ((size_t)a.K * sizeof(T) <= SHELF) {
         // K units of half 2^-S at most in error, and sums below 2^62
         const int S = std::min(51, 62 - ceil_log2(a.K));
-        if (a.K <= 512)
+        if (a.K <= 512 && a.D <= 64)
             hipLaunchKernelGGL((draw_row_kernel<T, 64, 512 * sizeof(T)>), dim3(a.rows), dim3(64), 0, s, a, S);
         else if (a.K <= 4096)
             hipLaunchKernelGGL((draw_row_kernel<T, 256, 4096 * sizeof(T)>), dim3(a.rows), dim3(256), 0, s, a, S);
