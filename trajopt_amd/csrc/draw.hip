@@ -1317,7 +1317,7 @@ template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspa
         if (a.K <= 512 && a.D <= 64)
             hipLaunchKernelGGL((draw_row_kernel<T, 64, 512 * sizeof(T)>), dim3(a.rows), dim3(64), 0, s, a, S);
         else if (a.K <= 4096)
-            hipLaunchKernelGGL((draw_row_kernel<T, 256, 4096 * sizeof(T)>), dim3(a.rows), dim3(256), 0, s, a, S);
+            hipLaunchKernelGGL((draw_row_kernel<T, 512, 4096 * sizeof(T)>), dim3(a.rows), dim3(512), 0, s, a, S);
         else
             hipLaunchKernelGGL((draw_row_kernel<T, 1024, SHELF>), dim3(a.rows), dim3(1024), 0, s, a, S);
         HIP_OK(hipGetLastError());

@@ -24,14 +24,24 @@ namespace {
 
 constexpr int BT = 256;                  // threads of a workgroup
 constexpr int CHUNK = 16384;             // entries of one tensor that a workgroup takes at a time
-constexpr int MAX_GROUPS = 1024;         // workgroups (= partial sums) of all norm launches together
-constexpr int TABLE = 128;               // tensors per launch: the table travels in the kernel's arguments (4 KB at most)
+constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums
+constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way
+constexpr int TABLE = 120;               // tensors whose table travels in a kernel's arguments (4 KB at most)
 
+struct Entry {
+    const void* g;
+    void* out;
+    long long n;
+    unsigned first;                      // chunks of the tensors before it
+    int type;
+};
 struct Table {
-    const void* g[TABLE];
-    void* out[TABLE];
-    long long n[TABLE];
-    unsigned first[TABLE];               // chunks of the tensors before it in this launch
+    Entry e[TABLE];
+    int tensors;
+    unsigned chunks;
+};
+struct FarTable {                        // more tensors: in the workspace, written there by table_kernel
+    const Entry* e;
     int tensors;
     unsigned chunks;
 };
@@ -55,22 +65,39 @@ template <> struct Io<__bf16> {
     static __device__ __forceinline__ float get(B b) { return __uint_as_float((uint32_t)b << 16); }
     static __device__ __forceinline__ B scaled(B b, double s) { return __builtin_bit_cast(B, (__bf16)(get(b) * (float)s)); }
 };
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+typedef Words LooseWords __attribute__((aligned(2), may_alias));
 template <class T> struct Pack {         // 16 bytes of entries, wherever they lie
-    typename Io<T>::B v[Io<T>::VEC];
-    __device__ __forceinline__ void load(const typename Io<T>::B* p) { __builtin_memcpy(this, p, 16); }
-    __device__ __forceinline__ void store(typename Io<T>::B* p) const { __builtin_memcpy(p, this, 16); }
+    using B = typename Io<T>::B;
+    static constexpr int PER = 4 / (int)sizeof(B);              // entries per word
+    Words w;
+    __device__ __forceinline__ void load(const B* p) { w = *(const LooseWords*)p; }
+    __device__ __forceinline__ void store(B* p) const { *(LooseWords*)p = w; }
+    __device__ __forceinline__ B get(int j) const { return (B)(w[j / PER] >> (j % PER * 16)); }
+    __device__ __forceinline__ void scale(double s) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (PER == 1) {
+                w[i] = Io<T>::scaled(get(i), s);
+            } else {
+                const uint32_t lo = Io<T>::scaled(get(2 * i), s), hi = Io<T>::scaled(get(2 * i + 1), s);
+                w[i] = hi << 16 | lo;
+            }
+        }
+    }
 };
 
 // tensor that holds chunk c, and the chunk's entries [lo, hi) in it
-__device__ __forceinline__ int locate(const Table& t, unsigned c, long long& lo, long long& hi) {
+template <class Tab> __device__ __forceinline__ const Entry& locate(const Tab& t, unsigned c, long long& lo, long long& hi) {
     int a = 0, b = t.tensors - 1;
     while (a < b) {
         const int m = (a + b + 1) >> 1;
-        if (t.first[m] <= c) a = m; else b = m - 1;
+        if (t.e[m].first <= c) a = m; else b = m - 1;
     }
-    lo = (long long)(c - t.first[a]) * CHUNK;
-    hi = lo + CHUNK < t.n[a] ? lo + CHUNK : t.n[a];
-    return a;
+    const Entry& e = t.e[a];
+    lo = (long long)(c - e.first) * CHUNK;
+    hi = lo + CHUNK < e.n ? lo + CHUNK : e.n;
+    return e;
 }
 
 // one entry into a running sum of squares, or largest magnitude (as its bits: NaN is above infinity)
@@ -82,7 +109,7 @@ template <bool MAX> __device__ __forceinline__ void take(double& acc, uint32_t& 
         acc = fma((double)x, (double)x, acc);
     }
 }
-template <bool MAX> __device__ double group_total(double acc, uint32_t top, double* s) {
+template <bool MAX, int NT> __device__ double group_total(double acc, uint32_t top, double* s) {
     double v = MAX ? (double)top : acc;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) {
@@ -92,38 +119,100 @@ template <bool MAX> __device__ double group_total(double acc, uint32_t top, doub
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     v = s[0];
-    for (int w = 1; w < BT / 64; w++) v = MAX ? fmax(v, s[w]) : v + s[w];
+    for (int w = 1; w < NT / 64; w++) v = MAX ? fmax(v, s[w]) : v + s[w];
     __syncthreads();
     return v;
 }
+template <bool MAX> __device__ __forceinline__ double norm_of_total(double v) { return MAX ? (double)__uint_as_float((uint32_t)v) : sqrt(v); }
 
-template <class T, bool MAX> __global__ void __launch_bounds__(BT) gradient_partials_kernel(Table t, double* __restrict__ partials) {
+// entries [lo, hi) of a tensor, AHEAD packs of a thread under way at a time
+template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(const void* p, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
     using B = typename Io<T>::B;
-    constexpr int VEC = Io<T>::VEC;
+    constexpr int VEC = Io<T>::VEC, STEP = NT * VEC;
+    const B* g = (const B*)p;
+    long long i = lo + threadIdx.x * VEC;
+    for (; i + (AHEAD - 1) * STEP + VEC <= hi; i += AHEAD * STEP) {
+        Pack<T> x[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) x[k].load(g + i + k * STEP);
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) take<MAX>(acc[j % 4], top, Io<T>::get(x[k].get(j)));
+    }
+    for (; i + VEC <= hi; i += STEP) {
+        Pack<T> x;
+        x.load(g + i);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) take<MAX>(acc[j % 4], top, Io<T>::get(x.get(j)));
+    }
+    for (; i < hi; i++) take<MAX>(acc[0], top, Io<T>::get(g[i]));      // the last, shorter pack
+}
+// times the scale, or bit for bit
+template <class T, bool SCALED, int NT> __device__ __forceinline__ void write_span(const void* from, void* to, long long lo, long long hi, double scale) {
+    using B = typename Io<T>::B;
+    constexpr int VEC = Io<T>::VEC, STEP = NT * VEC;
+    const B* g = (const B*)from;
+    B* out = (B*)to;
+    long long i = lo + threadIdx.x * VEC;
+    for (; i + (AHEAD - 1) * STEP + VEC <= hi; i += AHEAD * STEP) {
+        Pack<T> x[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) x[k].load(g + i + k * STEP);
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            if (SCALED) x[k].scale(scale);
+            x[k].store(out + i + k * STEP);
+        }
+    }
+    for (; i + VEC <= hi; i += STEP) {
+        Pack<T> x;
+        x.load(g + i);
+        if (SCALED) x.scale(scale);
+        x.store(out + i);
+    }
+    for (; i < hi; i++) out[i] = SCALED ? Io<T>::scaled(g[i], scale) : g[i];
+}
+template <bool MAX, int NT> __device__ __forceinline__ void read_chunk(const Entry& e, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
+    if (e.type == MPPI_F32) read_span<float, MAX, NT>(e.g, lo, hi, acc, top);
+    else if (e.type == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, lo, hi, acc, top);
+    else read_span<__bf16, MAX, NT>(e.g, lo, hi, acc, top);
+}
+template <int NT> __device__ __forceinline__ void write_chunk(const Entry& e, long long lo, long long hi, bool clip, double scale) {
+    if (!clip && e.out == e.g) return;
+    if (e.type == MPPI_F32) {
+        if (clip) write_span<float, true, NT>(e.g, e.out, lo, hi, scale);
+        else write_span<float, false, NT>(e.g, e.out, lo, hi, scale);
+    } else if (!clip) {
+        write_span<__bf16, false, NT>(e.g, e.out, lo, hi, scale);      // (bits are bits)
+    } else if (e.type == MPPI_F16) {
+        write_span<_Float16, true, NT>(e.g, e.out, lo, hi, scale);
+    } else {
+        write_span<__bf16, true, NT>(e.g, e.out, lo, hi, scale);
+    }
+}
+
+__global__ void __launch_bounds__(BT) table_kernel(Table t, int at, Entry* __restrict__ e) {
+    for (int i = threadIdx.x; i < t.tensors; i += BT) e[at + i] = t.e[i];
+}
+
+template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_partials_kernel(Tab t, double* __restrict__ partials) {
     __shared__ double s[BT / 64];
-    double acc = 0.0;
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};      // four chains of dependent additions
     uint32_t top = 0;
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         long long lo, hi;
-        const B* g = (const B*)t.g[locate(t, c, lo, hi)];
-        long long i = lo + threadIdx.x * VEC;
-        for (; i + VEC <= hi; i += BT * VEC) {
-            Pack<T> p;
-            p.load(g + i);
-#pragma unroll
-            for (int j = 0; j < VEC; j++) take<MAX>(acc, top, Io<T>::get(p.v[j]));
-        }
-        for (; i < hi; i++) take<MAX>(acc, top, Io<T>::get(g[i]));      // the last, shorter pack
+        const Entry& e = locate(t, c, lo, hi);
+        read_chunk<MAX, BT>(e, lo, hi, acc, top);
     }
-    const double v = group_total<MAX>(acc, top, s);
+    const double v = group_total<MAX, BT>((acc[0] + acc[1]) + (acc[2] + acc[3]), top, s);
     if (threadIdx.x == 0) partials[blockIdx.x] = v;
 }
 
 template <bool MAX> __device__ double norm_of(const double* __restrict__ partials, int n, double* s) {
     double acc = 0.0;
     for (int i = threadIdx.x; i < n; i += BT) acc = MAX ? fmax(acc, partials[i]) : acc + partials[i];
-    acc = group_total<MAX>(acc, (uint32_t)acc, s);
-    return MAX ? (double)__uint_as_float((uint32_t)acc) : sqrt(acc);
+    return norm_of_total<MAX>(group_total<MAX, BT>(acc, (uint32_t)acc, s));
 }
 
 template <bool MAX> __global__ void __launch_bounds__(BT) gradient_norm_kernel(const double* __restrict__ partials, int n, float* __restrict__ norm_out) {
@@ -132,59 +221,37 @@ template <bool MAX> __global__ void __launch_bounds__(BT) gradient_norm_kernel(c
     if (threadIdx.x == 0) *norm_out = (float)norm;
 }
 
-template <class T, bool MAX> __global__ void __launch_bounds__(BT) gradient_clip_kernel(Table t, const double* __restrict__ partials, int n_partials,
-                                                                                     double max_norm, float* __restrict__ norm_out) {
-    using B = typename Io<T>::B;
-    constexpr int VEC = Io<T>::VEC;
+// Every workgroup takes the chunks it took for the norm, the last one first: that one may still lie in its caches.
+template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_clip_kernel(Tab t, const double* __restrict__ partials, int n_partials,
+                                                                                       double max_norm, float* __restrict__ norm_out) {
     __shared__ double s[BT / 64];
     const double norm = norm_of<MAX>(partials, n_partials, s);
-    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const bool clip = norm > max_norm && norm < INFINITY;
     const double scale = clip ? max_norm / norm : 1.0;
-    for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const unsigned last = blockIdx.x + (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x;
+    for (unsigned c = last;; c -= gridDim.x) {
         long long lo, hi;
-        const int k = locate(t, c, lo, hi);
-        const B* g = (const B*)t.g[k];
-        B* out = (B*)t.out[k];
-        if (!clip && out == g) continue;
-        long long i = lo + threadIdx.x * VEC;
-        for (; i + VEC <= hi; i += BT * VEC) {
-            Pack<T> p;
-            p.load(g + i);
-            if (clip) {
-#pragma unroll
-                for (int j = 0; j < VEC; j++) p.v[j] = Io<T>::scaled(p.v[j], scale);
-            }
-            p.store(out + i);
-        }
-        for (; i < hi; i++) out[i] = clip ? Io<T>::scaled(g[i], scale) : g[i];
+        const Entry& e = locate(t, c, lo, hi);
+        write_chunk<BT>(e, lo, hi, clip, scale);
+        if (c < gridDim.x) break;
     }
 }
 
-// tensors of one element type, in launches of at most TABLE
-struct Batch {
-    Table t;
-    int dtype;
-    int groups, first_partial;
-};
-
-template <bool MAX> hipError_t launch_partials(const Batch& b, double* partials, hipStream_t s) {
-    double* at = partials + b.first_partial;
-    switch (b.dtype) {
-    case MPPI_F32: hipLaunchKernelGGL((gradient_partials_kernel<float, MAX>), dim3(b.groups), dim3(BT), 0, s, b.t, at); break;
-    case MPPI_F16: hipLaunchKernelGGL((gradient_partials_kernel<_Float16, MAX>), dim3(b.groups), dim3(BT), 0, s, b.t, at); break;
-    default: hipLaunchKernelGGL((gradient_partials_kernel<__bf16, MAX>), dim3(b.groups), dim3(BT), 0, s, b.t, at); break;
-    }
-    return hipGetLastError();
-}
-template <bool MAX> hipError_t launch_clip(const Batch& b, const double* partials, int n, double max_norm, float* norm, hipStream_t s) {
-    const int groups = (int)std::min<unsigned>(b.t.chunks, 2048u);
-    switch (b.dtype) {
-    case MPPI_F32: hipLaunchKernelGGL((gradient_clip_kernel<float, MAX>), dim3(groups), dim3(BT), 0, s, b.t, partials, n, max_norm, norm); break;
-    case MPPI_F16: hipLaunchKernelGGL((gradient_clip_kernel<_Float16, MAX>), dim3(groups), dim3(BT), 0, s, b.t, partials, n, max_norm, norm); break;
-    default: hipLaunchKernelGGL((gradient_clip_kernel<__bf16, MAX>), dim3(groups), dim3(BT), 0, s, b.t, partials, n, max_norm, norm); break;
-    }
-    return hipGetLastError();
+// Few entries: one workgroup does all of it, and its second reading comes from the cache of its XCD.
+constexpr int ST = 1024;
+constexpr size_t SMALL = 128 << 10;      // bytes
+template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(Table t, bool write, double max_norm, float* __restrict__ norm_out) {
+    __shared__ double s[ST / 64];
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};      // four chains of dependent additions
+    uint32_t top = 0;
+    for (int k = 0; k < t.tensors; k++) read_chunk<MAX, ST>(t.e[k], 0, t.e[k].n, acc, top);
+    const double norm = norm_of_total<MAX>(group_total<MAX, ST>((acc[0] + acc[1]) + (acc[2] + acc[3]), top, s));
+    if (threadIdx.x == 0) *norm_out = (float)norm;
+    if (!write) return;
+    const bool clip = norm > max_norm && norm < INFINITY;
+    const double scale = clip ? max_norm / norm : 1.0;
+    for (int k = 0; k < t.tensors; k++) write_chunk<ST>(t.e[k], 0, t.e[k].n, clip, scale);
 }
 
 int element_size(int dtype) { return dtype == MPPI_F32 ? 4 : 2; }
@@ -210,15 +277,41 @@ int check_overlap(int32_t n, const void* const* g, void* const* out, const int64
     return 0;
 }
 
-template <bool MAX> int run(std::vector<Batch>& batches, int n_partials, double* partials, const double* max_norm, float* norm, hipStream_t s) {
-    for (const Batch& b : batches) HIP_OK(launch_partials<MAX>(b, partials, s));
-    if (!max_norm || batches.empty()) {
-        hipLaunchKernelGGL((gradient_norm_kernel<MAX>), dim3(1), dim3(BT), 0, s, (const double*)partials, n_partials, norm);
-        HIP_OK(hipGetLastError());
-        return 0;
-    }
-    for (size_t i = 0; i < batches.size(); i++) HIP_OK(launch_clip<MAX>(batches[i], partials, n_partials, *max_norm, i == 0 ? norm : nullptr, s));
+template <class Tab, bool MAX> int run(const Tab& t, double* partials, const double* max_norm, float* norm, hipStream_t s) {
+    const int groups = (int)std::min<unsigned>(t.chunks, (unsigned)GROUPS);
+    hipLaunchKernelGGL((gradient_partials_kernel<Tab, MAX>), dim3(groups), dim3(BT), 0, s, t, partials);
+    HIP_OK(hipGetLastError());
+    if (max_norm)
+        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX>), dim3(groups), dim3(BT), 0, s, t, (const double*)partials, groups, *max_norm, norm);
+    else
+        hipLaunchKernelGGL((gradient_norm_kernel<MAX>), dim3(1), dim3(BT), 0, s, (const double*)partials, groups, norm);
+    HIP_OK(hipGetLastError());
     return 0;
+}
+template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t bytes, char* workspace, const double* max_norm, float* norm, hipStream_t s) {
+    double* partials = (double*)workspace;
+    if (e.size() <= (size_t)TABLE) {
+        Table t;
+        std::copy(e.begin(), e.end(), t.e);
+        t.tensors = (int)e.size();
+        t.chunks = chunks;
+        if (bytes <= SMALL) {
+            hipLaunchKernelGGL((gradient_small_kernel<MAX>), dim3(1), dim3(ST), 0, s, t, max_norm != nullptr, max_norm ? *max_norm : 0.0, norm);
+            HIP_OK(hipGetLastError());
+            return 0;
+        }
+        return run<Table, MAX>(t, partials, max_norm, norm, s);
+    }
+    Entry* far = (Entry*)(workspace + GROUPS * sizeof(double));
+    for (size_t at = 0; at < e.size(); at += TABLE) {
+        Table t;
+        t.tensors = (int)std::min((size_t)TABLE, e.size() - at);
+        std::copy(e.begin() + at, e.begin() + at + t.tensors, t.e);
+        t.chunks = 0;
+        hipLaunchKernelGGL(table_kernel, dim3(1), dim3(BT), 0, s, t, (int)at, far);
+        HIP_OK(hipGetLastError());
+    }
+    return run<FarTable, MAX>(FarTable{far, (int)e.size(), chunks}, partials, max_norm, norm, s);
 }
 
 int gradients(int32_t device, int32_t n, const void* const* g, void* const* out, const int64_t* sizes, const int32_t* dtypes,
@@ -241,42 +334,26 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
         const int rc = check_overlap(n, g, out, sizes, dtypes);
         if (rc) return rc;
     }
-    std::vector<Batch> batches;
-    for (const int dtype : {MPPI_F32, MPPI_F16, MPPI_BF16}) {
-        Batch* b = nullptr;
-        for (int i = 0; i < n; i++) {
-            if (dtypes[i] != dtype || sizes[i] == 0) continue;
-            const long long chunks = (sizes[i] + CHUNK - 1) / CHUNK;
-            if (!b || b->t.tensors == TABLE || (long long)b->t.chunks + chunks > 0x7fffffffll) {
-                batches.emplace_back();
-                b = &batches.back();
-                b->dtype = dtype;
-                b->t.tensors = 0;
-                b->t.chunks = 0;
-            }
-            const int k = b->t.tensors++;
-            b->t.g[k] = g[i]; b->t.out[k] = max_norm ? out[i] : nullptr; b->t.n[k] = sizes[i]; b->t.first[k] = b->t.chunks;
-            b->t.chunks += (unsigned)chunks;
-        }
-    }
-    // every launch gets its share of the partial sums
-    int n_partials = 0;
-    const int most = batches.empty() ? 0 : std::max(1, MAX_GROUPS / (int)batches.size());
-    for (Batch& b : batches) {
-        b.groups = (int)std::min<unsigned>(b.t.chunks, (unsigned)most);
-        b.first_partial = n_partials;
-        n_partials += b.groups;
+    std::vector<Entry> entries;
+    entries.reserve(n);
+    long long chunks = 0;
+    size_t bytes = 0;
+    for (int i = 0; i < n; i++) {
+        if (sizes[i] == 0) continue;
+        entries.push_back({g[i], max_norm ? out[i] : nullptr, (long long)sizes[i], (unsigned)chunks, dtypes[i]});
+        chunks += (sizes[i] + CHUNK - 1) / CHUNK;
+        bytes += (size_t)sizes[i] * element_size(dtypes[i]);
+        if (chunks > 0x7fffffffll) return fail(-6, "more entries than one call can take");
     }
     size_t need = 0;
     (void)mppi_gradient_workspace(n, &need);
-    if ((size_t)n_partials * 8 > need) return fail(-8, "workspace formula");
-    if (n_partials > 0 && (!d_workspace || workspace_bytes < (size_t)n_partials * 8)) return fail(-1, "workspace too small (mppi_gradient_workspace)");
+    if (!d_workspace || workspace_bytes < need) return fail(-1, "workspace too small (mppi_gradient_workspace)");
     if ((uintptr_t)d_workspace & 7) return fail(-1, "workspace must be a multiple of 8 bytes");
     mppi::DeviceGuard guard;
     HIP_OK(guard.enter(device));
-    double* partials = (double*)d_workspace;
-    return norm_type == MPPI_NORM_MAX ? run<true>(batches, n_partials, partials, max_norm, d_norm, (hipStream_t)stream)
-                                      : run<false>(batches, n_partials, partials, max_norm, d_norm, (hipStream_t)stream);
+    char* ws = (char*)d_workspace;
+    return norm_type == MPPI_NORM_MAX ? run<true>(entries, (unsigned)chunks, bytes, ws, max_norm, d_norm, (hipStream_t)stream)
+                                      : run<false>(entries, (unsigned)chunks, bytes, ws, max_norm, d_norm, (hipStream_t)stream);
 }
 
 }  // namespace
@@ -285,8 +362,7 @@ extern "C" {
 
 int mppi_gradient_workspace(int32_t n, size_t* bytes) {
     if (n < 0 || !bytes) return fail(-1, "bad argument");
-    // launches of at least one partial sum each: up to n / TABLE full ones and one more per element type
-    *bytes = (size_t)(MAX_GROUPS + n / TABLE + 3) * 8;
+    *bytes = GROUPS * sizeof(double) + (n > TABLE ? (size_t)n * sizeof(Entry) : 0);
     return 0;
 }
 
