@@ -23,7 +23,7 @@ using mppi::fail;
 namespace {
 
 constexpr int BT = 256;                  // threads of a workgroup
-constexpr int CHUNK = 16384;             // entries of one tensor that a workgroup takes at a time
+constexpr int CHUNK = 65536;             // bytes of one tensor that a workgroup takes at a time
 constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums
 constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way
 constexpr int TABLE = 120;               // tensors whose table travels in a kernel's arguments (4 KB at most)
@@ -71,8 +71,13 @@ template <class T> struct Pack {         // 16 bytes of entries, wherever they l
     using B = typename Io<T>::B;
     static constexpr int PER = 4 / (int)sizeof(B);              // entries per word
     Words w;
-    __device__ __forceinline__ void load(const B* p) { w = *(const LooseWords*)p; }
-    __device__ __forceinline__ void store(B* p) const { *(LooseWords*)p = w; }
+    template <bool STREAM = false> __device__ __forceinline__ void load(const B* p) {
+        w = STREAM ? __builtin_nontemporal_load((const LooseWords*)p) : *(const LooseWords*)p;
+    }
+    template <bool STREAM> __device__ __forceinline__ void store(B* p) const {
+        if (STREAM) __builtin_nontemporal_store(w, (LooseWords*)p);
+        else *(LooseWords*)p = w;
+    }
     __device__ __forceinline__ B get(int j) const { return (B)(w[j / PER] >> (j % PER * 16)); }
     __device__ __forceinline__ void scale(double s) {
 #pragma unroll
@@ -95,8 +100,9 @@ template <class Tab> __device__ __forceinline__ const Entry& locate(const Tab& t
         if (t.e[m].first <= c) a = m; else b = m - 1;
     }
     const Entry& e = t.e[a];
-    lo = (long long)(c - e.first) * CHUNK;
-    hi = lo + CHUNK < e.n ? lo + CHUNK : e.n;
+    const int per = e.type == MPPI_F32 ? CHUNK / 4 : CHUNK / 2;
+    lo = (long long)(c - e.first) * per;
+    hi = lo + per < e.n ? lo + per : e.n;
     return e;
 }
 
@@ -149,7 +155,7 @@ template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(c
     for (; i < hi; i++) take<MAX>(acc[0], top, Io<T>::get(g[i]));      // the last, shorter pack
 }
 // times the scale, or bit for bit
-template <class T, bool SCALED, int NT> __device__ __forceinline__ void write_span(const void* from, void* to, long long lo, long long hi, double scale) {
+template <class T, bool SCALED, int NT, bool STREAM> __device__ __forceinline__ void write_span(const void* from, void* to, long long lo, long long hi, double scale) {
     using B = typename Io<T>::B;
     constexpr int VEC = Io<T>::VEC, STEP = NT * VEC;
     const B* g = (const B*)from;
@@ -158,18 +164,18 @@ template <class T, bool SCALED, int NT> __device__ __forceinline__ void write_sp
     for (; i + (AHEAD - 1) * STEP + VEC <= hi; i += AHEAD * STEP) {
         Pack<T> x[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) x[k].load(g + i + k * STEP);
+        for (int k = 0; k < AHEAD; k++) x[k].template load<STREAM>(g + i + k * STEP);
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             if (SCALED) x[k].scale(scale);
-            x[k].store(out + i + k * STEP);
+            x[k].template store<STREAM>(out + i + k * STEP);
         }
     }
     for (; i + VEC <= hi; i += STEP) {
         Pack<T> x;
-        x.load(g + i);
+        x.template load<STREAM>(g + i);
         if (SCALED) x.scale(scale);
-        x.store(out + i);
+        x.template store<STREAM>(out + i);
     }
     for (; i < hi; i++) out[i] = SCALED ? Io<T>::scaled(g[i], scale) : g[i];
 }
@@ -178,17 +184,17 @@ template <bool MAX, int NT> __device__ __forceinline__ void read_chunk(const Ent
     else if (e.type == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, lo, hi, acc, top);
     else read_span<__bf16, MAX, NT>(e.g, lo, hi, acc, top);
 }
-template <int NT> __device__ __forceinline__ void write_chunk(const Entry& e, long long lo, long long hi, bool clip, double scale) {
+template <int NT, bool STREAM> __device__ __forceinline__ void write_chunk(const Entry& e, long long lo, long long hi, bool clip, double scale) {
     if (!clip && e.out == e.g) return;
     if (e.type == MPPI_F32) {
-        if (clip) write_span<float, true, NT>(e.g, e.out, lo, hi, scale);
-        else write_span<float, false, NT>(e.g, e.out, lo, hi, scale);
+        if (clip) write_span<float, true, NT, STREAM>(e.g, e.out, lo, hi, scale);
+        else write_span<float, false, NT, STREAM>(e.g, e.out, lo, hi, scale);
     } else if (!clip) {
-        write_span<__bf16, false, NT>(e.g, e.out, lo, hi, scale);      // (bits are bits)
+        write_span<__bf16, false, NT, STREAM>(e.g, e.out, lo, hi, scale);      // (bits are bits)
     } else if (e.type == MPPI_F16) {
-        write_span<_Float16, true, NT>(e.g, e.out, lo, hi, scale);
+        write_span<_Float16, true, NT, STREAM>(e.g, e.out, lo, hi, scale);
     } else {
-        write_span<__bf16, true, NT>(e.g, e.out, lo, hi, scale);
+        write_span<__bf16, true, NT, STREAM>(e.g, e.out, lo, hi, scale);
     }
 }
 
@@ -222,7 +228,7 @@ template <bool MAX> __global__ void __launch_bounds__(BT) gradient_norm_kernel(c
 }
 
 // Every workgroup takes the chunks it took for the norm, the last one first: that one may still lie in its caches.
-template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_clip_kernel(Tab t, const double* __restrict__ partials, int n_partials,
+template <class Tab, bool MAX, bool STREAM> __global__ void __launch_bounds__(BT) gradient_clip_kernel(Tab t, const double* __restrict__ partials, int n_partials,
                                                                                        double max_norm, float* __restrict__ norm_out) {
     __shared__ double s[BT / 64];
     const double norm = norm_of<MAX>(partials, n_partials, s);
@@ -233,7 +239,7 @@ template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_cl
     for (unsigned c = last;; c -= gridDim.x) {
         long long lo, hi;
         const Entry& e = locate(t, c, lo, hi);
-        write_chunk<BT>(e, lo, hi, clip, scale);
+        write_chunk<BT, STREAM>(e, lo, hi, clip, scale);
         if (c < gridDim.x) break;
     }
 }
@@ -241,6 +247,7 @@ template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_cl
 // Few entries: one workgroup does all of it, and its second reading comes from the cache of its XCD.
 constexpr int ST = 1024;
 constexpr size_t SMALL = 128 << 10;      // bytes
+constexpr size_t STREAMED = 24 << 20;    // bytes
 template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(Table t, bool write, double max_norm, float* __restrict__ norm_out) {
     __shared__ double s[ST / 64];
     double acc[4] = {0.0, 0.0, 0.0, 0.0};      // four chains of dependent additions
@@ -251,7 +258,7 @@ template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(
     if (!write) return;
     const bool clip = norm > max_norm && norm < INFINITY;
     const double scale = clip ? max_norm / norm : 1.0;
-    for (int k = 0; k < t.tensors; k++) write_chunk<ST>(t.e[k], 0, t.e[k].n, clip, scale);
+    for (int k = 0; k < t.tensors; k++) write_chunk<ST, false>(t.e[k], 0, t.e[k].n, clip, scale);
 }
 
 int element_size(int dtype) { return dtype == MPPI_F32 ? 4 : 2; }
@@ -277,12 +284,14 @@ int check_overlap(int32_t n, const void* const* g, void* const* out, const int64
     return 0;
 }
 
-template <class Tab, bool MAX> int run(const Tab& t, double* partials, const double* max_norm, float* norm, hipStream_t s) {
+template <class Tab, bool MAX> int run(const Tab& t, size_t bytes, double* partials, const double* max_norm, float* norm, hipStream_t s) {
     const int groups = (int)std::min<unsigned>(t.chunks, (unsigned)GROUPS);
     hipLaunchKernelGGL((gradient_partials_kernel<Tab, MAX>), dim3(groups), dim3(BT), 0, s, t, partials);
     HIP_OK(hipGetLastError());
-    if (max_norm)
-        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX>), dim3(groups), dim3(BT), 0, s, t, (const double*)partials, groups, *max_norm, norm);
+    if (max_norm && bytes > STREAMED)
+        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX, true>), dim3(groups), dim3(BT), 0, s, t, (const double*)partials, groups, *max_norm, norm);
+    else if (max_norm)
+        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX, false>), dim3(groups), dim3(BT), 0, s, t, (const double*)partials, groups, *max_norm, norm);
     else
         hipLaunchKernelGGL((gradient_norm_kernel<MAX>), dim3(1), dim3(BT), 0, s, (const double*)partials, groups, norm);
     HIP_OK(hipGetLastError());
@@ -300,7 +309,7 @@ template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t
             HIP_OK(hipGetLastError());
             return 0;
         }
-        return run<Table, MAX>(t, partials, max_norm, norm, s);
+        return run<Table, MAX>(t, bytes, partials, max_norm, norm, s);
     }
     Entry* far = (Entry*)(workspace + GROUPS * sizeof(double));
     for (size_t at = 0; at < e.size(); at += TABLE) {
@@ -311,7 +320,7 @@ template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t
         hipLaunchKernelGGL(table_kernel, dim3(1), dim3(BT), 0, s, t, (int)at, far);
         HIP_OK(hipGetLastError());
     }
-    return run<FarTable, MAX>(FarTable{far, (int)e.size(), chunks}, partials, max_norm, norm, s);
+    return run<FarTable, MAX>(FarTable{far, (int)e.size(), chunks}, bytes, partials, max_norm, norm, s);
 }
 
 int gradients(int32_t device, int32_t n, const void* const* g, void* const* out, const int64_t* sizes, const int32_t* dtypes,
@@ -341,8 +350,9 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
     for (int i = 0; i < n; i++) {
         if (sizes[i] == 0) continue;
         entries.push_back({g[i], max_norm ? out[i] : nullptr, (long long)sizes[i], (unsigned)chunks, dtypes[i]});
-        chunks += (sizes[i] + CHUNK - 1) / CHUNK;
-        bytes += (size_t)sizes[i] * element_size(dtypes[i]);
+        const int64_t size = sizes[i] * element_size(dtypes[i]);
+        chunks += (size + CHUNK - 1) / CHUNK;
+        bytes += (size_t)size;
         if (chunks > 0x7fffffffll) return fail(-6, "more entries than one call can take");
     }
     size_t need = 0;
