@@ -131,12 +131,12 @@ template <bool MAX, int NT> __device__ double group_total(double acc, uint32_t t
 }
 template <bool MAX> __device__ __forceinline__ double norm_of_total(double v) { return MAX ? (double)__uint_as_float((uint32_t)v) : sqrt(v); }
 
-// entries [lo, hi) of a tensor, AHEAD packs of a thread under way at a time
-template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(const void* p, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
+// entries [lo, hi) of a tensor by NT threads (tid: which one), AHEAD packs of a thread under way at a time
+template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(const void* p, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
     using B = typename Io<T>::B;
     constexpr int VEC = Io<T>::VEC, STEP = NT * VEC;
     const B* g = (const B*)p;
-    long long i = lo + threadIdx.x * VEC;
+    long long i = lo + tid * VEC;
     for (; i + (AHEAD - 1) * STEP + VEC <= hi; i += AHEAD * STEP) {
         Pack<T> x[AHEAD];
 #pragma unroll
@@ -155,12 +155,12 @@ template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(c
     for (; i < hi; i++) take<MAX>(acc[0], top, Io<T>::get(g[i]));      // the last, shorter pack
 }
 // times the scale, or bit for bit
-template <class T, bool SCALED, int NT, bool STREAM> __device__ __forceinline__ void write_span(const void* from, void* to, long long lo, long long hi, double scale) {
+template <class T, bool SCALED, int NT, bool STREAM> __device__ __forceinline__ void write_span(const void* from, void* to, int tid, long long lo, long long hi, double scale) {
     using B = typename Io<T>::B;
     constexpr int VEC = Io<T>::VEC, STEP = NT * VEC;
     const B* g = (const B*)from;
     B* out = (B*)to;
-    long long i = lo + threadIdx.x * VEC;
+    long long i = lo + tid * VEC;
     for (; i + (AHEAD - 1) * STEP + VEC <= hi; i += AHEAD * STEP) {
         Pack<T> x[AHEAD];
 #pragma unroll
@@ -179,22 +179,22 @@ template <class T, bool SCALED, int NT, bool STREAM> __device__ __forceinline__ 
     }
     for (; i < hi; i++) out[i] = SCALED ? Io<T>::scaled(g[i], scale) : g[i];
 }
-template <bool MAX, int NT> __device__ __forceinline__ void read_chunk(const Entry& e, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
-    if (e.type == MPPI_F32) read_span<float, MAX, NT>(e.g, lo, hi, acc, top);
-    else if (e.type == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, lo, hi, acc, top);
-    else read_span<__bf16, MAX, NT>(e.g, lo, hi, acc, top);
+template <bool MAX, int NT> __device__ __forceinline__ void read_chunk(const Entry& e, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
+    if (e.type == MPPI_F32) read_span<float, MAX, NT>(e.g, tid, lo, hi, acc, top);
+    else if (e.type == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, tid, lo, hi, acc, top);
+    else read_span<__bf16, MAX, NT>(e.g, tid, lo, hi, acc, top);
 }
-template <int NT, bool STREAM> __device__ __forceinline__ void write_chunk(const Entry& e, long long lo, long long hi, bool clip, double scale) {
+template <int NT, bool STREAM> __device__ __forceinline__ void write_chunk(const Entry& e, int tid, long long lo, long long hi, bool clip, double scale) {
     if (!clip && e.out == e.g) return;
     if (e.type == MPPI_F32) {
-        if (clip) write_span<float, true, NT, STREAM>(e.g, e.out, lo, hi, scale);
-        else write_span<float, false, NT, STREAM>(e.g, e.out, lo, hi, scale);
+        if (clip) write_span<float, true, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
+        else write_span<float, false, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
     } else if (!clip) {
-        write_span<__bf16, false, NT, STREAM>(e.g, e.out, lo, hi, scale);      // (bits are bits)
+        write_span<__bf16, false, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);      // (bits are bits)
     } else if (e.type == MPPI_F16) {
-        write_span<_Float16, true, NT, STREAM>(e.g, e.out, lo, hi, scale);
+        write_span<_Float16, true, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
     } else {
-        write_span<__bf16, true, NT, STREAM>(e.g, e.out, lo, hi, scale);
+        write_span<__bf16, true, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
     }
 }
 
@@ -209,7 +209,7 @@ template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_pa
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         long long lo, hi;
         const Entry& e = locate(t, c, lo, hi);
-        read_chunk<MAX, BT>(e, lo, hi, acc, top);
+        read_chunk<MAX, BT>(e, threadIdx.x, lo, hi, acc, top);
     }
     const double v = group_total<MAX, BT>((acc[0] + acc[1]) + (acc[2] + acc[3]), top, s);
     if (threadIdx.x == 0) partials[blockIdx.x] = v;
@@ -239,47 +239,85 @@ template <class Tab, bool MAX, bool STREAM> __global__ void __launch_bounds__(BT
     for (unsigned c = last;; c -= gridDim.x) {
         long long lo, hi;
         const Entry& e = locate(t, c, lo, hi);
-        write_chunk<BT, STREAM>(e, lo, hi, clip, scale);
+        write_chunk<BT, STREAM>(e, threadIdx.x, lo, hi, clip, scale);
         if (c < gridDim.x) break;
     }
 }
 
-// Few entries: one workgroup does all of it, and its second reading comes from the cache of its XCD.
-constexpr int ST = 1024;
-constexpr size_t SMALL = 128 << 10;      // bytes
-constexpr size_t STREAMED = 24 << 20;    // bytes
+// Few entries: one workgroup does all of it, a wave for every PIECE, and its second reading comes from the cache of its XCD.  A
+// round of pieces takes about a microsecond; MOST_PIECES is three rounds, where two launches take as long.
+constexpr int ST = 1024, PIECE = 4096 /* bytes */, MOST_PIECES = 48;
+constexpr size_t MOST_BYTES = 128 << 10;
 template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(Table t, bool write, double max_norm, float* __restrict__ norm_out) {
     __shared__ double s[ST / 64];
-    double acc[4] = {0.0, 0.0, 0.0, 0.0};      // four chains of dependent additions
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Lane l knows tensor l and where its pieces lie among all of them: the tensor of a piece is then a ballot away, where a search
+    // through the arguments would wait for a scalar load at every step.
+    const Entry& own = t.e[lane < t.tensors ? lane : 0];
+    const unsigned long long g = (unsigned long long)own.g, out = (unsigned long long)own.out;
+    const int n = (int)own.n, type = own.type, per = type == MPPI_F32 ? PIECE / 4 : PIECE / 2;
+    const int count = lane < t.tensors ? (n + per - 1) / per : 0;
+    int end = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(end, d, 64);
+        if (lane >= d) end += o;
+    }
+    const auto far = [](unsigned long long v, int l) {
+        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, l), hi = (unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l);
+        return (unsigned long long)hi << 32 | lo;
+    };
+    const int all = __builtin_amdgcn_readlane(end, 63);
+    const auto pieces = [&](auto f) {                // f(tensor, entries of a piece): this wave's pieces
+        for (int p = wave; p < all; p += ST / 64) {
+            const int k = __popcll(__ballot(end <= p));
+            Entry e;
+            e.g = (const void*)far(g, k);
+            e.out = (void*)far(out, k);
+            e.n = __builtin_amdgcn_readlane(n, k);
+            e.type = __builtin_amdgcn_readlane(type, k);
+            e.first = 0;
+            const int size = e.type == MPPI_F32 ? PIECE / 4 : PIECE / 2;
+            const long long lo = (long long)(p - __builtin_amdgcn_readlane(end - count, k)) * size;
+            f(e, lo, lo + size < e.n ? lo + size : e.n);
+        }
+    };
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
     uint32_t top = 0;
-    for (int k = 0; k < t.tensors; k++) read_chunk<MAX, ST>(t.e[k], 0, t.e[k].n, acc, top);
+    pieces([&](const Entry& e, long long lo, long long hi) { read_chunk<MAX, 64>(e, lane, lo, hi, acc, top); });
     const double norm = norm_of_total<MAX>(group_total<MAX, ST>((acc[0] + acc[1]) + (acc[2] + acc[3]), top, s));
     if (threadIdx.x == 0) *norm_out = (float)norm;
     if (!write) return;
     const bool clip = norm > max_norm && norm < INFINITY;
     const double scale = clip ? max_norm / norm : 1.0;
-    for (int k = 0; k < t.tensors; k++) write_chunk<ST, false>(t.e[k], 0, t.e[k].n, clip, scale);
+    pieces([&](const Entry& e, long long lo, long long hi) { write_chunk<64, false>(e, lane, lo, hi, clip, scale); });
 }
+constexpr size_t STREAMED = 24 << 20;    // bytes
 
 int element_size(int dtype) { return dtype == MPPI_F32 ? 4 : 2; }
 
 // What is written may be read only as the same tensor (in place) and written only once.
 int check_overlap(int32_t n, const void* const* g, void* const* out, const int64_t* sizes, const int32_t* dtypes) {
-    struct Span { uintptr_t lo, hi; int who; bool written; };
-    std::vector<Span> spans;
-    spans.reserve(2 * (size_t)n);
+    struct Span { uintptr_t lo, hi; int who; };
+    const auto by_address = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+    std::vector<Span> written, read;
+    written.reserve(n);
     for (int i = 0; i < n; i++) {
         if (sizes[i] == 0) continue;
         const uintptr_t bytes = (uintptr_t)sizes[i] * element_size(dtypes[i]);
-        spans.push_back({(uintptr_t)out[i], (uintptr_t)out[i] + bytes, i, true});
-        if (g[i] != out[i]) spans.push_back({(uintptr_t)g[i], (uintptr_t)g[i] + bytes, i, false});
+        written.push_back({(uintptr_t)out[i], (uintptr_t)out[i] + bytes, i});
+        if (g[i] != out[i]) read.push_back({(uintptr_t)g[i], (uintptr_t)g[i] + bytes, i});
     }
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
-    uintptr_t any_end = 0, written_end = 0;
-    for (const Span& x : spans) {
-        if (x.lo < written_end || (x.written && x.lo < any_end)) return fail(-1, "clipped gradients overlap each other or their inputs (tensor " + std::to_string(x.who) + ")");
-        any_end = std::max(any_end, x.hi);
-        if (x.written) written_end = std::max(written_end, x.hi);
+    for (std::vector<Span>* v : {&written, &read})               // (allocations and views of a buffer mostly ascend)
+        if (!std::is_sorted(v->begin(), v->end(), by_address)) std::sort(v->begin(), v->end(), by_address);
+    const auto refuse = [](int i) { return fail(-1, "clipped gradients overlap each other or their inputs (tensor " + std::to_string(i) + ")"); };
+    for (size_t i = 1; i < written.size(); i++)
+        if (written[i].lo < written[i - 1].hi) return refuse(written[i].who);
+    size_t w = 0;                                                // the first written span that ends behind the read one's start
+    for (const Span& r : read) {
+        // spans that are read may overlap each other, but their starts ascend
+        while (w < written.size() && written[w].hi <= r.lo) w++;
+        if (w < written.size() && written[w].lo < r.hi) return refuse(r.who);
     }
     return 0;
 }
@@ -297,14 +335,14 @@ template <class Tab, bool MAX> int run(const Tab& t, size_t bytes, double* parti
     HIP_OK(hipGetLastError());
     return 0;
 }
-template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t bytes, char* workspace, const double* max_norm, float* norm, hipStream_t s) {
+template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t pieces, size_t bytes, char* workspace, const double* max_norm, float* norm, hipStream_t s) {
     double* partials = (double*)workspace;
     if (e.size() <= (size_t)TABLE) {
         Table t;
         std::copy(e.begin(), e.end(), t.e);
         t.tensors = (int)e.size();
         t.chunks = chunks;
-        if (bytes <= SMALL) {
+        if (pieces <= MOST_PIECES && bytes <= MOST_BYTES && t.tensors <= 64) {
             hipLaunchKernelGGL((gradient_small_kernel<MAX>), dim3(1), dim3(ST), 0, s, t, max_norm != nullptr, max_norm ? *max_norm : 0.0, norm);
             HIP_OK(hipGetLastError());
             return 0;
@@ -346,13 +384,14 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
     std::vector<Entry> entries;
     entries.reserve(n);
     long long chunks = 0;
-    size_t bytes = 0;
+    size_t bytes = 0, pieces = 0;
     for (int i = 0; i < n; i++) {
         if (sizes[i] == 0) continue;
         entries.push_back({g[i], max_norm ? out[i] : nullptr, (long long)sizes[i], (unsigned)chunks, dtypes[i]});
         const int64_t size = sizes[i] * element_size(dtypes[i]);
         chunks += (size + CHUNK - 1) / CHUNK;
         bytes += (size_t)size;
+        pieces += (size_t)(size + PIECE - 1) / PIECE;
         if (chunks > 0x7fffffffll) return fail(-6, "more entries than one call can take");
     }
     size_t need = 0;
@@ -362,8 +401,8 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
     mppi::DeviceGuard guard;
     HIP_OK(guard.enter(device));
     char* ws = (char*)d_workspace;
-    return norm_type == MPPI_NORM_MAX ? run<true>(entries, (unsigned)chunks, bytes, ws, max_norm, d_norm, (hipStream_t)stream)
-                                      : run<false>(entries, (unsigned)chunks, bytes, ws, max_norm, d_norm, (hipStream_t)stream);
+    return norm_type == MPPI_NORM_MAX ? run<true>(entries, (unsigned)chunks, pieces, bytes, ws, max_norm, d_norm, (hipStream_t)stream)
+                                      : run<false>(entries, (unsigned)chunks, pieces, bytes, ws, max_norm, d_norm, (hipStream_t)stream);
 }
 
 }  // namespace

@@ -129,52 +129,57 @@ PyObject* draw(PyObject* const* args) {
     return out;
 }
 
-std::vector<at::Tensor> tensors(PyObject* o, const char* what) {
-    std::vector<at::Tensor> list;
-    auto add = [&](PyObject* item) {
-        if (!is_tensor(item)) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
-        const at::Tensor& t = tensor(item);
-        if (!t.is_cuda() || t.layout() != at::kStrided) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
-        if (!t.is_non_overlapping_and_dense())
-            raise(PyExc_ValueError, std::string(what) + " must fill their memory without gaps or overlaps (a slice or an expanded tensor does not)");
-        list.push_back(t);
-    };
-    if (is_tensor(o)) {
-        add(o);
-        return list;
+// The tensors of a list, borrowed: `owner` keeps the list alive.
+struct List {
+    std::vector<const at::Tensor*> t;
+    PyObject* owner = nullptr;
+    ~List() { Py_XDECREF(owner); }
+    List() = default;
+    List(const List&) = delete;
+    void fill(PyObject* o, const char* what) {
+        PyObject* const* items = &o;
+        Py_ssize_t n = 1;
+        if (!is_tensor(o)) {
+            owner = PySequence_Fast(o, "a list of tensors is needed");
+            if (!owner) throw Raised();
+            items = PySequence_Fast_ITEMS(owner);
+            n = PySequence_Fast_GET_SIZE(owner);
+        }
+        t.reserve(n);
+        for (Py_ssize_t i = 0; i < n; i++) {
+            if (!is_tensor(items[i])) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
+            const at::Tensor& x = tensor(items[i]);
+            if (!x.is_cuda() || x.layout() != at::kStrided) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
+            if (!x.is_non_overlapping_and_dense())
+                raise(PyExc_ValueError, std::string(what) + " must fill their memory without gaps or overlaps (a slice or an expanded tensor does not)");
+            t.push_back(&x);
+        }
     }
-    PyObject* seq = PySequence_Fast(o, "a list of tensors is needed");
-    if (!seq) throw Raised();
-    struct Owned { PyObject* o; ~Owned() { Py_DECREF(o); } } owned{seq};
-    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
-    list.reserve(n);
-    for (Py_ssize_t i = 0; i < n; i++) add(PySequence_Fast_GET_ITEM(seq, i));
-    return list;
-}
+};
 
 // gradients(grads, out or None, norm type, max_norm or None) -> norm
 PyObject* gradients(PyObject* const* args) {
-    const std::vector<at::Tensor> grads = tensors(args[0], "gradients");
-    if (grads.empty()) raise(PyExc_ValueError, "no gradients");
-    if (grads.size() > INT32_MAX) raise(PyExc_ValueError, "too many gradients");
     const bool clip = args[3] != Py_None, elsewhere = args[1] != Py_None;
-    const std::vector<at::Tensor> outs = elsewhere ? tensors(args[1], "outputs") : std::vector<at::Tensor>();
-    if (elsewhere && outs.size() != grads.size())
-        raise(PyExc_ValueError, std::to_string(grads.size()) + " gradients, " + std::to_string(outs.size()) + " outputs");
-    const at::Device device = grads[0].device();
-    const size_t n = grads.size();
+    List grads, outs;
+    grads.fill(args[0], "gradients");
+    if (grads.t.empty()) raise(PyExc_ValueError, "no gradients");
+    if (grads.t.size() > INT32_MAX) raise(PyExc_ValueError, "too many gradients");
+    if (elsewhere) outs.fill(args[1], "outputs");
+    const size_t n = grads.t.size();
+    if (elsewhere && outs.t.size() != n) raise(PyExc_ValueError, std::to_string(n) + " gradients, " + std::to_string(outs.t.size()) + " outputs");
+    const at::Device device = grads.t[0]->device();
     std::vector<const void*> in(n);
     std::vector<void*> out(n);
     std::vector<int64_t> sizes(n);
     std::vector<int32_t> types(n);
     for (size_t i = 0; i < n; i++) {
-        const at::Tensor& g = grads[i];
+        const at::Tensor& g = *grads.t[i];
         if (g.device() != device) raise(PyExc_ValueError, "all tensors must lie on one device");
         types[i] = element_type(g, false);
         sizes[i] = g.numel();
         in[i] = g.const_data_ptr();
         if (!clip) continue;
-        const at::Tensor& o = elsewhere ? outs[i] : g;
+        const at::Tensor& o = elsewhere ? *outs.t[i] : g;
         if (elsewhere) {
             if (o.device() != device) raise(PyExc_ValueError, "all tensors must lie on one device");
             if (o.scalar_type() != g.scalar_type() || o.sizes() != g.sizes() || o.strides() != g.strides())
@@ -191,8 +196,8 @@ PyObject* gradients(PyObject* const* args) {
         const double most = number(args[3]);
         check(clip_gradients(device.index(), (int32_t)n, in.data(), out.data(), sizes.data(), types.data(), kind, most,
                              (float*)norm.mutable_data_ptr(), ws.mutable_data_ptr(), bytes, stream_of(device)));
-        for (const at::Tensor& o : elsewhere ? outs : grads)
-            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();        // written in place: autograd has to know
+        for (const at::Tensor* o : elsewhere ? outs.t : grads.t)
+            if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();        // written in place: autograd has to know
     } else {
         check(gradient_norm(device.index(), (int32_t)n, in.data(), sizes.data(), types.data(), kind, (float*)norm.mutable_data_ptr(),
                             ws.mutable_data_ptr(), bytes, stream_of(device)));
