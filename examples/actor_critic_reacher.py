@@ -9,7 +9,11 @@ sparse, alpha cooled by `eta` per epoch) and whose last reward is replaced by th
 environment reports the sparse reward; the solution goes into a replay buffer twice, as in the reference, and the
 critic takes temporal-difference steps against a target copy of itself.
 
+With --draw K the epochs explore: every step applies one sampled sequence, drawn with the planner's weights among its K
+best, instead of their mean.  With --device cuda the critic trains on the GPU, and --clip bounds the norm of its gradients.
+
     python examples/actor_critic_reacher.py [--epochs 4] [--steps 100] [--iters 200] [--noise host|philox]
+                                            [--draw K] [--device cpu|cuda] [--clip NORM]
 """
 import argparse
 import os
@@ -53,21 +57,24 @@ def dense_solution(steps, noise):
     return agent
 
 
-def critic_steps(critic, target, replay, optimizer, iters):
+def critic_steps(critic, target, replay, optimizer, iters, max_norm=None):
     """Temporal-difference regression of the critic on minibatches of the replay buffer; rewards above 10 mark the
     goal and end the bootstrap.  The target copy follows the critic eight times per call."""
     loss_fn = torch.nn.MSELoss()
+    device = next(critic.parameters()).device
     loss = None
     for i in range(iters):
         batch = replay.get_minibatch(size=min(critic.batch_size, len(replay.buffer)))
-        state = torch.tensor(np.array([d.state for d in batch]), dtype=torch.float32)
-        nxt = torch.tensor(np.array([d.next_state for d in batch]), dtype=torch.float32)
-        reward = torch.tensor([float(d.reward) for d in batch], dtype=torch.float32).unsqueeze(1)
+        state = torch.tensor(np.array([d.state for d in batch]), dtype=torch.float32, device=device)
+        nxt = torch.tensor(np.array([d.next_state for d in batch]), dtype=torch.float32, device=device)
+        reward = torch.tensor([float(d.reward) for d in batch], dtype=torch.float32, device=device).unsqueeze(1)
         with torch.no_grad():
             boot = torch.where(reward > 10.0, torch.zeros_like(reward), critic.gamma * target(nxt))
         loss = loss_fn(critic(state), reward + boot)
         optimizer.zero_grad()
         loss.backward()
+        if max_norm is not None:
+            critic.clip_gradients(max_norm)
         optimizer.step()
         if i % max(iters // 8, 1) == 0:
             target.load_state_dict(critic.state_dict())
@@ -83,7 +90,12 @@ def main(argv=None):
     ap.add_argument('--lr', type=float, default=1e-2)
     ap.add_argument('--dim', type=int, default=14)
     ap.add_argument('--noise', default='host')
+    ap.add_argument('--draw', type=int, default=0, help="apply a sequence drawn among this many best samples (0: their mean)")
+    ap.add_argument('--device', default='cpu', help="where the critic trains")
+    ap.add_argument('--clip', type=float, default=None, help="largest norm of the critic's gradients (needs --device cuda)")
     args = ap.parse_args(argv)
+    if args.clip is not None and args.device == 'cpu':
+        ap.error("--clip needs --device cuda: gradients are clipped on the GPU")
 
     t0 = time.time()
     reference = hand_positions(dense_solution(args.steps + H, args.noise))
@@ -98,6 +110,7 @@ def main(argv=None):
     for net in (critic, target):
         net.eval()
         net.float()
+        net.to(args.device)
     optimizer = torch.optim.Adam(critic.parameters(), lr=args.lr)
     replay = ReplayBuffer(max_size=10000)
 
@@ -108,11 +121,12 @@ def main(argv=None):
         goal = e.get_env_state()['target_pos']
         agent = planner(e, args.noise, reward_type='cooling', reference=reference)
         for _ in range(args.steps):
-            agent.train_step(critic=critic, niter=N_ITER, goal=goal, dim=args.dim)
+            agent.train_step(critic=critic, niter=N_ITER, goal=goal, dim=args.dim,
+                             draw=dict(top_k=args.draw) if args.draw else None)
         samples = critic.compress_agent(agent, dim=args.dim)
         samples += critic.compress_agent(agent, dim=args.dim)   # the solution goes in twice
         replay.concatenate(samples)
-        loss = critic_steps(critic, target, replay, optimizer, critic.num_iters)
+        loss = critic_steps(critic, target, replay, optimizer, critic.num_iters, args.clip)
         ret, dist = float(np.sum(agent.sol_reward)), float(agent.sol_obs[-1][-1])
         print("epoch %d: alpha %.3f, sparse return %.0f, final distance %.3f m, critic loss %s, %.2f s"
               % (epoch, alpha, ret, dist, "%.3g" % loss if loss is not None else "-", time.time() - t0))

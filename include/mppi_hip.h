@@ -53,6 +53,7 @@ enum {
     MPPI_READ_STATUS = 6,       /* int32[1]             MPPI_STATUS_* bits, sticky since the planner was created */
     MPPI_READ_RMAX = 7,         /* double[1]            best return                                      */
     MPPI_READ_PARTIALS = 8,     /* double[3+H*M]        this shard's (Rmax, argmax, den, num[H*M])      */
+    MPPI_READ_DRAW = 10,        /* double[2]            sample that mppi_draw picked (-1: none) and its weight      */
     MPPI_READ_STATUS_DETAIL = 9 /* int32[4]             status bits; for the first capped solve reported by a     */
                                 /*                      rollout with dumps, a reference or a sparse reward: 1 +    */
                                 /*                      first sample of its wave, env step, planner (else zeros)   */
@@ -204,6 +205,15 @@ int mppi_rollout(mppi_planner* p, void* stream);
 /* niter x [rollouts, `MPPI.update`] with the same noise, as the loop of `MPPI.train_step`
  * (trajopt/algos/mppi.py:131-193, 56-65); single-rank form. */
 int mppi_iterate(mppi_planner* p, int32_t niter, void* stream);
+/* Rollouts and, in the place of `MPPI.update`, a draw: act_sequence becomes the sequence of ONE sample, drawn with the
+ * weights the update would average with, exp(kappa (R_k - Rmax)), among the samples that top_k, top_p and min_p keep (see
+ * mppi_draw_filter; 0, 1, 0 keep all).  u: one uniform number in [0, 1) per planner, host or device memory.  The reference only
+ * ever applies the mean (trajopt/algos/mppi.py:56-65); applied draws explore, which is what a critic's replay buffer wants.
+ * MPPI_READ_DRAW tells the sample and its weight; a planner whose samples all diverged keeps its act_sequence (-1).  Works on
+ * explicit action sequences (mppi_upload_actions) as well.  -4 on a planner that owns only a shard of its samples
+ * (mppi_comm_init, cfg.k_offset).  The first call on a planner allocates; best return and sample (MPPI_READ_RMAX,
+ * MPPI_READ_ARGMAX) stay those of the last update. */
+int mppi_draw(mppi_planner* p, const double* u, int64_t top_k, double top_p, double min_p, void* stream);
 /* Sharded form of one iteration: rollouts + this shard's sufficient statistics
  * (Rmax, argmax, sum S, sum S*eps) into the buffer at mppi_partials_ptr; after the caller
  * has all-gathered the nranks buffers (rank order), mppi_merge applies `MPPI.update`.

@@ -17,7 +17,7 @@ NORMS = {"l2": 0, "max": 1}
 REWARD_TYPES = {"dense": 0, "sparse": 1, "tracking": 2, "cooling": 3}
 TAIL = {"repeat": 0, "mean": 1}
 (READ_RETURNS, READ_ACT_SEQ, READ_ARGMAX, READ_ACTIONS, READ_NEXT_OBS, READ_REWARDS, READ_STATUS, READ_RMAX,
- READ_PARTIALS, READ_STATUS_DETAIL) = range(10)
+ READ_PARTIALS, READ_STATUS_DETAIL, READ_DRAW) = range(11)
 
 LIB_PATH = os.environ.get("MPPI_HIP_LIBRARY") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmppi_hip.so")
 
@@ -84,6 +84,7 @@ _PROTOS = {
     "mppi_upload_actions": (C.c_int, [_vp, _vp, _vp]),
     "mppi_rollout": (C.c_int, [_vp, _vp]),
     "mppi_iterate": (C.c_int, [_vp, _i32, _vp]),
+    "mppi_draw": (C.c_int, [_vp, _vp, C.c_int64, _d, _d, _vp]),
     "mppi_local_partials": (C.c_int, [_vp, _vp]),
     "mppi_partials_ptr": (C.c_int, [_vp, C.POINTER(_vp), C.POINTER(C.c_size_t)]),
     "mppi_merge": (C.c_int, [_vp, _vp, _i32, _vp]),

@@ -154,15 +154,23 @@ class MPPI(Trajectory):
                                      seed, goal, self.reward_type, self.reference, self.env.alpha,
                                      self.paths_per_cpu, self.num_cpu)
 
-    def train_step(self, critic=None, niter=1, act_sequence=None, goal=None, dim=14):
+    def train_step(self, critic=None, niter=1, act_sequence=None, goal=None, dim=14, draw=None):
+        """One planning step.  `draw` (an addition; None plans as the reference does) replaces the last iteration's update by
+        a draw: act_sequence becomes one sampled sequence, picked with the update's weights.  It is a dict with any of top_k,
+        top_p, min_p (which samples may be picked, see `trajopt_amd.device.draw_from_returns`) and u, the uniform number to
+        draw with (default: a generator of its own seeded with the step's seed; numpy's global one is left alone)."""
         t = len(self.sol_state) - 1
         weights = _critic_weights(critic, dim)
+        if draw is not None:
+            draw = self._draw_arguments(draw, self.seed + t, niter)
+            if self.env.env_name not in _KERNEL_ENVS or (critic is not None and weights is None):
+                raise ValueError("a draw needs rollouts on the device: not with this environment or critic")
         if self.env.env_name in _KERNEL_ENVS and (critic is None or weights is not None):
             if act_sequence is None and self._real_env_steps_on_the_device():
                 # the whole step, the real environment's included, without leaving the device
-                self._plan_on_device(self.seed + t, niter, dim if critic is not None else 0, weights, advance=True)
+                self._plan_on_device(self.seed + t, niter, dim if critic is not None else 0, weights, advance=True, draw=draw)
                 return []
-            self._plan_on_device(self.seed + t, niter, dim if critic is not None else 0, weights)
+            self._plan_on_device(self.seed + t, niter, dim if critic is not None else 0, weights, draw=draw)
         else:
             # an arbitrary Python critic can only be evaluated on the host: rollouts come back as paths
             for _ in range(niter):
@@ -171,6 +179,19 @@ class MPPI(Trajectory):
                 self.update(paths, use_critic=(critic is not None))
         self.advance_time(act_sequence=act_sequence)
         return []
+
+    @staticmethod
+    def _draw_arguments(draw, seed, niter):
+        d = dict(top_k=0, top_p=1.0, min_p=0.0, u=None)
+        unknown = set(draw) - set(d)
+        if unknown:
+            raise ValueError("unknown draw argument %s" % sorted(unknown))
+        if niter < 1:
+            raise ValueError("a draw takes the place of the last iteration: niter must be at least 1")
+        d.update(draw)
+        if d["u"] is None:
+            d["u"] = np.random.default_rng(seed % 2 ** 64).random()
+        return d
 
     # ---- device-resident iteration ------------------------------------------------------
     def _real_env_steps_on_the_device(self):
@@ -210,10 +231,10 @@ class MPPI(Trajectory):
         return (d is not None and d[0] == id(p) and np.shape(self.act_sequence) == (self.H, self.m)
                 and np.asarray(self.act_sequence, dtype=np.float64).tobytes() == d[1])
 
-    def _plan_on_device(self, seed, niter, critic_dim=0, critic_weights=None, advance=False):
+    def _plan_on_device(self, seed, niter, critic_dim=0, critic_weights=None, advance=False, draw=None):
         """niter iterations on the device from sol_state[-1] and act_sequence.  advance: also `advance_time` there
         (real-env step with the new act_sequence[0], logs, shift); otherwise act_sequence is read back and the
-        caller advances."""
+        caller advances.  draw: the last iteration draws a sample instead of updating."""
         s = self.sol_state[-1]
         H = self.H
         rt, reference = rollout_objective(self.env.env_name, self.reward_type, self.reference)
@@ -234,8 +255,20 @@ class MPPI(Trajectory):
         p.set_critic(critic_dim, critic_weights)         # a no-op while dim and weights stay what they were
         if advance:
             p.set_env_reward(self._env_reward())
+        def iterations():
+            if draw is None:
+                p.iterate(niter)
+            else:
+                p.iterate(niter - 1)
+                p.draw(draw["u"], draw["top_k"], draw["top_p"], draw["min_p"])
+
         if self.noise == 'philox':
-            if advance:
+            if draw is not None:
+                p.generate_noise(seed)
+                iterations()
+                if advance:
+                    p.advance()
+            elif advance:
                 # the device keys its stream with seed argument + time step of its state; one launch of the captured step
                 p.plan(seed - int(s['timestep']), niter, 1)
             else:
@@ -248,23 +281,23 @@ class MPPI(Trajectory):
             # numpy generator is moved when the draws are consumed, as if they had been made then (one worker runs
             # in-process in the reference, trajopt/utils.py:171-172, and leaves the global generator behind its draws;
             # pool workers re-seed only their own copies).
-            def draw(sd):
+            def host_noise(sd):
                 return p.draw_noise(worker_seeds(sd, self.paths_per_cpu, self.num_cpu), _host_threads(),
                                     want_state=self.num_cpu == 1)
             want = (id(p), seed, self.paths_per_cpu, self.num_cpu, H, self.m)
             if self._ahead is not None and self._ahead[0] == want:
                 state = self._ahead[1]
             else:
-                state = draw(seed)
+                state = host_noise(seed)
             self._ahead = None
             if state is not None:
                 _set_numpy_state(state)
             p.commit_noise()
-            p.iterate(niter)
+            iterations()
             if advance:
                 p.advance()
             if self.draw_ahead and 0 <= seed + 1 + (self.num_cpu - 1) * self.paths_per_cpu < 2 ** 32:
-                self._ahead = ((id(p), seed + 1, self.paths_per_cpu, self.num_cpu, H, self.m), draw(seed + 1))
+                self._ahead = ((id(p), seed + 1, self.paths_per_cpu, self.num_cpu, H, self.m), host_noise(seed + 1))
         if not advance:
             self.act_sequence = p.act_sequence()
             self._dev_seq = (id(p), self.act_sequence.tobytes())

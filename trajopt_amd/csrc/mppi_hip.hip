@@ -14,6 +14,7 @@
 //   shift_kernel                                receding-horizon shift + tail fill
 //   env_step_kernel<MD>                         one fp64 env.step for the real environment
 //   critic_kernel                               terminal value of the 128-wide tanh MLP
+//   draw_apply_kernel                           act_sequence from one drawn sample (the draw itself: draw.hip)
 //
 // Layout in HBM: eps is stored step-major, sample-minor ([H][M][K]) so that the 64 lanes of
 // a wave read 64 consecutive values per (t, j); returns are [K]; act_sequence is [H][M] fp64.
@@ -56,6 +57,20 @@ extern "C" void mppi_philox4x32(const uint32_t ctr[4], const uint32_t key[2], ui
     uint32_t c[4] = {ctr[0], ctr[1], ctr[2], ctr[3]};
     philox4x32_10(c, key[0], key[1]);
     for (int i = 0; i < 4; i++) out[i] = c[i];
+}
+
+// act_sequence <- the sequence of the drawn sample: base + eps_k, formed in the rollouts' type as they form it
+template <class T>
+__global__ void __launch_bounds__(256) draw_apply_kernel(const int64_t* __restrict__ index, const T* __restrict__ eps, int K, int HM, int explicit_act,
+                                                         double* __restrict__ base) {
+    const int64_t k = index[blockIdx.y];
+    if (k < 0) return;
+    eps += (size_t)blockIdx.y * HM * K;
+    base += (size_t)blockIdx.y * HM;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < HM; i += gridDim.x * 256) {
+        const T e = eps[(size_t)i * K + k];
+        base[i] = explicit_act ? (double)e : (double)((T)base[i] + e);
+    }
 }
 
 // act_sequence = sum_k S_k (base + eps_k) / (sum S + 1e-6) from nranks shard statistics, rank order
@@ -340,6 +355,8 @@ struct mppi_planner {
     int comm_rank, comm_nranks;
     double* d_gathered;             // [nranks][P][3 + HM]; d_part then points at this rank's row of it (in-place gather)
     double* d_part_alloc;           // the allocation d_part pointed at before
+    char* d_draw;                   // mppi_draw: workspace, then [P] index, [P] u, [P] weight (made on the first call)
+    size_t draw_workspace;
     bool profiling;
     std::vector<hipEvent_t>* prof_events;   // start/stop pairs around every rollout launch
     std::vector<DevState>* h_state;         // host mirror of the fields the host sets (alpha, ref_len, start state)
@@ -571,6 +588,7 @@ void mppi_planner_destroy(mppi_planner* p) {
     if (p->ev_raw_free) (void)hipEventDestroy(p->ev_raw_free);
     if (p->ev_upload_done) (void)hipEventDestroy(p->ev_upload_done);
     if (p->d_weights) (void)hipFree(p->d_weights);
+    if (p->d_draw) (void)hipFree(p->d_draw);
     void* bufs[] = {p->d_state, p->d_base, p->d_base_tmp, p->d_mean, p->d_eps, p->d_raw, p->d_ref, p->d_R,
                     p->d_part_alloc ? p->d_part_alloc : p->d_part, p->d_result, p->d_obs, p->d_rew, p->d_status, p->d_log, p->d_log_count, p->d_fobs, p->d_critic, p->d_next_step, p->d_last_row, p->d_noise_key};
     for (void* b : bufs)
@@ -1010,6 +1028,47 @@ int mppi_merge(mppi_planner* p, const void* gathered, int32_t nranks, void* stre
     return fail(-8, std::string("host exception: ") + e.what());
 }
 
+static int64_t* draw_index(mppi_planner* p) { return (int64_t*)(p->d_draw + p->draw_workspace); }
+static double* draw_numbers(mppi_planner* p) { return (double*)(draw_index(p) + p->P); }
+static float* draw_weight(mppi_planner* p) { return (float*)(draw_numbers(p) + p->P); }
+
+int mppi_draw(mppi_planner* p, const double* u, int64_t top_k, double top_p, double min_p, void* stream) try {
+    if (!p || !u) return fail(-1, "null argument");
+    if (p->comm || p->cfg.k_offset != 0) return fail(-4, "mppi_draw needs every sample of the planner on one GPU");
+    mppi_draw_filter f;
+    std::memset(&f, 0, sizeof(f));
+    f.kappa = p->cfg.kappa; f.top_k = top_k; f.top_p = top_p; f.min_p = min_p;
+    // the checks of the draw itself come before anything is launched (no rows: nothing else)
+    int rc = mppi_draw_from_returns(p->cfg.device, nullptr, p->cfg.dtype, 0, p->cfg.K, 0, 0, nullptr, 1, &f, nullptr, nullptr, nullptr, 0, nullptr);
+    if (!rc) rc = reference_covers(p, p->cfg.H, p->cfg.reward_type);
+    if (rc) return rc;
+    HIP_OK(hipSetDevice(p->cfg.device));
+    hipStream_t s = pick(p, stream);
+    if (!p->d_draw) {
+        size_t bytes = 0;
+        rc = mppi_draw_workspace(p->cfg.dtype, p->P, p->cfg.K, &bytes);
+        if (rc) return rc;
+        p->draw_workspace = (bytes + 255) & ~(size_t)255;
+        HIP_OK(hipMalloc(&p->d_draw, p->draw_workspace + (size_t)p->P * (8 + 8 + 4)));
+    }
+    HIP_OK(copy_now(draw_numbers(p), u, (size_t)p->P * 8, hipMemcpyDefault, s));
+    act_sequence_changed(p);
+    rc = launch_rollout_only(p, s);
+    if (rc) return rc;
+    rc = mppi_draw_from_returns(p->cfg.device, p->d_R, p->cfg.dtype, p->P, p->cfg.K, p->cfg.K, 1, draw_numbers(p), 1, &f, draw_index(p),
+                                draw_weight(p), p->d_draw, p->draw_workspace, s);
+    if (rc) return rc;
+    const dim3 grid((p->HM + 255) / 256, p->P);
+    if (p->cfg.dtype == MPPI_F32)
+        hipLaunchKernelGGL((draw_apply_kernel<float>), grid, dim3(256), 0, s, draw_index(p), (const float*)p->d_eps, p->cfg.K, p->HM, p->explicit_act, p->d_base);
+    else
+        hipLaunchKernelGGL((draw_apply_kernel<double>), grid, dim3(256), 0, s, draw_index(p), (const double*)p->d_eps, p->cfg.K, p->HM, p->explicit_act, p->d_base);
+    HIP_OK(hipGetLastError());
+    return 0;
+} catch (const std::exception& e) {
+    return fail(-8, std::string("host exception: ") + e.what());
+}
+
 static int build_graph(mppi_planner* p) {
     if (p->graph) { HIP_OK(hipGraphExecDestroy(p->graph)); p->graph = nullptr; }
     p->graph_gen = 0;
@@ -1379,6 +1438,16 @@ int mppi_read(mppi_planner* p, int32_t what, void* dst, size_t bytes) try {
         if (!need(16)) return fail(-1, "STATUS_DETAIL needs four int32");
         HIP_OK(copy_now(dst, p->d_status, 16, hipMemcpyDeviceToHost, p->stream));
         return 0;
+    case MPPI_READ_DRAW: {
+        if (!p->d_draw) return fail(-4, "mppi_draw has not been called on this planner");
+        if (!need(P * 16)) return fail(-1, "DRAW needs 2 doubles per planner");
+        std::vector<int64_t> k(P);
+        std::vector<float> w(P);
+        HIP_OK(copy_now(k.data(), draw_index(p), 8 * P, hipMemcpyDeviceToHost, p->stream));
+        HIP_OK(copy_now(w.data(), draw_weight(p), 4 * P, hipMemcpyDeviceToHost, p->stream));
+        for (size_t b = 0; b < P; b++) { ((double*)dst)[2 * b] = (double)k[b]; ((double*)dst)[2 * b + 1] = (double)w[b]; }
+        return 0;
+    }
     case MPPI_READ_PARTIALS:
         if (!need(P * (3 + HM) * 8)) return fail(-1, "PARTIALS needs P*(3+H*M) doubles");
         HIP_OK(copy_now(dst, p->d_part, P * (3 + HM) * 8, hipMemcpyDeviceToHost, p->stream));

@@ -1,6 +1,7 @@
 """Thin object wrappers over the C ABI: a model bound to its compiled kernels and a
 device-resident planner."""
 import ctypes as C
+import operator
 import os
 
 import numpy as np
@@ -286,6 +287,15 @@ class DevicePlanner:
     def iterate(self, niter=1, stream=None):
         L.check(L.lib().mppi_iterate(self._h, int(niter), stream))
 
+    def draw(self, u, top_k=0, top_p=1.0, min_p=0.0, stream=None):
+        """Rollouts and, in the place of the update, a draw: act_sequence becomes the sequence of one sample, drawn with the
+        update's own weights among the samples that top_k, top_p and min_p keep (see `draw_from_returns`).  u: a uniform
+        number in [0, 1), one per planner.  `drawn` tells which sample it was."""
+        u = L.f64(u).reshape(-1)
+        if u.shape != (self.P,):
+            raise ValueError("one number per planner: %d planners, %d numbers" % (self.P, len(u)))
+        L.check(L.lib().mppi_draw(self._h, L.ptr(u), operator.index(top_k), float(top_p), float(min_p), stream))
+
     def local_partials(self, stream=None):
         L.check(L.lib().mppi_local_partials(self._h, stream))
 
@@ -364,6 +374,11 @@ class DevicePlanner:
 
     def rewards(self):
         return self._read(L.READ_REWARDS, self._lead(self.K, self.H))
+
+    def drawn(self):
+        """(sample, weight) of the last draw; arrays for batches.  Sample -1: no sample's return was finite."""
+        d = self._read(L.READ_DRAW, (self.P, 2))
+        return (int(d[0, 0]), float(d[0, 1])) if self.P == 1 else (d[:, 0].astype(np.int64), d[:, 1])
 
     def status(self):
         return int(self._read(L.READ_STATUS, (1,), np.int32)[0])
