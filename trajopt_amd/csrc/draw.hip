@@ -22,6 +22,7 @@
 #include <cstdint>
 #include <exception>
 #include <new>
+#include <type_traits>
 
 using mppi::fail;
 
@@ -39,6 +40,8 @@ __device__ __forceinline__ float value_of(Bfloat x) { return __uint_as_float((un
 
 __device__ __forceinline__ float minus_infinity(float*) { return -INFINITY; }
 __device__ __forceinline__ double minus_infinity(double*) { return -INFINITY; }
+__device__ __forceinline__ float lowest(float*) { return -3.402823466e38f; }
+__device__ __forceinline__ double lowest(double*) { return -1.7976931348623157e308; }
 __device__ __forceinline__ Half minus_infinity(Half*) { return {0xfc00}; }
 __device__ __forceinline__ Bfloat minus_infinity(Bfloat*) { return {0xff80}; }
 
@@ -199,7 +202,7 @@ template <class V> struct Weights {
         best = best_;
         scale = __longlong_as_double((long long)(1023 + S) << 52);
         const V bound = (V)((double)best - (S + 1.01) * 0.6931471805599453 / kappa * (1.0 + 1e-6));
-        from = worst > bound ? worst : bound;
+        from = worst > bound ? worst : bound;        // (finite, as worst is)
     }
     // kappa (best - v) of a sample that takes part (of one that does not: that of the last that does).  Both ends of fp64 may be
     // apart by more than its range, and 0 times that is 0.
@@ -251,17 +254,19 @@ template <class V, int NT> struct BorderArea {
 
 // Among the samples of `src` in [low, high]: BY_COUNT: sample number `target` of the order.  BY_MASS: the last sample with less than
 // `target` of the mass before it.  BY_SHARE: the same with `share` (< 1) of their whole mass for a target.  False: there is no such
-// sample (too few of them; a share so small that nothing is kept, then src.from is raised to infinity).  `most`: as many samples as
-// there can be.  Every thread has to call.
+// sample (too few of them; a share so small that nothing is kept, then src.from is raised to infinity).  `bottom`: about the lowest of
+// them (the bins of the first pass reach down to it, the last one further).  `most`: as many samples as there can be.  Every thread has
+// to call.
 enum Aim { BY_COUNT, BY_MASS, BY_SHARE };
 template <Aim AIM, int NT, class Src, class V>
-__device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, unsigned long long target, double share, V low, V high, unsigned most) {
+__device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, unsigned long long target, double share, V low, V high, V bottom,
+                            unsigned most) {
     using U = typename Traits<V>::U;
     using Area = BorderArea<V, NT>;
     constexpr bool MASS = AIM != BY_COUNT;
     constexpr int BINS = Area::BINS, PER = BINS / NT, LIST = Area::LIST, VEC = Src::VEC;
     // bins linear in high - v first (monotone: every step rounds monotonically); per = 0 where that range overflows
-    const V per = high > low ? (V)BINS / (high - low) : (V)0;
+    const V per = high > bottom ? (V)BINS / (high - bottom) : (V)0;
     V lo = low, hi = high;
     int shift = -1, bin = 0;                         // -1: linear bins; else bits of key(hi) - key(v)
     U top = 0;
@@ -445,7 +450,7 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
 // ------------------------------------------------------------------------------------------
 // rows of up to 128 KB: one workgroup each
 // ------------------------------------------------------------------------------------------
-// The row lies in LDS as it came (what takes no part as -inf of its type).  Thread t owns the C samples from t C on, in GP
+// The row lies in LDS as it came, behind its end -inf; what is not finite fails the comparison with the lowest or the highest.  Thread t owns the C samples from t C on, in GP
 // pieces of 16 bytes; it visits them from piece t mod GP on, so that the lanes of a wave read from all banks.  All loops over
 // samples stay rolled: unrolled, a kernel of this many passes is larger than the instruction cache.  A pass tests values
 // against the lowest one that takes part, in the type of the row (fp32 or fp64); exponentials, in fp64, are evaluated only for
@@ -453,12 +458,13 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
 template <class T, int NT, int BYTES> struct Shelf {
     using V = typename Traits<T>::V;
     static constexpr int VEC = 16 / sizeof(T);
-    static constexpr int FEW = BYTES >= 131072 ? 1024 : 0;     // up to this many samples that take part move together
+    static constexpr int FEW = BYTES >= 131072 ? 1024 : 128;   // up to this many samples that take part can move together
+    static constexpr int LAST = 128;                           // up to this many are left to one wave (finish)
     struct alignas(16) Piece { T v[VEC]; };
     using Area = BorderArea<V, NT>;
     struct Shared {
         Piece row[(BYTES / (int)sizeof(T) + FEW) / VEC];
-        unsigned few_idx[FEW ? FEW : 1];
+        unsigned few_idx[FEW];
         Area b;
         __device__ unsigned long long* ends() { return b.mass; }           // (once the borders are found; NT <= BINS)
     };
@@ -467,6 +473,7 @@ template <class T, int NT, int BYTES> struct Shelf {
     int GP, start, base;              // pieces of this thread, the one it begins with, the row's first piece
     int C;                            // samples per thread
 
+    V bottom;                         // about the lowest value that takes part (at first)
     Group<NT> group;
     unsigned most;                    // samples that can take part
 
@@ -499,7 +506,7 @@ template <class T, int NT, int BYTES> struct Shelf {
     // raises w.from to a value that at least k threads' own values `mine` reach (one per thread), near the highest such
     __device__ void raise(V mine, unsigned k) {
         constexpr int BINS = Area::BINS, PER = BINS / NT;
-        const V per = w.best > w.from ? (V)BINS / (w.best - w.from) : (V)0;
+        const V per = w.best > bottom ? (V)BINS / (w.best - bottom) : (V)0;
         const bool in = mine >= w.from;
         int b = in ? (int)((w.best - mine) * per) : 0;
         b = b < BINS ? b : BINS - 1;
@@ -534,7 +541,7 @@ template <class T, int NT, int BYTES> struct Shelf {
                 const Piece x = s.row[p * NT + (int)threadIdx.x];
                 unsigned in = 0;
 #pragma unroll
-                for (int j = 0; j < VEC; j++) in |= at(x, j) >= w.from ? 1u << j : 0u;
+                for (int j = 0; j < VEC; j++) in |= at(x, j) >= w.from && at(x, j) <= w.best ? 1u << j : 0u;
                 bits |= (unsigned long long)in << (p * VEC);
                 mine[p / 4] += (unsigned long long)__popc(in) << (p % 4 * 16);
             }
@@ -568,6 +575,81 @@ template <class T, int NT, int BYTES> struct Shelf {
         GP = threadIdx.x < FEW / VEC ? 1 : 0;
         start = 0;
         C = VEC;
+    }
+
+    // The rest of the way for n <= 64 E samples in the order of their indices, in the first wave alone: ranks by comparing each with
+    // each, masses in the order of the ranks for top-p, and in that of the indices for the draws.  Lane l holds samples l, l + 64;
+    // returns their values, masses, the mass before each, and the whole mass.
+    template <int E> __device__ unsigned long long finish(unsigned n, const Param& par, V (&v)[E], unsigned long long (&q)[E], unsigned long long (&before)[E]) {
+        const int lane = threadIdx.x & 63;
+        unsigned long long* line = s.b.mass;
+        const auto settle = []() {                   // what the wave's lanes wrote to LDS is there for all of them
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        const bool by_count = par.top_k > 0 && par.top_k < (long long)n, by_share = !(par.top_p >= 1.0);
+        unsigned live = 0, rank[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const unsigned at_ = e * 64 + lane;
+            v[e] = at_ < n ? at(s.row[base + at_ / VEC], at_ % VEC) : (V)-INFINITY;
+            if (v[e] >= w.from && v[e] <= w.best) {
+                live |= 1u << e;
+            } else {
+                v[e] = (V)-INFINITY;
+                if (at_ < n) s.row[base + at_ / VEC].v[at_ % VEC] = minus_infinity((T*)nullptr);
+            }
+            rank[e] = 0;
+        }
+        if (by_count || by_share) {
+            settle();
+#pragma unroll 16 / VEC
+            for (unsigned p = 0; p * VEC < n; p++) { // every lane reads the same piece: one access for VEC comparisons
+                const Piece x = s.row[base + p];
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const V ov = at(x, j);
+#pragma unroll
+                    for (int e = 0; e < E; e++) rank[e] += ov > v[e] || (ov == v[e] && p * VEC + j < (unsigned)(e * 64 + lane)) ? 1u : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (by_count && (long long)rank[e] >= par.top_k) live &= ~(1u << e);
+        if (by_share) {
+            w.masses(v, live, 0.0, q);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (e * 64 + lane < (int)n) line[rank[e]] = q[e];
+            settle();
+            unsigned long long run = 0, ahead[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const unsigned long long m = e * 64 + lane < (int)n ? line[e * 64 + lane] : 0ull, inc = wave_scan(m, 0ull, Add());
+                ahead[e] = run + inc - m;
+                run += lane_value(inc, 63);
+            }
+            settle();
+#pragma unroll
+            for (int e = 0; e < E; e++) line[e * 64 + lane] = ahead[e];
+            settle();
+            const unsigned long long part = share_of(par.top_p, run);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (!(e * 64 + lane < (int)n && line[rank[e]] < part)) live &= ~(1u << e);
+        }
+        w.masses(v, live, par.min_p, q);
+        unsigned long long run = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const unsigned long long inc = wave_scan(q[e], 0ull, Add());
+            before[e] = run + inc - q[e];
+            run += lane_value(inc, 63);
+        }
+        settle();                                    // (line may be written again)
+        return run;
     }
 
     // leaves out what lies behind the border that was found
@@ -615,8 +697,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 
     const double u_wave = wave < a.D ? u[wave] : 0.0, u_thread = tid < a.D ? u[tid] : 0.0;      // asked for before anything waits
     // the row into LDS, AHEAD pieces requested at a time
-    constexpr int AHEAD = BYTES >= 131072 ? 8 : 4;
-    V best = (V)-INFINITY, worst = (V)INFINITY, top[AHEAD];
+    constexpr int AHEAD = BYTES >= 131072 ? 8 : 4, DIRECT = 8;
+    V best = (V)-INFINITY, some = (V)INFINITY, top[AHEAD];               // some: the lowest of every fourth sample
 #pragma unroll 1
     for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {                            // (once where few samples may move together)
         Piece in[AHEAD];
@@ -628,13 +710,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             top[k] = (V)-INFINITY;
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                const V v = H::at(in[k], j);
-                if (!isfinite(v)) {
-                    in[k].v[j] = minus_infinity((T*)nullptr);
-                } else {
-                    top[k] = v > top[k] ? v : top[k];
-                    worst = v < worst ? v : worst;
-                }
+                const V v = H::at(in[k], j), fine = isfinite(v) ? v : (V)-INFINITY;
+                top[k] = fine > top[k] ? fine : top[k];
+                if (j % 4 == 0) some = isfinite(v) && v < some ? v : some;
             }
             best = top[k] > best ? top[k] : best;
             s.row[(p0 + k) * NT + tid] = in[k];
@@ -642,22 +720,74 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     }
     const V mine = best;                                                  // best of what this thread loaded
     best = h.group.reduce(best, (V)-INFINITY, Max());
-    worst = h.group.reduce(worst, (V)INFINITY, Min());
+    some = h.group.reduce(some, (V)INFINITY, Min());
     if (NT == 64) __syncthreads();                                        // (the row is there; larger groups have just waited)
     if (!par.valid() || !(best > (V)-INFINITY)) return nothing();
-    h.w.set(par.kappa, best, worst, S);
-    // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
-    // thread next to nothing else passes that bound.
-    if (BYTES >= 131072 && par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
-    if constexpr (H::FEW > 0) {
-        static_assert(AHEAD * NT * 16 >= BYTES, "the row is loaded in one go");
-        if (h.GP > 1) h.gather_few(top);
+    h.w.set(par.kappa, best, lowest((V*)nullptr), S);
+    h.bottom = some > h.w.from && some <= best ? some : h.w.from;
+
+    auto answer = [&](int d, int i, double w, unsigned long long mass) {
+        index[d] = h.base ? (long long)s.few_idx[i] : i;
+        if (weight) weight[d] = (float)(w * h.w.scale / (double)mass);
+    };
+    auto finish = [&](auto one) __attribute__((always_inline)) {                                         // few samples: the first wave does the rest
+        constexpr int E = decltype(one)::value;
+        const unsigned n = h.most;
+        V v[E];
+        unsigned long long q[E], before[E], mass = 0;
+        if (wave == 0) {
+            mass = h.finish(n, par, v, q, before);
+            if (a.D <= DIRECT) {
+                for (int d = 0; d < a.D; d++) {
+                    const unsigned long long target = mass ? target_of(d == 0 ? u_wave : u[d], mass) : 0ull;
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if (target - before[e] < q[e]) answer(d, e * 64 + lane, h.w.weight(v[e]), mass);
+                    if (mass == 0 && lane == 0) { index[d] = -1; if (weight) weight[d] = 0.0f; }
+                }
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) s.ends()[e * 64 + lane] = before[e] + q[e];
+        }
+        if (a.D <= DIRECT) return;
+        __syncthreads();                                                  // many draws: a thread each
+        const unsigned long long* ends = s.ends();
+        mass = ends[n - 1];
+        if (mass == 0) return nothing();
+        for (int d = tid; d < a.D; d += NT) {
+            const unsigned long long target = target_of(d == tid ? u_thread : u[d], mass);
+            int lo = 0, hi = (int)n - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (ends[mid] > target) hi = mid; else lo = mid + 1;
+            }
+            answer(d, lo, h.w.weight(H::at(s.row[h.base + lo / VEC], lo % VEC)), mass);
+        }
+    };
+    static_assert(AHEAD * NT * 16 >= BYTES, "the row is loaded in one go, and top[] holds all of its pieces");
+    bool few = BYTES < 131072 && a.K <= H::LAST;
+    if (BYTES >= 131072) {
+        // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
+        // thread next to nothing else passes that bound.
+        if (par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
+        h.gather_few(top);
+        few = h.base && h.most <= H::LAST;
     }
-    if (par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, h.group, (unsigned long long)par.top_k, 0.0, h.w.from, best, h.most)) {
+    if (!few && par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, h.group, (unsigned long long)par.top_k, 0.0, h.w.from, best, h.bottom, h.most)) {
         h.cut_behind();
+        h.bottom = h.w.from;
         h.most = h.most < par.top_k ? h.most : (unsigned)par.top_k;
+        if (BYTES < 131072 && h.most <= H::LAST) {
+            h.gather_few(top);
+            few = true;
+        }
     }
-    if (!(par.top_p >= 1.0) && find_border<BY_SHARE>(h, s.b, h.group, 0, par.top_p, h.w.from, best, h.most)) h.cut_behind();
+    if (few) {
+        if (h.most <= 64) finish(std::integral_constant<int, 1>()); else finish(std::integral_constant<int, 2>());
+        return;
+    }
+    if (!(par.top_p >= 1.0) && find_border<BY_SHARE>(h, s.b, h.group, 0, par.top_p, h.w.from, best, h.bottom, h.most)) h.cut_behind();
 
     unsigned long long sum = 0, mass;
     h.each(h.w.from, best, [&](const V (&v)[VEC], unsigned live, int) {
@@ -675,11 +805,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     auto mass_of_sample = [&](int i, double& w) -> unsigned long long {
         const V v = H::at(s.row[h.base + i / VEC], i % VEC);
         w = h.w.weight(v);
-        return v >= h.w.from && w >= par.min_p ? whole(w * h.w.scale) : 0ull;
-    };
-    auto answer = [&](int d, int i, double w) {
-        index[d] = h.base ? (long long)s.few_idx[i] : i;
-        if (weight) weight[d] = (float)(w * h.w.scale / (double)mass);
+        return v >= h.w.from && v <= best && w >= par.min_p ? whole(w * h.w.scale) : 0ull;
     };
     const int C = h.C;
     // A wave for every draw (about 500 cycles each) or a thread for every draw (about 500 cycles for every piece it walks over)
@@ -694,7 +820,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             double w = 0.0;
             const unsigned long long m = lane < C ? mass_of_sample(owner * C + lane, w) : 0ull;      // C <= 64
             const unsigned long long at = ahead + wave_scan(m, 0ull, Add()) - m;
-            if (target - at < m) answer(d, owner * C + lane, w);
+            if (target - at < m) answer(d, owner * C + lane, w, mass);
         }
     } else {
         double next = u_thread;
@@ -717,7 +843,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 #pragma unroll
                 for (int j = 0; j < VEC; j++) {
                     v[j] = H::at(x, j);
-                    live |= v[j] >= h.w.from ? 1u << j : 0u;
+                    live |= v[j] >= h.w.from && v[j] <= best ? 1u << j : 0u;
                 }
                 h.w.masses(v, live, par.min_p, q);
 #pragma unroll
@@ -730,7 +856,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
                         if (target - c < q[j]) { chosen = v[j]; at = j; }
                         c += q[j];
                     }
-                    answer(d, p * VEC + at, h.w.weight(chosen));
+                    answer(d, p * VEC + at, h.w.weight(chosen), mass);
                     break;
                 }
                 c += sum;
@@ -1170,7 +1296,7 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
     const bool share = at.p_first <= at.p_last;
     if (at.k >= 0) {
         range(at.k, at.k, w.from, lo, hi);
-        (void)find_border<BY_COUNT>(list, s, group, (unsigned long long)par.top_k - at.k_before, 0.0, lo, hi, list.n);
+        (void)find_border<BY_COUNT>(list, s, group, (unsigned long long)par.top_k - at.k_before, 0.0, lo, hi, lo, list.n);
         found();
         if (share) {
             unsigned long long sum = 0;
@@ -1197,14 +1323,14 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
             return;
         }
         range(at.p_first, at.p_last, border, lo, hi);
-        if (find_border<BY_MASS>(list, s, group, target - at.mass_before, 0.0, lo, hi, list.n)) found();
+        if (find_border<BY_MASS>(list, s, group, target - at.mass_before, 0.0, lo, hi, lo, list.n)) found();
     }
     if (keep >= all) {
         last = UINT_MAX;
     } else if (last == UINT_MAX) {
         // more equal ones than a list of candidates holds: the keep-th of them by index
         Listed<V, true> equal{list.v, list.i, list.n, border, w};
-        (void)find_border<BY_COUNT>(equal, s, group, keep, 0.0, -(V)a.K, (V)0, list.n);
+        (void)find_border<BY_COUNT>(equal, s, group, keep, 0.0, -(V)a.K, (V)0, -(V)a.K, list.n);
         last = s.border_idx;
     }
     if (threadIdx.x == 0) { r.border = border; r.last = last; }
