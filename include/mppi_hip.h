@@ -207,7 +207,8 @@ int mppi_rollout(mppi_planner* p, void* stream);
 int mppi_iterate(mppi_planner* p, int32_t niter, void* stream);
 /* Rollouts and, in the place of `MPPI.update`, a draw: act_sequence becomes the sequence of ONE sample, drawn with the
  * weights the update would average with, exp(kappa (R_k - Rmax)), among the samples that top_k, top_p and min_p keep (see
- * mppi_draw_filter; 0, 1, 0 keep all).  u: one uniform number in [0, 1) per planner, host or device memory.  The reference only
+ * mppi_draw_filter; 0, 1, 0 keep all).  u: one uniform number in [0, 1) per planner, host or device memory, copied before the
+ * rollouts are launched (the call waits for what `stream` already holds).  The reference only
  * ever applies the mean (trajopt/algos/mppi.py:56-65); applied draws explore, which is what a critic's replay buffer wants.
  * MPPI_READ_DRAW tells the sample and its weight; a planner whose samples all diverged keeps its act_sequence (-1).  Works on
  * explicit action sequences (mppi_upload_actions) as well.  -4 on a planner that owns only a shard of its samples

@@ -208,6 +208,38 @@ def test_many_rows_and_many_draws():
     _check(R, u, kappa=0.5, top_p=0.9, top_k=60000)
 
 
+def test_many_small_rows():
+    """More rows than a grid's second dimension holds; compared with the two-sample formula in closed form."""
+    import torch
+    R, u = _returns(70001, 2, "float32", 5), _numbers(70001, 1, 5)
+    index, weight = _draw(R, u, kappa=0.8)
+    w = torch.exp(0.8 * (R.double() - R.double().amax(1, keepdim=True)))
+    want = (u[:, 0] * w.sum(1) >= w[:, 0]).long()
+    assert torch.equal(index[:, 0], want)
+    share = w.gather(1, index) / w.sum(1, keepdim=True)
+    assert ((weight.double() - share).abs() <= WEIGHT_RTOL * share).all()
+    for D in (8, 9, 100):                                    # rows that one wave finishes, few draws and many
+        for K in (3, 64, 65, 128, 129):
+            _check(_returns(4, K, "float64", K + D, masked=0.2), _numbers(4, D, K + D), kappa=1.0, top_k=K // 2 + 1, top_p=0.8, min_p=0.01)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_longest_row(dtype):
+    """The largest K there is: every index up to 2^24 - 1 is reached by its own chunk, and one sample more is refused."""
+    import torch
+    from trajopt_amd._lib import MppiError
+    K = 1 << 24
+    R = _returns(1, K, dtype, 1)
+    _check(R, _numbers(1, 7, 1), kappa=0.6, top_k=K // 5, top_p=0.9)
+    one = torch.full((1, K), float("-inf"), dtype=R.dtype, device="cuda")
+    for at in (0, K // 2 + 12345, K - 1):
+        one.fill_(float("-inf"))
+        one[0, at] = 2.0
+        assert _draw(one, _numbers(1, 2, 1), top_p=0.5)[0].tolist() == [[at, at]]
+    with pytest.raises(MppiError):
+        _draw(torch.zeros(1, K + 1, dtype=R.dtype, device="cuda"), _numbers(1, 1, 1))
+
+
 def test_nothing_to_do():
     import torch
     R, u = _returns(2, 10, "float32", 0), _numbers(2, 0, 0)

@@ -1,8 +1,8 @@
 """Gradient norm and clipping against the definition in 64 bits (oracle/ref_learn.py).
 
 Tolerances.  The norm: fp64 sums of fp64 squares (below 1e-12 relative at these sizes), rounded to float32 once, 2^-24.
-A clipped fp32 entry: one rounding of an fp64 product, 2^-24 relative.  A clipped 16-bit entry: the scale and the product are
-rounded to fp32 first (2 x 2^-24), then to the type: eps / 2 relative, or half the smallest subnormal step of the type."""
+A clipped fp32 entry: one rounding of an fp64 product, 2^-24 relative.  A clipped 16-bit entry: the product is rounded to fp32
+first (2^-24), then to the type: eps / 2 relative, or half the smallest subnormal step of the type."""
 import numpy as np
 import pytest
 
@@ -27,7 +27,7 @@ def _close(t, want):
     import torch
     f = torch.finfo(t.dtype)
     step = float(f.tiny) * float(f.eps)
-    extra = 0.0 if t.dtype == torch.float32 else 2 * 2.0 ** -24
+    extra = 0.0 if t.dtype == torch.float32 else 2.0 ** -24
     got = t.double().cpu().numpy()
     assert np.all(np.abs(got - want) <= (f.eps / 2 + extra) * 1.0000001 * np.abs(want) + step / 2), np.abs(got - want).max()
 
@@ -141,6 +141,10 @@ def test_large_and_small_magnitudes():
     g = [torch.full((100,), 3e38, device="cuda")]
     assert float(clip_gradients(g, 1.0)) == float("inf")
     assert torch.allclose(g[0], torch.full_like(g[0], 0.1))
+    # a scale below fp32's range
+    for n in (300, 200000):
+        g = [torch.full((n,), 3e38, device="cuda").to(torch.bfloat16), torch.full((n,), 1e30, device="cuda")]
+        _check(g, 1e-7)
     for dtype in (torch.float16, torch.bfloat16):
         g = [torch.full((4096,), torch.finfo(dtype).max / 2, dtype=dtype, device="cuda")]
         _check(g, 1.0)

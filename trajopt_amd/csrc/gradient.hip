@@ -3,10 +3,10 @@
 //     l2: sqrt(sum g^2)      max: max |g|        over all entries of all tensors
 //     out = g s,  s = max_norm / norm if norm > max_norm, else 1; a norm that is not finite changes nothing
 //
-// Numbers.  Squares and their sums are fp64, so no fp32 gradient overflows or vanishes in them, and every sum has a fixed
-// order: a thread adds what it reads, the lanes of a workgroup are added by a tree, the workgroups in the order of their
-// partial sums, of which the launch shape alone says what each covers.  fp32 gradients are scaled in fp64 and rounded once;
-// 16-bit ones are exact in fp32, scaled there and rounded once more (the first rounding is 2^-16 of the second's step).
+// Numbers.  Squares and their sums are fp64, so no fp32 gradient overflows or vanishes in them, and every sum has a fixed order: a
+// thread adds what it reads, the lanes of a workgroup are added by a tree, the workgroups in the order of their partial sums, of
+// which the sizes of the tensors alone say what each covers.  Entries are scaled in fp64 (the scale of large gradients may lie below
+// fp32's range) and rounded to fp32; 16-bit ones from there to their type, 2^-16 of whose step the first rounding is at most.
 //
 // Two passes over the data: no entry can be scaled before all have been read.
 #include "abi_common.hpp"
@@ -57,13 +57,13 @@ template <> struct Io<_Float16> {
     static constexpr int VEC = 8;
     using B = uint16_t;
     static __device__ __forceinline__ float get(B b) { return (float)__builtin_bit_cast(_Float16, b); }
-    static __device__ __forceinline__ B scaled(B b, double s) { return __builtin_bit_cast(B, (_Float16)(get(b) * (float)s)); }
+    static __device__ __forceinline__ B scaled(B b, double s) { return __builtin_bit_cast(B, (_Float16)(float)((double)get(b) * s)); }
 };
 template <> struct Io<__bf16> {
     static constexpr int VEC = 8;
     using B = uint16_t;
     static __device__ __forceinline__ float get(B b) { return __uint_as_float((uint32_t)b << 16); }
-    static __device__ __forceinline__ B scaled(B b, double s) { return __builtin_bit_cast(B, (__bf16)(get(b) * (float)s)); }
+    static __device__ __forceinline__ B scaled(B b, double s) { return __builtin_bit_cast(B, (__bf16)(float)((double)get(b) * s)); }
 };
 typedef uint32_t Words __attribute__((ext_vector_type(4)));
 typedef Words LooseWords __attribute__((aligned(2), may_alias));
