@@ -223,6 +223,41 @@ def test_many_small_rows():
             _check(_returns(4, K, "float64", K + D, masked=0.2), _numbers(4, D, K + D), kappa=1.0, top_k=K // 2 + 1, top_p=0.8, min_p=0.01)
 
 
+def test_more_rows_than_one_grid_holds():
+    """2^26 + 5 rows of one sample, a wave each: 2^32 threads are more than a grid can have.  Rows with a NaN stay empty."""
+    import torch
+    rows = (1 << 26) + 5
+    R = torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda")
+    bad = [0, 12345, (1 << 26) - 2, (1 << 26) - 1, 1 << 26, rows - 2]
+    R[bad] = float("nan")
+    index, weight = _draw(R, torch.full((rows, 1), 0.3, dtype=torch.float64, device="cuda"))
+    assert (index[bad] == -1).all() and (weight[bad] == 0).all()
+    assert (index.count_nonzero(), weight.count_nonzero()) == (len(bad), rows - len(bad))
+    assert (weight.max(), index.min(), index.max()) == (1, -1, 0)
+
+
+def test_more_draws_than_one_workgroup_takes():
+    for K, D, dtype in ((300, 16385, "float64"), (3000, 33000, "float32"), (9000, 40000, "bfloat16")):
+        _check(_returns(2, K, dtype, K, masked=0.1), _numbers(2, D, K), kappa=0.7, top_p=0.99)
+
+
+def test_negated_views():
+    """A view that torch negates lazily: its memory holds the other sign."""
+    import torch
+    z = torch.complex(torch.zeros(2, 50, device="cuda"), _returns(2, 50, "float32", 3))
+    u = _numbers(2, 4, 3)
+    lazy = z.conj().imag
+    assert lazy.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        _draw(lazy, u)
+    _check(lazy.resolve_neg(), u, kappa=0.5)
+    half = torch.complex(torch.zeros_like(u), -u).conj().imag                 # as u, and as a row's parameter
+    assert half.is_neg() and torch.equal(half.resolve_neg(), u)
+    want = _draw(z.imag, u, top_p=u[:, 0].contiguous())
+    got = _draw(z.imag, half, top_p=half[:, 0])
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_longest_row(dtype):
     """The largest K there is: every index up to 2^24 - 1 is reached by its own chunk, and one sample more is refused."""

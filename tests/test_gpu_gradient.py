@@ -263,3 +263,15 @@ def test_refusals():
         clip_gradients([g], 1.0, out=[g.half()])
     assert abs(float(gradient_norm([g, g])) - np.sqrt(200.0)) < 1e-5      # reading twice is no harm: counted twice
     assert (g == 1).all()
+
+
+def test_negated_views_are_refused():
+    """A view that torch negates lazily: its memory holds the other sign."""
+    import torch
+    from trajopt_amd.device import clip_gradients, gradient_norm
+    lazy = torch.complex(torch.zeros(1, device="cuda"), torch.ones(1, device="cuda")).conj().imag
+    assert lazy.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        gradient_norm([lazy])
+    with pytest.raises(ValueError, match="negated"):
+        clip_gradients([torch.ones(1, device="cuda")], 1.0, out=[lazy])

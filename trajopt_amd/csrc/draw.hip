@@ -21,7 +21,6 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
-#include <new>
 #include <type_traits>
 
 using mppi::fail;
@@ -65,6 +64,8 @@ struct DrawArgs {
     mppi_draw_filter f;
     long long* index;
     float* weight;
+    long long first;                  // row (long_draw: draw) of the launch's first workgroup
+    int per;                          // draws of one workgroup
 };
 
 // ------------------------------------------------------------------------------------------
@@ -679,7 +680,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     constexpr int VEC = H::VEC, NW = NT / 64;
     __shared__ typename H::Shared s;
     H h(s);
-    const long long row = blockIdx.x;
+    const long long row = a.first + blockIdx.x, from_draw = row * a.D + (long long)blockIdx.y * a.per;
+    const int D = min(a.per, (int)(a.D - (long long)blockIdx.y * a.per));
     const T* R = (const T*)a.R + row * a.row_stride;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     h.GP = (a.K + NT * VEC - 1) / (NT * VEC);
@@ -688,14 +690,14 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     h.base = 0;
     h.most = (unsigned)a.K;
     const Param par(a.f, row);
-    long long* index = a.index + row * a.D;
-    float* weight = a.weight ? a.weight + row * a.D : nullptr;
-    const double* u = a.u + row * a.D;
+    long long* index = a.index + from_draw;
+    float* weight = a.weight ? a.weight + from_draw : nullptr;
+    const double* u = a.u + from_draw;
     auto nothing = [&]() {
-        for (int d = tid; d < a.D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
+        for (int d = tid; d < D; d += NT) { index[d] = -1; if (weight) weight[d] = 0.0f; }
     };
 
-    const double u_wave = wave < a.D ? u[wave] : 0.0, u_thread = tid < a.D ? u[tid] : 0.0;      // asked for before anything waits
+    const double u_wave = wave < D ? u[wave] : 0.0, u_thread = tid < D ? u[tid] : 0.0;      // asked for before anything waits
     // the row into LDS, AHEAD pieces requested at a time
     constexpr int AHEAD = BYTES >= 131072 ? 8 : 4, DIRECT = 8;
     V best = (V)-INFINITY, some = (V)INFINITY, top[AHEAD];               // some: the lowest of every fourth sample
@@ -737,8 +739,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         unsigned long long q[E], before[E], mass = 0;
         if (wave == 0) {
             mass = h.finish(n, par, v, q, before);
-            if (a.D <= DIRECT) {
-                for (int d = 0; d < a.D; d++) {
+            if (D <= DIRECT) {
+                for (int d = 0; d < D; d++) {
                     const unsigned long long target = mass ? target_of(d == 0 ? u_wave : u[d], mass) : 0ull;
 #pragma unroll
                     for (int e = 0; e < E; e++)
@@ -750,12 +752,12 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 #pragma unroll
             for (int e = 0; e < E; e++) s.ends()[e * 64 + lane] = before[e] + q[e];
         }
-        if (a.D <= DIRECT) return;
+        if (D <= DIRECT) return;
         __syncthreads();                                                  // many draws: a thread each
         const unsigned long long* ends = s.ends();
         mass = ends[n - 1];
         if (mass == 0) return nothing();
-        for (int d = tid; d < a.D; d += NT) {
+        for (int d = tid; d < D; d += NT) {
             const unsigned long long target = target_of(d == tid ? u_thread : u[d], mass);
             int lo = 0, hi = (int)n - 1;
             while (lo < hi) {
@@ -809,9 +811,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     };
     const int C = h.C;
     // A wave for every draw (about 500 cycles each) or a thread for every draw (about 500 cycles for every piece it walks over)
-    if ((a.D + NW - 1) / NW <= (a.D + NT - 1) / NT * (C / VEC)) {
+    if ((D + NW - 1) / NW <= (D + NT - 1) / NT * (C / VEC)) {
 #pragma unroll 1
-        for (int d = wave; d < a.D; d += NW) {
+        for (int d = wave; d < D; d += NW) {
             const unsigned long long target = target_of(d == wave ? u_wave : u[d], mass);
             int owner = 0;                                     // number of threads that end at or below the target
 #pragma unroll
@@ -825,9 +827,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     } else {
         double next = u_thread;
 #pragma unroll 1
-        for (int d = tid; d < a.D; d += NT) {
+        for (int d = tid; d < D; d += NT) {
             const unsigned long long target = target_of(next, mass);
-            next = d + NT < a.D ? u[d + NT] : 0.0;
+            next = d + NT < D ? u[d + NT] : 0.0;
             int lo = 0, hi = NT - 1;                           // the first thread that ends above the target
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
@@ -1360,7 +1362,7 @@ template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawAr
     using V = typename Traits<T>::V;
     using C = Chunk<T>;
     constexpr int VEC = C::VEC;
-    const long long row = blockIdx.x / a.D, at = blockIdx.x;
+    const long long at = a.first + blockIdx.x, row = (unsigned)at / (unsigned)a.D;       // (below 2^31)
     const LongRow<V>& r = l.row[row];
     const Param par(a.f, row);
     const int lane = threadIdx.x;
@@ -1435,26 +1437,38 @@ int ceil_log2(int n) {
 
 constexpr size_t SHELF = 131072;                     // bytes of the longest row that one workgroup holds in LDS
 
-template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+// A grid has at most 2^32 - 1 threads along its first axis: more workgroups than that go into several launches.  `f(count)` makes
+// one of workgroups a.first ... a.first + count - 1.
+template <class F> int in_grids(DrawArgs& a, long long groups, int threads, F f) {
+    const long long most = 0xffffffffll / threads;
+    for (a.first = 0; a.first < groups; a.first += most) {
+        f((unsigned)std::min(most, groups - a.first));
+        HIP_OK(hipGetLastError());
+    }
+    return 0;
+}
+template <class T, int NT, int BYTES> int launch_rows(DrawArgs a, hipStream_t s) {
+    // K units of half 2^-S at most in error, and sums below 2^62
+    const int S = std::min(51, 62 - ceil_log2(a.K));
+    const long long most = 32 * NT, per = std::max(most, ((long long)a.D + 65534) / 65535);
+    const unsigned parts = (unsigned)((a.D + per - 1) / per);
+    a.per = (int)std::min(per, (long long)a.D);
+    return in_grids(a, a.rows, NT, [&](unsigned n) { hipLaunchKernelGGL((draw_row_kernel<T, NT, BYTES>), dim3(n, parts), dim3(NT), 0, s, a, S); });
+}
+template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_bytes, hipStream_t s) {
     using V = typename Traits<T>::V;
     if ((size_t)a.K * sizeof(T) <= SHELF) {
-        // K units of half 2^-S at most in error, and sums below 2^62
-        const int S = std::min(51, 62 - ceil_log2(a.K));
-        if (a.K <= 512 && a.D <= 64)
-            hipLaunchKernelGGL((draw_row_kernel<T, 64, 512 * sizeof(T)>), dim3(a.rows), dim3(64), 0, s, a, S);
-        else if (a.K <= 4096)
-            hipLaunchKernelGGL((draw_row_kernel<T, 512, 4096 * sizeof(T)>), dim3(a.rows), dim3(512), 0, s, a, S);
-        else
-            hipLaunchKernelGGL((draw_row_kernel<T, 1024, SHELF>), dim3(a.rows), dim3(1024), 0, s, a, S);
-        HIP_OK(hipGetLastError());
-        return 0;
+        if (a.K <= 512 && a.D <= 64) return launch_rows<T, 64, 512 * sizeof(T)>(a, s);
+        if (a.K <= 4096) return launch_rows<T, 512, 4096 * sizeof(T)>(a, s);
+        return launch_rows<T, 1024, SHELF>(a, s);
     }
     LongArea<V> l;
     if (!workspace || workspace_bytes < LongArea<V>::carve(&l, (char*)workspace, a.rows, a.K))
         return fail(-1, "workspace too small (mppi_draw_workspace)");
-    if ((long long)a.rows * l.chunks > INT_MAX || (long long)a.rows * a.D > INT_MAX)
-        return fail(-6, "more than 2^31 - 1 chunks or draws in one call of long rows");
-    const dim3 chunks((unsigned)((long long)a.rows * l.chunks));
+    const long long n = (long long)a.rows * l.chunks;
+    if (n > 0xffffffffll / LT || (long long)a.rows * a.D > INT_MAX)
+        return fail(-6, "more than 2^23 - 1 chunks of 8192 samples, or than 2^31 - 1 draws, in one call of long rows");
+    const dim3 chunks((unsigned)n);
     hipLaunchKernelGGL((chunk_best_kernel<T>), chunks, dim3(LT), 0, s, a, l);
     HIP_OK(hipGetLastError());
     hipLaunchKernelGGL((chunk_bins_kernel<T>), chunks, dim3(LT), 0, s, a, l);
@@ -1465,9 +1479,7 @@ template <class T> int launch(const DrawArgs& a, void* workspace, size_t workspa
         hipLaunchKernelGGL((row_border_kernel<T>), dim3(a.rows), dim3(BT), 0, s, a, l);
         HIP_OK(hipGetLastError());
     }
-    hipLaunchKernelGGL((long_draw_kernel<T>), dim3((unsigned)((long long)a.rows * a.D)), dim3(64), 0, s, a, l);
-    HIP_OK(hipGetLastError());
-    return 0;
+    return in_grids(a, (long long)a.rows * a.D, 64, [&](unsigned n) { hipLaunchKernelGGL((long_draw_kernel<T>), dim3(n), dim3(64), 0, s, a, l); });
 }
 
 size_t workspace_of(int dtype, size_t rows, size_t K) {
@@ -1516,7 +1528,7 @@ int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32
         return fail(-1, "workspace too small (mppi_draw_workspace) or not aligned to 256 bytes");
     mppi::DeviceGuard guard;
     HIP_OK(guard.enter(device));
-    DrawArgs a;
+    DrawArgs a{};
     a.R = d_R; a.row_stride = row_stride; a.col_stride = col_stride;
     a.rows = rows; a.K = K; a.D = D;
     a.u = d_u; a.f = *filter;

@@ -67,7 +67,7 @@ struct PerRow {
             raise(PyExc_ValueError, std::string(name) + ": one value per row, shape (" + std::to_string(rows) + ",), got " + text(t.sizes()));
         if (t.is_complex() || (type == at::kLong && t.is_floating_point()))
             raise(PyExc_TypeError, std::string(name) + ": unsupported element type " + c10::toString(t.scalar_type()));
-        held = t.detach().to(type).contiguous();
+        held = t.detach().to(type).contiguous().resolve_neg();
         data = held.const_data_ptr();
     }
 };
@@ -97,6 +97,7 @@ PyObject* draw(PyObject* const* args) {
     if (u.device() != device) raise(PyExc_ValueError, "u lies on " + text(u.device()) + ", the returns on " + text(device));
     if (u.scalar_type() != at::kDouble && u.scalar_type() != at::kFloat)
         raise(PyExc_TypeError, std::string("u must be float64 or float32, got ") + c10::toString(u.scalar_type()));
+    if (R.is_neg()) raise(PyExc_ValueError, "the returns are a lazily negated view: resolve_neg() them first");
     const int type = element_type(R, true);
     const bool one = R.dim() == 1;
     const int64_t rows = one ? 1 : R.size(0), K = R.size(one ? 0 : 1), D = u.size(one ? 0 : 1);
@@ -112,7 +113,7 @@ PyObject* draw(PyObject* const* args) {
     f.kappa_of = (const double*)kappa.data; f.top_k_of = (const int64_t*)top_k.data;
     f.top_p_of = (const double*)top_p.data; f.min_p_of = (const double*)min_p.data;
     at::Tensor u64 = u;
-    if (u.scalar_type() != at::kDouble || !u.is_contiguous()) u64 = u.detach().to(at::kDouble).contiguous();
+    if (u.scalar_type() != at::kDouble || !u.is_contiguous() || u.is_neg()) u64 = u.detach().to(at::kDouble).contiguous().resolve_neg();
     at::Tensor index = at::empty(u.sizes(), at::TensorOptions().dtype(at::kLong).device(device));
     at::Tensor weight = at::empty(u.sizes(), at::TensorOptions().dtype(at::kFloat).device(device));
     size_t bytes = 0;
@@ -152,6 +153,7 @@ struct List {
             if (!x.is_cuda() || x.layout() != at::kStrided) raise(PyExc_TypeError, std::string(what) + " must be dense CUDA tensors");
             if (!x.is_non_overlapping_and_dense())
                 raise(PyExc_ValueError, std::string(what) + " must fill their memory without gaps or overlaps (a slice or an expanded tensor does not)");
+            if (x.is_neg()) raise(PyExc_ValueError, std::string(what) + " must not be lazily negated views (resolve_neg())");
             t.push_back(&x);
         }
     }
