@@ -699,7 +699,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 
     const double u_wave = wave < D ? u[wave] : 0.0, u_thread = tid < D ? u[tid] : 0.0;      // asked for before anything waits
     // the row into LDS, AHEAD pieces requested at a time
-    constexpr int AHEAD = BYTES >= 131072 ? 8 : 4, DIRECT = 8;
+    constexpr int AHEAD = BYTES >= 65536 ? 8 : 4, DIRECT = 8;
     V best = (V)-INFINITY, some = (V)INFINITY, top[AHEAD];               // some: the lowest of every fourth sample
 #pragma unroll 1
     for (int p0 = 0; p0 < h.GP; p0 += AHEAD) {                            // (once where few samples may move together)
@@ -1450,7 +1450,11 @@ template <class F> int in_grids(DrawArgs& a, long long groups, int threads, F f)
 template <class T, int NT, int BYTES> int launch_rows(DrawArgs a, hipStream_t s) {
     // K units of half 2^-S at most in error, and sums below 2^62
     const int S = std::min(51, 62 - ceil_log2(a.K));
-    const long long most = 32 * NT, per = std::max(most, ((long long)a.D + 65534) / 65535);
+    // Many draws are shared by as many workgroups as leave no CU idle, each of which finds the kept samples for itself; fewer than NT / 4
+    // draws of one pay for no further one.  (1 row of 4096 fp32 and 300000 draws: 11.5 us for 256 workgroups, 13.8 for 512, 1403 for one;
+    // 16 rows of 30000 and 16384 draws each: 32, 50 and 228 us.)
+    const long long want = std::max(1ll, 256ll / a.rows);
+    const long long per = std::max({(long long)NT / 4, (a.D + want - 1) / want, ((long long)a.D + 65534) / 65535});
     const unsigned parts = (unsigned)((a.D + per - 1) / per);
     a.per = (int)std::min(per, (long long)a.D);
     return in_grids(a, a.rows, NT, [&](unsigned n) { hipLaunchKernelGGL((draw_row_kernel<T, NT, BYTES>), dim3(n, parts), dim3(NT), 0, s, a, S); });
@@ -1459,7 +1463,9 @@ template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_byte
     using V = typename Traits<T>::V;
     if ((size_t)a.K * sizeof(T) <= SHELF) {
         if (a.K <= 512 && a.D <= 64) return launch_rows<T, 64, 512 * sizeof(T)>(a, s);
-        if (a.K <= 4096) return launch_rows<T, 512, 4096 * sizeof(T)>(a, s);
+        if (a.K * sizeof(T) <= 32768) return launch_rows<T, 512, 32768>(a, s);
+        if constexpr (sizeof(T) >= 4)
+            if (a.K * sizeof(T) <= 65536) return launch_rows<T, 512, 65536>(a, s);
         return launch_rows<T, 1024, SHELF>(a, s);
     }
     LongArea<V> l;
