@@ -26,20 +26,23 @@ constexpr int BT = 256;                  // threads of a workgroup
 constexpr int CHUNK = 65536;             // bytes of one tensor that a workgroup takes at a time
 constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums
 constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way
-constexpr int TABLE = 120;               // tensors whose table travels in a kernel's arguments (4 KB at most)
+constexpr int TABLE = 168;               // tensors whose table travels in a kernel's arguments (4 KB at most)
 
 struct Entry {
     const void* g;
     void* out;
-    long long n;
     unsigned first;                      // chunks of the tensors before it
-    int type;
+    unsigned last_type;                  // 4 times the entries of its last chunk, plus its type
+    __host__ __device__ __forceinline__ int type() const { return (int)(last_type & 3u); }
+    __device__ __forceinline__ int per() const { return type() == MPPI_F32 ? CHUNK / 4 : CHUNK / 2; }
 };
+static_assert(MPPI_F32 < 4 && MPPI_F16 < 4 && MPPI_BF16 < 4, "two bits");
 struct Table {
     Entry e[TABLE];
     int tensors;
     unsigned chunks;
 };
+static_assert(sizeof(Table) + 40 <= 4096, "and the kernels' other arguments");
 struct FarTable {                        // more tensors: in the workspace, written there by table_kernel
     const Entry* e;
     int tensors;
@@ -100,9 +103,10 @@ template <class Tab> __device__ __forceinline__ const Entry& locate(const Tab& t
         if (t.e[m].first <= c) a = m; else b = m - 1;
     }
     const Entry& e = t.e[a];
-    const int per = e.type == MPPI_F32 ? CHUNK / 4 : CHUNK / 2;
+    const unsigned end = a + 1 < t.tensors ? t.e[a + 1].first : t.chunks;
+    const int per = e.per();
     lo = (long long)(c - e.first) * per;
-    hi = lo + per < e.n ? lo + per : e.n;
+    hi = lo + (c + 1 < end ? per : (int)(e.last_type >> 2));
     return e;
 }
 
@@ -180,18 +184,18 @@ template <class T, bool SCALED, int NT, bool STREAM> __device__ __forceinline__ 
     for (; i < hi; i++) out[i] = SCALED ? Io<T>::scaled(g[i], scale) : g[i];
 }
 template <bool MAX, int NT> __device__ __forceinline__ void read_chunk(const Entry& e, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
-    if (e.type == MPPI_F32) read_span<float, MAX, NT>(e.g, tid, lo, hi, acc, top);
-    else if (e.type == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, tid, lo, hi, acc, top);
+    if (e.type() == MPPI_F32) read_span<float, MAX, NT>(e.g, tid, lo, hi, acc, top);
+    else if (e.type() == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, tid, lo, hi, acc, top);
     else read_span<__bf16, MAX, NT>(e.g, tid, lo, hi, acc, top);
 }
 template <int NT, bool STREAM> __device__ __forceinline__ void write_chunk(const Entry& e, int tid, long long lo, long long hi, bool clip, double scale) {
     if (!clip && e.out == e.g) return;
-    if (e.type == MPPI_F32) {
+    if (e.type() == MPPI_F32) {
         if (clip) write_span<float, true, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
         else write_span<float, false, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
     } else if (!clip) {
         write_span<__bf16, false, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);      // (bits are bits)
-    } else if (e.type == MPPI_F16) {
+    } else if (e.type() == MPPI_F16) {
         write_span<_Float16, true, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
     } else {
         write_span<__bf16, true, NT, STREAM>(e.g, e.out, tid, lo, hi, scale);
@@ -255,7 +259,8 @@ template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(
     // through the arguments would wait for a scalar load at every step.
     const Entry& own = t.e[lane < t.tensors ? lane : 0];
     const unsigned long long g = (unsigned long long)own.g, out = (unsigned long long)own.out;
-    const int n = (int)own.n, type = own.type, per = type == MPPI_F32 ? PIECE / 4 : PIECE / 2;
+    const int type = own.type(), per = type == MPPI_F32 ? PIECE / 4 : PIECE / 2;
+    const int n = (int)((lane + 1 < t.tensors ? t.e[lane + 1].first : t.chunks) - own.first - 1) * own.per() + (int)(own.last_type >> 2);
     const int count = lane < t.tensors ? (n + per - 1) / per : 0;
     int end = count;
 #pragma unroll
@@ -274,12 +279,11 @@ template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(
             Entry e;
             e.g = (const void*)far(g, k);
             e.out = (void*)far(out, k);
-            e.n = __builtin_amdgcn_readlane(n, k);
-            e.type = __builtin_amdgcn_readlane(type, k);
             e.first = 0;
-            const int size = e.type == MPPI_F32 ? PIECE / 4 : PIECE / 2;
-            const long long lo = (long long)(p - __builtin_amdgcn_readlane(end - count, k)) * size;
-            f(e, lo, lo + size < e.n ? lo + size : e.n);
+            e.last_type = (unsigned)__builtin_amdgcn_readlane(type, k);
+            const int size = e.type() == MPPI_F32 ? PIECE / 4 : PIECE / 2;
+            const int lo = (p - __builtin_amdgcn_readlane(end - count, k)) * size, all_of = __builtin_amdgcn_readlane(n, k);
+            f(e, (long long)lo, (long long)(lo + size < all_of ? lo + size : all_of));
         }
     };
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
@@ -387,9 +391,9 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
     size_t bytes = 0, pieces = 0;
     for (int i = 0; i < n; i++) {
         if (sizes[i] == 0) continue;
-        entries.push_back({g[i], max_norm ? out[i] : nullptr, (long long)sizes[i], (unsigned)chunks, dtypes[i]});
-        const int64_t size = sizes[i] * element_size(dtypes[i]);
-        chunks += (size + CHUNK - 1) / CHUNK;
+        const int64_t size = sizes[i] * element_size(dtypes[i]), per = CHUNK / element_size(dtypes[i]), parts = (sizes[i] + per - 1) / per;
+        entries.push_back({g[i], max_norm ? out[i] : nullptr, (unsigned)chunks, (unsigned)(sizes[i] - (parts - 1) * per) << 2 | (unsigned)dtypes[i]});
+        chunks += parts;
         bytes += (size_t)size;
         pieces += (size_t)(size + PIECE - 1) / PIECE;
         if (chunks > 0x7fffffffll) return fail(-6, "more entries than one call can take");
