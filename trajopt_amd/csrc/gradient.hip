@@ -23,7 +23,7 @@ using mppi::fail;
 namespace {
 
 constexpr int BT = 256;                  // threads of a workgroup
-constexpr int CHUNK = 65536;             // bytes of one tensor that a workgroup takes at a time
+constexpr int CHUNK = 65536, SMALL_CHUNK = 16384;      // bytes of one tensor that a workgroup takes at a time
 constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums
 constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way
 constexpr int TABLE = 168;               // tensors whose table travels in a kernel's arguments (4 KB at most)
@@ -34,18 +34,18 @@ struct Entry {
     unsigned first;                      // chunks of the tensors before it
     unsigned last_type;                  // 4 times the entries of its last chunk, plus its type
     __host__ __device__ __forceinline__ int type() const { return (int)(last_type & 3u); }
-    __device__ __forceinline__ int per() const { return type() == MPPI_F32 ? CHUNK / 4 : CHUNK / 2; }
+    __device__ __forceinline__ int per(int chunk) const { return type() == MPPI_F32 ? chunk / 4 : chunk / 2; }       // entries
 };
 static_assert(MPPI_F32 < 4 && MPPI_F16 < 4 && MPPI_BF16 < 4, "two bits");
 struct Table {
     Entry e[TABLE];
-    int tensors;
+    int tensors, chunk;                  // chunk: bytes
     unsigned chunks;
 };
 static_assert(sizeof(Table) + 40 <= 4096, "and the kernels' other arguments");
 struct FarTable {                        // more tensors: in the workspace, written there by table_kernel
     const Entry* e;
-    int tensors;
+    int tensors, chunk;                  // chunk: bytes
     unsigned chunks;
 };
 
@@ -97,14 +97,17 @@ template <class T> struct Pack {         // 16 bytes of entries, wherever they l
 
 // tensor that holds chunk c, and the chunk's entries [lo, hi) in it
 template <class Tab> __device__ __forceinline__ const Entry& locate(const Tab& t, unsigned c, long long& lo, long long& hi) {
-    int a = 0, b = t.tensors - 1;
-    while (a < b) {
-        const int m = (a + b + 1) >> 1;
-        if (t.e[m].first <= c) a = m; else b = m - 1;
+    // the lanes look at 64 tensors at a time: a wait or two, where halving the table would wait eight times and more
+    const int lane = threadIdx.x & 63;
+    int a = 0, b = t.tensors;
+    while (b - a > 1) {
+        const int step = (b - a + 63) >> 6, i = a + lane * step;
+        a += (__popcll(__ballot(i < b && t.e[i < b ? i : a].first <= c)) - 1) * step;
+        b = a + step < b ? a + step : b;
     }
     const Entry& e = t.e[a];
     const unsigned end = a + 1 < t.tensors ? t.e[a + 1].first : t.chunks;
-    const int per = e.per();
+    const int per = e.per(t.chunk);
     lo = (long long)(c - e.first) * per;
     hi = lo + (c + 1 < end ? per : (int)(e.last_type >> 2));
     return e;
@@ -220,8 +223,11 @@ template <class Tab, bool MAX> __global__ void __launch_bounds__(BT) gradient_pa
 }
 
 template <bool MAX> __device__ double norm_of(const double* __restrict__ partials, int n, double* s) {
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < n; i += BT) acc = MAX ? fmax(acc, partials[i]) : acc + partials[i];
+    double acc = 0.0, v[GROUPS / BT];                // (all asked for at once)
+#pragma unroll
+    for (int k = 0; k < GROUPS / BT; k++) v[k] = (int)threadIdx.x + k * BT < n ? partials[threadIdx.x + k * BT] : 0.0;
+#pragma unroll
+    for (int k = 0; k < GROUPS / BT; k++) acc = MAX ? fmax(acc, v[k]) : acc + v[k];
     return norm_of_total<MAX>(group_total<MAX, BT>(acc, (uint32_t)acc, s));
 }
 
@@ -260,7 +266,7 @@ template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(
     const Entry& own = t.e[lane < t.tensors ? lane : 0];
     const unsigned long long g = (unsigned long long)own.g, out = (unsigned long long)own.out;
     const int type = own.type(), per = type == MPPI_F32 ? PIECE / 4 : PIECE / 2;
-    const int n = (int)((lane + 1 < t.tensors ? t.e[lane + 1].first : t.chunks) - own.first - 1) * own.per() + (int)(own.last_type >> 2);
+    const int n = (int)((lane + 1 < t.tensors ? t.e[lane + 1].first : t.chunks) - own.first - 1) * own.per(t.chunk) + (int)(own.last_type >> 2);
     const int count = lane < t.tensors ? (n + per - 1) / per : 0;
     int end = count;
 #pragma unroll
@@ -339,12 +345,13 @@ template <class Tab, bool MAX> int run(const Tab& t, size_t bytes, double* parti
     HIP_OK(hipGetLastError());
     return 0;
 }
-template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t pieces, size_t bytes, char* workspace, const double* max_norm, float* norm, hipStream_t s) {
+template <bool MAX> int run(const std::vector<Entry>& e, int chunk, unsigned chunks, size_t pieces, size_t bytes, char* workspace, const double* max_norm, float* norm, hipStream_t s) {
     double* partials = (double*)workspace;
     if (e.size() <= (size_t)TABLE) {
         Table t;
         std::copy(e.begin(), e.end(), t.e);
         t.tensors = (int)e.size();
+        t.chunk = chunk;
         t.chunks = chunks;
         if (pieces <= MOST_PIECES && bytes <= MOST_BYTES && t.tensors <= 64) {
             hipLaunchKernelGGL((gradient_small_kernel<MAX>), dim3(1), dim3(ST), 0, s, t, max_norm != nullptr, max_norm ? *max_norm : 0.0, norm);
@@ -358,11 +365,12 @@ template <bool MAX> int run(const std::vector<Entry>& e, unsigned chunks, size_t
         Table t;
         t.tensors = (int)std::min((size_t)TABLE, e.size() - at);
         std::copy(e.begin() + at, e.begin() + at + t.tensors, t.e);
+        t.chunk = 0;
         t.chunks = 0;
         hipLaunchKernelGGL(table_kernel, dim3(1), dim3(BT), 0, s, t, (int)at, far);
         HIP_OK(hipGetLastError());
     }
-    return run<FarTable, MAX>(FarTable{far, (int)e.size(), chunks}, bytes, partials, max_norm, norm, s);
+    return run<FarTable, MAX>(FarTable{far, (int)e.size(), chunk, chunks}, bytes, partials, max_norm, norm, s);
 }
 
 int gradients(int32_t device, int32_t n, const void* const* g, void* const* out, const int64_t* sizes, const int32_t* dtypes,
@@ -385,17 +393,21 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
         const int rc = check_overlap(n, g, out, sizes, dtypes);
         if (rc) return rc;
     }
+    size_t bytes = 0, pieces = 0;
+    for (int i = 0; i < n; i++) {
+        const size_t size = (size_t)sizes[i] * element_size(dtypes[i]);
+        bytes += size;
+        pieces += (size + PIECE - 1) / PIECE;
+    }
+    const int chunk = bytes <= (size_t)GROUPS * SMALL_CHUNK ? SMALL_CHUNK : CHUNK;
     std::vector<Entry> entries;
     entries.reserve(n);
     long long chunks = 0;
-    size_t bytes = 0, pieces = 0;
     for (int i = 0; i < n; i++) {
         if (sizes[i] == 0) continue;
-        const int64_t size = sizes[i] * element_size(dtypes[i]), per = CHUNK / element_size(dtypes[i]), parts = (sizes[i] + per - 1) / per;
+        const int64_t per = chunk / element_size(dtypes[i]), parts = (sizes[i] + per - 1) / per;
         entries.push_back({g[i], max_norm ? out[i] : nullptr, (unsigned)chunks, (unsigned)(sizes[i] - (parts - 1) * per) << 2 | (unsigned)dtypes[i]});
         chunks += parts;
-        bytes += (size_t)size;
-        pieces += (size_t)(size + PIECE - 1) / PIECE;
         if (chunks > 0x7fffffffll) return fail(-6, "more entries than one call can take");
     }
     size_t need = 0;
@@ -405,8 +417,8 @@ int gradients(int32_t device, int32_t n, const void* const* g, void* const* out,
     mppi::DeviceGuard guard;
     HIP_OK(guard.enter(device));
     char* ws = (char*)d_workspace;
-    return norm_type == MPPI_NORM_MAX ? run<true>(entries, (unsigned)chunks, pieces, bytes, ws, max_norm, d_norm, (hipStream_t)stream)
-                                      : run<false>(entries, (unsigned)chunks, pieces, bytes, ws, max_norm, d_norm, (hipStream_t)stream);
+    return norm_type == MPPI_NORM_MAX ? run<true>(entries, chunk, (unsigned)chunks, pieces, bytes, ws, max_norm, d_norm, (hipStream_t)stream)
+                                      : run<false>(entries, chunk, (unsigned)chunks, pieces, bytes, ws, max_norm, d_norm, (hipStream_t)stream);
 }
 
 }  // namespace
