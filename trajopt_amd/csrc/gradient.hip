@@ -241,16 +241,18 @@ template <bool MAX> __global__ void __launch_bounds__(BT) gradient_norm_kernel(c
 template <class Tab, bool MAX, bool STREAM> __global__ void __launch_bounds__(BT) gradient_clip_kernel(Tab t, const double* __restrict__ partials, int n_partials,
                                                                                        double max_norm, float* __restrict__ norm_out) {
     __shared__ double s[BT / 64];
+    unsigned c = blockIdx.x + (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x;
+    long long lo, hi;
+    const Entry* e = &locate(t, c, lo, hi);          // (while the partial sums are on their way)
     const double norm = norm_of<MAX>(partials, n_partials, s);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const bool clip = norm > max_norm && norm < INFINITY;
     const double scale = clip ? max_norm / norm : 1.0;
-    const unsigned last = blockIdx.x + (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x;
-    for (unsigned c = last;; c -= gridDim.x) {
-        long long lo, hi;
-        const Entry& e = locate(t, c, lo, hi);
-        write_chunk<BT, STREAM>(e, threadIdx.x, lo, hi, clip, scale);
+    while (true) {
+        write_chunk<BT, STREAM>(*e, threadIdx.x, lo, hi, clip, scale);
         if (c < gridDim.x) break;
+        c -= gridDim.x;
+        e = &locate(t, c, lo, hi);
     }
 }
 
