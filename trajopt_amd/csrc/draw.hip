@@ -990,10 +990,12 @@ template <class T> __global__ void __launch_bounds__(LT, 4) chunk_best_kernel(Dr
     if (par.valid() && best > (V)-INFINITY) {
         Weights<V> w;
         w.set(par.kappa, best, worst, 51);
+        float some = 0.0f;                           // (it says how large the sums become; fp32 is enough for that)
 #pragma unroll
         for (int p = 0; p < c.PIECES; p++)
 #pragma unroll
-            for (int j = 0; j < c.VEC; j++) sum += c.x[p][j] >= w.from ? w.weight(c.x[p][j]) : 0.0;
+            for (int j = 0; j < c.VEC; j++) some += c.x[p][j] >= w.from ? __expf(-(float)w.distance(c.x[p][j])) : 0.0f;
+        sum = some;
     }
     sum = group.reduce(sum, 0.0, Add());
     if (threadIdx.x == 0) {
@@ -1044,7 +1046,7 @@ template <class T> __global__ void __launch_bounds__(LT, 4) chunk_bins_kernel(Dr
         }
         sum = group.reduce(sum, 0.0, Add());
         int e;
-        (void)frexp(sum, &e);                         // sum < 2^e
+        (void)frexp(sum * 1.001, &e);                 // the sum is below 2^e (the weights of chunk_best are good to 10^-5)
         const int S = 62 - e < 51 ? 62 - e : 51;
         w.set(par.kappa, best, worst, S);
         state = wants_border(par, a.K) ? 2 : 1;
@@ -1101,6 +1103,7 @@ struct Where {
     int k, p_first, p_last;
     unsigned k_before;
     unsigned long long k_mass_before, mass_before;   // mass_before: before p_first
+    unsigned long long mass;                         // of all bins
     bool nothing;
 };
 struct WhereArea {
@@ -1126,6 +1129,7 @@ template <int NT> __device__ Where where(const Param& par, int K, const unsigned
     r.p_first = 1; r.p_last = 0;
     r.k_before = 0;
     r.k_mass_before = r.mass_before = 0;
+    r.mass = mtotal;
     r.nothing = false;
     unsigned long long least = mtotal, most = mtotal;          // bounds of the mass that top-k keeps
     if (par.top_k > 0 && par.top_k < K && (unsigned long long)par.top_k <= ctotal) {
@@ -1278,6 +1282,53 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
     if (at.k < 0 && at.p_first > at.p_last) return;  // all of them are kept
     const Weights<V> w = r.w;
     const LongBins<V> bins(w);
+    const bool share = at.p_first <= at.p_last;
+    if (r.listed <= BT) {
+        // A thread for each: ranks by comparing each with each, masses in the order of the ranks.  The bins of the mass border come first
+        // in that order, behind them, if it is another, the bin of the count border.
+        const unsigned n = r.listed, t = threadIdx.x;
+        V* line_v = (V*)(s.mass + BT);
+        static_assert(3 * BT <= BorderArea<V, BT>::BINS, "masses, values and ranks");
+        const bool in = t < n;
+        const V v = in ? l.list_v[row * a.K + t] : (V)-INFINITY;
+        const unsigned idx = in ? l.list_i[row * a.K + t] : UINT_MAX;
+        line_v[t] = v;
+        s.cnt[t] = idx;
+        const int bin = in ? bins.of(v) : LONG_BINS;
+        const double weight = w.weight(v);
+        const unsigned long long q = in ? whole(weight * w.scale) : 0ull;
+        const unsigned before_k = group.reduce(bin < at.k ? 1u : 0u, 0u, Add());             // (and line_v, cnt are there)
+        unsigned rank = 0;
+#pragma unroll 2
+        for (unsigned o = 0; o < n; o += 4) {
+#pragma unroll
+            for (unsigned j = 0; j < 4; j++) rank += line_v[o + j] > v || (line_v[o + j] == v && s.cnt[o + j] < idx) ? 1u : 0u;
+        }
+        bool keep = in && (at.k < 0 || bin < at.k || (bin == at.k && (long long)(rank - before_k) < par.top_k - (long long)at.k_before));
+        if (share) {
+            const unsigned long long some = group.reduce(keep && bin == at.k ? q : 0ull, 0ull, Add());
+            const unsigned long long target = share_of(par.top_p, at.k >= 0 ? at.k_mass_before + some : at.mass);
+            if (target == 0) {
+                if (t == 0) r.state = 0;
+                return;
+            }
+            if (in) s.mass[rank] = q;
+            __syncthreads();
+            unsigned long long total;
+            const unsigned long long ahead = group.scan(in ? s.mass[t] : 0ull, total);
+            s.mass[2 * BT + t] = at.mass_before + ahead;
+            __syncthreads();
+            keep = keep && bin <= at.p_last && s.mass[2 * BT + rank] < target;
+        }
+        const unsigned last = group.reduce(keep ? rank : 0u, 0u, Max());                     // (some sample is kept)
+        if (keep && rank == last) { r.border = v; r.last = idx; }
+        if (keep && weight >= par.min_p && q) {
+            const long long chunk = row * l.chunks + idx / CHUNK;
+            atomicAdd(&l.kept[chunk], q);
+            atomicAdd(&l.seg[chunk * Chunk<T>::SEGS + idx % CHUNK / Chunk<T>::SEG], q);
+        }
+        return;
+    }
     Listed<V, false> list{l.list_v + row * a.K, l.list_i + row * a.K, r.listed, (V)0, w};
     // values of the listed samples in bins first ... last
     auto range = [&](int first, int last, V low, V& lo, V& hi) {
@@ -1296,7 +1347,6 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
     unsigned keep = 0, all = 0, last = UINT_MAX;
     auto found = [&]() { border = s.border; keep = s.border_keep; all = s.border_all; last = s.border_idx; __syncthreads(); };
     unsigned long long mass = 0;                      // of what top-k keeps, where top-p asks
-    const bool share = at.p_first <= at.p_last;
     if (at.k >= 0) {
         range(at.k, at.k, w.from, lo, hi);
         (void)find_border<BY_COUNT>(list, s, group, (unsigned long long)par.top_k - at.k_before, 0.0, lo, hi, lo, list.n);
@@ -1315,9 +1365,7 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
             mass = at.k_mass_before + group.reduce(sum, 0ull, Add()) + keep * w.mass_of(border);
         }
     } else {
-        unsigned long long m = 0;
-        for (int i = threadIdx.x; i < LONG_BINS; i += BT) m += l.mass[row * LONG_BINS + i];
-        mass = group.reduce(m, 0ull, Add());
+        mass = at.mass;
     }
     if (share) {
         const unsigned long long target = share_of(par.top_p, mass);
