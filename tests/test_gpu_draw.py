@@ -275,6 +275,22 @@ def test_longest_row(dtype):
         _draw(torch.zeros(1, K + 1, dtype=R.dtype, device="cuda"), _numbers(1, 1, 1))
 
 
+@pytest.mark.parametrize("D", [1, 8, 9, 30])
+@pytest.mark.parametrize("step", [0.0, 0.01, 0.5])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_draws_of_long_rows(dtype, step, D):
+    """Few and many samples near the border (returns rounded to multiples of a step share values), with either border, both of
+    them, and neither."""
+    K = 70001
+    R = _returns(3, K, dtype, D, masked=0.01)
+    if step:
+        R = ((R.double() / step).round() * step).to(R.dtype)
+    u = _numbers(3, D, D)
+    for f in (dict(top_k=1), dict(top_k=900), dict(top_p=0.9), dict(top_k=5000, top_p=0.6), dict(top_k=30000, top_p=0.99, min_p=0.01),
+              dict(top_k=K - 1), dict(min_p=0.2)):
+        _check(R, u, kappa=0.9, **f)
+
+
 def test_nothing_to_do():
     import torch
     R, u = _returns(2, 10, "float32", 0), _numbers(2, 0, 0)

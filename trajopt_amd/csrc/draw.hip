@@ -1264,23 +1264,20 @@ template <class V, bool BY_INDEX> struct Listed {
     }
 };
 
-template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
-    using V = typename Traits<T>::V;
-    __shared__ BorderArea<V, BT> s;
-    __shared__ WhereArea sw;
-    Group<BT> group(s.slots);
-    const long long row = blockIdx.x;
-    LongRow<V>& r = l.row[row];
-    if (r.state != 2) return;
-    const Param par(a.f, row);
+// what is kept of a row: above the border, or equal to it with an index up to last
+template <class V> struct Kept {
+    V border;
+    unsigned last;
+    bool some;
+};
+template <class T, class V = typename Traits<T>::V>
+__device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long long row, const LongRow<V>& r, const Param& par, BorderArea<V, BT>& s, WhereArea& sw,
+                               Group<BT>& group) {
+    const Kept<V> nothing{(V)0, 0, false};
     const Where at = where<BT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, sw, group);
-    if (at.nothing) {
-        __syncthreads();
-        if (threadIdx.x == 0) r.state = 0;
-        return;
-    }
-    if (at.k < 0 && at.p_first > at.p_last) return;  // all of them are kept
+    if (at.nothing) return nothing;
     const Weights<V> w = r.w;
+    if (at.k < 0 && at.p_first > at.p_last) return {w.from, UINT_MAX, true};             // all of them are kept
     const LongBins<V> bins(w);
     const bool share = at.p_first <= at.p_last;
     if (r.listed <= BT) {
@@ -1308,10 +1305,7 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
         if (share) {
             const unsigned long long some = group.reduce(keep && bin == at.k ? q : 0ull, 0ull, Add());
             const unsigned long long target = share_of(par.top_p, at.k >= 0 ? at.k_mass_before + some : at.mass);
-            if (target == 0) {
-                if (t == 0) r.state = 0;
-                return;
-            }
+            if (target == 0) return nothing;
             if (in) s.mass[rank] = q;
             __syncthreads();
             unsigned long long total;
@@ -1321,13 +1315,14 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
             keep = keep && bin <= at.p_last && s.mass[2 * BT + rank] < target;
         }
         const unsigned last = group.reduce(keep ? rank : 0u, 0u, Max());                     // (some sample is kept)
-        if (keep && rank == last) { r.border = v; r.last = idx; }
+        if (keep && rank == last) { s.border = v; s.border_idx = idx; }
         if (keep && weight >= par.min_p && q) {
             const long long chunk = row * l.chunks + idx / CHUNK;
             atomicAdd(&l.kept[chunk], q);
             atomicAdd(&l.seg[chunk * Chunk<T>::SEGS + idx % CHUNK / Chunk<T>::SEG], q);
         }
-        return;
+        __syncthreads();
+        return {s.border, s.border_idx, true};
     }
     Listed<V, false> list{l.list_v + row * a.K, l.list_i + row * a.K, r.listed, (V)0, w};
     // values of the listed samples in bins first ... last
@@ -1369,10 +1364,7 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
     }
     if (share) {
         const unsigned long long target = share_of(par.top_p, mass);
-        if (target == 0) {
-            if (threadIdx.x == 0) r.state = 0;
-            return;
-        }
+        if (target == 0) return nothing;
         range(at.p_first, at.p_last, border, lo, hi);
         if (find_border<BY_MASS>(list, s, group, target - at.mass_before, 0.0, lo, hi, lo, list.n)) found();
     }
@@ -1384,7 +1376,6 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
         (void)find_border<BY_COUNT>(equal, s, group, keep, 0.0, -(V)a.K, (V)0, -(V)a.K, list.n);
         last = s.border_idx;
     }
-    if (threadIdx.x == 0) { r.border = border; r.last = last; }
     // what the list keeps joins the chunks
     list.each(border, w.best, [&](const V (&x)[4], unsigned live, int o) {
         unsigned in = 0;
@@ -1404,26 +1395,25 @@ template <class T> __global__ void __launch_bounds__(BT) row_border_kernel(DrawA
                 atomicAdd(&l.seg[chunk * Chunk<T>::SEGS + idx[j] % CHUNK / Chunk<T>::SEG], q[j]);
             }
     });
+    return {border, last, true};
 }
 
-// A wave for every draw: the chunk, its segment, the sample
-template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
-    using V = typename Traits<T>::V;
+// Draw number `at` of all by one wave: the chunk, its segment, the sample.  FRESH: masses that this workgroup has just added to.
+template <class T, bool FRESH, class V = typename Traits<T>::V>
+__device__ void draw_one(const DrawArgs& a, const LongArea<V>& l, long long row, long long at, const Param& par, const Weights<V>& w, const Kept<V>& r) {
     using C = Chunk<T>;
     constexpr int VEC = C::VEC;
-    const long long at = a.first + blockIdx.x, row = (unsigned)at / (unsigned)a.D;       // (below 2^31)
-    const LongRow<V>& r = l.row[row];
-    const Param par(a.f, row);
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 63;
+    const auto mass_at = [](const unsigned long long* p) { return FRESH ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p; };
     const unsigned long long* kept = l.kept + row * l.chunks;
     unsigned long long mass = 0, target = 0, run = 0;
     int chunk = 0;
-    if (r.state != 0) {
+    if (r.some) {
         const int PER = (l.chunks + 63) / 64;                   // neighbouring chunks of a lane
         unsigned long long sum = 0;
         for (int i = 0; i < PER; i++) {
             const int c = lane * PER + i;
-            sum += c < l.chunks ? kept[c] : 0ull;
+            sum += c < l.chunks ? mass_at(kept + c) : 0ull;
         }
         const unsigned long long inc = wave_scan(sum, 0ull, Add());
         mass = lane_value(inc, 63);
@@ -1434,7 +1424,7 @@ template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawAr
             run = lane_value(run, owner);
             chunk = owner * PER;
             for (int i = 0; i < PER - 1; i++) {                  // (the same in every lane)
-                const unsigned long long m = kept[chunk];
+                const unsigned long long m = mass_at(kept + chunk);
                 if (target - run < m) break;
                 run += m;
                 chunk++;
@@ -1445,12 +1435,11 @@ template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawAr
         if (lane == 0) { a.index[at] = -1; if (a.weight) a.weight[at] = 0.0f; }
         return;
     }
-    const unsigned long long m = lane < C::SEGS ? l.seg[(row * l.chunks + chunk) * C::SEGS + lane] : 0ull;
+    const unsigned long long m = lane < C::SEGS ? mass_at(l.seg + (row * l.chunks + chunk) * C::SEGS + lane) : 0ull;
     const unsigned long long inc = wave_scan(m, 0ull, Add());
     const int seg = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(target - (run + inc - m) < m)) - 1);
     run += lane_value(inc - m, seg);
 
-    const Weights<V> w = r.w;
     const int first = chunk * CHUNK + seg * C::SEG + lane * VEC;
     T raw[VEC];
     load_piece((const T*)a.R + row * a.row_stride, a.col_stride, (long long)first, a.K, raw);
@@ -1476,6 +1465,39 @@ template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawAr
             run += q[j];
         }
     }
+}
+
+// DRAW: the rows' draws as well, by the waves that found the borders
+constexpr int FEW_DRAWS = 8;
+template <class T, bool DRAW> __global__ void __launch_bounds__(BT) row_border_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    using V = typename Traits<T>::V;
+    __shared__ BorderArea<V, BT> s;
+    __shared__ WhereArea sw;
+    Group<BT> group(s.slots);
+    const long long row = blockIdx.x;
+    LongRow<V>& r = l.row[row];
+    const Param par(a.f, row);
+    const int state = r.state;
+    if (!DRAW && state != 2) return;
+    Kept<V> k{r.border, UINT_MAX, state != 0};
+    if (state == 2) {
+        k = keep_listed<T>(a, l, row, r, par, s, sw, group);
+        if (!DRAW && threadIdx.x == 0) {
+            r.border = k.border;
+            r.last = k.last;
+            r.state = k.some ? 2 : 0;
+        }
+    }
+    if (DRAW) {
+        __threadfence();                             // (the masses added by any of the threads, for all of them)
+        __syncthreads();
+        for (int d = threadIdx.x >> 6; d < a.D; d += BT / 64) draw_one<T, true>(a, l, row, row * a.D + d, par, r.w, k);
+    }
+}
+template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+    const long long at = a.first + blockIdx.x, row = (unsigned)at / (unsigned)a.D;       // (below 2^31)
+    const LongRow<typename Traits<T>::V>& r = l.row[row];
+    draw_one<T, false>(a, l, row, at, Param(a.f, row), r.w, {r.border, r.last, r.state != 0});
 }
 
 int ceil_log2(int n) {
@@ -1531,8 +1553,12 @@ template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_byte
     if (a.f.top_k_of || a.f.top_p_of || (a.f.top_k > 0 && a.f.top_k < a.K) || a.f.top_p < 1.0) {
         hipLaunchKernelGGL((chunk_split_kernel<T>), chunks, dim3(LT), 0, s, a, l);
         HIP_OK(hipGetLastError());
-        hipLaunchKernelGGL((row_border_kernel<T>), dim3(a.rows), dim3(BT), 0, s, a, l);
+        if (a.D <= FEW_DRAWS)
+            hipLaunchKernelGGL((row_border_kernel<T, true>), dim3(a.rows), dim3(BT), 0, s, a, l);
+        else
+            hipLaunchKernelGGL((row_border_kernel<T, false>), dim3(a.rows), dim3(BT), 0, s, a, l);
         HIP_OK(hipGetLastError());
+        if (a.D <= FEW_DRAWS) return 0;
     }
     return in_grids(a, (long long)a.rows * a.D, 64, [&](unsigned n) { hipLaunchKernelGGL((long_draw_kernel<T>), dim3(n), dim3(64), 0, s, a, l); });
 }
