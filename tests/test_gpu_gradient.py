@@ -79,7 +79,7 @@ def test_clipping_to_nothing_and_to_no_bound():
 
 
 @pytest.mark.parametrize("kind", ["l2", "max"])
-@pytest.mark.parametrize("n", [2, 127, 128, 129, 300, 1200])
+@pytest.mark.parametrize("n", [2, 127, 128, 129, 167, 168, 169, 300, 335, 336, 337, 1200])
 def test_many_tensors_of_mixed_types(n, kind):
     rng = np.random.RandomState(n)
     grads = []

@@ -43,7 +43,7 @@ struct Table {
     unsigned chunks;
 };
 static_assert(sizeof(Table) + 40 <= 4096, "and the kernels' other arguments");
-struct FarTable {                        // of more tensors: in the workspace, left there by the first pass
+struct FarTable {                        // of more tensors: in the workspace, put there by table_kernel
     const Entry* e;
     int tensors, chunk;                  // chunk: bytes
     unsigned chunks;
@@ -205,31 +205,32 @@ template <int NT, bool STREAM> __device__ __forceinline__ void write_chunk(const
     }
 }
 
-// far: where the table is to be left for the second pass, `before` chunks behind the start of all (NULL: it needs none)
-template <bool MAX> __global__ void __launch_bounds__(BT) gradient_partials_kernel(Table t, Entry* __restrict__ far, unsigned before, double* __restrict__ partials) {
+__global__ void __launch_bounds__(BT) table_kernel(Table t, Entry* __restrict__ far) {
+    for (int i = threadIdx.x; i < t.tensors; i += BT) far[i] = t.e[i];
+}
+
+// FAR: t holds the last tensors only, those before it, with `before` chunks, lie in far; it is put behind them for the second pass
+template <bool MAX, bool FAR> __global__ void __launch_bounds__(BT) gradient_partials_kernel(Table t, Entry* far, int tensors, unsigned before, double* __restrict__ partials) {
     __shared__ double s[BT / 64];
     double acc[4] = {0.0, 0.0, 0.0, 0.0};      // four chains of dependent additions
     uint32_t top = 0;
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         long long lo, hi;
-        const Entry& e = locate(t, c, lo, hi);
+        const Entry& e = FAR && c < before ? locate(FarTable{far, tensors, t.chunk, before}, c, lo, hi) : locate(t, c, lo, hi);
         read_chunk<MAX, BT>(e, threadIdx.x, lo, hi, acc, top);
     }
-    if (far && blockIdx.x == gridDim.x - 1)
-        for (int i = threadIdx.x; i < t.tensors; i += BT) far[i] = Entry{t.e[i].g, t.e[i].out, t.e[i].first + before, t.e[i].last_type};
+    if (FAR && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < t.tensors; i += BT) far[tensors + i] = t.e[i];
     const double v = group_total<MAX, BT>((acc[0] + acc[1]) + (acc[2] + acc[3]), top, s);
     if (threadIdx.x == 0) partials[blockIdx.x] = v;
 }
 
 template <bool MAX> __device__ double norm_of(const double* __restrict__ partials, int n, double* s) {
-    double acc = 0.0;
-    for (int first = threadIdx.x; first < n; first += GROUPS) {           // (once, but with more tables than GROUPS leaves room for)
-        double v[GROUPS / BT];                       // all asked for at once
+    double acc = 0.0, v[GROUPS / BT];                // (all asked for at once)
 #pragma unroll
-        for (int k = 0; k < GROUPS / BT; k++) v[k] = first + k * BT < n ? partials[first + k * BT] : 0.0;
+    for (int k = 0; k < GROUPS / BT; k++) v[k] = (int)threadIdx.x + k * BT < n ? partials[threadIdx.x + k * BT] : 0.0;
 #pragma unroll
-        for (int k = 0; k < GROUPS / BT; k++) acc = MAX ? fmax(acc, v[k]) : acc + v[k];
-    }
+    for (int k = 0; k < GROUPS / BT; k++) acc = MAX ? fmax(acc, v[k]) : acc + v[k];
     return norm_of_total<MAX>(group_total<MAX, BT>(acc, (uint32_t)acc, s));
 }
 
@@ -336,51 +337,45 @@ int check_overlap(int32_t n, const void* const* g, void* const* out, const int64
     return 0;
 }
 
-int tables(size_t n) { return (int)((n + TABLE - 1) / TABLE); }
-
 // second pass: the norm, and what it does to the entries
-template <class Tab, bool MAX> int second(const Tab& t, size_t bytes, const double* partials, int n, const double* max_norm, float* norm, hipStream_t s) {
-    const int groups = (int)std::min<unsigned>(t.chunks, (unsigned)GROUPS);
+template <class Tab, bool MAX> int second(const Tab& t, int groups, size_t bytes, const double* partials, const double* max_norm, float* norm, hipStream_t s) {
     if (!max_norm)
-        hipLaunchKernelGGL((gradient_norm_kernel<MAX>), dim3(1), dim3(BT), 0, s, partials, n, norm);
+        hipLaunchKernelGGL((gradient_norm_kernel<MAX>), dim3(1), dim3(BT), 0, s, partials, groups, norm);
     else if (bytes > STREAMED)
-        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX, true>), dim3(groups), dim3(BT), 0, s, t, partials, n, *max_norm, norm);
+        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX, true>), dim3(groups), dim3(BT), 0, s, t, partials, groups, *max_norm, norm);
     else
-        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX, false>), dim3(groups), dim3(BT), 0, s, t, partials, n, *max_norm, norm);
+        hipLaunchKernelGGL((gradient_clip_kernel<Tab, MAX, false>), dim3(groups), dim3(BT), 0, s, t, partials, groups, *max_norm, norm);
     HIP_OK(hipGetLastError());
     return 0;
 }
 template <bool MAX> int run(const std::vector<Entry>& e, int chunk, unsigned chunks, size_t pieces, size_t bytes, char* workspace, const double* max_norm, float* norm, hipStream_t s) {
-    const bool one = e.size() <= (size_t)TABLE;
+    const int groups = (int)std::min<unsigned>(chunks, (unsigned)GROUPS);
     double* partials = (double*)workspace;
-    Entry* far = one || !max_norm ? nullptr : (Entry*)(workspace + (GROUPS + tables(e.size())) * sizeof(double));
+    Entry* far = (Entry*)(workspace + GROUPS * sizeof(double));
     Table t;
     t.chunk = chunk;
-    t.tensors = (int)e.size();
     t.chunks = chunks;
-    if (one && pieces <= MOST_PIECES && bytes <= MOST_BYTES && t.tensors <= 64) {
-        std::copy(e.begin(), e.end(), t.e);
+    size_t at = 0;
+    for (;; at += TABLE) {                                   // all tables but the last go ahead
+        t.tensors = (int)std::min((size_t)TABLE, e.size() - at);
+        std::copy(e.begin() + at, e.begin() + at + t.tensors, t.e);
+        if (at + t.tensors == e.size()) break;
+        hipLaunchKernelGGL(table_kernel, dim3(1), dim3(BT), 0, s, t, far + at);
+        HIP_OK(hipGetLastError());
+    }
+    if (at > 0) {
+        hipLaunchKernelGGL((gradient_partials_kernel<MAX, true>), dim3(groups), dim3(BT), 0, s, t, far, (int)at, e[at].first, partials);
+        HIP_OK(hipGetLastError());
+        return second<FarTable, MAX>(FarTable{far, (int)e.size(), chunk, chunks}, groups, bytes, partials, max_norm, norm, s);
+    }
+    if (pieces <= MOST_PIECES && bytes <= MOST_BYTES && t.tensors <= 64) {
         hipLaunchKernelGGL((gradient_small_kernel<MAX>), dim3(1), dim3(ST), 0, s, t, max_norm != nullptr, max_norm ? *max_norm : 0.0, norm);
         HIP_OK(hipGetLastError());
         return 0;
     }
-    int sums = 0;
-    for (size_t at = 0; at < e.size(); at += TABLE) {        // first pass: a launch for every table, with its share of the workgroups
-        const size_t end = std::min(at + TABLE, e.size());
-        const unsigned before = e[at].first;
-        t.tensors = (int)(end - at);
-        t.chunks = (end < e.size() ? e[end].first : chunks) - before;
-        for (size_t i = at; i < end; i++) {
-            t.e[i - at] = e[i];
-            t.e[i - at].first -= before;
-        }
-        const unsigned share = chunks <= (unsigned)GROUPS ? t.chunks : std::max(1u, (unsigned)((unsigned long long)t.chunks * GROUPS / chunks));
-        hipLaunchKernelGGL((gradient_partials_kernel<MAX>), dim3(share), dim3(BT), 0, s, t, far ? far + at : nullptr, before, partials + sums);
-        HIP_OK(hipGetLastError());
-        sums += (int)share;
-    }
-    if (one) return second<Table, MAX>(t, bytes, partials, sums, max_norm, norm, s);
-    return second<FarTable, MAX>(FarTable{far, (int)e.size(), chunk, chunks}, bytes, partials, sums, max_norm, norm, s);
+    hipLaunchKernelGGL((gradient_partials_kernel<MAX, false>), dim3(groups), dim3(BT), 0, s, t, (Entry*)nullptr, 0, 0u, partials);
+    HIP_OK(hipGetLastError());
+    return second<Table, MAX>(t, groups, bytes, partials, max_norm, norm, s);
 }
 
 int gradients(int32_t device, int32_t n, const void* const* g, void* const* out, const int64_t* sizes, const int32_t* dtypes,
@@ -437,7 +432,7 @@ extern "C" {
 
 int mppi_gradient_workspace(int32_t n, size_t* bytes) {
     if (n < 0 || !bytes) return fail(-1, "bad argument");
-    *bytes = (GROUPS + tables((size_t)n)) * sizeof(double) + (n > TABLE ? (size_t)n * sizeof(Entry) : 0);
+    *bytes = GROUPS * sizeof(double) + (n > TABLE ? (size_t)n * sizeof(Entry) : 0);
     return 0;
 }
 
