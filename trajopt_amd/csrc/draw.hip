@@ -21,7 +21,6 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
-#include <type_traits>
 
 using mppi::fail;
 
@@ -459,8 +458,8 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
 template <class T, int NT, int BYTES> struct Shelf {
     using V = typename Traits<T>::V;
     static constexpr int VEC = 16 / sizeof(T);
-    static constexpr int FEW = BYTES >= 131072 ? 1024 : 128;   // up to this many samples that take part can move together
-    static constexpr int LAST = 128;                           // up to this many are left to one wave (finish)
+    static constexpr int FEW = NT >= 512 ? 1024 : 64;          // up to this many samples that take part can move together
+    static constexpr int LAST = 64;                            // up to this many are left to one wave (finish)
     struct alignas(16) Piece { T v[VEC]; };
     using Area = BorderArea<V, NT>;
     struct Shared {
@@ -578,79 +577,50 @@ template <class T, int NT, int BYTES> struct Shelf {
         C = VEC;
     }
 
-    // The rest of the way for n <= 64 E samples in the order of their indices, in the first wave alone: ranks by comparing each with
-    // each, masses in the order of the ranks for top-p, and in that of the indices for the draws.  Lane l holds samples l, l + 64;
-    // returns their values, masses, the mass before each, and the whole mass.
-    template <int E> __device__ unsigned long long finish(unsigned n, const Param& par, V (&v)[E], unsigned long long (&q)[E], unsigned long long (&before)[E]) {
-        const int lane = threadIdx.x & 63;
-        unsigned long long* line = s.b.mass;
-        const auto settle = []() {                   // what the wave's lanes wrote to LDS is there for all of them
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        };
+    // The rest of the way for n <= 64 samples in the order of their indices, by one wave, a sample per lane: ranks by comparing each with
+    // each, masses in the order of the ranks for top-p, and in that of the indices for the draws.  The lane's sample, its weight, its
+    // mass (0: it may not be drawn) and the mass before it; returns the whole mass.
+    __device__ unsigned long long finish(unsigned n, const Param& par, V& v, double& weight, unsigned long long& q, unsigned long long& before) {
+        const unsigned lane = threadIdx.x & 63;
         const bool by_count = par.top_k > 0 && par.top_k < (long long)n, by_share = !(par.top_p >= 1.0);
-        unsigned live = 0, rank[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const unsigned at_ = e * 64 + lane;
-            v[e] = at_ < n ? at(s.row[base + at_ / VEC], at_ % VEC) : (V)-INFINITY;
-            if (v[e] >= w.from && v[e] <= w.best) {
-                live |= 1u << e;
-            } else {
-                v[e] = (V)-INFINITY;
-                if (at_ < n) s.row[base + at_ / VEC].v[at_ % VEC] = minus_infinity((T*)nullptr);
-            }
-            rank[e] = 0;
-        }
+        v = lane < n ? at(s.row[base + lane / VEC], lane % VEC) : (V)-INFINITY;
+        bool live = v >= w.from && v <= w.best;
+        v = live ? v : (V)-INFINITY;
+        weight = w.weight(v);
+        const unsigned long long mass = whole(weight * w.scale);
         if (by_count || by_share) {
-            settle();
-#pragma unroll 16 / VEC
-            for (unsigned p = 0; p * VEC < n; p++) { // every lane reads the same piece: one access for VEC comparisons
-                const Piece x = s.row[base + p];
+            unsigned rank = 0;                       // (the lanes behind n come last, in their order)
+            if constexpr (sizeof(V) == 4) {          // value and index in one number
+                const unsigned long long place = (unsigned long long)key_of(v) << 32 | (63u - lane);
+                for (unsigned o = 0; o < n; o += 4) {
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const V ov = at(x, j);
+                    for (unsigned j = 0; j < 4; j++) rank += lane_value(place, o + j) > place ? 1u : 0u;
+                }
+            } else {
+                for (unsigned o = 0; o < n; o += 4) {
 #pragma unroll
-                    for (int e = 0; e < E; e++) rank[e] += ov > v[e] || (ov == v[e] && p * VEC + j < (unsigned)(e * 64 + lane)) ? 1u : 0u;
+                    for (unsigned j = 0; j < 4; j++) {
+                        const V ov = lane_value(v, o + j);
+                        rank += ov > v || (ov == v && o + j < lane) ? 1u : 0u;
+                    }
                 }
             }
-        }
-#pragma unroll
-        for (int e = 0; e < E; e++)
-            if (by_count && (long long)rank[e] >= par.top_k) live &= ~(1u << e);
-        if (by_share) {
-            w.masses(v, live, 0.0, q);
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                if (e * 64 + lane < (int)n) line[rank[e]] = q[e];
-            settle();
-            unsigned long long run = 0, ahead[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const unsigned long long m = e * 64 + lane < (int)n ? line[e * 64 + lane] : 0ull, inc = wave_scan(m, 0ull, Add());
-                ahead[e] = run + inc - m;
-                run += lane_value(inc, 63);
+            if (by_count) live = live && (long long)rank < par.top_k;
+            if (by_share) {
+                const unsigned long long m = live ? mass : 0ull;
+                const int to = (int)rank * 4;
+                const unsigned long long sorted = (unsigned long long)(unsigned)__builtin_amdgcn_ds_permute(to, (int)(m >> 32)) << 32 |
+                                                  (unsigned)__builtin_amdgcn_ds_permute(to, (int)(unsigned)m);
+                const unsigned long long inc = wave_scan(sorted, 0ull, Add()), ahead = inc - sorted;
+                const unsigned long long own = (unsigned long long)(unsigned)__builtin_amdgcn_ds_bpermute(to, (int)(ahead >> 32)) << 32 |
+                                               (unsigned)__builtin_amdgcn_ds_bpermute(to, (int)(unsigned)ahead);
+                live = live && own < share_of(par.top_p, lane_value(inc, 63));
             }
-            settle();
-#pragma unroll
-            for (int e = 0; e < E; e++) line[e * 64 + lane] = ahead[e];
-            settle();
-            const unsigned long long part = share_of(par.top_p, run);
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                if (!(e * 64 + lane < (int)n && line[rank[e]] < part)) live &= ~(1u << e);
         }
-        w.masses(v, live, par.min_p, q);
-        unsigned long long run = 0;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const unsigned long long inc = wave_scan(q[e], 0ull, Add());
-            before[e] = run + inc - q[e];
-            run += lane_value(inc, 63);
-        }
-        settle();                                    // (line may be written again)
-        return run;
+        q = live && weight >= par.min_p ? mass : 0ull;
+        const unsigned long long inc = wave_scan(q, 0ull, Add());
+        before = inc - q;
+        return lane_value(inc, 63);
     }
 
     // leaves out what lies behind the border that was found
@@ -732,30 +702,28 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         index[d] = h.base ? (long long)s.few_idx[i] : i;
         if (weight) weight[d] = (float)(w * h.w.scale / (double)mass);
     };
-    auto finish = [&](auto one) __attribute__((always_inline)) {                                         // few samples: the first wave does the rest
-        constexpr int E = decltype(one)::value;
+    auto finish = [&]() __attribute__((always_inline)) {                  // few samples: the first wave does the rest
         const unsigned n = h.most;
-        V v[E];
-        unsigned long long q[E], before[E], mass = 0;
+        unsigned long long mass = 0;
         if (wave == 0) {
-            mass = h.finish(n, par, v, q, before);
+            V v;
+            double own;
+            unsigned long long q, before;
+            mass = h.finish(n, par, v, own, q, before);
             if (D <= DIRECT) {
                 for (int d = 0; d < D; d++) {
                     const unsigned long long target = mass ? target_of(d == 0 ? u_wave : u[d], mass) : 0ull;
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-                        if (target - before[e] < q[e]) answer(d, e * 64 + lane, h.w.weight(v[e]), mass);
+                    if (target - before < q) answer(d, lane, own, mass);
                     if (mass == 0 && lane == 0) { index[d] = -1; if (weight) weight[d] = 0.0f; }
                 }
                 return;
             }
-#pragma unroll
-            for (int e = 0; e < E; e++) s.ends()[e * 64 + lane] = before[e] + q[e];
+            s.ends()[lane] = before + q;
         }
         if (D <= DIRECT) return;
         __syncthreads();                                                  // many draws: a thread each
         const unsigned long long* ends = s.ends();
-        mass = ends[n - 1];
+        mass = ends[63];
         if (mass == 0) return nothing();
         for (int d = tid; d < D; d += NT) {
             const unsigned long long target = target_of(d == tid ? u_thread : u[d], mass);
@@ -769,10 +737,9 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     };
     static_assert(AHEAD * NT * 16 >= BYTES, "the row is loaded in one go, and top[] holds all of its pieces");
     bool few = BYTES < 131072 && a.K <= H::LAST;
-    if (BYTES >= 131072) {
-        // Each thread's best is one sample, so the k best threads bound the k best samples from below: with many samples per
-        // thread next to nothing else passes that bound.
-        if (par.top_k > 0 && par.top_k <= NT / 4 && h.GP > 1) h.raise(mine, (unsigned)par.top_k);
+    const bool raised = NT >= 512 && par.top_k > 0 && par.top_k <= NT / 2 && h.GP > 1;
+    if (raised) h.raise(mine, (unsigned)par.top_k);
+    if (raised || BYTES >= 131072) {
         h.gather_few(top);
         few = h.base && h.most <= H::LAST;
     }
@@ -780,15 +747,12 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
         h.cut_behind();
         h.bottom = h.w.from;
         h.most = h.most < par.top_k ? h.most : (unsigned)par.top_k;
-        if (BYTES < 131072 && h.most <= H::LAST) {
+        if (BYTES < 131072 && !h.base && h.most <= H::LAST) {
             h.gather_few(top);
             few = true;
         }
     }
-    if (few) {
-        if (h.most <= 64) finish(std::integral_constant<int, 1>()); else finish(std::integral_constant<int, 2>());
-        return;
-    }
+    if (few) return finish();
     if (!(par.top_p >= 1.0) && find_border<BY_SHARE>(h, s.b, h.group, 0, par.top_p, h.w.from, best, h.bottom, h.most)) h.cut_behind();
 
     unsigned long long sum = 0, mass;
