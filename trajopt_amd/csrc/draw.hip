@@ -3,16 +3,25 @@
 //
 // Numbers.  A return that is NaN or infinite weighs nothing, as in the planner's updates.  Weights are evaluated in fp64 and
 // summed as 64-bit fixed point, q_i = round(w_i 2^S): integer sums do not depend on their order, so the histograms may use
-// atomics, a row gives the same answer however it is split, and ties are exact.  S is chosen from the row's own mass (its
-// fp64 sum, rounded up to a power of two), so the sum stays below 2^63 and K roundings of half a unit are at most
-// K 2^-62 of the mass.  Samples with kappa (max - R) > (S + 1) ln 2 round to zero; they cannot be drawn, so they are left
-// out from the start.
+// atomics, a row gives the same answer however it is split, and ties are exact.  The best sample weighs 1, so a mass is never
+// below 2^S, and each of K roundings is off by half a unit at most.  Rows in LDS take the largest S at which K weights of 1
+// stay below 2^62 (at most 51, where w 2^S still fits the 52 bits of a double's fraction: 46 for the longest row); longer
+// rows first sum their weights and take S from that sum, so that a row with few samples that count keeps 51 bits of them.
+// Samples with kappa (max - R) > (S + 1) ln 2 round to zero; they cannot be drawn, and are left out from the start.
 //
 // Borders.  The samples kept by top-k and top-p are a prefix of the order (return descending, index ascending), so either
-// filter is one pair (key of the last kept return, how many of the samples equal to it are kept).  It is found without
-// sorting: a histogram of counts (top-k) or masses (top-p) over bins that are linear in kappa (max - R), then, while the bin
-// with the border holds more than LIST samples of different returns, histograms over the bits of its keys, and last the
-// ranks of the LIST candidates by comparing each with each.
+// filter is one pair (the last return that is kept, and the index up to which samples equal to it are).  It is found without
+// sorting: a histogram of counts (top-k) or masses (top-p) over bins that are linear in max - R, then, while the bin with the
+// border holds more than 64 samples of different returns, histograms over the bits of its keys, and last the ranks of the up to
+// 64 candidates, a lane each, by comparing each with each.  (A linear bin holds about as many samples wherever it lies; bins
+// of the key's leading bits would put most returns of a planner, which are of one magnitude, into one.)
+//
+// What bounds it.  The bytes are few (the benchmark planner's row is 16 KB); what takes the time is one pass behind the other
+// over a row, with a barrier after each, and the instructions of code that runs once.  So a row stays in one workgroup's LDS as long
+// as it fits, passes test values in the type of the row and evaluate fp64 exponentials only where a sample passes, and loops are
+// rolled.  Per call, with the launch (3.6 us for the smallest kernel there is): 1 x 40 fp64 with top-k 5.7 us; 1 x 4096 fp32 with
+// top-p 9.2; 1024 x 512 fp32 with all three filters 8.8; 192 x 65535 bf16 with all three 17.2 (25 MB: 1.5 TB/s); 1 x 524288
+// fp32 with both borders 30; 16 x 262144 fp64 with top-p and 64 draws each 59.
 #include "abi_common.hpp"
 #include "../../include/mppi_hip.h"
 
@@ -323,7 +332,7 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
     };
     if (NT == 64) __syncthreads();                   // (larger groups have just met at a barrier)
     if (threadIdx.x == 0) s.n_list = 0;
-    if (most > 16) {                                 // (the histogram costs less than comparing as few as 32 with each other)
+    if (most > 16) {     // (comparing more with each other costs more than the histogram: 1 x 40 fp64 3.8 us of kernel with it, 4.9 without)
 #pragma unroll 1
         while (true) {
 #pragma unroll
@@ -450,16 +459,17 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
 // ------------------------------------------------------------------------------------------
 // rows of up to 128 KB: one workgroup each
 // ------------------------------------------------------------------------------------------
-// The row lies in LDS as it came, behind its end -inf; what is not finite fails the comparison with the lowest or the highest.  Thread t owns the C samples from t C on, in GP
-// pieces of 16 bytes; it visits them from piece t mod GP on, so that the lanes of a wave read from all banks.  All loops over
-// samples stay rolled: unrolled, a kernel of this many passes is larger than the instruction cache.  A pass tests values
-// against the lowest one that takes part, in the type of the row (fp32 or fp64); exponentials, in fp64, are evaluated only for
-// pieces with a sample that passes.
+// The row lies in LDS as it came, behind its end -inf; what is not finite fails the comparison with the lowest or the highest.
+// Thread t owns the C samples from t C on, in GP pieces of 16 bytes; it visits them from piece t mod GP on, so that the lanes of
+// a wave read from all banks.  All loops over samples stay rolled: unrolled, or with the row in registers, a kernel of this many
+// passes is larger than the instruction cache (192 x 65535 bf16: 424 us in registers, 88 with the same passes over LDS).  A pass
+// tests values against the lowest one that takes part, in the type of the row (fp32 or fp64); exponentials, in fp64, are evaluated
+// only for pieces with a sample that passes (88 -> 62 us).
 template <class T, int NT, int BYTES> struct Shelf {
     using V = typename Traits<T>::V;
     static constexpr int VEC = 16 / sizeof(T);
     static constexpr int FEW = NT >= 512 ? 1024 : 64;          // up to this many samples that take part can move together
-    static constexpr int LAST = 64;                            // up to this many are left to one wave (finish)
+    static constexpr int LAST = 64;                            // up to this many are left to one wave (finish): a sample per lane
     struct alignas(16) Piece { T v[VEC]; };
     using Area = BorderArea<V, NT>;
     struct Shared {
@@ -503,7 +513,7 @@ template <class T, int NT, int BYTES> struct Shelf {
         }
     }
 
-    // raises w.from to a value that at least k threads' own values `mine` reach (one per thread), near the highest such
+    // Raises w.from to a value that at least k threads' own values `mine` reach (one per thread), near the highest such.
     __device__ void raise(V mine, unsigned k) {
         constexpr int BINS = Area::BINS, PER = BINS / NT;
         const V per = w.best > bottom ? (V)BINS / (w.best - bottom) : (V)0;
@@ -737,6 +747,11 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     };
     static_assert(AHEAD * NT * 16 >= BYTES, "the row is loaded in one go, and top[] holds all of its pieces");
     bool few = BYTES < 131072 && a.K <= H::LAST;
+    // Each thread's best is one sample, so the k best threads bound the k best samples from below, and with many samples per thread
+    // little else passes that bound: what passes moves together, and the passes that follow go over it alone.  Up to NT / 2: beyond,
+    // more passes than can move (64 x 65535 bf16, k = 512: 56 us without the bound, 24 with it; k = 800: 55 and 56).  With two
+    // pieces per thread it gains little without top-p behind it (64 x 4096 fp32, k = 200: 9.3 and 10.2, with top-p 13.2 and 12.9),
+    // with four much (64 x 8192: 11.5 and 10.4, with top-p 17.9 and 13.3).
     const bool raised = NT >= 512 && par.top_k > 0 && par.top_k <= NT / 2 && h.GP > 1;
     if (raised) h.raise(mine, (unsigned)par.top_k);
     if (raised || BYTES >= 131072) {
@@ -833,16 +848,20 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 }
 
 // ------------------------------------------------------------------------------------------
-// longer rows: a workgroup for every chunk of CHUNK samples, five launches
+// longer rows: a workgroup for every chunk of CHUNK samples, up to five launches
 // ------------------------------------------------------------------------------------------
 //   chunk_best    highest, lowest and summed weight of every chunk; clears what the next ones add to
 //   chunk_bins    counts and masses over bins linear in best - v, a histogram per row
-//   chunk_split   the bins in which the borders can lie follow from the histogram: mass of what lies before them by chunk, and a
-//                 list of the samples in them
-//   row_border    the borders among the listed samples; their masses join those of their chunks
-//   long_draw     for every draw: the chunk, then the sample
-// Rows without top-k and top-p need no list: chunk_split and row_border leave their chunks' masses as chunk_bins wrote them.
-//                 (segment: the 64 VEC samples that one wave holds in one piece each)
+//   chunk_split   the bins in which the borders can lie follow from the histogram: mass of what lies before them by chunk and by
+//                 segment (the 64 VEC samples that one wave holds in one piece each), and a list of the samples in them
+//   row_border    the borders among the listed samples; their masses join those of their chunks; up to 4 draws
+//   long_draw     more draws, a wave for each: the chunk, then the segment, then the sample
+// Rows without top-k and top-p need no list: the masses of their chunks stay as chunk_bins wrote them, and long_draw follows.
+//
+// Each of the first three reads the row once, and only the first finds it outside the caches (in part: an L2 holds 4 MB).  A launch
+// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 4.6, 8.1, 8.3, 10.2 us; 16 x 262144 fp64 (34 MB) and 64 draws: 10.4, 13.5,
+// 16.2, 16.6, 4.5 us, i.e. 3.2 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
+// each for a wave) in the two that need masses.  Chunks of 4096 or 2048 samples instead of 8192: within 5 % on both.
 constexpr int MOST_SEGS = 64, LT = 512, CHUNK = 8192, HELD = CHUNK / LT, LONG_BINS = 1024, BT = 256;
 
 template <class V> struct LongRow {                  // what is known of a row (written by its first workgroup of chunk_bins)
@@ -1245,8 +1264,9 @@ __device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long lon
     const LongBins<V> bins(w);
     const bool share = at.p_first <= at.p_last;
     if (r.listed <= BT) {
-        // A thread for each: ranks by comparing each with each, masses in the order of the ranks.  The bins of the mass border come first
-        // in that order, behind them, if it is another, the bin of the count border.
+        // A thread for each: ranks by comparing each with each, masses in the order of the ranks (1 x 524288 fp32: 8.6 us, by the
+        // histograms below 11.6).  The bins of the mass border come first in that order, behind them, if it is another, the
+        // bin of the count border.
         const unsigned n = r.listed, t = threadIdx.x;
         V* line_v = (V*)(s.mass + BT);
         static_assert(3 * BT <= BorderArea<V, BT>::BINS, "masses, values and ranks");
@@ -1431,8 +1451,9 @@ __device__ void draw_one(const DrawArgs& a, const LongArea<V>& l, long long row,
     }
 }
 
-// DRAW: the rows' draws as well, by the waves that found the borders
-constexpr int FEW_DRAWS = 8;
+// DRAW: the rows' draws as well, a wave each by those that found the borders: less than another launch for one round of them (16 x
+// 262144 fp64, per call: 4 draws 51.2 us, 52.0 with a launch of their own; 8 draws 53.1 and 51.6, 64 draws 81 and 53).
+constexpr int FEW_DRAWS = BT / 64;
 template <class T, bool DRAW> __global__ void __launch_bounds__(BT) row_border_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ BorderArea<V, BT> s;
@@ -1455,7 +1476,8 @@ template <class T, bool DRAW> __global__ void __launch_bounds__(BT) row_border_k
     if (DRAW) {
         __threadfence();                             // (the masses added by any of the threads, for all of them)
         __syncthreads();
-        for (int d = threadIdx.x >> 6; d < a.D; d += BT / 64) draw_one<T, true>(a, l, row, row * a.D + d, par, r.w, k);
+        const int d = threadIdx.x >> 6;
+        if (d < a.D) draw_one<T, true>(a, l, row, row * a.D + d, par, r.w, k);
     }
 }
 template <class T> __global__ void __launch_bounds__(64) long_draw_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
@@ -1497,12 +1519,19 @@ template <class T, int NT, int BYTES> int launch_rows(DrawArgs a, hipStream_t s)
 template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_bytes, hipStream_t s) {
     using V = typename Traits<T>::V;
     if ((size_t)a.K * sizeof(T) <= SHELF) {
+        // One wave needs no barriers, but has every pass to itself: 1024 x 512 fp32 with all filters 9.8 us by 64 threads, 18.7 by 512;
+        // 1 x 512 and 64 draws 9.3 and 10.3, 200 draws 11.4 and 10.4.  More than 512 threads pay where a row would otherwise be more
+        // than 64 KB, or 64 samples per thread: 1024 x 4096 fp32 21 us by 512 threads, 64 by 1024; 1 x 8192 11.7 and 15.9; 1024 x
+        // 16384 40 and 64; 1 x 16384 15.8 and 14.9.  (Two sizes of 512: with LDS for 64 KB fewer workgroups share a CU, 1024 x 8192
+        // fp32 26 us with 32 KB, 33 with 64.)
         if (a.K <= 512 && a.D <= 64) return launch_rows<T, 64, 512 * sizeof(T)>(a, s);
         if (a.K * sizeof(T) <= 32768) return launch_rows<T, 512, 32768>(a, s);
         if constexpr (sizeof(T) >= 4)
             if (a.K * sizeof(T) <= 65536) return launch_rows<T, 512, 65536>(a, s);
         return launch_rows<T, 1024, SHELF>(a, s);
     }
+    // Five launches cost 30 us whatever the row; one workgroup is faster as long as it holds the row (1 x 32768 fp32: with both filters
+    // 17 us and 34, with top-p alone 32 and 33; 192 of them 19 and 58, 35 and 58).
     LongArea<V> l;
     if (!workspace || workspace_bytes < LongArea<V>::carve(&l, (char*)workspace, a.rows, a.K))
         return fail(-1, "workspace too small (mppi_draw_workspace)");

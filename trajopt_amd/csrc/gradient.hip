@@ -4,11 +4,14 @@
 //     out = g s,  s = max_norm / norm if norm > max_norm, else 1; a norm that is not finite changes nothing
 //
 // Numbers.  Squares and their sums are fp64, so no fp32 gradient overflows or vanishes in them, and every sum has a fixed order: a
-// thread adds what it reads, the lanes of a workgroup are added by a tree, the workgroups in the order of their partial sums, of
+// thread adds what it reads, the lanes of a workgroup are added by a tree, and so are the partial sums of the workgroups, of
 // which the sizes of the tensors alone say what each covers.  Entries are scaled in fp64 (the scale of large gradients may lie below
 // fp32's range) and rounded to fp32; 16-bit ones from there to their type, 2^-16 of whose step the first rounding is at most.
 //
-// Two passes over the data: no entry can be scaled before all have been read.
+// Two passes over the data: no entry can be scaled before all have been read.  Large sets are bound by memory: 1.07 GB of fp32 read
+// in 179 us (6.0 TB/s), 268 MB of bf16 read in 50 us and read again and written in 84 (6.4 TB/s; what a copy moves here: 4.8).  Small
+// ones are bound by launches and by the host: the six tensors of a critic take one launch, 6.3 us per call; 384 small tensors four,
+// of which two carry tables of addresses, 27 to 31 us per call, 17 of them in this library and 14 on the GPU.
 #include "abi_common.hpp"
 #include "../../include/mppi_hip.h"
 
@@ -23,9 +26,12 @@ using mppi::fail;
 namespace {
 
 constexpr int BT = 256;                  // threads of a workgroup
-constexpr int CHUNK = 65536, SMALL_CHUNK = 16384;      // bytes of one tensor that a workgroup takes at a time
-constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums
-constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way
+// Bytes of one tensor that a workgroup takes at a time: four rounds of its loads, or one where there would be too few workgroups (150
+// fp16 tensors of 10 MB: 14.0 us per call, 16.0 with the larger; 268 MB of bf16: 133 us, 149 with the smaller, 155 with 256 KB).
+constexpr int CHUNK = 65536, SMALL_CHUNK = 16384;
+constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums (4096: 131 us for 133)
+constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way (268 MB of bf16: 2: 135.7 us, 4: 133.4, 8: 134.3)
+constexpr size_t STREAMED = 24 << 20;    // bytes from which on entries go past the caches (gradient_clip_kernel)
 constexpr int TABLE = 168;               // tensors whose table travels in a kernel's arguments (4 KB at most)
 
 struct Entry {
@@ -240,7 +246,9 @@ template <bool MAX> __global__ void __launch_bounds__(BT) gradient_norm_kernel(c
     if (threadIdx.x == 0) *norm_out = (float)norm;
 }
 
-// Every workgroup takes the chunks it took for the norm, the last one first: that one may still lie in its caches.
+// Every workgroup takes the chunks it took for the norm, the last one first: that one may still lie in its caches.  STREAM: above 24 MB
+// loads and stores go past them, or the next call's reads wait for this one's writes to leave (per call out of place, with and
+// without: 16 MB 11.8 and 11.7 us, 32 MB 15.3 and 18.4, 256 MB 125 and 158; in place 64 MB 33.5 and 34.3, 256 MB 128 and 155).
 template <class Tab, bool MAX, bool STREAM> __global__ void __launch_bounds__(BT) gradient_clip_kernel(Tab t, const double* __restrict__ partials, int n_partials,
                                                                                        double max_norm, float* __restrict__ norm_out) {
     __shared__ double s[BT / 64];
@@ -260,7 +268,8 @@ template <class Tab, bool MAX, bool STREAM> __global__ void __launch_bounds__(BT
 }
 
 // Few entries: one workgroup does all of it, a wave for every PIECE, and its second reading comes from the cache of its XCD.  A
-// round of pieces takes about a microsecond; MOST_PIECES is three rounds, where two launches take as long.
+// round of 16 pieces takes about a microsecond, and three rounds as long as two launches (per call, this and two launches: 32 full
+// pieces 7.9 and 9.5 us, 45 full ones 10.6 and 9.6, 47 of 400 bytes 7.1 and 10.2); MOST_BYTES stops the full ones earlier.
 constexpr int ST = 1024, PIECE = 4096 /* bytes */, MOST_PIECES = 48;
 constexpr size_t MOST_BYTES = 128 << 10;
 template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(Table t, bool write, double max_norm, float* __restrict__ norm_out) {
@@ -307,7 +316,6 @@ template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(
     const double scale = clip ? max_norm / norm : 1.0;
     pieces([&](const Entry& e, long long lo, long long hi) { write_chunk<64, false>(e, lane, lo, hi, clip, scale); });
 }
-constexpr size_t STREAMED = 24 << 20;    // bytes
 
 int element_size(int dtype) { return dtype == MPPI_F32 ? 4 : 2; }
 
