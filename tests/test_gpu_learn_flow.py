@@ -109,6 +109,49 @@ def test_draw_of_explicit_actions_and_between_iterations(dm):
     p.close()
 
 
+def test_draws_with_a_critic_and_from_several_host_threads(dm):
+    """The critic's values belong to the returns that a draw weighs; planners of their own in threads of their own draw while others
+    capture their graphs, and give what they give one after the other."""
+    import threading
+    rng = np.random.RandomState(2)
+    W = [rng.normal(size=s).astype(np.float32) * 0.3 for s in ((128, 14), (128,), (128, 128), (128,), (1, 128), (1,))]
+    u = rng.uniform(size=(4, 6))
+
+    def run(i, out):
+        K, H, dtype = [(700, 6, "f32"), (64, 9, "f64"), (4096, 5, "f32"), (40000, 4, "f32")][i]
+        seen = []
+        for life in range(2):
+            p = _p(dm, K, H, dtype, kappa=3.0)
+            p.set_start_state(np.full(7, 0.1 * i), np.zeros(7), np.array([0.1, 0.0, 0.1]), 0)
+            p.set_base_actions(np.zeros((H, 7)))
+            if life == 0:
+                p.set_critic(14, W)
+            for t in range(6):
+                p.generate_noise(5 + t)
+                p.iterate(t % 3)
+                p.draw(u[i, t], top_k=(0, 20)[t % 2], top_p=(1.0, 0.8)[t % 2])
+                k, w = p.drawn()
+                R = p.returns()
+                want_k, want_w = ref_learn.draw(R, [u[i, t]], 3.0, top_k=(0, 20)[t % 2], top_p=(1.0, 0.8)[t % 2])
+                assert k == want_k[0] and abs(w - want_w[0]) <= WEIGHT_RTOL * want_w[0]
+                seen.append(np.r_[p.act_sequence().ravel(), R])
+                p.advance()
+            p.close()
+        out[i] = seen
+
+    serial, threaded = {}, {}
+    for i in range(4):
+        run(i, serial)
+    assert not np.array_equal(serial[0][0], serial[0][6])          # with and without the critic
+    threads = [threading.Thread(target=run, args=(i, threaded)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(4):
+        assert i in threaded and all(np.array_equal(a, b) for a, b in zip(serial[i], threaded[i])), i
+
+
 def test_draw_refusals(dm):
     from trajopt_amd._lib import MppiError
     p = _p(dm, 16, 3)
