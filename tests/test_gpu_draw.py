@@ -326,11 +326,12 @@ def test_rows_behind_the_last_are_left_alone():
         assert ctypes.sizeof(f) == 64
 
 
+@pytest.mark.parametrize("D", [2, 9])
 @pytest.mark.parametrize("K", [40, 3000, 100000])
-def test_captured_and_replayed(K):
+def test_captured_and_replayed(K, D):
     """Two graphs and eager calls in turn; every replay against the eager result of its own inputs."""
     import torch
-    R, u = _returns(2, K, "float32", K), _numbers(2, 9, K)
+    R, u = _returns(2, K, "float32", K), _numbers(2, D, K)
     _draw(R, u, kappa=1.0, top_k=30, top_p=0.9)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -345,7 +346,7 @@ def test_captured_and_replayed(K):
     torch.cuda.synchronize()
     for turn in range(4):
         for (r, v), g, out in zip(ins, graphs, outs):
-            v.copy_(_numbers(2, 9, 50 + turn))
+            v.copy_(_numbers(2, D, 50 + turn))
             r.copy_(_returns(2, K, "float32", 90 + turn))
             g.replay()
             want = _draw(r, v, kappa=1.0, top_k=30, top_p=0.9)

@@ -200,11 +200,12 @@ def test_same_bits_every_time_and_on_other_streams():
         assert torch.equal(norm, w[0]) and all(torch.equal(a, b) for a, b in zip(out, w[1]))
 
 
-def test_captured_and_replayed():
-    """Two graphs over different gradients, with eager calls between the replays."""
+@pytest.mark.parametrize("sizes", [((5000, 128, 300), (200000, 128, 300)), ((700,) * 170, (4001,) * 400)])
+def test_captured_and_replayed(sizes):
+    """Two graphs over different gradients, with eager calls between the replays; few tensors, and more than travel in arguments."""
     import torch
     from trajopt_amd.device import clip_gradients
-    base = [_tensors((n, 128, 300), "float32", n) for n in (5000, 200000)]
+    base = [_tensors(s, "float32", len(s)) for s in sizes]
     live = [[g.clone() for g in b] for b in base]
     clip_gradients([g.clone() for g in base[0]], 0.1)
     torch.cuda.synchronize()
