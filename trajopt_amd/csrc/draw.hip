@@ -848,7 +848,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 }
 
 // ------------------------------------------------------------------------------------------
-// longer rows: a workgroup for every chunk of CHUNK samples, up to five launches
+// longer rows: a workgroup for every chunk of 4096 or 8192 samples, up to five launches
 // ------------------------------------------------------------------------------------------
 //   chunk_best    highest, lowest and summed weight of every chunk; clears what the next ones add to
 //   chunk_bins    counts and masses over bins linear in best - v, a histogram per row
@@ -861,8 +861,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 // Each of the first three reads the row once, and only the first finds it outside the caches (in part: an L2 holds 4 MB).  A launch
 // takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 4.6, 8.1, 8.3, 10.2 us; 16 x 262144 fp64 (34 MB) and 64 draws: 10.4, 13.5,
 // 16.2, 16.6, 4.5 us, i.e. 3.2 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
-// each for a wave) in the two that need masses.  Chunks of 4096 or 2048 samples instead of 8192: within 5 % on both.
-constexpr int MOST_SEGS = 64, LT = 512, CHUNK = 8192, HELD = CHUNK / LT, LONG_BINS = 1024, BT = 256;
+// each for a wave) in the two that need masses.
+constexpr int MOST_SEGS = 64, LT = 512, LONG_BINS = 1024, BT = 256;
 
 template <class V> struct LongRow {                  // what is known of a row (written by its first workgroup of chunk_bins)
     Weights<V> w;
@@ -870,17 +870,21 @@ template <class V> struct LongRow {                  // what is known of a row (
     unsigned last, listed;
     int state;                                       // 0: nothing to draw, 1: every sample that takes part is kept, 2: borders
 };
+// log2 of a chunk's samples: smaller ones where there would be up to 128 workgroups (per call, top-p alone, 4096 and 8192: 1 x 70000 39 us and 44, 1 x 524288
+// 37 and 40; more of them add more to the histogram: 16 x 262144 fp64 58 and 57, 1 x 4000000 with top-k 64 and 51).
+__host__ __device__ __forceinline__ int chunk_shift(size_t rows, size_t K) { return rows * K <= (size_t)1 << 20 ? 12 : 13; }
 template <class V> struct LongArea {                 // the workspace, of all rows
     V *best, *worst;                                 // [rows][chunks]
     double* sum;
-    unsigned long long *kept, *seg, *mass;           // mass of a chunk, [rows][chunks], and of its segments; [rows][LONG_BINS]
+    unsigned long long *kept, *seg, *mass;           // mass of a chunk, [rows][chunks], and of its segments, [MOST_SEGS]; [rows][LONG_BINS]
     unsigned* cnt;
     LongRow<V>* row;
     V* list_v;                                       // [rows][K]
     unsigned* list_i;
     int chunks;
     static size_t carve(LongArea* a, char* p, size_t rows, size_t K) {
-        const size_t chunks = (K + CHUNK - 1) / CHUNK;
+        const int shift = chunk_shift(rows, K);
+        const size_t chunks = (K + (1u << shift) - 1) >> shift;
         size_t at = 0;
         auto take = [&](size_t bytes) { char* r = p + at; at += (bytes + 255) & ~(size_t)255; return r; };
         LongArea local;
@@ -901,9 +905,10 @@ template <class V> struct LongArea {                 // the workspace, of all ro
 };
 
 // the chunk of this workgroup, HELD samples per thread, in pieces of VEC neighbours
-template <class T> struct Chunk {
+template <class T> constexpr int segment = 64 * (16 / (int)sizeof(T));       // samples that one wave holds in a piece per lane
+template <class T, int CHUNK> struct Chunk {
     using V = typename Traits<T>::V;
-    static constexpr int VEC = 16 / sizeof(T), PIECES = HELD / VEC, SEG = 64 * VEC, SEGS = CHUNK / SEG;
+    static constexpr int HELD = CHUNK / LT, VEC = 16 / sizeof(T), PIECES = HELD / VEC, SEGS = CHUNK / segment<T>;
     static_assert(SEGS <= MOST_SEGS, "");
     V x[PIECES][VEC];
     int first;                                       // index of x[0][0]
@@ -944,13 +949,13 @@ template <class T> struct Chunk {
 
 __device__ __forceinline__ bool wants_border(const Param& par, int K) { return (par.top_k > 0 && par.top_k < K) || !(par.top_p >= 1.0); }
 
-template <class T> __global__ void __launch_bounds__(LT, 4) chunk_best_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_best_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ unsigned long long s_slots[LT / 32];
     Group<LT> group(s_slots);
     const long long row = blockIdx.x / l.chunks;
     const int chunk = (int)(blockIdx.x - row * l.chunks);
-    Chunk<T> c;
+    Chunk<T, CHUNK> c;
     c.load(a, row, chunk);
     const Param par(a.f, row);
     for (int i = chunk * LT + (int)threadIdx.x; i < LONG_BINS; i += l.chunks * LT) {
@@ -998,14 +1003,14 @@ template <class V> struct LongBins {
     }
 };
 
-template <class T> __global__ void __launch_bounds__(LT, 4) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ unsigned long long s_slots[LT / 32], s_mass[LONG_BINS];
     Group<LT> group(s_slots);
     __shared__ unsigned s_cnt[LONG_BINS];
     const long long row = blockIdx.x / l.chunks;
     const int chunk = (int)(blockIdx.x - row * l.chunks);
-    Chunk<T> c;
+    Chunk<T, CHUNK> c;
     c.load(a, row, chunk);
     const Param par(a.f, row);
     // the row's best, worst and mass from those of its chunks
@@ -1069,7 +1074,7 @@ template <class T> __global__ void __launch_bounds__(LT, 4) chunk_bins_kernel(Dr
         }
     }
     if (state != 2) {
-        Chunk<T>::store(kept, group, l.seg + (size_t)blockIdx.x * c.SEGS, l.kept + blockIdx.x);
+        c.store(kept, group, l.seg + (size_t)blockIdx.x * MOST_SEGS, l.kept + blockIdx.x);
         return;
     }
     __syncthreads();
@@ -1151,7 +1156,7 @@ template <int NT> __device__ Where where(const Param& par, int K, const unsigned
     return r;
 }
 
-template <class T> __global__ void __launch_bounds__(LT, 4) chunk_split_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
+template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_split_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ WhereArea s;
     __shared__ unsigned long long s_slots[LT / 32];
@@ -1160,7 +1165,7 @@ template <class T> __global__ void __launch_bounds__(LT, 4) chunk_split_kernel(D
     const long long row = blockIdx.x / l.chunks;
     const int chunk = (int)(blockIdx.x - row * l.chunks);
     if (l.row[row].state != 2) return;
-    Chunk<T> c;
+    Chunk<T, CHUNK> c;
     c.load(a, row, chunk);
     const Param par(a.f, row);
     const Weights<V> w = l.row[row].w;
@@ -1197,7 +1202,7 @@ template <class T> __global__ void __launch_bounds__(LT, 4) chunk_split_kernel(D
     }
     __syncthreads();                                  // (s_listed)
     unsigned to = mine ? atomicAdd(&s_listed, mine) : 0u;
-    Chunk<T>::store(kept, group, l.seg + (size_t)blockIdx.x * c.SEGS, l.kept + blockIdx.x);
+    c.store(kept, group, l.seg + (size_t)blockIdx.x * MOST_SEGS, l.kept + blockIdx.x);
     if (threadIdx.x == 0) {
         s_at = s_listed ? atomicAdd(&l.row[row].listed, s_listed) : 0u;
     }
@@ -1262,6 +1267,12 @@ __device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long lon
     const Weights<V> w = r.w;
     if (at.k < 0 && at.p_first > at.p_last) return {w.from, UINT_MAX, true};             // all of them are kept
     const LongBins<V> bins(w);
+    const int shift = chunk_shift(a.rows, a.K);
+    const auto add = [&](unsigned idx, unsigned long long q) {
+        const long long chunk = row * l.chunks + (idx >> shift);
+        atomicAdd(&l.kept[chunk], q);
+        atomicAdd(&l.seg[chunk * MOST_SEGS + (idx & ((1u << shift) - 1u)) / segment<T>], q);
+    };
     const bool share = at.p_first <= at.p_last;
     if (r.listed <= BT) {
         // A thread for each: ranks by comparing each with each, masses in the order of the ranks (1 x 524288 fp32: 8.6 us, by the
@@ -1301,9 +1312,7 @@ __device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long lon
         const unsigned last = group.reduce(keep ? rank : 0u, 0u, Max());                     // (some sample is kept)
         if (keep && rank == last) { s.border = v; s.border_idx = idx; }
         if (keep && weight >= par.min_p && q) {
-            const long long chunk = row * l.chunks + idx / CHUNK;
-            atomicAdd(&l.kept[chunk], q);
-            atomicAdd(&l.seg[chunk * Chunk<T>::SEGS + idx % CHUNK / Chunk<T>::SEG], q);
+            add(idx, q);
         }
         __syncthreads();
         return {s.border, s.border_idx, true};
@@ -1373,11 +1382,7 @@ __device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long lon
         w.masses(x, in, par.min_p, q);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (q[j]) {
-                const long long chunk = row * l.chunks + idx[j] / CHUNK;
-                atomicAdd(&l.kept[chunk], q[j]);
-                atomicAdd(&l.seg[chunk * Chunk<T>::SEGS + idx[j] % CHUNK / Chunk<T>::SEG], q[j]);
-            }
+            if (q[j]) add(idx[j], q[j]);
     });
     return {border, last, true};
 }
@@ -1385,9 +1390,8 @@ __device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long lon
 // Draw number `at` of all by one wave: the chunk, its segment, the sample.  FRESH: masses that this workgroup has just added to.
 template <class T, bool FRESH, class V = typename Traits<T>::V>
 __device__ void draw_one(const DrawArgs& a, const LongArea<V>& l, long long row, long long at, const Param& par, const Weights<V>& w, const Kept<V>& r) {
-    using C = Chunk<T>;
-    constexpr int VEC = C::VEC;
-    const int lane = threadIdx.x & 63;
+    constexpr int SEG = segment<T>, VEC = SEG / 64;
+    const int lane = threadIdx.x & 63, shift = chunk_shift(a.rows, a.K);
     const auto mass_at = [](const unsigned long long* p) { return FRESH ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p; };
     const unsigned long long* kept = l.kept + row * l.chunks;
     unsigned long long mass = 0, target = 0, run = 0;
@@ -1419,12 +1423,12 @@ __device__ void draw_one(const DrawArgs& a, const LongArea<V>& l, long long row,
         if (lane == 0) { a.index[at] = -1; if (a.weight) a.weight[at] = 0.0f; }
         return;
     }
-    const unsigned long long m = lane < C::SEGS ? mass_at(l.seg + (row * l.chunks + chunk) * C::SEGS + lane) : 0ull;
+    const unsigned long long m = lane < (1 << shift) / SEG ? mass_at(l.seg + (row * l.chunks + chunk) * MOST_SEGS + lane) : 0ull;
     const unsigned long long inc = wave_scan(m, 0ull, Add());
     const int seg = __builtin_amdgcn_readfirstlane(__ffsll((long long)__ballot(target - (run + inc - m) < m)) - 1);
     run += lane_value(inc - m, seg);
 
-    const int first = chunk * CHUNK + seg * C::SEG + lane * VEC;
+    const int first = (chunk << shift) + seg * SEG + lane * VEC;
     T raw[VEC];
     load_piece((const T*)a.R + row * a.row_stride, a.col_stride, (long long)first, a.K, raw);
     V v[VEC];
@@ -1516,6 +1520,17 @@ template <class T, int NT, int BYTES> int launch_rows(DrawArgs a, hipStream_t s)
     a.per = (int)std::min(per, (long long)a.D);
     return in_grids(a, a.rows, NT, [&](unsigned n) { hipLaunchKernelGGL((draw_row_kernel<T, NT, BYTES>), dim3(n, parts), dim3(NT), 0, s, a, S); });
 }
+template <class T, int CHUNK> int launch_chunks(const DrawArgs& a, const LongArea<typename Traits<T>::V>& l, unsigned n, bool borders, hipStream_t s) {
+    hipLaunchKernelGGL((chunk_best_kernel<T, CHUNK>), dim3(n), dim3(LT), 0, s, a, l);
+    HIP_OK(hipGetLastError());
+    hipLaunchKernelGGL((chunk_bins_kernel<T, CHUNK>), dim3(n), dim3(LT), 0, s, a, l);
+    HIP_OK(hipGetLastError());
+    if (borders) {
+        hipLaunchKernelGGL((chunk_split_kernel<T, CHUNK>), dim3(n), dim3(LT), 0, s, a, l);
+        HIP_OK(hipGetLastError());
+    }
+    return 0;
+}
 template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_bytes, hipStream_t s) {
     using V = typename Traits<T>::V;
     if ((size_t)a.K * sizeof(T) <= SHELF) {
@@ -1538,14 +1553,10 @@ template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_byte
     const long long n = (long long)a.rows * l.chunks;
     if (n > 0xffffffffll / LT || (long long)a.rows * a.D > INT_MAX)
         return fail(-6, "more than 2^23 - 1 chunks of 8192 samples, or than 2^31 - 1 draws, in one call of long rows");
-    const dim3 chunks((unsigned)n);
-    hipLaunchKernelGGL((chunk_best_kernel<T>), chunks, dim3(LT), 0, s, a, l);
-    HIP_OK(hipGetLastError());
-    hipLaunchKernelGGL((chunk_bins_kernel<T>), chunks, dim3(LT), 0, s, a, l);
-    HIP_OK(hipGetLastError());
-    if (a.f.top_k_of || a.f.top_p_of || (a.f.top_k > 0 && a.f.top_k < a.K) || a.f.top_p < 1.0) {
-        hipLaunchKernelGGL((chunk_split_kernel<T>), chunks, dim3(LT), 0, s, a, l);
-        HIP_OK(hipGetLastError());
+    const bool borders = a.f.top_k_of || a.f.top_p_of || (a.f.top_k > 0 && a.f.top_k < a.K) || a.f.top_p < 1.0;
+    const int rc = chunk_shift(a.rows, a.K) == 12 ? launch_chunks<T, 4096>(a, l, (unsigned)n, borders, s) : launch_chunks<T, 8192>(a, l, (unsigned)n, borders, s);
+    if (rc) return rc;
+    if (borders) {
         if (a.D <= FEW_DRAWS)
             hipLaunchKernelGGL((row_border_kernel<T, true>), dim3(a.rows), dim3(BT), 0, s, a, l);
         else
