@@ -599,21 +599,27 @@ template <class T, int NT, int BYTES> struct Shelf {
         weight = w.weight(v);
         const unsigned long long mass = whole(weight * w.scale);
         if (by_count || by_share) {
-            unsigned rank = 0;                       // (the lanes behind n come last, in their order)
-            if constexpr (sizeof(V) == 4) {          // value and index in one number
+            unsigned rank = 0;
+            if constexpr (sizeof(V) == 4) {          // value and index in one number (16-bit returns are often equal); the others come last
                 const unsigned long long place = (unsigned long long)key_of(v) << 32 | (63u - lane);
                 for (unsigned o = 0; o < n; o += 4) {
 #pragma unroll
                     for (unsigned j = 0; j < 4; j++) rank += lane_value(place, o + j) > place ? 1u : 0u;
                 }
-            } else {
+            } else {                                 // how many are higher, and where there are equal ones, how many of these come first
+                const V x = live ? v : (V)NAN;
                 for (unsigned o = 0; o < n; o += 4) {
 #pragma unroll
-                    for (unsigned j = 0; j < 4; j++) {
-                        const V ov = lane_value(v, o + j);
-                        rank += ov > v || (ov == v && o + j < lane) ? 1u : 0u;
+                    for (unsigned j = 0; j < 4; j++) rank += lane_value(x, o + j) > x ? 1u : 0u;
+                }
+                const unsigned all = (unsigned)__popcll(__ballot(live));
+                if (lane_value(wave_scan(live ? rank : 0u, 0u, Add()), 63) != all * (all - 1) / 2) {
+                    for (unsigned o = 0; o < n; o += 4) {
+#pragma unroll
+                        for (unsigned j = 0; j < 4; j++) rank += lane_value(x, o + j) == x && o + j < lane ? 1u : 0u;
                     }
                 }
+                rank = live ? rank : 63u;            // (where some lane takes no part, no rank is 63)
             }
             if (by_count) live = live && (long long)rank < par.top_k;
             if (by_share) {
