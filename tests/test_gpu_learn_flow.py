@@ -353,3 +353,19 @@ def test_example_actor_critic_script_with_draws_and_clipping():
     assert len(results) == 2 and all(np.isfinite(r[3]) for r in results)
     with pytest.raises(SystemExit):
         mod.main(["--clip", "1.0"])
+
+
+def test_results_in_inference_mode():
+    """Tensors made inside are inference tensors, tensors made outside are not, and either kind may be clipped or drawn from."""
+    import torch
+    from trajopt_amd.device import clip_gradients, draw_from_returns
+    R, u, g = torch.randn(2, 9, device="cuda"), torch.rand(2, 3, device="cuda", dtype=torch.float64), torch.ones(16, device="cuda")
+    want = draw_from_returns(R, u)
+    assert not want[0].is_inference() and not want[1].requires_grad
+    with torch.inference_mode():
+        got = draw_from_returns(R + 0.0, u)
+        norm = clip_gradients([g * 1.0], 1.0)
+        clip_gradients([g], 2.0)
+    assert got[0].is_inference() and norm.is_inference() and float(norm) == 4.0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert (g == 0.5).all()
