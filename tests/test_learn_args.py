@@ -80,8 +80,8 @@ def test_workspace_query():
         assert L.lib().mppi_draw_workspace(*bad, C.byref(need)) < 0
     assert L.lib().mppi_draw_workspace(L.F32, 1, 5, None) == -1
     assert L.lib().mppi_gradient_workspace(-1, C.byref(need)) == -1 and L.lib().mppi_gradient_workspace(1, None) == -1
-    for n in (0, 1, 120, 121, 100000):         # partial sums of at most 2048 workgroups, and a table entry of at most 32 bytes per tensor
-        assert L.lib().mppi_gradient_workspace(n, C.byref(need)) == 0 and 2048 * 8 <= need.value <= 2048 * 8 + 32 * n
+    for n in (0, 1, 168, 169, 100000):         # partial sums of 1024 workgroups, and a table entry of 24 bytes where they do not travel
+        assert L.lib().mppi_gradient_workspace(n, C.byref(need)) == 0 and need.value == 1024 * 8 + (24 * n if n > 168 else 0)
 
 
 def test_python_refusals():

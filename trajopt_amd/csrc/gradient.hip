@@ -9,7 +9,7 @@
 // fp32's range) and rounded to fp32; 16-bit ones from there to their type, 2^-16 of whose step the first rounding is at most.
 //
 // Two passes over the data: no entry can be scaled before all have been read.  Large sets are bound by memory: 1.07 GB of fp32 read
-// in 179 us (6.0 TB/s), 268 MB of bf16 read in 50 us and read again and written in 84 (6.4 TB/s; what a copy moves here: 4.8).  Small
+// in 155 us (6.9 TB/s), 268 MB of bf16 read in 48 us and read again and written in 86 (6.2 TB/s; what a copy moves here: 4.8).  Small
 // ones are bound by launches and by the host: the six tensors of a critic take one launch, 6.3 us per call; 384 small tensors four,
 // of which two carry tables of addresses, 27 to 31 us per call, 17 of them in this library and 14 on the GPU.
 #include "abi_common.hpp"
@@ -26,12 +26,14 @@ using mppi::fail;
 namespace {
 
 constexpr int BT = 256;                  // threads of a workgroup
-// Bytes of one tensor that a workgroup takes at a time: four rounds of its loads, or one where there would be too few workgroups (150
-// fp16 tensors of 10 MB: 14.0 us per call, 16.0 with the larger; 268 MB of bf16: 133 us, 149 with the smaller, 155 with 256 KB).
-constexpr int CHUNK = 65536, SMALL_CHUNK = 16384;
-constexpr int GROUPS = 2048;             // most workgroups of a launch (eight per CU), and so most partial sums (4096: 131 us for 133)
+// Bytes of one tensor that a workgroup takes at a time: two rounds of its loads, or one where there would be too few workgroups (per
+// call, clipping bf16 out of place, 16, 32 and 64 KB: 8 MB 10.8, 11.1 and 14.0 us, 48 MB 30.0, 27.5 and 26.3, 256 MB 129.7, 128.1 and
+// 128.6; tensors end inside a chunk, so that smaller ones are filled better).
+constexpr int CHUNK = 32768, SMALL_CHUNK = 16384;
+constexpr int GROUPS = 1024;             // most workgroups of a launch (four per CU), and so most partial sums (512 MB: 258 us, 2048: 261, 512: 8 % more)
 constexpr int AHEAD = 4;                 // loads of 16 bytes that a thread has under way (268 MB of bf16: 2: 135.7 us, 4: 133.4, 8: 134.3)
-constexpr size_t STREAMED = 24 << 20;    // bytes from which on entries go past the caches (gradient_clip_kernel)
+constexpr size_t STREAMED = 24 << 20;    // bytes from which on what is clipped goes past the caches (gradient_clip_kernel),
+constexpr size_t READ_ONCE = 128 << 20;  // and what only a norm is taken of (gradient_partials_kernel)
 constexpr int TABLE = 168;               // tensors whose table travels in a kernel's arguments (4 KB at most)
 
 struct Entry {
@@ -145,7 +147,7 @@ template <bool MAX, int NT> __device__ double group_total(double acc, uint32_t t
 template <bool MAX> __device__ __forceinline__ double norm_of_total(double v) { return MAX ? (double)__uint_as_float((uint32_t)v) : sqrt(v); }
 
 // entries [lo, hi) of a tensor by NT threads (tid: which one), AHEAD packs of a thread under way at a time
-template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(const void* p, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
+template <class T, bool MAX, int NT, bool STREAM> __device__ __forceinline__ void read_span(const void* p, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
     using B = typename Io<T>::B;
     constexpr int VEC = Io<T>::VEC, STEP = NT * VEC;
     const B* g = (const B*)p;
@@ -153,7 +155,7 @@ template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(c
     for (; i + (AHEAD - 1) * STEP + VEC <= hi; i += AHEAD * STEP) {
         Pack<T> x[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) x[k].load(g + i + k * STEP);
+        for (int k = 0; k < AHEAD; k++) x[k].template load<STREAM>(g + i + k * STEP);
 #pragma unroll
         for (int k = 0; k < AHEAD; k++)
 #pragma unroll
@@ -161,7 +163,7 @@ template <class T, bool MAX, int NT> __device__ __forceinline__ void read_span(c
     }
     for (; i + VEC <= hi; i += STEP) {
         Pack<T> x;
-        x.load(g + i);
+        x.template load<STREAM>(g + i);
 #pragma unroll
         for (int j = 0; j < VEC; j++) take<MAX>(acc[j % 4], top, Io<T>::get(x.get(j)));
     }
@@ -192,10 +194,10 @@ template <class T, bool SCALED, int NT, bool STREAM> __device__ __forceinline__ 
     }
     for (; i < hi; i++) out[i] = SCALED ? Io<T>::scaled(g[i], scale) : g[i];
 }
-template <bool MAX, int NT> __device__ __forceinline__ void read_chunk(const Entry& e, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
-    if (e.type() == MPPI_F32) read_span<float, MAX, NT>(e.g, tid, lo, hi, acc, top);
-    else if (e.type() == MPPI_F16) read_span<_Float16, MAX, NT>(e.g, tid, lo, hi, acc, top);
-    else read_span<__bf16, MAX, NT>(e.g, tid, lo, hi, acc, top);
+template <bool MAX, int NT, bool STREAM> __device__ __forceinline__ void read_chunk(const Entry& e, int tid, long long lo, long long hi, double (&acc)[4], uint32_t& top) {
+    if (e.type() == MPPI_F32) read_span<float, MAX, NT, STREAM>(e.g, tid, lo, hi, acc, top);
+    else if (e.type() == MPPI_F16) read_span<_Float16, MAX, NT, STREAM>(e.g, tid, lo, hi, acc, top);
+    else read_span<__bf16, MAX, NT, STREAM>(e.g, tid, lo, hi, acc, top);
 }
 template <int NT, bool STREAM> __device__ __forceinline__ void write_chunk(const Entry& e, int tid, long long lo, long long hi, bool clip, double scale) {
     if (!clip && e.out == e.g) return;
@@ -215,15 +217,17 @@ __global__ void __launch_bounds__(BT) table_kernel(Table t, Entry* __restrict__ 
     for (int i = threadIdx.x; i < t.tensors; i += BT) far[i] = t.e[i];
 }
 
+// STREAM: nothing is read again, and what is read need not push anything out of the caches (per call, the norm of bf16 with and without:
+// 128 MB 25.4 and 26.2 us, 256 MB 44 and 48, 512 MB 82 and 92; 1.07 GB of fp32 158 and 183, i.e. 6.8 TB/s).
 // FAR: t holds the last tensors only, those before it, with `before` chunks, lie in far; it is put behind them for the second pass
-template <bool MAX, bool FAR> __global__ void __launch_bounds__(BT) gradient_partials_kernel(Table t, Entry* far, int tensors, unsigned before, double* __restrict__ partials) {
+template <bool MAX, bool FAR, bool STREAM> __global__ void __launch_bounds__(BT) gradient_partials_kernel(Table t, Entry* far, int tensors, unsigned before, double* __restrict__ partials) {
     __shared__ double s[BT / 64];
     double acc[4] = {0.0, 0.0, 0.0, 0.0};      // four chains of dependent additions
     uint32_t top = 0;
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         long long lo, hi;
         const Entry& e = FAR && c < before ? locate(FarTable{far, tensors, t.chunk, before}, c, lo, hi) : locate(t, c, lo, hi);
-        read_chunk<MAX, BT>(e, threadIdx.x, lo, hi, acc, top);
+        read_chunk<MAX, BT, STREAM>(e, threadIdx.x, lo, hi, acc, top);
     }
     if (FAR && blockIdx.x == 0)
         for (int i = threadIdx.x; i < t.tensors; i += BT) far[tensors + i] = t.e[i];
@@ -308,7 +312,7 @@ template <bool MAX> __global__ void __launch_bounds__(ST) gradient_small_kernel(
     };
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     uint32_t top = 0;
-    pieces([&](const Entry& e, long long lo, long long hi) { read_chunk<MAX, 64>(e, lane, lo, hi, acc, top); });
+    pieces([&](const Entry& e, long long lo, long long hi) { read_chunk<MAX, 64, false>(e, lane, lo, hi, acc, top); });
     const double norm = norm_of_total<MAX>(group_total<MAX, ST>((acc[0] + acc[1]) + (acc[2] + acc[3]), top, s));
     if (threadIdx.x == 0) *norm_out = (float)norm;
     if (!write) return;
@@ -371,8 +375,12 @@ template <bool MAX> int run(const std::vector<Entry>& e, int chunk, unsigned chu
         hipLaunchKernelGGL(table_kernel, dim3(1), dim3(BT), 0, s, t, far + at);
         HIP_OK(hipGetLastError());
     }
+    const bool once = !max_norm && bytes > READ_ONCE;
     if (at > 0) {
-        hipLaunchKernelGGL((gradient_partials_kernel<MAX, true>), dim3(groups), dim3(BT), 0, s, t, far, (int)at, e[at].first, partials);
+        if (once)
+            hipLaunchKernelGGL((gradient_partials_kernel<MAX, true, true>), dim3(groups), dim3(BT), 0, s, t, far, (int)at, e[at].first, partials);
+        else
+            hipLaunchKernelGGL((gradient_partials_kernel<MAX, true, false>), dim3(groups), dim3(BT), 0, s, t, far, (int)at, e[at].first, partials);
         HIP_OK(hipGetLastError());
         return second<FarTable, MAX>(FarTable{far, (int)e.size(), chunk, chunks}, groups, bytes, partials, max_norm, norm, s);
     }
@@ -381,7 +389,10 @@ template <bool MAX> int run(const std::vector<Entry>& e, int chunk, unsigned chu
         HIP_OK(hipGetLastError());
         return 0;
     }
-    hipLaunchKernelGGL((gradient_partials_kernel<MAX, false>), dim3(groups), dim3(BT), 0, s, t, (Entry*)nullptr, 0, 0u, partials);
+    if (once)
+        hipLaunchKernelGGL((gradient_partials_kernel<MAX, false, true>), dim3(groups), dim3(BT), 0, s, t, (Entry*)nullptr, 0, 0u, partials);
+    else
+        hipLaunchKernelGGL((gradient_partials_kernel<MAX, false, false>), dim3(groups), dim3(BT), 0, s, t, (Entry*)nullptr, 0, 0u, partials);
     HIP_OK(hipGetLastError());
     return second<Table, MAX>(t, groups, bytes, partials, max_norm, norm, s);
 }
