@@ -19,9 +19,9 @@
 // What bounds it.  The bytes are few (the benchmark planner's row is 16 KB); what takes the time is one pass behind the other
 // over a row, with a barrier after each, and the instructions of code that runs once.  So a row stays in one workgroup's LDS as long
 // as it fits, passes test values in the type of the row and evaluate fp64 exponentials only where a sample passes, and loops are
-// rolled.  Per call, with the launch (3.6 us for the smallest kernel there is): 1 x 40 fp64 with top-k 5.7 us; 1 x 4096 fp32 with
+// rolled.  Per call, with the launch (3.6 us for the smallest kernel there is): 1 x 40 fp64 with top-k 5.3 us; 1 x 4096 fp32 with
 // top-p 9.2; 1024 x 512 fp32 with all three filters 8.8; 192 x 65535 bf16 with all three 17.2 (25 MB: 1.5 TB/s); 1 x 524288
-// fp32 with both borders 30; 16 x 262144 fp64 with top-p and 64 draws each 59.
+// fp32 with both borders 29; 16 x 262144 fp64 with top-p and 64 draws each 58.
 #include "abi_common.hpp"
 #include "../../include/mppi_hip.h"
 
@@ -332,7 +332,7 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
     };
     if (NT == 64) __syncthreads();                   // (larger groups have just met at a barrier)
     if (threadIdx.x == 0) s.n_list = 0;
-    if (most > 16) {     // (comparing more with each other costs more than the histogram: 1 x 40 fp64 3.8 us of kernel with it, 4.9 without)
+    if (most > 16) {     // (comparing more with each other costs more than the histogram: 1024 x 512 11.5 us with it, 13.9 without)
 #pragma unroll 1
         while (true) {
 #pragma unroll
@@ -865,8 +865,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 // Rows without top-k and top-p need no list: the masses of their chunks stay as chunk_bins wrote them, and long_draw follows.
 //
 // Each of the first three reads the row once, and only the first finds it outside the caches (in part: an L2 holds 4 MB).  A launch
-// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 4.6, 8.1, 8.3, 10.2 us; 16 x 262144 fp64 (34 MB) and 64 draws: 10.4, 13.5,
-// 16.2, 16.6, 4.5 us, i.e. 3.2 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
+// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 3.9, 8.3, 6.5, 10.3 us; 16 x 262144 fp64 (34 MB) and 64 draws: 10.9, 13.2,
+// 16.2, 16.4, 4.8 us, i.e. 3.1 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
 // each for a wave) in the two that need masses.
 constexpr int MOST_SEGS = 64, LT = 512, LONG_BINS = 1024, BT = 256;
 
@@ -1551,7 +1551,7 @@ template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_byte
             if (a.K * sizeof(T) <= 65536) return launch_rows<T, 512, 65536>(a, s);
         return launch_rows<T, 1024, SHELF>(a, s);
     }
-    // Five launches cost 30 us whatever the row; one workgroup is faster as long as it holds the row (1 x 32768 fp32: with both filters
+    // The launches of a long row take 27 us and more; one workgroup is faster as long as it holds the row (1 x 32768 fp32: with both filters
     // 17 us and 34, with top-p alone 32 and 33; 192 of them 19 and 58, 35 and 58).
     LongArea<V> l;
     if (!workspace || workspace_bytes < LongArea<V>::carve(&l, (char*)workspace, a.rows, a.K))
