@@ -241,6 +241,19 @@ def test_more_draws_than_one_workgroup_takes():
         _check(_returns(2, K, dtype, K, masked=0.1), _numbers(2, D, K), kappa=0.7, top_p=0.99)
 
 
+def test_more_draws_of_a_long_row_than_one_grid_holds():
+    """2^26 + 5 draws, a wave each, from a row with two samples."""
+    import torch
+    D, K = (1 << 26) + 5, 40000
+    R = torch.full((1, K), float("-inf"), device="cuda")
+    R[0, 77] = R[0, 39999] = 3.0
+    u = torch.full((1, D), 0.25, dtype=torch.float64, device="cuda")
+    u[0, 1::2] = 0.75
+    u[0, [0, (1 << 26) - 2, (1 << 26) - 1, 1 << 26, D - 1]] = 0.5
+    index, weight = _draw(R, u)
+    assert torch.equal(index, torch.where(u < 0.5, 77, 39999)) and (weight == 0.5).all()
+
+
 def test_negated_views():
     """A view that torch negates lazily: its memory holds the other sign."""
     import torch
