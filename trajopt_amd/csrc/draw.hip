@@ -870,8 +870,18 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 // each for a wave) in the two that need masses.
 constexpr int MOST_SEGS = 64, LT = 512, LONG_BINS = 1024, BT = 256;
 
+// Where the borders can lie: the count border in bin k (-1: none) with so many samples and so much mass before it, the mass border in
+// bins p_first ... p_last (none: p_first > p_last)
+struct Where {
+    int k, p_first, p_last;
+    unsigned k_before;
+    unsigned long long k_mass_before, mass_before;   // mass_before: before p_first
+    unsigned long long mass;                         // of all bins
+    bool nothing;
+};
 template <class V> struct LongRow {                  // what is known of a row (written by its first workgroup of chunk_bins)
     Weights<V> w;
+    Where at;                                        // (of chunk_split)
     V border;                                        // kept: above the border, or equal to it with an index up to last
     unsigned last, listed;
     int state;                                       // 0: nothing to draw, 1: every sample that takes part is kept, 2: borders
@@ -1091,15 +1101,6 @@ template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_bin
         }
 }
 
-// Where the borders can lie: the count border in bin k (-1: none) with so many samples and so much mass before it, the mass border in
-// bins p_first ... p_last (none: p_first > p_last)
-struct Where {
-    int k, p_first, p_last;
-    unsigned k_before;
-    unsigned long long k_mass_before, mass_before;   // mass_before: before p_first
-    unsigned long long mass;                         // of all bins
-    bool nothing;
-};
 struct WhereArea {
     unsigned long long k_mass_before, k_mass, p_before;
     unsigned k_before;
@@ -1178,6 +1179,7 @@ template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_spl
     const LongBins<V> bins(w);
     if (threadIdx.x == 0) s_listed = 0;
     const Where at = where<LT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, s, group);
+    if (chunk == 0 && threadIdx.x == 0) l.row[row].at = at;
     // before `first` everything is kept; with neither border (top-k of more samples than there are) that is all of it
     const int first = at.nothing ? 0 : at.p_first <= at.p_last ? at.p_first : at.k >= 0 ? at.k : LONG_BINS;
     unsigned long long kept[c.PIECES];
@@ -1265,10 +1267,10 @@ template <class V> struct Kept {
     bool some;
 };
 template <class T, class V = typename Traits<T>::V>
-__device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long long row, const LongRow<V>& r, const Param& par, BorderArea<V, BT>& s, WhereArea& sw,
+__device__ Kept<V> keep_listed(const DrawArgs& a, const LongArea<V>& l, long long row, const LongRow<V>& r, const Param& par, BorderArea<V, BT>& s,
                                Group<BT>& group) {
     const Kept<V> nothing{(V)0, 0, false};
-    const Where at = where<BT>(par, a.K, l.cnt + row * LONG_BINS, l.mass + row * LONG_BINS, sw, group);
+    const Where at = r.at;
     if (at.nothing) return nothing;
     const Weights<V> w = r.w;
     if (at.k < 0 && at.p_first > at.p_last) return {w.from, UINT_MAX, true};             // all of them are kept
@@ -1467,7 +1469,6 @@ constexpr int FEW_DRAWS = BT / 64;
 template <class T, bool DRAW> __global__ void __launch_bounds__(BT) row_border_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
     using V = typename Traits<T>::V;
     __shared__ BorderArea<V, BT> s;
-    __shared__ WhereArea sw;
     Group<BT> group(s.slots);
     const long long row = blockIdx.x;
     LongRow<V>& r = l.row[row];
@@ -1476,7 +1477,7 @@ template <class T, bool DRAW> __global__ void __launch_bounds__(BT) row_border_k
     if (!DRAW && state != 2) return;
     Kept<V> k{r.border, UINT_MAX, state != 0};
     if (state == 2) {
-        k = keep_listed<T>(a, l, row, r, par, s, sw, group);
+        k = keep_listed<T>(a, l, row, r, par, s, group);
         if (!DRAW && threadIdx.x == 0) {
             r.border = k.border;
             r.last = k.last;
