@@ -865,8 +865,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 // Rows without top-k and top-p need no list: the masses of their chunks stay as chunk_bins wrote them, and long_draw follows.
 //
 // Each of the first three reads the row once, and only the first finds it outside the caches (in part: an L2 holds 4 MB).  A launch
-// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 3.9, 8.3, 6.5, 10.3 us; 16 x 262144 fp64 (34 MB) and 64 draws: 10.9, 13.2,
-// 16.2, 16.4, 4.8 us, i.e. 3.1 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
+// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 3.9, 8.0, 6.6, 9.7 us; 16 x 262144 fp64 (34 MB) and 64 draws: 11.3, 13.1,
+// 16.0, 16.1, 4.7 us, i.e. 3.0 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
 // each for a wave) in the two that need masses.
 constexpr int MOST_SEGS = 64, LT = 512, LONG_BINS = 1024, BT = 256;
 
