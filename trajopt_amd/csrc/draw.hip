@@ -473,14 +473,15 @@ template <class T, int NT, int BYTES> struct Shelf {
     struct alignas(16) Piece { T v[VEC]; };
     using Area = BorderArea<V, NT>;
     struct Shared {
-        Piece row[(BYTES / (int)sizeof(T) + FEW) / VEC];
-        unsigned few_idx[FEW];
+        Piece row[BYTES / 16];
         Area b;
+        __device__ unsigned* few_idx() { return (unsigned*)&row[FEW / VEC]; }       // (behind what has moved together)
         __device__ unsigned long long* ends() { return b.mass; }           // (once the borders are found; NT <= BINS)
     };
     Shared& s;
     Weights<V> w;
-    int GP, start, base;              // pieces of this thread, the one it begins with, the row's first piece
+    int GP, start;                    // pieces of this thread, the one it begins with
+    bool moved;                       // the row is what has moved together
     int C;                            // samples per thread
 
     V bottom;                         // about the lowest value that takes part (at first)
@@ -491,12 +492,12 @@ template <class T, int NT, int BYTES> struct Shelf {
     __device__ __forceinline__ static V at(const Piece& p, int j) { return value_of(p.v[j]); }
     // the thread's pieces in the order in which it visits them
     __device__ __forceinline__ int piece(int o) const { const int g = start + o; return (int)threadIdx.x * GP + (g < GP ? g : g - GP); }
-    __device__ __forceinline__ V value(int o, int j) const { return at(s.row[base + piece(o)], j); }
+    __device__ __forceinline__ V value(int o, int j) const { return at(s.row[piece(o)], j); }
     __device__ __forceinline__ unsigned index(int o, int j) const { return (unsigned)(piece(o) * VEC + j); }
 
     // f(v, live, o): the pieces with samples in [low, high]; live: bit j for sample v[j] of the o-th piece visited
     template <class F> __device__ __forceinline__ void each(V low, V high, F f) {
-        const int own = base + (int)threadIdx.x * GP;
+        const int own = (int)threadIdx.x * GP;
         int g = start;
 #pragma unroll 1
         for (int o = 0; o < GP; o++) {
@@ -565,23 +566,26 @@ template <class T, int NT, int BYTES> struct Shelf {
         }
         most = all;
         if (all > FEW) return;
-        constexpr int first = BYTES / 16;
-        if (threadIdx.x < FEW / VEC) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) s.row[first + threadIdx.x].v[j] = minus_infinity((T*)nullptr);
-        }
-        __syncthreads();
+        // over the areas of the histogram, and from there to where the row was
+        static_assert(FEW <= Area::BINS && FEW * (sizeof(T) + 4) <= BYTES, "values and indices");
+        T* values = (T*)s.b.mass;
+        for (int e = (int)all + (int)threadIdx.x; e < FEW; e += NT) values[e] = minus_infinity((T*)nullptr);
 #pragma unroll 1
         for (; bits; bits &= bits - 1) {             // (in the order of the pieces, and in it within each)
             const int at = __ffsll((long long)bits) - 1, p = at / VEC, j = at % VEC, from = p * NT + (int)threadIdx.x;
             const int field = p % 4 * 16;
             const unsigned e = (unsigned)((p < 4 ? to[0] : to[1]) >> field & 0xffffu);
             if (p < 4) to[0] += 1ull << field; else to[1] += 1ull << field;
-            s.row[first + e / VEC].v[e % VEC] = s.row[from].v[j];
-            s.few_idx[e] = (unsigned)(from * VEC + j);
+            values[e] = s.row[from].v[j];
+            s.b.cnt[e] = (unsigned)(from * VEC + j);
         }
         __syncthreads();
-        base = first;
+        for (int e = threadIdx.x; e < FEW; e += NT) {
+            s.row[e / VEC].v[e % VEC] = values[e];
+            s.few_idx()[e] = s.b.cnt[e];
+        }
+        __syncthreads();
+        moved = true;
         GP = threadIdx.x < FEW / VEC ? 1 : 0;
         start = 0;
         C = VEC;
@@ -593,7 +597,7 @@ template <class T, int NT, int BYTES> struct Shelf {
     __device__ unsigned long long finish(unsigned n, const Param& par, V& v, double& weight, unsigned long long& q, unsigned long long& before) {
         const unsigned lane = threadIdx.x & 63;
         const bool by_count = par.top_k > 0 && par.top_k < (long long)n, by_share = !(par.top_p >= 1.0);
-        v = lane < n ? at(s.row[base + lane / VEC], lane % VEC) : (V)-INFINITY;
+        v = lane < n ? at(s.row[lane / VEC], lane % VEC) : (V)-INFINITY;
         bool live = v >= w.from && v <= w.best;
         v = live ? v : (V)-INFINITY;
         weight = w.weight(v);
@@ -649,7 +653,7 @@ template <class T, int NT, int BYTES> struct Shelf {
             unsigned rank = group.scan(mine, total);
 #pragma unroll 1
             for (int g = 0; g < GP && mine > 0; g++) {
-                Piece& p = s.row[base + (int)threadIdx.x * GP + g];
+                Piece& p = s.row[(int)threadIdx.x * GP + g];
 #pragma unroll
                 for (int j = 0; j < VEC; j++)
                     if (at(p, j) == w.from && rank++ >= keep) p.v[j] = minus_infinity((T*)nullptr);
@@ -673,7 +677,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     h.GP = (a.K + NT * VEC - 1) / (NT * VEC);
     h.C = h.GP * VEC;
     h.start = tid % h.GP;
-    h.base = 0;
+    h.moved = false;
     h.most = (unsigned)a.K;
     const Param par(a.f, row);
     long long* index = a.index + from_draw;
@@ -715,7 +719,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     h.bottom = some > h.w.from && some <= best ? some : h.w.from;
 
     auto answer = [&](int d, int i, double w, unsigned long long mass) {
-        index[d] = h.base ? (long long)s.few_idx[i] : i;
+        index[d] = h.moved ? (long long)s.few_idx()[i] : i;
         if (weight) weight[d] = (float)(w * h.w.scale / (double)mass);
     };
     auto finish = [&]() __attribute__((always_inline)) {                  // few samples: the first wave does the rest
@@ -748,7 +752,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
                 const int mid = (lo + hi) >> 1;
                 if (ends[mid] > target) hi = mid; else lo = mid + 1;
             }
-            answer(d, lo, h.w.weight(H::at(s.row[h.base + lo / VEC], lo % VEC)), mass);
+            answer(d, lo, h.w.weight(H::at(s.row[lo / VEC], lo % VEC)), mass);
         }
     };
     static_assert(AHEAD * NT * 16 >= BYTES, "the row is loaded in one go, and top[] holds all of its pieces");
@@ -762,13 +766,13 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     if (raised) h.raise(mine, (unsigned)par.top_k);
     if (raised || BYTES >= 131072) {
         h.gather_few(top);
-        few = h.base && h.most <= H::LAST;
+        few = h.moved && h.most <= H::LAST;
     }
     if (!few && par.top_k > 0 && par.top_k < a.K && find_border<BY_COUNT>(h, s.b, h.group, (unsigned long long)par.top_k, 0.0, h.w.from, best, h.bottom, h.most)) {
         h.cut_behind();
         h.bottom = h.w.from;
         h.most = h.most < par.top_k ? h.most : (unsigned)par.top_k;
-        if (BYTES < 131072 && !h.base && h.most <= H::LAST) {
+        if (BYTES < 131072 && !h.moved && h.most <= H::LAST) {
             h.gather_few(top);
             few = true;
         }
@@ -790,7 +794,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
     __syncthreads();
     // mass of sample i of the row, zero if it may not be drawn
     auto mass_of_sample = [&](int i, double& w) -> unsigned long long {
-        const V v = H::at(s.row[h.base + i / VEC], i % VEC);
+        const V v = H::at(s.row[i / VEC], i % VEC);
         w = h.w.weight(v);
         return v >= h.w.from && v <= best && w >= par.min_p ? whole(w * h.w.scale) : 0ull;
     };
@@ -824,7 +828,7 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
             unsigned long long c = lo > 0 ? ends[lo - 1] : 0ull;
 #pragma unroll 1
             for (int p = lo * C / VEC; p < (lo + 1) * C / VEC; p++) {
-                const Piece x = s.row[h.base + p];
+                const Piece x = s.row[p];
                 V v[VEC];
                 unsigned live = 0;
                 unsigned long long q[VEC], sum = 0;
