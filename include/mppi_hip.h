@@ -338,10 +338,10 @@ typedef struct mppi_draw_filter {
  * whose update is the mean over the same weights (trajopt/algos/mppi.py:56-65).
  * All arrays are device memory: returns of type `dtype` (MPPI_F32, F64, F16, BF16), element k of row r at
  * r * row_stride + k * col_stride elements; u (rows, D), index (rows, D) and weight (rows, D) contiguous; d_workspace of at
- * least mppi_draw_workspace bytes (0 for rows of up to 128 KB), aligned to 256 bytes, that nothing else uses until the work
+ * least mppi_draw_workspace bytes (0 for rows of up to 16384 samples), aligned to 256 bytes, that nothing else uses until the work
  * on `stream` is done.  The work is enqueued on `stream` (NULL: the default stream); nothing is allocated or synchronised, and
  * it may be captured.  K up to MPPI_DRAW_MAX_K, and of rows longer
- * than 128 KB at most 2^31 - 1 draws in all (-6 beyond).  The current device of the calling thread is left as it was. */
+ * than 16384 samples at most 2^31 - 1 draws in all (-6 beyond).  The current device of the calling thread is left as it was. */
 int mppi_draw_workspace(int32_t dtype, int32_t rows, int32_t K, size_t* bytes);
 int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32_t rows, int32_t K, int64_t row_stride,
                            int64_t col_stride, const double* d_u, int32_t D, const mppi_draw_filter* filter, int64_t* d_index,

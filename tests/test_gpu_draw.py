@@ -288,6 +288,15 @@ def test_longest_row(dtype):
         _draw(torch.zeros(1, K + 1, dtype=R.dtype, device="cuda"), _numbers(1, 1, 1))
 
 
+@pytest.mark.parametrize("rows,K,dtype", [(39, 20001, "float32"), (40, 20001, "float32"), (40, 20001, "bfloat16"), (41, 16385, "float16"), (32, 16385, "bfloat16"),
+                                          (64, 32768, "float32"), (63, 32768, "float32"), (128, 65536, "bfloat16"), (129, 65535, "float16"), (33, 16384, "float64")])
+def test_many_long_rows(rows, K, dtype):
+    """As many rows as are taken by one workgroup each, or one less."""
+    R, u = _returns(rows, K, dtype, rows, masked=0.02), _numbers(rows, 2, rows)
+    for f in (dict(), dict(top_k=300), dict(top_k=5000, top_p=0.8), dict(top_p=0.9, min_p=0.02)):
+        _check(R, u, kappa=0.8, **f)
+
+
 @pytest.mark.parametrize("D", [1, 8, 9, 30])
 @pytest.mark.parametrize("step", [0.0, 0.01, 0.5])
 @pytest.mark.parametrize("dtype", TYPES)

@@ -1509,6 +1509,12 @@ int ceil_log2(int n) {
 
 constexpr size_t SHELF = 131072;                     // bytes of the longest row that one workgroup holds in LDS
 
+// Long rows of which there are few are cut into chunks also where one workgroup could hold them: its passes take the longer the longer the
+// row is, those over chunks the longer the more samples there are in all (per call, LDS and chunks, top-p alone: 1 x 20000 fp32 26 us and
+// 23, 32 rows 28 and 27, 64 rows 27 and 32; 1 x 32768 34 and 25, 64 rows 35 and 34, 128 rows 35 and 47; 1 x 65536 bf16 69 and 28, 128
+// rows 68 and 68, 192 rows 68 and 89; no filter: 28 and 13, 30 and 31, 31 and 40; 1 x 16384 fp64 24 and 24).
+bool few_long_rows(size_t rows, size_t K) { return K > 16384 && rows * 512 <= K; }
+
 // A grid has at most 2^32 - 1 threads along its first axis: more workgroups than that go into several launches.  `f(count)` makes
 // one of workgroups a.first ... a.first + count - 1.
 template <class F> int in_grids(DrawArgs& a, long long groups, int threads, F f) {
@@ -1544,7 +1550,9 @@ template <class T, int CHUNK> int launch_chunks(const DrawArgs& a, const LongAre
 }
 template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_bytes, hipStream_t s) {
     using V = typename Traits<T>::V;
-    if ((size_t)a.K * sizeof(T) <= SHELF) {
+    // (not where top-k leaves little to do behind the first pass: 1 x 65536 bf16 with k = 64 22 us and 25, 64 rows 25 and 41)
+    const bool few = few_long_rows(a.rows, a.K) && (a.f.top_k_of || a.f.top_k == 0 || a.f.top_k > 512);
+    if ((size_t)a.K * sizeof(T) <= SHELF && !few) {
         // One wave needs no barriers, but has every pass to itself: 1024 x 512 fp32 with all filters 9.8 us by 64 threads, 18.7 by 512;
         // 1 x 512 and 64 draws 9.3 and 10.3, 200 draws 11.4 and 10.4.  More than 512 threads pay where a row would otherwise be more
         // than 64 KB, or 64 samples per thread: 1024 x 4096 fp32 21 us by 512 threads, 64 by 1024; 1 x 8192 11.7 and 15.9; 1024 x
@@ -1556,8 +1564,6 @@ template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_byte
             if (a.K * sizeof(T) <= 65536) return launch_rows<T, 512, 65536>(a, s);
         return launch_rows<T, 1024, SHELF>(a, s);
     }
-    // The launches of a long row take 27 us and more; one workgroup is faster as long as it holds the row (1 x 32768 fp32: with both filters
-    // 17 us and 34, with top-p alone 32 and 33; 192 of them 19 and 58, 35 and 58).
     LongArea<V> l;
     if (!workspace || workspace_bytes < LongArea<V>::carve(&l, (char*)workspace, a.rows, a.K))
         return fail(-1, "workspace too small (mppi_draw_workspace)");
@@ -1580,7 +1586,7 @@ template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_byte
 
 size_t workspace_of(int dtype, size_t rows, size_t K) {
     const size_t size = dtype == MPPI_F64 ? 8 : dtype == MPPI_F32 ? 4 : 2;
-    if (K * size <= SHELF) return 0;
+    if (K * size <= SHELF && !few_long_rows(rows, K)) return 0;
     return dtype == MPPI_F64 ? LongArea<double>::carve(nullptr, nullptr, rows, K) : LongArea<float>::carve(nullptr, nullptr, rows, K);
 }
 
