@@ -237,7 +237,7 @@ def test_more_rows_than_one_grid_holds():
 
 
 def test_more_draws_than_one_workgroup_takes():
-    for K, D, dtype in ((300, 16385, "float64"), (3000, 33000, "float32"), (9000, 40000, "bfloat16")):
+    for K, D, dtype in ((300, 16385, "float64"), (3000, 33000, "float32"), (9000, 40000, "bfloat16"), (20000, 8192, "float32"), (20000, 8193, "float32")):
         _check(_returns(2, K, dtype, K, masked=0.1), _numbers(2, D, K), kappa=0.7, top_p=0.99)
 
 

@@ -1550,8 +1550,10 @@ template <class T, int CHUNK> int launch_chunks(const DrawArgs& a, const LongAre
 }
 template <class T> int launch(DrawArgs a, void* workspace, size_t workspace_bytes, hipStream_t s) {
     using V = typename Traits<T>::V;
-    // (not where top-k leaves little to do behind the first pass: 1 x 65536 bf16 with k = 64 22 us and 25, 64 rows 25 and 41)
-    const bool few = few_long_rows(a.rows, a.K) && (a.f.top_k_of || a.f.top_k == 0 || a.f.top_k > 512);
+    // (Not where top-k leaves little to do behind the first pass: 1 x 65536 bf16 with k = 64 22 us and 25, 64 rows 25 and 41.  Nor for very
+    // many draws, which evaluate their segment's weights each: 1 x 32768 fp32, 16384 draws 23 and 24, 65536 24 and 51; 32 rows, 256 draws
+    // each 25 and 19, 1024 each 24 and 34.)
+    const bool few = few_long_rows(a.rows, a.K) && (a.f.top_k_of || a.f.top_k == 0 || a.f.top_k > 512) && (long long)a.rows * a.D <= 16384;
     if ((size_t)a.K * sizeof(T) <= SHELF && !few) {
         // One wave needs no barriers, but has every pass to itself: 1024 x 512 fp32 with all filters 9.8 us by 64 threads, 18.7 by 512;
         // 1 x 512 and 64 draws 9.3 and 10.3, 200 draws 11.4 and 10.4.  More than 512 threads pay where a row would otherwise be more
