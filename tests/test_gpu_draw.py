@@ -197,6 +197,31 @@ def test_parameters_per_row(K):
     assert index32.shape == index.shape
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float64"])
+@pytest.mark.parametrize("K", [30, 500, 6000, 20000, 70000])
+def test_parameters_per_row_outside_their_range(K, dtype):
+    """Every parameter alone, on either side of its range: its row has no samples (a negative top_k: all), the rows beside it
+    are drawn from as ever."""
+    import torch
+    inf, nan = float("inf"), float("nan")
+    bad = [("kappa", v) for v in (-1.0, -inf, inf, nan)] + [("top_p", v) for v in (1.5, inf, 1.0 + 2.0 ** -52, 0.0, -0.5, -inf, nan)] + \
+          [("min_p", v) for v in (-0.1, -inf, -5e-324, 1.0 + 2.0 ** -52, inf, nan)]
+    rows = 2 * len(bad) + 2
+    R = _returns(rows, K, dtype, K, masked=0.02)
+    for D in (1, 9):
+        u = _numbers(rows, D, K + D)
+        for usual in (dict(kappa=0.8, top_k=0, top_p=0.9, min_p=0.01), dict(kappa=0.8, top_k=K // 3, top_p=1.0, min_p=0.0)):
+            of = {name: torch.full((rows,), usual[name], dtype=torch.int64 if name == "top_k" else torch.float64, device="cuda") for name in usual}
+            for i, (name, value) in enumerate(bad):
+                of[name][2 * i + 1] = value
+            of["top_k"][rows - 1] = -3
+            index, weight = _draw(R, u, **of)
+            for i, (name, value) in enumerate(bad):
+                assert (index[2 * i + 1] == -1).all() and (weight[2 * i + 1] == 0).all(), (name, value)
+            _check(R[::2], u[::2], got=(index[::2], weight[::2]), **usual)
+            _check(R[-1:], u[-1:], got=(index[-1:], weight[-1:]), **dict(usual, top_k=0))
+
+
 def test_many_rows_and_many_draws():
     R, u = _returns(700, 130, "float32", 1), _numbers(700, 1, 1)
     _check(R, u, kappa=2.0, top_k=64, top_p=0.95, min_p=0.01)

@@ -156,7 +156,8 @@ struct Param {
     __device__ Param(const mppi_draw_filter& f, long long row)
         : kappa(f.kappa_of ? f.kappa_of[row] : f.kappa), top_p(f.top_p_of ? f.top_p_of[row] : f.top_p),
           min_p(f.min_p_of ? f.min_p_of[row] : f.min_p), top_k(f.top_k_of ? f.top_k_of[row] : f.top_k) {}
-    __device__ bool valid() const { return kappa >= 0.0 && kappa < INFINITY; }
+    // Values that the host has not seen, one per row: outside its range (or NaN) any of them leaves the row without samples.
+    __device__ bool valid() const { return kappa >= 0.0 && kappa < INFINITY && top_p > 0.0 && top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0; }
 };
 // u in [0, 1) -> a whole number below the mass
 __device__ __forceinline__ unsigned long long target_of(double u, unsigned long long mass) {

@@ -81,7 +81,8 @@ def draw_from_returns(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0):
     top_k   the best k samples (equal returns: lower index first); 0: all
     top_p   of these, the best that hold this fraction of their weight (the one that crosses it included), in (0, 1]
     min_p   of these, the ones with at least this fraction of the best sample's weight, in [0, 1]
-    Each of the four parameters may also be a (P,) tensor, one value per planner.
+    Each of the four parameters may also be a (P,) tensor, one value per planner; there a value outside its range leaves its
+    row without samples (a negative top_k: with all of them), as it cannot be refused without waiting for the device.
 
     Returns (index, weight) of u's shape: index (int64) is the smallest one at which the running sum of the kept weights
     exceeds u times their sum, weight (float32) its share of that sum.  A row without samples gives -1 and 0.  Runs on
