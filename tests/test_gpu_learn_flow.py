@@ -181,6 +181,43 @@ def test_draw_refusals(dm):
     p.close()
 
 
+def test_no_shard_draws(dm):
+    """The first shard of a caller-made exchange has offset 0 like a whole planner; that its statistics go out tells it from one."""
+    import torch
+    from trajopt_amd._lib import MppiError
+    K, H = 64, 4
+    shards = [_p(dm, K, H, "f64", k_offset=r * K) for r in range(2)]
+    for s in shards:
+        s.set_start_state(np.zeros(7), np.zeros(7), np.zeros(3), 0)
+        s.set_base_actions(np.zeros((H, 7)))
+        s.generate_noise(3)
+    for begin in (lambda p: p.partials_ptr(), lambda p: p.local_partials()):
+        for s in shards:
+            begin(s)
+            with pytest.raises(MppiError, match="every sample"):
+                s.draw(0.5)
+            s.synchronize()
+    gathered = torch.from_numpy(np.stack([s.partials() for s in shards])).cuda()
+    torch.cuda.synchronize()
+    for s in shards:
+        s.merge(gathered.data_ptr(), 2)
+        seq = s.act_sequence()
+        with pytest.raises(MppiError, match="every sample"):
+            s.draw(0.5)
+        assert np.array_equal(s.act_sequence(), seq)
+        s.close()
+    # a world of one rank: the same calls, and all samples there are
+    p = _p(dm, K, H, "f64")
+    p.set_start_state(np.zeros(7), np.zeros(7), np.zeros(3), 0)
+    p.set_base_actions(np.zeros((H, 7)))
+    p.generate_noise(3)
+    p.local_partials()
+    p.merge(p.partials_ptr()[0], 1)
+    p.draw(0.5)
+    assert p.drawn()[0] == ref_learn.draw(p.returns(), [0.5], 25.0)[0][0]
+    p.close()
+
+
 def _agent(noise, dtype="f64", **kw):
     from trajopt.algos.mppi import MPPI
     from trajopt.envs.utils import get_environment

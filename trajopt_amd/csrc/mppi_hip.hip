@@ -357,6 +357,7 @@ struct mppi_planner {
     double* d_part_alloc;           // the allocation d_part pointed at before
     char* d_draw;                   // mppi_draw: workspace, then [P] index, [P] u, [P] weight (made on the first call)
     size_t draw_workspace;
+    bool shard;                     // statistics of these samples go out to be merged with other ranks' (mppi_partials_ptr, mppi_local_partials, mppi_merge)
     bool profiling;
     std::vector<hipEvent_t>* prof_events;   // start/stop pairs around every rollout launch
     std::vector<DevState>* h_state;         // host mirror of the fields the host sets (alpha, ref_len, start state)
@@ -1003,6 +1004,7 @@ int mppi_local_partials(mppi_planner* p, void* stream) try {
     }
     HIP_OK(hipSetDevice(p->cfg.device));
     hipStream_t s = pick(p, stream);
+    p->shard = true;
     int rc = launch_rollout_only(p, s);
     if (rc) return rc;
     return launch_partials(p, s);
@@ -1012,6 +1014,7 @@ int mppi_local_partials(mppi_planner* p, void* stream) try {
 
 int mppi_partials_ptr(mppi_planner* p, void** ptr, size_t* bytes) try {
     if (!p || !ptr || !bytes) return fail(-1, "null argument");
+    p->shard = true;
     *ptr = p->d_part;
     *bytes = (size_t)(3 + p->HM) * p->P * 8;
     return 0;
@@ -1023,6 +1026,7 @@ int mppi_merge(mppi_planner* p, const void* gathered, int32_t nranks, void* stre
     if (!p || !gathered || nranks < 1) return fail(-1, "bad argument");
     HIP_OK(hipSetDevice(p->cfg.device));
     act_sequence_changed(p);
+    p->shard = nranks > 1;                         // (merged with nothing else: the samples are all there are)
     return launch_merge(p, (const double*)gathered, nranks, pick(p, stream));
 } catch (const std::exception& e) {
     return fail(-8, std::string("host exception: ") + e.what());
@@ -1034,7 +1038,7 @@ static float* draw_weight(mppi_planner* p) { return (float*)(draw_numbers(p) + p
 
 int mppi_draw(mppi_planner* p, const double* u, int64_t top_k, double top_p, double min_p, void* stream) try {
     if (!p || !u) return fail(-1, "null argument");
-    if (p->comm || p->cfg.k_offset != 0) return fail(-4, "mppi_draw needs every sample of the planner on one GPU");
+    if (p->comm || p->cfg.k_offset != 0 || p->shard) return fail(-4, "mppi_draw needs every sample of the planner on one GPU");
     mppi_draw_filter f;
     std::memset(&f, 0, sizeof(f));
     f.kappa = p->cfg.kappa; f.top_k = top_k; f.top_p = top_p; f.min_p = min_p;
