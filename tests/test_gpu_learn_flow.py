@@ -218,6 +218,28 @@ def test_no_shard_draws(dm):
     p.close()
 
 
+def test_a_group_of_one_rank_draws(dm):
+    """After mppi_comm_init with one rank the planner still owns every sample: drawn steps and iterations in turn, as without."""
+    from trajopt_amd.device import DevicePlanner
+    out = []
+    for grouped in (False, True):
+        p = _p(dm, 128, 5, "f64", kappa=2.0)
+        p.set_start_state(np.zeros(7), np.zeros(7), np.zeros(3), 0)
+        p.set_base_actions(np.zeros((5, 7)))
+        if grouped:
+            p.comm_init(DevicePlanner.comm_unique_id(), 0, 1)
+        p.generate_noise(4)
+        p.draw(0.3, top_k=30)
+        first = p.drawn(), p.act_sequence()
+        assert first[0][0] == ref_learn.draw(p.returns(), [0.3], 2.0, 30)[0][0]
+        p.iterate(1)
+        p.draw(0.8, top_p=0.7)
+        out.append((first, p.drawn(), p.act_sequence()))
+        p.close()
+    for (a, b) in ((out[0][0], out[1][0]), (out[0][1:], out[1][1:])):
+        assert a[0] == b[0] and np.array_equal(a[1], b[1])
+
+
 def _agent(noise, dtype="f64", **kw):
     from trajopt.algos.mppi import MPPI
     from trajopt.envs.utils import get_environment

@@ -1038,7 +1038,7 @@ static float* draw_weight(mppi_planner* p) { return (float*)(draw_numbers(p) + p
 
 int mppi_draw(mppi_planner* p, const double* u, int64_t top_k, double top_p, double min_p, void* stream) try {
     if (!p || !u) return fail(-1, "null argument");
-    if (p->comm || p->cfg.k_offset != 0 || p->shard) return fail(-4, "mppi_draw needs every sample of the planner on one GPU");
+    if ((p->comm && p->comm_nranks > 1) || p->cfg.k_offset != 0 || p->shard) return fail(-4, "mppi_draw needs every sample of the planner on one GPU");
     mppi_draw_filter f;
     std::memset(&f, 0, sizeof(f));
     f.kappa = p->cfg.kappa; f.top_k = top_k; f.top_p = top_p; f.min_p = min_p;
