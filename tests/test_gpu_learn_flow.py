@@ -363,6 +363,59 @@ def test_clipping_tells_autograd_that_it_wrote():
         z.backward()
 
 
+def test_no_graph_is_dropped_in_silence():
+    """Autograd's tensors are refused while it records and taken while it does not; nothing is written by a refused call, and
+    tensors that stand for others (vmap, forward mode, without memory) are refused as well."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from trajopt_amd.device import clip_gradients, draw_from_returns, gradient_norm
+    leaf = torch.randn(40, device="cuda", requires_grad=True)
+    u = torch.tensor([0.1, 0.9], device="cuda", dtype=torch.float64)
+    keep, plain = leaf.detach().clone(), torch.ones(40, device="cuda")
+    for call in (lambda: draw_from_returns(leaf, u), lambda: gradient_norm([leaf]), lambda: clip_gradients([leaf * 1.0], 0.1),
+                 lambda: clip_gradients([leaf], 0.1), lambda: clip_gradients([plain], 0.1, out=[leaf])):
+        with pytest.raises(RuntimeError, match="no derivative"):
+            call()
+    assert torch.equal(leaf, keep) and (plain == 1).all()
+    with torch.no_grad():
+        a, b = draw_from_returns(leaf, u), draw_from_returns(keep, u)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and not a[1].requires_grad
+        assert torch.equal(gradient_norm([leaf]), gradient_norm([keep]))
+        version = leaf._version
+        clip_gradients([leaf], 0.1)
+        clip_gradients([keep], 0.1)
+        assert torch.equal(leaf, keep) and leaf._version > version
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(plain, torch.ones_like(plain))
+        for call in (lambda: draw_from_returns(dual, u), lambda: gradient_norm([dual]), lambda: clip_gradients([dual], 0.1)):
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call()
+    for call in (lambda x: draw_from_returns(x, u)[1], lambda x: gradient_norm([x]), lambda x: clip_gradients([x], 0.1)):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(plain.reshape(4, 10))
+        with pytest.raises(RuntimeError), FakeTensorMode():
+            call(torch.ones(40, device="cuda"))
+    assert (plain == 1).all()
+
+
+def test_critic_clips_gradients_that_have_a_graph_of_their_own():
+    import torch
+    from trajopt.models.critic_nets import Critic
+    torch.manual_seed(3)
+    critic = Critic(input_dim=14, inner_layer=128).cuda()
+    (critic(torch.randn(8, 14, device="cuda")) ** 2).sum().backward(create_graph=True)
+    grads = [p.grad for p in critic.parameters()]
+    assert any(g.requires_grad for g in grads)
+    want_norm, want = ref_learn.clip([g.detach().double().cpu().numpy() for g in grads], 0.01)
+    assert want_norm > 0.01
+    norm = critic.clip_gradients(0.01)
+    assert not norm.requires_grad and abs(float(norm) - want_norm) <= (2.0 ** -24 + 1e-12) * want_norm
+    for g, w in zip(grads, want):
+        assert np.all(np.abs(g.detach().double().cpu().numpy() - w) <= 2.0 ** -24 * 1.0000001 * np.abs(w) + 2.0 ** -150)
+    for p in critic.parameters():
+        p.grad = None                                         # (a graph that holds its own leaves)
+
+
 def test_epochs_of_drawn_steps_and_clipped_training():
     """The whole loop: drawn steps fill the replay buffer, the critic trains on the GPU with clipped gradients, the next
     epoch's rollouts end in the trained critic's value."""

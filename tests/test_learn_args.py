@@ -100,6 +100,25 @@ def test_python_refusals():
         clip_gradients([], 1.0)
 
 
+def test_tensors_that_autograd_follows_are_refused():
+    """There are no derivatives: what would drop a graph without a word is refused before anything is launched (tensors
+    without memory, so that no GPU is needed)."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from trajopt_amd.device import clip_gradients, draw_from_returns, gradient_norm
+    with FakeTensorMode():
+        x = torch.empty(3, 4, device="cuda")
+        leaf = torch.empty(3, 4, device="cuda", requires_grad=True)
+        row = torch.empty(3, dtype=torch.float64, device="cuda", requires_grad=True)
+        u = torch.empty(3, 1, device="cuda", dtype=torch.float64)
+        for call in (lambda: draw_from_returns(leaf, u), lambda: draw_from_returns(leaf * 2.0, u), lambda: draw_from_returns(x, u, kappa=row),
+                     lambda: draw_from_returns(x, u, top_p=row), lambda: draw_from_returns(x, u, min_p=row),
+                     lambda: gradient_norm([x, leaf]), lambda: gradient_norm(leaf * 2.0), lambda: clip_gradients([leaf], 1.0),
+                     lambda: clip_gradients([leaf * 2.0], 1.0), lambda: clip_gradients([x], 1.0, out=[leaf])):
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call()
+
+
 def test_oracle_draws():
     R = np.array([1.0, 3.0, np.nan, 2.0, 3.0, -np.inf])
     assert np.allclose(ref_learn.kept_weights(R, 1.0), [np.exp(-2), 1, 0, np.exp(-1), 1, 0])

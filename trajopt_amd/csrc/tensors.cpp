@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 
 #include <vector>
@@ -59,6 +60,13 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& d
 bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
 const at::Tensor& tensor(PyObject* o) { return THPVariable_Unpack(o); }
 
+// None of these functions has a derivative.  A tensor that autograd would have to follow through one is refused: the result would look
+// like a constant, and a write would go past the graph.
+void untracked(const at::Tensor& t, const char* what) {
+    if ((c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())
+        raise(PyExc_RuntimeError, std::string(what) + ": part of a graph, and this function has no derivative (detach() it, or call under torch.no_grad())");
+}
+
 // a draw's parameter: a number, or a tensor of one value per row
 struct PerRow {
     at::Tensor held;
@@ -71,6 +79,7 @@ struct PerRow {
             raise(PyExc_ValueError, std::string(name) + ": one value per row, shape (" + std::to_string(rows) + ",), got " + text(t.sizes()));
         if (t.is_complex() || (type == at::kLong && t.is_floating_point()))
             raise(PyExc_TypeError, std::string(name) + ": unsupported element type " + c10::toString(t.scalar_type()));
+        if (type == at::kDouble) untracked(t, name);
         held = t.detach().to(type).contiguous().resolve_neg();
         data = held.const_data_ptr();
     }
@@ -102,6 +111,7 @@ PyObject* draw(PyObject* const* args) {
     if (u.scalar_type() != at::kDouble && u.scalar_type() != at::kFloat)
         raise(PyExc_TypeError, std::string("u must be float64 or float32, got ") + c10::toString(u.scalar_type()));
     if (R.is_neg()) raise(PyExc_ValueError, "the returns are a lazily negated view: resolve_neg() them first");
+    untracked(R, "the returns");
     const int type = element_type(R, true);
     const bool one = R.dim() == 1;
     const int64_t rows = one ? 1 : R.size(0), K = R.size(one ? 0 : 1), D = u.size(one ? 0 : 1);
@@ -158,6 +168,7 @@ struct List {
             if (!x.is_non_overlapping_and_dense())
                 raise(PyExc_ValueError, std::string(what) + " must fill their memory without gaps or overlaps (a slice or an expanded tensor does not)");
             if (x.is_neg()) raise(PyExc_ValueError, std::string(what) + " must not be lazily negated views (resolve_neg())");
+            untracked(x, what);
             t.push_back(&x);
         }
     }

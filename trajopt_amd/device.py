@@ -86,7 +86,8 @@ def draw_from_returns(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
     Returns (index, weight) of u's shape: index (int64) is the smallest one at which the running sum of the kept weights
     exceeds u times their sum, weight (float32) its share of that sum.  A row without samples gives -1 and 0.  Runs on
-    the current stream of R's device, without synchronising; can be captured into a graph."""
+    the current stream of R's device, without synchronising; can be captured into a graph.  A draw has no derivative: returns
+    and parameters that require grad are refused unless grad mode is off."""
     return L.tensors().draw(R, u, kappa, top_k, top_p, min_p)
 
 
@@ -98,7 +99,8 @@ def _norm_type(norm):
 
 def gradient_norm(grads, norm="l2"):
     """Norm over all entries of a list of CUDA tensors (float32, float16, bfloat16, mixed freely): 'l2' or 'max', as a
-    float32 scalar tensor.  Sums of squares are fp64.  Runs on the device's current stream, without synchronising."""
+    float32 scalar tensor.  Sums of squares are fp64.  Runs on the device's current stream, without synchronising.  The norm
+    has no derivative: tensors that require grad are refused unless grad mode is off."""
     return L.tensors().gradients(grads, None, _norm_type(norm), None)
 
 
@@ -106,7 +108,8 @@ def clip_gradients(grads, max_norm, norm="l2", out=None):
     """Scales a list of gradients so that their norm over all entries is at most max_norm, in place or into `out` (tensors
     of the same shapes, types and layouts), and returns the norm before as a float32 scalar tensor.  A norm that is not
     finite leaves the gradients as they are: the caller sees it in the result and can skip the step.  Runs on the device's
-    current stream, without synchronising; can be captured into a graph, which then clips the same tensors."""
+    current stream, without synchronising; can be captured into a graph, which then clips the same tensors.  Tensors that
+    require grad are refused unless grad mode is off, `out` among them."""
     return L.tensors().gradients(grads, out, _norm_type(norm), float(max_norm))
 
 

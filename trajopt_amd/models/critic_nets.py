@@ -42,9 +42,11 @@ class Critic(nn.Module):
     def clip_gradients(self, max_norm, norm='l2'):
         """Scales the parameters' gradients, in place, so that their norm over all of them ('l2' or 'max') is at most max_norm;
         returns the norm before, as a scalar tensor.  For a critic that trains on the GPU, between `backward` and the
-        optimizer's step; a norm that is not finite leaves the gradients as they are."""
+        optimizer's step; a norm that is not finite leaves the gradients as they are.  Not part of any graph, also where the
+        gradients are (`backward(create_graph=True)`)."""
         from ..device import clip_gradients
-        return clip_gradients([p.grad for p in self.parameters() if p.grad is not None], max_norm, norm=norm)
+        with torch.no_grad():
+            return clip_gradients([p.grad for p in self.parameters() if p.grad is not None], max_norm, norm=norm)
 
     def compress_state(self, state, dim=14):
         return _slice(state, dim)
