@@ -305,6 +305,37 @@ def test_train_step_draw_refusals():
     assert u[0] == u[1] != u[2] and 0.0 <= u[0] < 1.0
 
 
+BAD_DRAWS = [dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=2.0), dict(u=[0.1, 0.2]),
+             dict(u=[]), dict(u=float("nan")), dict(u=float("inf")), dict(u="x"), dict(top_k=2.5), dict(top_k="x"), dict(min_p=None), dict(topk=3)]
+
+
+@pytest.mark.parametrize("noise", ["host", "philox"])
+def test_a_refused_drawn_step_changes_nothing(noise):
+    """Every refusal of train_step(draw=...) comes before noise, numpy's generator, act_sequence or the device is touched: an agent with
+    refused calls between its steps goes on as one without."""
+    from trajopt_amd._lib import MppiError
+    a, b = _agent(noise), _agent(noise)
+    for t in range(3):
+        for ag in (a, b):
+            np.random.seed(5)
+            ag.train_step(niter=2, draw=dict(top_k=10) if t == 1 else None)
+        np.random.seed(77)
+        before = np.random.get_state()[1].copy()
+        seq, ahead, device = a.act_sequence.copy(), a._ahead, a._planner.act_sequence()
+        for bad in BAD_DRAWS:
+            with pytest.raises((MppiError, ValueError, TypeError)):
+                a.train_step(niter=2, draw=bad)
+        a.kappa = -1.0                                         # an update takes it, a draw does not
+        with pytest.raises(MppiError):
+            a.train_step(niter=2, draw={})
+        a.kappa = b.kappa
+        assert np.array_equal(np.random.get_state()[1], before) and a._ahead is ahead and len(a.sol_state) == t + 2
+        assert np.array_equal(a.act_sequence, seq) and np.array_equal(a._planner.act_sequence(), device)
+    for ag in (a, b):
+        ag.train_step(niter=2, draw=dict(u=np.array([0.25]), min_p=0.01))
+    assert np.array_equal(a.act_sequence, b.act_sequence) and np.array_equal(a.sol_state[-1]["qp"], b.sol_state[-1]["qp"])
+
+
 def test_critic_gradients_clipped_on_the_way_to_the_optimizer():
     """A temporal-difference step of the critic on the GPU: gradients against differences of the loss, their norm and the
     clipped values against the definition, and the step an SGD makes with them."""

@@ -119,6 +119,26 @@ def test_tensors_that_autograd_follows_are_refused():
                 call()
 
 
+def test_numbers_of_a_drawn_step_are_checked_without_a_device():
+    """What train_step(draw=...) asks before it touches anything: the argument's form, and whether a draw takes its numbers."""
+    from trajopt.algos.mppi import MPPI
+    from trajopt_amd._lib import MppiError
+    from trajopt_amd.device import check_draw
+    check_draw(8, 5.0)
+    check_draw(1 << 24, 0.0, 1 << 40, 1.0, 1.0)
+    for bad in ((0, 1.0), ((1 << 24) + 1, 1.0), (8, -1.0), (8, float("nan")), (8, 1.0, -1), (8, 1.0, 0, 0.0), (8, 1.0, 0, 1.1), (8, 1.0, 0, float("nan")),
+                (8, 1.0, 0, 1.0, -0.5), (8, 1.0, 0, 1.0, 1.5)):
+        with pytest.raises(MppiError):
+            check_draw(*bad)
+    with pytest.raises(TypeError):
+        check_draw(8, 1.0, 2.5)
+    for u in (0.25, np.float32(0.25), np.array([0.25]), [0.25]):
+        assert MPPI._draw_arguments(dict(u=u), 0, 1)["u"] == 0.25
+    for u in ([], [0.1, 0.2], float("nan"), float("inf"), "x"):
+        with pytest.raises(ValueError):
+            MPPI._draw_arguments(dict(u=u), 0, 1)
+
+
 def test_oracle_draws():
     R = np.array([1.0, 3.0, np.nan, 2.0, 3.0, -np.inf])
     assert np.allclose(ref_learn.kept_weights(R, 1.0), [np.exp(-2), 1, 0, np.exp(-1), 1, 0])

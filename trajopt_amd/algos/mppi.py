@@ -20,7 +20,7 @@ Two keyword arguments are additions with behaviour-preserving defaults:
 """
 import numpy as np
 
-from ..device import DeviceModel, DevicePlanner, update_from_returns
+from ..device import DeviceModel, DevicePlanner, check_draw, update_from_returns
 from ..utils import (ReplayBuffer, Tuple, _host_threads, _set_numpy_state, all_worker_normals,  # noqa: F401
                      gather_paths_parallel, rollout_objective, score_trajectory, worker_seeds)
 from .trajopt_base import Trajectory
@@ -165,6 +165,8 @@ class MPPI(Trajectory):
             draw = self._draw_arguments(draw, self.seed + t, niter)
             if self.env.env_name not in _KERNEL_ENVS or (critic is not None and weights is None):
                 raise ValueError("a draw needs rollouts on the device: not with this environment or critic")
+            # (here, before noise is drawn, numpy's generator moves or an iteration runs)
+            check_draw(self.paths_per_cpu * self.num_cpu, self.kappa, draw["top_k"], draw["top_p"], draw["min_p"])
         if self.env.env_name in _KERNEL_ENVS and (critic is None or weights is not None):
             if act_sequence is None and self._real_env_steps_on_the_device():
                 # the whole step, the real environment's included, without leaving the device
@@ -191,6 +193,10 @@ class MPPI(Trajectory):
         d.update(draw)
         if d["u"] is None:
             d["u"] = np.random.default_rng(seed % 2 ** 64).random()
+        u = np.asarray(d["u"], dtype=np.float64).reshape(-1)
+        if len(u) != 1 or not np.isfinite(u[0]):
+            raise ValueError("u is one finite number, got %r" % (d["u"],))
+        d["u"] = float(u[0])
         return d
 
     # ---- device-resident iteration ------------------------------------------------------

@@ -91,6 +91,12 @@ def draw_from_returns(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return L.tensors().draw(R, u, kappa, top_k, top_p, min_p)
 
 
+def check_draw(K, kappa, top_k=0, top_p=1.0, min_p=0.0):
+    """Raises what a draw from K returns with these numbers would raise, without launching or needing anything."""
+    f = L.DrawFilterC(kappa=float(kappa), top_k=operator.index(top_k), top_p=float(top_p), min_p=float(min_p))
+    L.check(L.lib().mppi_draw_from_returns(0, None, L.F64, 0, int(K), 0, 0, None, 0, C.byref(f), None, None, None, 0, None))
+
+
 def _norm_type(norm):
     if norm not in L.NORMS:
         raise ValueError("norm must be 'l2' or 'max', got %r" % (norm,))
