@@ -187,7 +187,9 @@ int mppi_host_staging(mppi_planner* p, double** buffer_out);
  * samples [i*K/nstreams, (i+1)*K/nstreams) of the staging buffer (mppi_host_staging) with numpy's legacy stream, and
  * every finished stretch goes to the device on a side stream.  The planner's own stream is left alone, so the call may
  * overlap the rollouts of the previous planning step; mppi_commit_noise then applies sigma and the filter on the
- * planner's stream (behind the upload) and makes the draws the noise of the next rollouts.  state_out as for
+ * planner's stream (behind the upload) and makes the draws the noise of the next rollouts.  The call waits until the
+ * upload of the draws before has left the staging buffer; it returns while its own may still be under way, so the caller
+ * writes to that buffer again only behind the work that mppi_commit_noise enqueues.  state_out as for
  * mppi_numpy_normals (one stream only), or NULL.  Single planners (P = 1). */
 int mppi_draw_noise(mppi_planner* p, const uint32_t* seeds, int32_t nstreams, int32_t nthreads, uint32_t* state_out);
 int mppi_commit_noise(mppi_planner* p, void* stream);

@@ -389,3 +389,30 @@ def test_horizons_beyond_the_device_resident_advance():
         assert np.array_equal(ag.act_sequence[-1], np.zeros(7))
         with pytest.raises(MppiError):
             ag._planner.plan(1, 1, 1)
+
+
+@pytest.mark.parametrize("streams", [1, 4])
+def test_draws_made_ahead_leave_the_ones_under_way_alone(dm, streams):
+    """The host's draws pass through one staging buffer.  The first upload is held up behind a tenth of a second of rollouts, so
+    that the next draws are asked for before it has run: what was committed has to be the first ones all the same."""
+    K, H = 256, 32
+    p = _p(dm, K, H, "f64")
+    p.set_start_state(np.zeros(7), np.zeros(7), np.zeros(3), 0)
+    p.set_base_actions(np.zeros((H, 7)))
+    p.generate_noise(1)
+    p.iterate(1)
+    p.synchronize()
+    seeds = [[100 * i + j for j in range(streams)] for i in range(3)]
+    raw = [np.concatenate([ref_mppi.raw_normals(s, K // streams, H, 7) for s in ss]) for ss in seeds]
+    p.iterate(300)
+    p.draw_noise(seeds[0], 2)
+    p.commit_noise()
+    p.draw_noise(seeds[1], 2)
+    assert np.abs(p.actions() - p.act_sequence() - ref_mppi.filter_noise(raw[0].copy(), FILTER)).max() < 1e-12
+    p.commit_noise()
+    p.iterate(300)
+    p.draw_noise(seeds[2], 2)
+    assert np.abs(p.actions() - p.act_sequence() - ref_mppi.filter_noise(raw[1].copy(), FILTER)).max() < 1e-12
+    p.commit_noise()
+    assert np.abs(p.actions() - p.act_sequence() - ref_mppi.filter_noise(raw[2].copy(), FILTER)).max() < 1e-12
+    p.close()

@@ -760,6 +760,9 @@ int mppi_draw_noise(mppi_planner* p, const uint32_t* seeds, int32_t nstreams, in
         HIP_OK(hipEventCreateWithFlags(&p->ev_upload_done, hipEventDisableTiming));
         HIP_OK(hipEventRecord(p->ev_raw_free, p->stream));
     }
+    // The generator writes to the staging buffer at once, so the upload of the draws before has to have left it: committing them does
+    // not wait for that (and the upload itself may wait, for work that still holds d_raw).
+    HIP_OK(hipStreamSynchronize(p->copy_stream));
     // d_raw is free once the filter kernel of the previous commit has read it
     HIP_OK(hipStreamWaitEvent(p->copy_stream, p->ev_raw_free, 0));
     p->raw_pending = true;
