@@ -416,3 +416,22 @@ def test_draws_made_ahead_leave_the_ones_under_way_alone(dm, streams):
     p.commit_noise()
     assert np.abs(p.actions() - p.act_sequence() - ref_mppi.filter_noise(raw[2].copy(), FILTER)).max() < 1e-12
     p.close()
+
+
+def test_planners_end_with_an_upload_under_way(dm):
+    """Draws that nobody committed are still on their way when the planner goes: it waits for them before their buffer is freed."""
+    K, H = 1024, 32
+    raw = ref_mppi.raw_normals(3, K, H, 7)
+    for _ in range(3):
+        p = _p(dm, K, H, "f64")
+        p.set_start_state(np.zeros(7), np.zeros(7), np.zeros(3), 0)
+        p.set_base_actions(np.zeros((H, 7)))
+        p.generate_noise(1)
+        p.iterate(50)
+        p.draw_noise([3], 2)
+        p.close()
+        p = _p(dm, K, H, "f64")
+        p.draw_noise([3], 2)
+        p.commit_noise()
+        assert np.abs(p.actions() - p.act_sequence() - ref_mppi.filter_noise(raw.copy(), FILTER)).max() < 1e-12
+        p.close()

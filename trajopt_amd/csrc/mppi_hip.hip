@@ -571,6 +571,7 @@ void mppi_planner_destroy(mppi_planner* p) {
     if (!p) return;
     (void)hipSetDevice(p->cfg.device);
     if (p->stream) (void)hipStreamSynchronize(p->stream);
+    if (p->copy_stream) (void)hipStreamSynchronize(p->copy_stream);      // (an upload may still read the staging buffer)
     if (p->prof_events) for (hipEvent_t e : *p->prof_events) (void)hipEventDestroy(e);
     delete p->prof_events;
     delete p->h_state;
@@ -585,7 +586,7 @@ void mppi_planner_destroy(mppi_planner* p) {
     if (p->h_stage) (void)hipHostFree(p->h_stage);
     if (p->h_step) (void)hipHostFree(p->h_step);
     if (p->h_mirror) (void)hipHostFree(p->h_mirror);
-    if (p->copy_stream) { (void)hipStreamSynchronize(p->copy_stream); (void)hipStreamDestroy(p->copy_stream); }
+    if (p->copy_stream) (void)hipStreamDestroy(p->copy_stream);
     if (p->ev_raw_free) (void)hipEventDestroy(p->ev_raw_free);
     if (p->ev_upload_done) (void)hipEventDestroy(p->ev_upload_done);
     if (p->d_weights) (void)hipFree(p->d_weights);
