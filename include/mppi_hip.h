@@ -212,7 +212,7 @@ int mppi_iterate(mppi_planner* p, int32_t niter, void* stream);
  * mppi_draw_filter; 0, 1, 0 keep all).  u: one uniform number in [0, 1) per planner, host or device memory, copied before the
  * rollouts are launched (the call waits for what `stream` already holds).  The reference only
  * ever applies the mean (trajopt/algos/mppi.py:56-65); applied draws explore, which is what a critic's replay buffer wants.
- * MPPI_READ_DRAW tells the sample and its weight; a planner whose samples all diverged keeps its act_sequence (-1).  Works on
+ * MPPI_READ_DRAW tells the sample and its weight (-4 before the first draw and after one that failed on its way); a planner whose samples all diverged keeps its act_sequence (-1).  Works on
  * explicit action sequences (mppi_upload_actions) as well.  -4 on a planner that owns only a shard of its samples: after
  * mppi_comm_init of more than one rank, with a cfg.k_offset, and on the first shard of a caller-made exchange, which has none, from its first
  * mppi_partials_ptr or mppi_local_partials on (until an mppi_merge of its own row alone, nranks 1, says that its samples are all

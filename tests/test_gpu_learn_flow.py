@@ -181,6 +181,39 @@ def test_draw_refusals(dm):
     p.close()
 
 
+def test_a_failed_draw_has_no_outcome(dm):
+    """A draw on a capturing stream fails (it has to wait for the stream) behind its allocations: there is nothing to be read then, and
+    the next one is as if it had been the first."""
+    import ctypes
+    from trajopt_amd import _lib as L
+    hip = L.lib()                                             # (the runtime's functions through the library that links it)
+    outcome = []
+    for fails in (False, True):
+        p = _p(dm, 64, 4, "f64", kappa=2.0)
+        p.set_start_state(np.zeros(7), np.zeros(7), np.zeros(3), 0)
+        p.set_base_actions(np.zeros((4, 7)))
+        p.generate_noise(1)
+        p.rollout()
+        p.synchronize()
+        if fails:
+            s, g = ctypes.c_void_p(), ctypes.c_void_p()
+            assert hip.hipStreamCreate(ctypes.byref(s)) == 0 and hip.hipStreamBeginCapture(s, 2) == 0
+            with pytest.raises(L.MppiError, match="error -2"):
+                p.draw(0.5, stream=s)
+            hip.hipStreamEndCapture(s, ctypes.byref(g))       # (no capture is left: the wait has ended it)
+            assert hip.hipStreamDestroy(s) == 0
+            hip.hipGetLastError()
+            with pytest.raises(L.MppiError, match="no draw"):
+                p.drawn()
+        p.draw(0.5)
+        outcome.append((p.drawn(), p.act_sequence()))
+        with pytest.raises(L.MppiError):
+            p.draw(0.5, top_p=2.0)                            # a refused draw leaves the last one's outcome
+        assert p.drawn() == outcome[-1][0]
+        p.close()
+    assert outcome[0][0] == outcome[1][0] and np.array_equal(outcome[0][1], outcome[1][1])
+
+
 def test_no_shard_draws(dm):
     """The first shard of a caller-made exchange has offset 0 like a whole planner; that its statistics go out tells it from one."""
     import torch

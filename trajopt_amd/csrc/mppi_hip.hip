@@ -357,6 +357,7 @@ struct mppi_planner {
     double* d_part_alloc;           // the allocation d_part pointed at before
     char* d_draw;                   // mppi_draw: workspace, then [P] index, [P] u, [P] weight (made on the first call)
     size_t draw_workspace;
+    bool drawn;                     // d_draw holds the outcome of the last draw
     bool shard;                     // statistics of these samples go out to be merged with other ranks' (mppi_partials_ptr, mppi_local_partials, mppi_merge)
     bool profiling;
     std::vector<hipEvent_t>* prof_events;   // start/stop pairs around every rollout launch
@@ -1060,6 +1061,7 @@ int mppi_draw(mppi_planner* p, const double* u, int64_t top_k, double top_p, dou
         HIP_OK(hipMalloc(&p->d_draw, p->draw_workspace + (size_t)p->P * (8 + 8 + 4)));
     }
     HIP_OK(copy_now(draw_numbers(p), u, (size_t)p->P * 8, hipMemcpyDefault, s));
+    p->drawn = false;                              // (until all of it has been launched)
     act_sequence_changed(p);
     rc = launch_rollout_only(p, s);
     if (rc) return rc;
@@ -1072,6 +1074,7 @@ int mppi_draw(mppi_planner* p, const double* u, int64_t top_k, double top_p, dou
     else
         hipLaunchKernelGGL((draw_apply_kernel<double>), grid, dim3(256), 0, s, draw_index(p), (const double*)p->d_eps, p->cfg.K, p->HM, p->explicit_act, p->d_base);
     HIP_OK(hipGetLastError());
+    p->drawn = true;
     return 0;
 } catch (const std::exception& e) {
     return fail(-8, std::string("host exception: ") + e.what());
@@ -1447,7 +1450,7 @@ int mppi_read(mppi_planner* p, int32_t what, void* dst, size_t bytes) try {
         HIP_OK(copy_now(dst, p->d_status, 16, hipMemcpyDeviceToHost, p->stream));
         return 0;
     case MPPI_READ_DRAW: {
-        if (!p->d_draw) return fail(-4, "mppi_draw has not been called on this planner");
+        if (!p->drawn) return fail(-4, "the planner holds no draw (mppi_draw has not been called, or failed)");
         if (!need(P * 16)) return fail(-1, "DRAW needs 2 doubles per planner");
         std::vector<int64_t> k(P);
         std::vector<float> w(P);
