@@ -141,6 +141,31 @@ def test_range_of_the_type():
             _check(close.repeat(1, K // 1000), u, kappa=1.0, top_k=K // 3 + 1, top_p=0.7)
 
 
+@pytest.mark.parametrize("dtype", ["float64", "float32"])
+@pytest.mark.parametrize("K", [200, 1000, 9000, 17000, 70000])
+def test_ranges_that_overflow(K, dtype):
+    """Both ends of the type in one row (their distance is infinite, the bins' quotient zero), ranges so small that the quotient is
+    infinite, and rows whose lowest values a look at every fourth sample misses."""
+    import torch
+    t = getattr(torch, dtype)
+    rng = np.random.RandomState(K)
+    big, small = torch.finfo(t).max, torch.finfo(t).tiny * torch.finfo(t).eps
+    u = _numbers(3, 7, K)
+    filters = (dict(), dict(top_k=K // 3), dict(top_p=0.6), dict(top_k=K // 2, top_p=0.7), dict(top_k=20))
+    ends = torch.tensor(rng.choice([-big, -big / 2, 0.0, big / 3, big], size=(3, K)), device="cuda", dtype=t)
+    for f in filters:
+        _check(ends, u, kappa=0.0, **f)
+    denormal = torch.tensor(rng.randint(0, 5, size=(3, K)) * small, device="cuda", dtype=t)
+    for f in filters:
+        _check(denormal, u, kappa=0.3, **f)
+    low = _returns(3, K, dtype, K)
+    at = torch.arange(K, device="cuda")
+    low = torch.where((at % 4 != 0) & (at % 5 == 1), torch.full_like(low, -big / 4), low)
+    for f in filters + (dict(top_k=K - 3), dict(top_p=0.999)):
+        _check(low, u, kappa=0.0, **f)
+        _check(low, u, kappa=0.9, **f)
+
+
 def test_numbers_at_the_ends():
     import torch
     for K in (40, 5000, 80000):

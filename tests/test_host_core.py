@@ -153,3 +153,32 @@ def test_runge_kutta_integrator(core):
     assert np.abs(hand - nobs_o[0, -1, 37:40]).max() < 1e-10 and abs(np.linalg.norm(q[3:7]) - 1) < 1e-14
     q, v, _, _, R32, _ = core(0, q0, v0, tgt, act, gamma=0.99, model=4)
     assert (np.abs(np.r_[q, v] - nobs_o[0, -1, :37]) / (1 + np.abs(nobs_o[0, -1, :37]))).max() < 2e-3
+
+
+def test_bins_of_any_distance(tmp_path):
+    """csrc/bins.hpp, evaluated by the compiler: a conversion without a value (a float beyond int, infinity) would not be a constant
+    expression.  The second source asks for one, so that the check is known to see it.  NaN, which compilers do not compare in
+    constants, is looked at in the program."""
+    source = tmp_path / "bins.cpp"
+    body = """#include "%s"
+    #include <limits>
+    template <class V> constexpr bool good() {
+        using L = std::numeric_limits<V>;
+        const V inf = L::infinity(), most = L::max();
+        int last = 0;
+        const V xs[] = {(V)0, -(V)0, L::denorm_min(), (V)0.99, (V)1, (V)1022.5, (V)1023, (V)1023.9, (V)1024, (V)1e9, (V)4e9, (V)1e30, most, inf};
+        for (V x : xs) {
+            const int b = bin_of(x, 1024);
+            if (b < last || b > 1023) return false;
+            last = b;
+        }
+        return bin_of((V)1022.5, 1024) == 1022 && bin_of((V)1023.9, 1024) == 1023 && bin_of(inf, 256) == 255 && last == 1023;
+    }
+    static_assert(good<float>() && good<double>(), "");
+    """ % os.path.join(ROOT, "trajopt_amd", "csrc", "bins.hpp")
+    for extra, fine in (("", True), ("constexpr int no_value = (int)1e30f;", False)):
+        source.write_text(body + extra + "\nint main(int n, char**) { return bin_of(0.0f / (n - 1), 256) == 255 && bin_of(0.0 / (n - 1), 256) == 255 ? 0 : 1; }\n")
+        done = subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "bins"), str(source)], capture_output=True, text=True)
+        assert (done.returncode == 0) == fine, done.stderr
+        if fine:
+            assert subprocess.run([str(tmp_path / "bins")]).returncode == 0

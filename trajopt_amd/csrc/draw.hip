@@ -23,6 +23,7 @@
 // top-p 9.2; 1024 x 512 fp32 with all three filters 8.8; 192 x 65535 bf16 with all three 17.2 (25 MB: 1.5 TB/s); 1 x 524288
 // fp32 with both borders 29; 16 x 262144 fp64 with top-p and 64 draws each 58.
 #include "abi_common.hpp"
+#include "bins.hpp"
 #include "../../include/mppi_hip.h"
 
 #include <algorithm>
@@ -282,10 +283,7 @@ __device__ bool find_border(Src& src, BorderArea<V, NT>& s, Group<NT>& group, un
     U top = 0;
     unsigned long long before = 0;
     unsigned n = most;
-    const auto linear = [&](V v) -> int {
-        const int b = (int)((high - v) * per);
-        return b < BINS ? b : BINS - 1;
-    };
+    const auto linear = [&](V v) -> int { return bin_of((high - v) * per, BINS); };
     const auto keyed = [&](V v) -> int { return (int)((top - key_of(v)) >> shift); };
     const auto fill = [&](auto bin_of) {
         src.each(lo, hi, [&](const V (&v)[VEC], unsigned live, int) {
@@ -520,8 +518,7 @@ template <class T, int NT, int BYTES> struct Shelf {
         constexpr int BINS = Area::BINS, PER = BINS / NT;
         const V per = w.best > bottom ? (V)BINS / (w.best - bottom) : (V)0;
         const bool in = mine >= w.from;
-        int b = in ? (int)((w.best - mine) * per) : 0;
-        b = b < BINS ? b : BINS - 1;
+        const int b = in ? bin_of((w.best - mine) * per, BINS) : 0;
 #pragma unroll
         for (int i = 0; i < PER; i++) s.b.cnt[threadIdx.x + i * NT] = 0;
         __syncthreads();
@@ -1018,10 +1015,7 @@ template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_bes
 template <class V> struct LongBins {
     V best, per;
     __device__ LongBins(const Weights<V>& w) : best(w.best), per(w.best > w.from ? (V)LONG_BINS / (w.best - w.from) : (V)0) {}
-    __device__ __forceinline__ int of(V v) const {
-        const int b = (int)((best - v) * per);
-        return b < LONG_BINS ? b : LONG_BINS - 1;
-    }
+    __device__ __forceinline__ int of(V v) const { return bin_of((best - v) * per, LONG_BINS); }
 };
 
 template <class T, int CHUNK> __global__ void __launch_bounds__(LT, 4) chunk_bins_kernel(DrawArgs a, LongArea<typename Traits<T>::V> l) {
