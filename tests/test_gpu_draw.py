@@ -166,6 +166,31 @@ def test_ranges_that_overflow(K, dtype):
         _check(low, u, kappa=0.9, **f)
 
 
+@pytest.mark.parametrize("K", [7, 64, 300, 1000, 9000, 17000, 70000])
+@pytest.mark.parametrize("kappa", [3e-308, 1e-308, 5e-309, 1e-310])
+def test_distances_beyond_the_range_of_fp64(K, kappa):
+    """Returns whose distance fp64 does not hold, at temperatures that tell them apart all the same; against 80-bit numbers."""
+    import torch
+    rng = np.random.RandomState(K)
+    big = np.finfo(np.float64).max
+    R = rng.uniform(-1.0, 1.0, size=K) * big
+    R[rng.randint(K)] = big
+    R[0] = -big
+    u = rng.uniform(size=33)
+    for top_k, min_p in ((0, 0.0), (K // 2 + 1, 0.0), (0, 0.2)):
+        x = R.astype(np.longdouble)
+        w = np.exp(-np.longdouble(kappa) * (x.max() - x))
+        if top_k:
+            w[np.argsort(-R, kind="stable")[top_k:]] = 0
+        w[w < min_p] = 0
+        upto = np.cumsum(w)
+        want = np.searchsorted(upto, u.astype(np.longdouble) * upto[-1], side="right")
+        index, weight = _draw(torch.tensor(R[None], device="cuda"), torch.tensor(u[None], device="cuda"), kappa=kappa, top_k=top_k, min_p=min_p)
+        assert np.array_equal(index.cpu().numpy()[0], want), (top_k, min_p)
+        share = (w[want] / upto[-1]).astype(np.float64)
+        assert np.all(np.abs(weight.cpu().numpy()[0] - share) <= WEIGHT_RTOL * share)
+
+
 def test_numbers_at_the_ends():
     import torch
     for K in (40, 5000, 80000):

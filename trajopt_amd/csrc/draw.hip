@@ -204,6 +204,8 @@ __device__ __forceinline__ unsigned long long whole(double x) {
 
 template <class V> struct Weights {
     double kappa, scale;              // scale: 2^S
+    double unit, top;                 // fp64: both ends may be apart by more than its range; then distances are taken in halves,
+                                      // unit = 1/2, top = best unit, and kappa is twice what it was
     V best, from;                     // highest value of the row, lowest that takes part
 
     // Samples further behind than (S + 1) ln 2 / kappa have masses below half a unit.  (A margin covers the rounding of this
@@ -214,12 +216,16 @@ template <class V> struct Weights {
         scale = __longlong_as_double((long long)(1023 + S) << 52);
         const V bound = (V)((double)best - (S + 1.01) * 0.6931471805599453 / kappa * (1.0 + 1e-6));
         from = worst > bound ? worst : bound;        // (finite, as worst is)
+        if (sizeof(V) == 8) {
+            unit = (double)best - (double)from < INFINITY ? 1.0 : 0.5;       // (not a large kappa's: its `from` is near)
+            top = unit * (double)best;
+            kappa /= unit;
+        }
     }
-    // kappa (best - v) of a sample that takes part (of one that does not: that of the last that does).  Both ends of fp64 may be
-    // apart by more than its range, and 0 times that is 0.
+    // kappa (best - v) of a sample that takes part (of one that does not: that of the last that does)
     __device__ __forceinline__ double distance(V v) const {
-        const double d = (double)best - (double)(v > from ? v : from);
-        return kappa * (sizeof(V) == 8 ? fmin(d, 1.7976931348623157e308) : d);
+        const double x = (double)(v > from ? v : from);
+        return kappa * (sizeof(V) == 8 ? fma(-x, unit, top) : (double)best - x);
     }
     __device__ __forceinline__ double weight(V v) const {
         const double d[1] = {distance(v)};
