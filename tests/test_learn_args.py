@@ -139,6 +139,19 @@ def test_numbers_of_a_drawn_step_are_checked_without_a_device():
             MPPI._draw_arguments(dict(u=u), 0, 1)
 
 
+def test_top_k_beyond_64_bits():
+    """Not its lowest 64 bits, which would keep 5 samples, or none of a filter."""
+    from trajopt_amd.device import DevicePlanner, check_draw
+    check_draw(8, 1.0, 2 ** 63 - 1)
+    for k in (2 ** 64 + 5, 2 ** 64, 2 ** 63, -2 ** 63 - 1):
+        with pytest.raises(OverflowError):
+            check_draw(8, 1.0, k)
+        p = DevicePlanner.__new__(DevicePlanner)              # (no device behind it: nothing may be called)
+        p.P, p._h = 1, None
+        with pytest.raises(OverflowError):
+            p.draw(0.5, top_k=k)
+
+
 def test_oracle_draws():
     R = np.array([1.0, 3.0, np.nan, 2.0, 3.0, -np.inf])
     assert np.allclose(ref_learn.kept_weights(R, 1.0), [np.exp(-2), 1, 0, np.exp(-1), 1, 0])

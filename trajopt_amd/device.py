@@ -91,9 +91,17 @@ def draw_from_returns(R, u, kappa=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return L.tensors().draw(R, u, kappa, top_k, top_p, min_p)
 
 
+def _int64(i):
+    """A whole number that fits the C ABI's 64 bits (ctypes would take its lowest ones)."""
+    i = operator.index(i)
+    if not -2 ** 63 <= i < 2 ** 63:
+        raise OverflowError("%d does not fit 64 bits" % i)
+    return i
+
+
 def check_draw(K, kappa, top_k=0, top_p=1.0, min_p=0.0):
     """Raises what a draw from K returns with these numbers would raise, without launching or needing anything."""
-    f = L.DrawFilterC(kappa=float(kappa), top_k=operator.index(top_k), top_p=float(top_p), min_p=float(min_p))
+    f = L.DrawFilterC(kappa=float(kappa), top_k=_int64(top_k), top_p=float(top_p), min_p=float(min_p))
     L.check(L.lib().mppi_draw_from_returns(0, None, L.F64, 0, int(K), 0, 0, None, 0, C.byref(f), None, None, None, 0, None))
 
 
@@ -304,7 +312,7 @@ class DevicePlanner:
         u = L.f64(u).reshape(-1)
         if u.shape != (self.P,):
             raise ValueError("one number per planner: %d planners, %d numbers" % (self.P, len(u)))
-        L.check(L.lib().mppi_draw(self._h, L.ptr(u), operator.index(top_k), float(top_p), float(min_p), stream))
+        L.check(L.lib().mppi_draw(self._h, L.ptr(u), _int64(top_k), float(top_p), float(min_p), stream))
 
     def local_partials(self, stream=None):
         L.check(L.lib().mppi_local_partials(self._h, stream))
