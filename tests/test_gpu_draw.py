@@ -388,6 +388,31 @@ def test_draws_of_long_rows(dtype, step, D):
         _check(R, u, kappa=0.9, **f)
 
 
+def test_offsets_beyond_32_bits():
+    """Rows, and samples of a row, further apart than 2^31 elements; and more than 2^31 samples in one call, of rows that one workgroup holds
+    and of rows in chunks (their lists lie as far apart)."""
+    import torch
+    far = 1 << 31
+    flat = torch.full((far + (1 << 20),), float("-inf"), dtype=torch.bfloat16, device="cuda")
+    for shape, strides in (((3, 50), (far // 2 + 7, 1)), ((3, 5000), (far // 2 + 7, 1)), ((2, 70001), (far + 11, 1)), ((2, 300), (5, far // 299)),
+                           ((2, 6000), (7, far // 5999)), ((2, 70001), (3, far // 70000))):
+        R = flat.as_strided(shape, strides)
+        R.copy_(_returns(*shape, "bfloat16", shape[1]))
+        _check(R, _numbers(shape[0], 5, shape[1]), kappa=0.8, top_k=shape[1] // 2, top_p=0.9)
+        R.fill_(float("-inf"))
+    del flat, R
+    for rows, K in ((40000, 65000), (33000, 70000)):
+        R = torch.full((rows, K), float("-inf"), dtype=torch.bfloat16, device="cuda")
+        first, gap = torch.arange(rows, device="cuda") * 7919 % (K - 200), torch.arange(rows, device="cuda") % 199 + 1
+        R.scatter_(1, torch.stack((first, first + gap), 1), 2.0)         # two samples of the same weight
+        u = torch.tensor([[0.25, 0.75]], dtype=torch.float64, device="cuda").repeat(rows, 1)
+        index, weight = _draw(R, u, top_p=0.9)
+        assert torch.equal(index, torch.stack((first, first + gap), 1)) and (weight == 0.5).all()
+        index, weight = _draw(R, u, top_p=0.4)
+        assert torch.equal(index, torch.stack((first, first), 1)) and (weight == 1).all()
+        del R
+
+
 def test_nothing_to_do():
     import torch
     R, u = _returns(2, 10, "float32", 0), _numbers(2, 0, 0)

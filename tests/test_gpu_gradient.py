@@ -276,3 +276,26 @@ def test_negated_views_are_refused():
         gradient_norm([lazy])
     with pytest.raises(ValueError, match="negated"):
         clip_gradients([torch.ones(1, device="cuda")], 1.0, out=[lazy])
+
+
+@pytest.mark.parametrize("kind", ["l2", "max"])
+def test_one_tensor_beyond_32_bits(kind):
+    """More than 2^31 entries in one tensor (and 2^32 bytes): entries at its ends and around 2^31, zeros between them."""
+    import torch
+    from trajopt_amd.device import clip_gradients, gradient_norm
+    n = (1 << 31) + 12345
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, (1 << 30) + 3, (1 << 31) - 1, 1 << 31, (1 << 31) + 1, n - 2, n - 1], device="cuda")
+    values = torch.tensor([3.0, -4.0, 2.0, 6.0, -1.0, 5.0, 8.0, -7.0], dtype=torch.bfloat16, device="cuda")
+    g[at] = values
+    small = torch.full((100,), 0.5, device="cuda")
+    both = [g, small]
+    want_norm, want = ref_learn.clip([values.double().cpu().numpy(), small.double().cpu().numpy()], 2.0, kind)
+    assert want_norm > 2.0
+    norm = gradient_norm(both, norm=kind)
+    assert abs(float(norm) - want_norm) <= (2.0 ** -24 + 1e-12) * want_norm
+    assert torch.equal(clip_gradients(both, 2.0, norm=kind), norm)
+    _close(g[at], want[0])
+    _close(small, want[1])
+    g[at] = 0
+    assert not g.any()
