@@ -276,7 +276,7 @@ int mppi_read_log(mppi_planner* p, int32_t planner, double* rows, int32_t max_ro
  * that step's kernel also writes both, and then the count of steps logged, into page-locked host memory of the planner,
  * and this call only waits for the count (it looks at the stream now and then, so a launch that failed cannot hang
  * it).  Every other case (batched planners, the last step inside a multi-step replay, act_sequence changed since by
- * mppi_set_base_actions / mppi_iterate / mppi_merge / mppi_shift) is two copies behind the stream of the last step and
+ * mppi_set_base_actions / mppi_iterate / mppi_draw / mppi_merge / mppi_shift) is two copies behind the stream of the last step and
  * one wait. */
 int mppi_read_step(mppi_planner* p, double* rows_out, double* act_seq_out);
 
@@ -357,7 +357,8 @@ int mppi_draw_from_returns(int32_t device, const void* d_R, int32_t dtype, int32
  * Tensor i has sizes[i] contiguous entries of type dtypes[i] (MPPI_F32, MPPI_F16 or MPPI_BF16) at the device address
  * d_grads[i], a multiple of the entry's size; the four arrays themselves are host memory and are read before the call returns.
  * d_out[i] = d_grads[i] clips in place; otherwise nothing that is written may overlap another tensor (-1).  Sums of squares
- * are fp64.  *d_norm (device memory) receives the norm before clipping, rounded to float.  d_workspace: device memory of at
+ * are fp64.  *d_norm (device memory) receives the norm before clipping, rounded to float (infinite where float ends, though
+ * the norm itself is finite and clips).  d_workspace: device memory of at
  * least mppi_gradient_workspace bytes, 8-byte aligned, that nothing else uses until the work on `stream` is done.  The work
  * is enqueued on `stream` (NULL: the default stream); nothing is allocated on the device or synchronised, and it may be
  * captured (with the addresses it was given).  The current device of the calling thread is left as it was. */

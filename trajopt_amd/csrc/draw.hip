@@ -4,7 +4,8 @@
 // Numbers.  A return that is NaN or infinite weighs nothing, as in the planner's updates.  Weights are evaluated in fp64 and
 // summed as 64-bit fixed point, q_i = round(w_i 2^S): integer sums do not depend on their order, so the histograms may use
 // atomics, a row gives the same answer however it is split, and ties are exact.  The best sample weighs 1, so a mass is never
-// below 2^S, and each of K roundings is off by half a unit at most.  Rows in LDS take the largest S at which K weights of 1
+// below 2^S, and each of K roundings is off by half a unit at most: a border between two samples lies within K 2^-(S + 1) of the mass
+// of where it would be without them (2^-31 for 65536 samples in LDS).  Rows in LDS take the largest S at which K weights of 1
 // stay below 2^62 (at most 51, where w 2^S still fits the 52 bits of a double's fraction: 46 for the longest row); longer
 // rows first sum their weights and take S from that sum, so that a row with few samples that count keeps 51 bits of them.
 // Samples with kappa (max - R) > (S + 1) ln 2 round to zero; they cannot be drawn, and are left out from the start.
@@ -19,9 +20,9 @@
 // What bounds it.  The bytes are few (the benchmark planner's row is 16 KB); what takes the time is one pass behind the other
 // over a row, with a barrier after each, and the instructions of code that runs once.  So a row stays in one workgroup's LDS as long
 // as it fits, passes test values in the type of the row and evaluate fp64 exponentials only where a sample passes, and loops are
-// rolled.  Per call, with the launch (3.6 us for the smallest kernel there is): 1 x 40 fp64 with top-k 5.3 us; 1 x 4096 fp32 with
-// top-p 9.2; 1024 x 512 fp32 with all three filters 8.8; 192 x 65535 bf16 with all three 17.2 (25 MB: 1.5 TB/s); 1 x 524288
-// fp32 with both borders 29; 16 x 262144 fp64 with top-p and 64 draws each 58.
+// rolled.  Per call in a row of calls (3.6 us for the smallest kernel there is): 1 x 40 fp64 with top-k 5.4 us; 1 x 4096 fp32 with
+// top-p 9.3; 1024 x 512 fp32 with all three filters 8.8; 192 x 65535 bf16 with all three 17.3 or 20, one of the two for as long as a
+// process runs (25 MB: 1.3 to 1.5 TB/s); 1 x 524288 fp32 with both borders 28.5; 16 x 262144 fp64 with top-p and 64 draws each 58.5.
 #include "abi_common.hpp"
 #include "bins.hpp"
 #include "../../include/mppi_hip.h"
@@ -873,8 +874,8 @@ template <class T, int NT, int BYTES> __global__ void __launch_bounds__(NT) draw
 // Rows without top-k and top-p need no list: the masses of their chunks stay as chunk_bins wrote them, and long_draw follows.
 //
 // Each of the first three reads the row once, and only the first finds it outside the caches (in part: an L2 holds 4 MB).  A launch
-// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 3.9, 8.0, 6.6, 9.7 us; 16 x 262144 fp64 (34 MB) and 64 draws: 11.3, 13.1,
-// 16.0, 16.1, 4.7 us, i.e. 3.0 TB/s for the reading alone and 2.1 TB/s with fp64 exponentials (some 20 operations of 4 cycles
+// takes 4 us by itself; by kernel, 1 x 524288 fp32 (2 MB): 3.9, 8.3, 6.7, 9.5 us; 16 x 262144 fp64 (34 MB) and 64 draws: 10.8, 13.5,
+// 16.2, 15.5, 4.8 us, i.e. 3.1 TB/s for the reading alone and 2.1 to 2.5 TB/s with fp64 exponentials (some 20 operations of 4 cycles
 // each for a wave) in the two that need masses.
 constexpr int MOST_SEGS = 64, LT = 512, LONG_BINS = 1024, BT = 256;
 

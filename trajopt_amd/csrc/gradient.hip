@@ -6,12 +6,13 @@
 // Numbers.  Squares and their sums are fp64, so no fp32 gradient overflows or vanishes in them, and every sum has a fixed order: a
 // thread adds what it reads, the lanes of a workgroup are added by a tree, and so are the partial sums of the workgroups, of
 // which the sizes of the tensors alone say what each covers.  Entries are scaled in fp64 (the scale of large gradients may lie below
-// fp32's range) and rounded to fp32; 16-bit ones from there to their type, 2^-16 of whose step the first rounding is at most.
+// fp32's range) and rounded to fp32; 16-bit ones from there to their type, of whose step the first rounding is at most 2^-14
+// (fp16) or 2^-17 (bf16).
 //
 // Two passes over the data: no entry can be scaled before all have been read.  Large sets are bound by memory: 1.07 GB of fp32 read
-// in 155 us (6.9 TB/s), 268 MB of bf16 read in 48 us and read again and written in 86 (6.2 TB/s; what a copy moves here: 4.8).  Small
+// in 155 us (6.9 TB/s), 268 MB of bf16 read in 48 us and read again and written in 85 to 92 (6 TB/s; what a copy moves here: 4.8).  Small
 // ones are bound by launches and by the host: the six tensors of a critic take one launch, 6.3 us per call; 384 small tensors four,
-// of which two carry tables of addresses, 27 to 31 us per call, 17 of them in this library and 14 on the GPU.
+// of which two carry tables of addresses, 28 to 35 us per call, of which the GPU works 12.
 #include "abi_common.hpp"
 #include "../../include/mppi_hip.h"
 

@@ -121,7 +121,8 @@ def gradient_norm(grads, norm="l2"):
 def clip_gradients(grads, max_norm, norm="l2", out=None):
     """Scales a list of gradients so that their norm over all entries is at most max_norm, in place or into `out` (tensors
     of the same shapes, types and layouts), and returns the norm before as a float32 scalar tensor.  A norm that is not
-    finite leaves the gradients as they are: the caller sees it in the result and can skip the step.  Runs on the device's
+    finite leaves the gradients as they are: the caller sees it in the result and can skip the step.  (A finite one beyond
+    float32's range is infinite in the result only: the gradients are clipped by it.)  Runs on the device's
     current stream, without synchronising; can be captured into a graph, which then clips the same tensors.  Tensors that
     require grad are refused unless grad mode is off, `out` among them."""
     return L.tensors().gradients(grads, out, _norm_type(norm), float(max_norm))
