@@ -280,7 +280,7 @@ def test_negated_views_are_refused():
 
 @pytest.mark.parametrize("kind", ["l2", "max"])
 def test_one_tensor_beyond_32_bits(kind):
-    """More than 2^31 entries in one tensor (and 2^32 bytes): entries at its ends and around 2^31, zeros between them."""
+    """More than 2^31 entries in one tensor (and 2^32 bytes): entries at its ends and near 2^31, zeros between them."""
     import torch
     from trajopt_amd.device import clip_gradients, gradient_norm
     n = (1 << 31) + 12345
